@@ -202,7 +202,8 @@ def run(state):
     if case["kind"] == "attend" and case["weights"]:
         cache["weight"].copy_(state["before"])   # every pass adds to the sums as they were before the step
     if own:
-        lib, handle, stream = state["lib"], state["store"].handle, torch.cuda.current_stream().cuda_stream
+        # (a null stream stands for the context's own; 1 is CUDA's handle of the default stream that torch works on)
+        lib, handle, stream = state["lib"], state["store"].handle, torch.cuda.current_stream().cuda_stream or 1
         if case["kind"] == "append":
             lib.check(lib.swlm_op_kv8_append_dev(handle, state["described"], state["call"], stream))
         elif case["kind"] == "attend":
