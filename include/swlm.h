@@ -294,6 +294,114 @@ int swlm_op_flash_decode_noalloc_dev(swlm_ctx* ctx, int b, int heads, int kv_hea
                                      int ctx_stride, float scale, const void* q_dev, const void* k_dev,
                                      const void* v_dev, void* out_dev, void* cuda_stream);
 
+/* ---- a caller's key/value cache held in 8 bits, one scale per block of tokens and head -----------------------------
+ * No counterpart in the reference, whose 8-bit caches (SWLM_KV_Q8G*) scale every 32 to 128 values of one token. A cached value is
+ * code * scale[block]; codes are signed bytes of -127..127 or e4m3 numbers. The three operators work on one layer's cache:
+ *
+ *   append    a step's new keys and values (already rotated) are quantized behind the tokens that a sequence has,
+ *   attend    the step's queries attend over the cache; each cached token's weight may be added to its running sum,
+ *   evict     every (sequence, KV head) keeps the tokens of the largest sums, in place or in a smaller cache.
+ *
+ * All of them are enqueued on `cuda_stream` (NULL = the context's own stream) without synchronising and without allocating, take
+ * their lengths from device memory, and can be captured into a graph. Pointers are device memory of the context's device. What two
+ * calls at once may share is what both only read: concurrent calls need scratch of their own. The counters
+ *
+ *   lengths[b]   tokens in the cache of sequence b before the step, the same for all layers; none of the calls changes it
+ *   counts[b]    its tokens in this step (NULL: n each); starts[b] the row of the first of them in the step's arrays (NULL: b * n)
+ *   seen[b]      position of the first of them: how many tokens the sequence has had, evicted ones included
+ *
+ * are advanced behind the last layer with swlm_op_kv8_lengths_dev. */
+enum { SWLM_KV8_INT8 = 0, SWLM_KV8_E4M3 = 1 };   /* swlm_kv8_cache.code */
+enum { SWLM_KV8_BF16 = 0, SWLM_KV8_FP16 = 1 };   /* type of keys, values, queries and results */
+
+typedef struct swlm_kv8_cache {
+    void* k;            /* codes [batch][kv_heads][capacity][head_dim], 16-byte aligned as v is */
+    void* v;
+    float* k_scale;     /* [batch][kv_heads][capacity / block] */
+    float* v_scale;
+    float* weight;      /* [batch][kv_heads][capacity]: attention weight that each slot's token has had so far; NULL: not kept */
+    int32_t* slot_pos;  /* [batch][kv_heads][capacity]: position of each slot's token; NULL: not kept (eviction needs both) */
+    int32_t batch, kv_heads;
+    int32_t head_dim;   /* 64 or 128 */
+    int32_t capacity;   /* slots of a sequence, a multiple of block */
+    int32_t block;      /* tokens of a scale: 16, 32, 64 or 128 */
+    int32_t code;       /* SWLM_KV8_INT8 or SWLM_KV8_E4M3 */
+} swlm_kv8_cache;
+
+/* New tokens. Row r of KV head h lies at k + r * k_stride + h * head_dim (strides in elements, multiples of 8). A block's scale is the
+ * largest |value| that it has taken over 127 (int8) or 448 (e4m3): s = max(old scale, max |new| / 127), codes are round(x / s), ties to
+ * even, and where s grows the block's older codes c become round(c * old / s). A block that takes an infinity or a NaN reads as NaN from
+ * then on. Slots get weight 0 and the position seen[b] + i.
+ * A sequence is refused as a whole - nothing of it is changed, refused[b] = 1 - where lengths[b] or counts[b] is negative, counts[b] > n,
+ * its rows are not within 0..rows-1, or it has no room for them; refused[b] = 0 otherwise (refused may be NULL). */
+typedef struct swlm_kv8_append {
+    const void* k;
+    const void* v;
+    int64_t k_stride, v_stride;
+    const int32_t* lengths;
+    const int32_t* counts;
+    const int32_t* starts;
+    const int32_t* seen;   /* needed where the cache has slot_pos */
+    int32_t* refused;
+    int32_t dtype;         /* SWLM_KV8_BF16 or SWLM_KV8_FP16 */
+    int32_t n;             /* most tokens of a sequence in this step */
+    int32_t rows;          /* rows of k and v */
+} swlm_kv8_append;
+int swlm_op_kv8_append_dev(swlm_ctx* ctx, const swlm_kv8_cache* cache, const swlm_kv8_append* step, void* cuda_stream);
+
+/* Queries of the same step, after its append: query i of sequence b attends the slots below lengths[b] + i + 1, cut to max_len and the
+ * capacity; one that attends nothing (lengths[b] < 0 parks a sequence) gets zeros. Row r of query head h lies at q + r * q_stride +
+ * h * head_dim; query heads h * heads / kv_heads ... share KV head h. Rows of `out` that no sequence has stay as they are, as do the rows of
+ * a sequence whose rows are not within 0..rows-1 or whose counts[b] > n or < 0 (nothing of such a sequence is worked on).
+ * accumulate: weight[b][h][slot] += the softmax weights that the step's queries of all heads of the group have for the slot.
+ * Scores, softmax and sums are fp32; probabilities meet the values as fp16. An infinity or NaN in a query makes that query's results (and,
+ * accumulated, the weights that it adds) NaN.
+ * scratch: swlm_op_kv8_attend_scratch_bytes() (0: none needed), 16-byte aligned, not shared by calls that may overlap. */
+typedef struct swlm_kv8_attend {
+    const void* q;
+    void* out;
+    int64_t q_stride, out_stride;
+    const int32_t* lengths;
+    const int32_t* counts;
+    const int32_t* starts;
+    void* scratch;
+    uint64_t scratch_bytes;
+    float scale;           /* of the scores, > 0 */
+    int32_t dtype;         /* of q and out */
+    int32_t heads;         /* query heads, a multiple of kv_heads */
+    int32_t n;             /* most queries of a sequence in this step */
+    int32_t rows;          /* rows of q and out */
+    int32_t max_len;       /* no sequence has more tokens than this, its new ones included; what lies behind is not attended */
+    int32_t accumulate;
+} swlm_kv8_attend;
+size_t swlm_op_kv8_attend_scratch_bytes(const swlm_kv8_cache* cache, const swlm_kv8_attend* step);   /* the pointers are not looked at; 0 for what the call refuses */
+int swlm_op_kv8_attend_dev(swlm_ctx* ctx, const swlm_kv8_cache* cache, const swlm_kv8_attend* step, void* cuda_stream);
+
+/* Of every (sequence, KV head) with more than `keep` tokens: the tokens of positions below `sink` and the last `recent` ones (positions from
+ * seen[b] - recent on; seen[b] counts all tokens so far here) are protected, then those of the largest weights stay (a NaN counts as the
+ * smallest, of equal ones the lowest slot stays). Tokens below slot `keep` that stay keep their slots; the i-th free slot
+ * below `keep` takes the i-th token that stays from behind. Blocks that take such tokens are scaled anew: s = max |c * scale| / 127 over their slots,
+ * codes round(c * scale / s); the other blocks stay as they are. What a sequence has afterwards is min(lengths[b], keep) tokens
+ * (swlm_op_kv8_lengths_dev with that limit).
+ * `to` may be the same cache (all pointers equal) or another one, no array of which overlaps one of `cache`, with the same batch,
+ * kv_heads, head_dim, block and code, and a capacity of at least `keep`; sequences with fewer tokens are copied there. Slots
+ * of `to` from min(lengths[b], keep) on stay as they are. sink + recent <= keep. Both caches need weight and slot_pos. */
+typedef struct swlm_kv8_evict {
+    const int32_t* lengths;
+    const int32_t* seen;
+    void* scratch;             /* swlm_op_kv8_evict_scratch_bytes(), 16-byte aligned */
+    uint64_t scratch_bytes;
+    int32_t keep, sink, recent;
+    int32_t max_len;           /* no sequence has more tokens than this; what lies behind is not looked at */
+} swlm_kv8_evict;
+size_t swlm_op_kv8_evict_scratch_bytes(const swlm_kv8_cache* cache, const swlm_kv8_evict* how);
+int swlm_op_kv8_evict_dev(swlm_ctx* ctx, const swlm_kv8_cache* cache, const swlm_kv8_cache* to, const swlm_kv8_evict* how, void* cuda_stream);
+
+/* out[b] = min(in[b] + counts[b], limit) (counts NULL: n each; out may be in; where refused[b] != 0, refused not NULL, out[b] = in[b]):
+ * what a step adds to lengths (limit: the capacity) and to seen (limit: INT32_MAX), what an eviction leaves (n = 0, limit: keep). */
+int swlm_op_kv8_lengths_dev(swlm_ctx* ctx, int batch, const int32_t* in, const int32_t* counts, int n, int limit, const int32_t* refused,
+                            int32_t* out, void* cuda_stream);
+
 #ifdef __cplusplus
 }
 #endif

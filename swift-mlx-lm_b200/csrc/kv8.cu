@@ -1,0 +1,552 @@
+// A cache of 8-bit codes with one scale per block of tokens and head: appending to it and evicting from it.
+//
+// append   s = max(s0, max |x| / top), c = round(x / s) with IEEE quotients, so that a code is the same whatever the launch. One CTA per
+//          (block of tokens, KV head, keys or values): the new values of the block stay in registers between the search for the largest and
+//          the rounding, each is read once.
+// evict    select: one CTA per (sequence, KV head) finds the `keep` largest keys by radix selection and pairs the free slots below `keep`
+//          with the tokens that stay from behind. move: one CTA per (block below `keep`, KV head, keys or values) gathers what the
+//          block takes, scales it anew and stores it. Only slots from `keep` on are sources of another block's slots and only slots below
+//          `keep` are written, so that the blocks need no order among them, also in place; the scales of the sources, which the last block
+//          may share with slots that are written, are taken along by the first kernel.
+#include <cuda_fp8.h>
+
+#include <algorithm>
+#include <climits>
+
+#include "kv8.h"
+#include "swlm_runtime.h"
+
+namespace swlm {
+namespace {
+
+constexpr float kTopInt8 = 127.f, kTopE4m3 = 448.f;
+
+template <int CODE> __device__ __forceinline__ constexpr float kv8_top() { return CODE == SWLM_KV8_INT8 ? kTopInt8 : kTopE4m3; }
+
+// the nearest code of y = x / s, as a byte (|y| <= top but for the last place; the clamp is for scales that are subnormal)
+template <int CODE> __device__ __forceinline__ unsigned kv8_code(float y) {
+    if (CODE == SWLM_KV8_INT8) return (unsigned)__float2int_rn(fminf(fmaxf(y, -kTopInt8), kTopInt8)) & 0xFFu;
+    return (unsigned)__nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+}
+template <int CODE> __device__ __forceinline__ float kv8_number(unsigned byte) {
+    if (CODE == SWLM_KV8_INT8) return (float)(int)(signed char)byte;
+    return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)));
+}
+
+// Largest of a CTA's unsigned numbers, to all of its threads.
+__device__ __forceinline__ unsigned block_max(unsigned v, unsigned* warps) {
+    v = __reduce_max_sync(0xffffffffu, v);
+    if (blockDim.x == 32) return v;
+    if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0;
+    for (int w = 0; w < (int)blockDim.x / 32; ++w) v = max(v, warps[w]);
+    return v;
+}
+
+// ---- append ----------------------------------------------------------------------------------------------------------------
+
+constexpr int kAppendThreads = 256, kAppendUnits = 8;   // a unit: eight values of a token, at most 128 * 128 / 8 of them in a block
+static_assert(kAppendThreads * kAppendUnits * 8 >= kKv8MaxBlock * 128, "a block fits its CTA");
+
+__device__ __forceinline__ float half_bits(unsigned bits, bool f16) {
+    return f16 ? __half2float(__ushort_as_half((unsigned short)bits)) : __uint_as_float(bits << 16);
+}
+
+template <int CODE>
+__global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const swlm_kv8_cache c, const swlm_kv8_append a) {
+    __shared__ unsigned warps[kAppendThreads / 32];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int b = blockIdx.z, h = blockIdx.y >> 1, which = blockIdx.y & 1, tid = threadIdx.x, T = c.block;
+    const Kv8Part part = kv8_part(b, a.lengths, a.counts, a.starts, a.n, a.rows);
+    const bool ok = part.fits && part.len >= 0 && (long long)part.len + part.count <= c.capacity;
+    if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0 && a.refused) a.refused[b] = ok ? 0 : 1;
+    if (!ok) return;
+    const int blk = part.len / T + (int)blockIdx.x, base = blk * T;
+    const int low = max(part.len, base), high = min(part.len + part.count, base + T);   // new slots of this block
+    if (low >= high) return;
+    const int old = low - base;   // tokens that it has
+    const bool f16 = a.dtype == SWLM_KV8_FP16;
+    const unsigned short* x = static_cast<const unsigned short*>(which ? a.v : a.k);
+    const int64_t stride = which ? a.v_stride : a.k_stride;
+    unsigned char* codes = static_cast<unsigned char*>(which ? c.v : c.k) + ((size_t)(b * (size_t)c.kv_heads + h) * c.capacity + base) * c.head_dim;
+    float* scale = (which ? c.v_scale : c.k_scale) + (size_t)(b * (size_t)c.kv_heads + h) * (c.capacity / T) + blk;
+    const float s0 = old ? *scale : 0.f;
+
+    const int per = c.head_dim >> 3, units = (high - low) * per;   // units of a token, new units
+    uint4 raw[kAppendUnits];
+    unsigned top = 0;   // largest |value| as its 15 bits: the order of the numbers, infinity and NaN above all
+#pragma unroll
+    for (int u = 0; u < kAppendUnits; ++u) {
+        const int i = tid + u * (int)blockDim.x;
+        raw[u] = make_uint4(0, 0, 0, 0);
+        if (i < units) {
+            const int slot = low + i / per, d = i % per * 8;
+            raw[u] = *reinterpret_cast<const uint4*>(x + (int64_t)(part.start + slot - part.len) * stride + (size_t)h * c.head_dim + d);
+        }
+        const unsigned m = __vmaxu2(__vmaxu2(raw[u].x & 0x7FFF7FFFu, raw[u].y & 0x7FFF7FFFu), __vmaxu2(raw[u].z & 0x7FFF7FFFu, raw[u].w & 0x7FFF7FFFu));
+        top = max(top, max(m & 0xFFFFu, m >> 16));
+    }
+    top = block_max(top, warps);   // (all have read the old scale when it returns, or are the only warp)
+    const bool finite = top < (f16 ? 0x7C00u : 0x7F80u) && s0 == s0;
+    const float s = finite ? fmaxf(s0, __fdiv_rn(half_bits(top, f16), kv8_top<CODE>())) : kKv8NaN;
+    if (blockDim.x == 32) __syncwarp();
+    if (tid == 0) *scale = s;
+    const bool grows = old && finite && s > s0;
+#pragma unroll
+    for (int u = 0; u < kAppendUnits; ++u) {
+        const int i = tid + u * (int)blockDim.x;
+        if (i < units) {
+            const unsigned w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+            unsigned out[2] = {0, 0};
+            if (finite && s > 0.f)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) out[e >> 2] |= kv8_code<CODE>(__fdiv_rn(half_bits((w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu, f16), s)) << (8 * (e & 3));
+            *reinterpret_cast<uint2*>(codes + (size_t)(low - base + i / per) * c.head_dim + i % per * 8) = make_uint2(out[0], out[1]);
+        }
+    }
+    if (grows)
+        for (int i = tid; i < old * per; i += blockDim.x) {
+            uint2* at = reinterpret_cast<uint2*>(codes + (size_t)i * 8);
+            const uint2 was = *at;
+            const unsigned w[2] = {was.x, was.y};
+            unsigned out[2] = {0, 0};
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                out[e >> 2] |= kv8_code<CODE>(__fdiv_rn(kv8_number<CODE>((w[e >> 2] >> (8 * (e & 3))) & 0xFFu) * s0, s)) << (8 * (e & 3));
+            *at = make_uint2(out[0], out[1]);
+        }
+    if (which == 0)
+        for (int slot = low + tid; slot < high; slot += blockDim.x) {
+            const size_t at = (size_t)(b * (size_t)c.kv_heads + h) * c.capacity + slot;
+            if (c.weight) c.weight[at] = 0.f;
+            if (c.slot_pos) c.slot_pos[at] = (int)((unsigned)a.seen[b] + (unsigned)(slot - part.len));
+        }
+}
+
+__global__ void kv8_lengths_kernel(int batch, const int32_t* in, const int32_t* counts, int n, int limit, const int32_t* refused, int32_t* out) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int b = blockIdx.x * blockDim.x + threadIdx.x;
+    if (b >= batch) return;
+    const long long sum = (long long)in[b] + (refused && refused[b] ? 0 : counts ? counts[b] : n);
+    out[b] = refused && refused[b] ? in[b] : (int)max(min(sum, (long long)limit), (long long)INT32_MIN);
+}
+
+// ---- evict -----------------------------------------------------------------------------------------------------------------
+
+constexpr int kSelectThreads = 1024, kSelectWarps = kSelectThreads / 32;
+constexpr int kDigitBits = 11, kDigits = 1 << kDigitBits;
+constexpr int kCachedKeys = 48 * 1024;   // keys that stay in shared memory between the passes (192 KB of 227)
+
+// Scratch of one (sequence, KV head): where slot j < keep comes from (j itself, or ~i: the i-th of the tokens that move), the slots of the
+// tokens that move and the scales of their keys and values.
+struct EvictPlan {
+    int* source; int* moved; float* k_scale; float* v_scale;
+    __host__ __device__ EvictPlan(void* scratch, size_t head, int keep) {
+        int* p = static_cast<int*>(scratch) + head * (size_t)keep * 4;
+        source = p; moved = p + keep; k_scale = reinterpret_cast<float*>(p + 2 * (size_t)keep); v_scale = k_scale + keep;
+    }
+};
+
+// Floats in the order of unsigned numbers, both zeros alike, NaN below all; protected tokens above all.
+__device__ __forceinline__ unsigned evict_key(float w, int pos, int sink, long long recent_from) {
+    if (pos < sink || pos >= recent_from) return 0xFFFFFFFFu;
+    if (w != w) return 0u;
+    const unsigned u = __float_as_uint(w + 0.f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+template <bool CACHED>
+__global__ void __launch_bounds__(kSelectThreads) kv8_select_kernel(const swlm_kv8_cache c, const swlm_kv8_evict a) {
+    extern __shared__ unsigned keys[];
+    __shared__ unsigned hist[kDigits];
+    __shared__ int seg[3][kSelectWarps];
+    __shared__ unsigned found_digit, found_above;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int b = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int len = min(min(a.lengths[b], a.max_len), c.capacity), keep = a.keep;
+    if (len <= keep) return;   // nothing leaves: the second kernel does not look at the plan
+    const size_t head = (size_t)b * c.kv_heads + h;
+    const float* weight = c.weight + head * c.capacity;
+    const int32_t* pos = c.slot_pos + head * c.capacity;
+    const long long recent_from = (long long)a.seen[b] - a.recent;
+    auto key_of = [&](int i) { return evict_key(weight[i], pos[i], a.sink, recent_from); };
+    if (CACHED)
+        for (int i = tid; i < len; i += kSelectThreads) keys[i] = key_of(i);
+    auto key = [&](int i) { return CACHED ? keys[i] : key_of(i); };
+
+    // radix selection of the keep-th largest key, from the top digit down
+    unsigned prefix = 0, mask = 0;
+    int want = keep;   // how many keys are still to be found among those that share the prefix
+    for (int shift = 32 - kDigitBits; ; shift = max(shift - kDigitBits, 0)) {
+        for (int i = tid; i < kDigits; i += kSelectThreads) hist[i] = 0;
+        __syncthreads();
+        for (int i = tid; i < len; i += kSelectThreads) {
+            const unsigned k = key(i);
+            if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (kDigits - 1)], 1u);
+        }
+        __syncthreads();
+        if (warp == 0) {   // lane l has the 64 digits from the (31 - l)-th group on: counts from the top down
+            constexpr int PER = kDigits / 32;
+            const int first = (31 - lane) * PER;
+            unsigned sum = 0;
+            for (int i = 0; i < PER; ++i) sum += hist[first + i];
+            unsigned above = sum;
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned v = __shfl_up_sync(0xffffffffu, above, o);
+                if (lane >= o) above += v;
+            }
+            above -= sum;   // keys of higher groups
+            if (above < (unsigned)want && above + sum >= (unsigned)want) {
+                int d = first + PER - 1;
+                while (above + hist[d] < (unsigned)want) above += hist[d--];
+                found_digit = (unsigned)d;
+                found_above = above;
+            }
+        }
+        __syncthreads();
+        const unsigned digits = (unsigned)(kDigits - 1) << shift;
+        prefix = (prefix & ~digits) | found_digit << shift;   // (the last digit overlaps the one before it, with the same bits there)
+        mask |= digits;
+        want -= (int)found_above;
+        __syncthreads();
+        if (shift == 0) break;
+    }
+    const unsigned limit = prefix;   // keys above it stay, and the first `want` of those equal to it
+
+    // a run of slots per warp: ties first, then free slots below `keep` and staying ones from it on, each numbered in slot order
+    const int run = (len + kSelectThreads - 1) / kSelectThreads * 32, from = min(warp * run, len), to = min(from + run, len);
+    const unsigned below = (1u << lane) - 1u;
+    int ties = 0;
+    for (int i = from; i < to; i += 32) ties += __popc(__ballot_sync(0xffffffffu, i + lane < to && key(min(i + lane, len - 1)) == limit));
+    if (lane == 0) seg[0][warp] = ties;
+    __syncthreads();
+    int tie0 = 0;
+    for (int w = 0; w < warp; ++w) tie0 += seg[0][w];
+    auto walk = [&](auto&& each) {   // each(slot, within, stays)
+        int t = tie0;
+        for (int i = from; i < to; i += 32) {
+            const int slot = i + lane;
+            const bool in = slot < to;
+            const unsigned k = key(min(slot, len - 1));
+            const unsigned tied = __ballot_sync(0xffffffffu, in && k == limit);
+            const bool stays = in && (k > limit || (k == limit && t + __popc(tied & below) < want));
+            t += __popc(tied);
+            each(slot, in, stays);
+        }
+    };
+    int free_slots = 0, moving = 0;
+    walk([&](int slot, bool in, bool stays) {
+        free_slots += __popc(__ballot_sync(0xffffffffu, in && slot < keep && !stays));
+        moving += __popc(__ballot_sync(0xffffffffu, stays && slot >= keep));
+    });
+    if (lane == 0) { seg[1][warp] = free_slots; seg[2][warp] = moving; }
+    __syncthreads();
+    int free0 = 0, move0 = 0;
+    for (int w = 0; w < warp; ++w) { free0 += seg[1][w]; move0 += seg[2][w]; }
+    const EvictPlan plan(a.scratch, head, keep);
+    const float* ks = c.k_scale + head * (c.capacity / c.block);
+    const float* vs = c.v_scale + head * (c.capacity / c.block);
+    walk([&](int slot, bool in, bool stays) {
+        const unsigned f = __ballot_sync(0xffffffffu, in && slot < keep && !stays), m = __ballot_sync(0xffffffffu, stays && slot >= keep);
+        if (in && slot < keep) plan.source[slot] = stays ? slot : ~(free0 + __popc(f & below));
+        if (stays && slot >= keep) {
+            const int i = move0 + __popc(m & below);
+            plan.moved[i] = slot;
+            plan.k_scale[i] = ks[slot / c.block];
+            plan.v_scale[i] = vs[slot / c.block];
+        }
+        free0 += __popc(f);
+        move0 += __popc(m);
+    });
+}
+
+constexpr int kMoveThreads = 256, kMoveUnits = 4;   // a unit: 16 codes
+static_assert(kMoveThreads * kMoveUnits * 16 >= kKv8MaxBlock * 128, "a block fits its CTA");
+
+template <int CODE>
+__global__ void __launch_bounds__(kMoveThreads) kv8_move_kernel(const swlm_kv8_cache c, const swlm_kv8_cache to, const swlm_kv8_evict a, const int in_place) {
+    __shared__ int source[kKv8MaxBlock];
+    __shared__ float scales[kKv8MaxBlock];
+    __shared__ unsigned warps[kMoveThreads / 32];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int b = blockIdx.z, h = blockIdx.y >> 1, which = blockIdx.y & 1, tid = threadIdx.x, T = c.block, keep = a.keep;
+    const int len = min(min(a.lengths[b], a.max_len), c.capacity);
+    const int base = (int)blockIdx.x * T, n = min(min(len, keep) - base, T);   // slots of this block
+    if (n <= 0) return;
+    const size_t head = (size_t)b * c.kv_heads + h;
+    const EvictPlan plan(a.scratch, head, keep);
+    const float own = (which ? c.v_scale : c.k_scale)[head * (c.capacity / T) + blockIdx.x];
+    bool takes = false;
+    for (int i = tid; i < n; i += blockDim.x) {
+        int src = base + i;
+        float s = own;
+        if (len > keep) {
+            src = plan.source[base + i];
+            if (src < 0) {
+                const int m = ~src;
+                s = which ? plan.v_scale[m] : plan.k_scale[m];
+                src = plan.moved[m];
+                takes = true;
+            }
+        }
+        source[i] = src;
+        scales[i] = s;
+    }
+    const bool changed = __syncthreads_or(takes);
+    if (!changed && in_place) return;
+    const unsigned char* from = static_cast<const unsigned char*>(which ? c.v : c.k) + head * c.capacity * c.head_dim;
+    unsigned char* dst = static_cast<unsigned char*>(which ? to.v : to.k) + (head * to.capacity + base) * c.head_dim;
+    const int per = c.head_dim >> 4, units = n * per;
+    uint4 raw[kMoveUnits];
+    unsigned top = 0;   // largest |value|, as the bits of a float that is not negative
+#pragma unroll
+    for (int u = 0; u < kMoveUnits; ++u) {
+        const int i = tid + u * (int)blockDim.x;
+        if (i >= units) continue;
+        raw[u] = *reinterpret_cast<const uint4*>(from + (size_t)source[i / per] * c.head_dim + i % per * 16);
+        if (changed) {
+            const unsigned w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+            unsigned m = 0;   // of each byte's |code|: an integer, or the seven bits of an e4m3 number
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m = __vmaxu4(m, CODE == SWLM_KV8_INT8 ? __vabsss4(w[e]) : w[e] & 0x7F7F7F7Fu);
+            m = __vmaxu4(m, m >> 16);
+            m = max(m & 0xFFu, (m >> 8) & 0xFFu);
+            top = max(top, __float_as_uint(fabsf(kv8_number<CODE>(m) * scales[i / per])));
+        }
+    }
+    if (!changed) {
+#pragma unroll
+        for (int u = 0; u < kMoveUnits; ++u) {
+            const int i = tid + u * (int)blockDim.x;
+            if (i < units) *reinterpret_cast<uint4*>(dst + (size_t)i * 16) = raw[u];
+        }
+        if (tid == 0) (which ? to.v_scale : to.k_scale)[head * (to.capacity / T) + blockIdx.x] = own;
+    } else {
+        top = block_max(top, warps);
+        const bool finite = top < 0x7F800000u;
+        const float s = finite ? __fdiv_rn(__uint_as_float(top), kv8_top<CODE>()) : kKv8NaN;
+        if (tid == 0) (which ? to.v_scale : to.k_scale)[head * (to.capacity / T) + blockIdx.x] = s;
+#pragma unroll
+        for (int u = 0; u < kMoveUnits; ++u) {
+            const int i = tid + u * (int)blockDim.x;
+            if (i >= units) continue;
+            const unsigned w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+            unsigned out[4] = {0, 0, 0, 0};
+            const float mine = scales[i / per];
+            if (finite && s > 0.f)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    out[e >> 2] |= kv8_code<CODE>(__fdiv_rn(kv8_number<CODE>((w[e >> 2] >> (8 * (e & 3))) & 0xFFu) * mine, s)) << (8 * (e & 3));
+            *reinterpret_cast<uint4*>(dst + (size_t)i * 16) = make_uint4(out[0], out[1], out[2], out[3]);
+        }
+    }
+    if (which == 0)
+        for (int i = tid; i < n; i += blockDim.x) {
+            const size_t at = head * c.capacity + source[i], put = head * to.capacity + base + i;
+            const float w = c.weight[at];
+            const int32_t p = c.slot_pos[at];
+            to.weight[put] = w;
+            to.slot_pos[put] = p;
+        }
+}
+
+int after_launch(cudaError_t e, const char* what) { return e == cudaSuccess ? SWLM_OK : cuda_fail(e, what); }
+
+}  // namespace
+
+int launch_kv8_append(const swlm_kv8_cache& c, const swlm_kv8_append& a, cudaStream_t s) {
+    // blocks that a sequence's tokens may touch: the first one may have room for a single token
+    const unsigned blocks = (unsigned)((a.n + c.block - 2) / c.block + 1);
+    // (a whole block in at most 8 units per thread; a single token's few values need no more than a warp, its block's older codes do)
+    const int threads = std::min(kAppendThreads, std::max(32, c.block * c.head_dim / (8 * kAppendUnits)));
+    const dim3 grid(blocks, 2u * (unsigned)c.kv_heads, (unsigned)c.batch);
+    return after_launch(c.code == SWLM_KV8_INT8 ? launch_k(kv8_append_kernel<SWLM_KV8_INT8>, grid, dim3(threads), 0, s, c, a)
+                                                : launch_k(kv8_append_kernel<SWLM_KV8_E4M3>, grid, dim3(threads), 0, s, c, a), "kv8 append launch");
+}
+
+int launch_kv8_lengths(int batch, const int32_t* in, const int32_t* counts, int n, int limit, const int32_t* refused, int32_t* out, cudaStream_t s) {
+    return after_launch(launch_k(kv8_lengths_kernel, dim3((unsigned)(batch + 127) / 128), dim3(128), 0, s, batch, in, counts, n, limit, refused, out), "kv8 lengths launch");
+}
+
+int kv8_init() {
+    SWLM_CUDA(cudaFuncSetAttribute(kv8_select_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kCachedKeys * 4));
+    return kv8_attend_init();
+}
+
+size_t kv8_evict_scratch(const swlm_kv8_cache& c, const swlm_kv8_evict& a) { return (size_t)c.batch * c.kv_heads * a.keep * 16; }
+
+int launch_kv8_evict(const swlm_kv8_cache& c, const swlm_kv8_cache& to, const swlm_kv8_evict& a, cudaStream_t s) {
+    const int span = std::min(a.max_len, c.capacity);
+    cudaError_t e = cudaSuccess;
+    if (span > a.keep) {
+        const dim3 grid((unsigned)c.kv_heads, (unsigned)c.batch);
+        if (span <= kCachedKeys) {
+            e = launch_k(kv8_select_kernel<true>, grid, dim3(kSelectThreads), (size_t)span * 4, s, c, a);
+        } else {
+            e = launch_k(kv8_select_kernel<false>, grid, dim3(kSelectThreads), 0, s, c, a);
+        }
+        if (e != cudaSuccess) return cuda_fail(e, "kv8 selection launch");
+    } else if (c.k == to.k) {
+        return SWLM_OK;   // in place, and no sequence can have more than `keep` tokens
+    }
+    const int threads = std::min(kMoveThreads, std::max(32, c.block * c.head_dim / (16 * kMoveUnits)));
+    const dim3 grid((unsigned)((std::min(a.keep, span) + c.block - 1) / c.block), 2u * (unsigned)c.kv_heads, (unsigned)c.batch);
+    const int in_place = c.k == to.k;
+    return after_launch(c.code == SWLM_KV8_INT8 ? launch_k(kv8_move_kernel<SWLM_KV8_INT8>, grid, dim3(threads), 0, s, c, to, a, in_place)
+                                                : launch_k(kv8_move_kernel<SWLM_KV8_E4M3>, grid, dim3(threads), 0, s, c, to, a, in_place), "kv8 move launch");
+}
+
+}  // namespace swlm
+
+// ---- entry points: arguments are checked before anything is launched; what only the device knows is checked by the kernels -----------------
+
+using namespace swlm;
+
+namespace {
+
+int refuse(const char* what) {
+    set_error("kv8: %s", what);
+    return SWLM_ERR_INVALID;
+}
+
+bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+int cache_shape_ok(const swlm_kv8_cache& c) {
+    if (c.batch < 1 || c.batch > kKv8MaxBatch || c.kv_heads < 1 || c.kv_heads > kKv8MaxKvHeads) return refuse("batch or KV heads out of range");
+    if (c.head_dim != 64 && c.head_dim != 128) { set_error("kv8: heads of %d (64 and 128 are supported)", c.head_dim); return SWLM_ERR_UNSUPPORTED; }
+    if (c.block < kKv8MinBlock || c.block > kKv8MaxBlock || (c.block & (c.block - 1))) return refuse("a block has 16, 32, 64 or 128 tokens");
+    if (c.capacity < c.block || c.capacity % c.block || c.capacity > kKv8MaxLen) return refuse("the capacity is a multiple of the block, at most 2^30");
+    if (c.code != SWLM_KV8_INT8 && c.code != SWLM_KV8_E4M3) return refuse("unknown code");
+    return SWLM_OK;
+}
+int cache_ok(const swlm_kv8_cache& c) {
+    const int rc = cache_shape_ok(c);
+    if (rc) return rc;
+    if (!c.k || !c.v || !c.k_scale || !c.v_scale) return refuse("null cache array");
+    if (!aligned(c.k, 16) || !aligned(c.v, 16)) return refuse("codes must be 16-byte aligned");
+    if (!aligned(c.k_scale, 4) || !aligned(c.v_scale, 4) || !aligned(c.weight, 4) || !aligned(c.slot_pos, 4)) return refuse("scales, weights and positions must be 4-byte aligned");
+    return SWLM_OK;
+}
+int counters_ok(const int32_t* lengths, const int32_t* counts, const int32_t* starts, const int32_t* seen) {
+    if (!lengths) return refuse("null lengths");
+    if (!aligned(lengths, 4) || !aligned(counts, 4) || !aligned(starts, 4) || !aligned(seen, 4)) return refuse("counters must be 4-byte aligned");
+    return SWLM_OK;
+}
+int step_ok(int dtype, int n, int rows) {
+    if (dtype != SWLM_KV8_BF16 && dtype != SWLM_KV8_FP16) return refuse("unknown dtype");
+    if (n < 1 || n > kKv8MaxLen / 2 || rows < 0) return refuse("tokens or rows out of range");
+    return SWLM_OK;
+}
+bool rows_ok(const void* p, int64_t stride, int64_t width) { return aligned(p, 16) && stride >= width && stride % 8 == 0 && stride <= (int64_t)1 << 40; }
+
+int attend_shape_ok(const swlm_kv8_cache& c, const swlm_kv8_attend& a) {
+    int rc = cache_shape_ok(c);
+    if (rc || (rc = step_ok(a.dtype, a.n, a.rows))) return rc;
+    if (a.heads < 1 || a.heads % c.kv_heads) { set_error("kv8: %d query heads do not divide by %d KV heads", a.heads, c.kv_heads); return SWLM_ERR_INVALID; }
+    if ((int64_t)a.n * (a.heads / c.kv_heads) > kKv8MaxLen) return refuse("too many query rows");
+    if (a.max_len < 1 || a.max_len > kKv8MaxLen) return refuse("max_len out of range");
+    return SWLM_OK;
+}
+
+struct Range { uintptr_t from, to; };
+void ranges_of(const swlm_kv8_cache& c, Range* r) {
+    const size_t heads = (size_t)c.batch * c.kv_heads, codes = heads * c.capacity * c.head_dim, scales = heads * (c.capacity / c.block) * 4, slots = heads * c.capacity * 4;
+    const void* p[6] = {c.k, c.v, c.k_scale, c.v_scale, c.weight, c.slot_pos};
+    const size_t n[6] = {codes, codes, scales, scales, slots, slots};
+    for (int i = 0; i < 6; ++i) r[i] = {reinterpret_cast<uintptr_t>(p[i]), reinterpret_cast<uintptr_t>(p[i]) + n[i]};
+}
+
+int evict_shape_ok(const swlm_kv8_cache& c, const swlm_kv8_evict& a) {
+    const int rc = cache_shape_ok(c);
+    if (rc) return rc;
+    if (a.keep < 1 || a.keep > kKv8MaxLen || a.sink < 0 || a.recent < 0 || (int64_t)a.sink + a.recent > a.keep) return refuse("keep is positive and at least sink + recent, neither of them negative");
+    if (a.max_len < 1 || a.max_len > kKv8MaxLen) return refuse("max_len out of range");
+    return SWLM_OK;
+}
+
+cudaStream_t stream_of(swlm_ctx* ctx, void* s) { return s ? static_cast<cudaStream_t>(s) : ctx->stream; }
+
+}  // namespace
+
+extern "C" {
+
+int swlm_op_kv8_append_dev(swlm_ctx* ctx, const swlm_kv8_cache* cache, const swlm_kv8_append* step, void* cuda_stream) {
+    if (!ctx || !cache || !step || !step->k || !step->v) return refuse("null argument");
+    const swlm_kv8_cache& c = *cache;
+    const swlm_kv8_append& a = *step;
+    int rc = cache_ok(c);
+    if (rc || (rc = step_ok(a.dtype, a.n, a.rows)) || (rc = counters_ok(a.lengths, a.counts, a.starts, a.seen))) return rc;
+    if (!aligned(a.refused, 4)) return refuse("counters must be 4-byte aligned");
+    if (c.slot_pos && !a.seen) return refuse("a cache with slot_pos needs seen");
+    const int64_t width = (int64_t)c.kv_heads * c.head_dim;
+    if (!rows_ok(a.k, a.k_stride, width) || !rows_ok(a.v, a.v_stride, width)) return refuse("k and v must be 16-byte aligned, their strides multiples of 8 and at least kv_heads * head_dim");
+    SWLM_CUDA(cudaSetDevice(ctx->device));
+    return launch_kv8_append(c, a, stream_of(ctx, cuda_stream));
+}
+
+size_t swlm_op_kv8_attend_scratch_bytes(const swlm_kv8_cache* cache, const swlm_kv8_attend* step) {
+    if (!cache || !step || attend_shape_ok(*cache, *step)) return 0;
+    return kv8_attend_scratch(*cache, *step);
+}
+
+int swlm_op_kv8_attend_dev(swlm_ctx* ctx, const swlm_kv8_cache* cache, const swlm_kv8_attend* step, void* cuda_stream) {
+    if (!ctx || !cache || !step || !step->q || !step->out) return refuse("null argument");
+    const swlm_kv8_cache& c = *cache;
+    const swlm_kv8_attend& a = *step;
+    int rc = cache_ok(c);
+    if (rc || (rc = attend_shape_ok(c, a)) || (rc = counters_ok(a.lengths, a.counts, a.starts, nullptr))) return rc;
+    const int64_t width = (int64_t)a.heads * c.head_dim;
+    if (!rows_ok(a.q, a.q_stride, width) || !rows_ok(a.out, a.out_stride, width)) return refuse("q and out must be 16-byte aligned, their strides multiples of 8 and at least heads * head_dim");
+    if (!(a.scale > 0.f) || a.scale > 1e30f) return refuse("the scale must be positive and finite");
+    if (a.accumulate && !c.weight) return refuse("accumulate needs the cache's weight array");
+    const size_t need = kv8_attend_scratch(c, a);
+    if (need && (!a.scratch || !aligned(a.scratch, 16) || a.scratch_bytes < need)) { set_error("kv8: %zu bytes of 16-byte aligned scratch are needed", need); return SWLM_ERR_INVALID; }
+    SWLM_CUDA(cudaSetDevice(ctx->device));
+    return launch_kv8_attend(c, a, stream_of(ctx, cuda_stream));
+}
+
+size_t swlm_op_kv8_evict_scratch_bytes(const swlm_kv8_cache* cache, const swlm_kv8_evict* how) {
+    if (!cache || !how || evict_shape_ok(*cache, *how)) return 0;
+    return kv8_evict_scratch(*cache, *how);
+}
+
+int swlm_op_kv8_evict_dev(swlm_ctx* ctx, const swlm_kv8_cache* cache, const swlm_kv8_cache* to, const swlm_kv8_evict* how, void* cuda_stream) {
+    if (!ctx || !cache || !to || !how) return refuse("null argument");
+    const swlm_kv8_cache &c = *cache, &d = *to;
+    const swlm_kv8_evict& a = *how;
+    int rc = cache_ok(c);
+    if (rc || (rc = cache_ok(d)) || (rc = evict_shape_ok(c, a)) || (rc = counters_ok(a.lengths, nullptr, nullptr, a.seen))) return rc;
+    if (!a.seen) return refuse("null seen");
+    if (!c.weight || !c.slot_pos || !d.weight || !d.slot_pos) return refuse("eviction needs weight and slot_pos of both caches");
+    if (c.batch != d.batch || c.kv_heads != d.kv_heads || c.head_dim != d.head_dim || c.block != d.block || c.code != d.code) return refuse("the two caches differ in shape or code");
+    const bool same = c.k == d.k && c.v == d.v && c.k_scale == d.k_scale && c.v_scale == d.v_scale && c.weight == d.weight && c.slot_pos == d.slot_pos;
+    if (same ? c.capacity != d.capacity : d.capacity < std::min(a.keep, std::min(a.max_len, c.capacity))) return refuse("the second cache has no room for the tokens that stay");
+    if (!same) {
+        Range x[6], y[6];
+        ranges_of(c, x);
+        ranges_of(d, y);
+        for (const Range& i : x)
+            for (const Range& j : y)
+                if (i.from < j.to && j.from < i.to) return refuse("the two caches share some memory but are not the same");
+    }
+    const size_t need = kv8_evict_scratch(c, a);
+    if (!a.scratch || !aligned(a.scratch, 16) || a.scratch_bytes < need) { set_error("kv8: %zu bytes of 16-byte aligned scratch are needed", need); return SWLM_ERR_INVALID; }
+    SWLM_CUDA(cudaSetDevice(ctx->device));
+    return launch_kv8_evict(c, d, a, stream_of(ctx, cuda_stream));
+}
+
+int swlm_op_kv8_lengths_dev(swlm_ctx* ctx, int batch, const int32_t* in, const int32_t* counts, int n, int limit, const int32_t* refused,
+                            int32_t* out, void* cuda_stream) {
+    if (!ctx || !in || !out) return refuse("null argument");
+    if (batch < 1 || batch > kKv8MaxBatch) return refuse("batch out of range");
+    if (!aligned(in, 4) || !aligned(counts, 4) || !aligned(refused, 4) || !aligned(out, 4)) return refuse("counters must be 4-byte aligned");
+    SWLM_CUDA(cudaSetDevice(ctx->device));
+    return launch_kv8_lengths(batch, in, counts, n, limit, refused, out, stream_of(ctx, cuda_stream));
+}
+
+}  // extern "C"

@@ -19,6 +19,7 @@
 
 #include <sys/mman.h>
 
+#include "kv8.h"
 #include "swlm_runtime.h"
 
 namespace swlm {
@@ -1395,6 +1396,7 @@ int swlm_ctx_create(int device_id, int tp_rank, int tp_size, swlm_ctx** out) {
     if (!rc) rc = routed_init();
     if (!rc) rc = grouped_init();
     if (!rc) rc = retention_init();
+    if (!rc) rc = kv8_init();
     if (rc) { cudaStreamDestroy(ctx->stream); delete ctx; return rc; }
     *out = ctx;
     return SWLM_OK;

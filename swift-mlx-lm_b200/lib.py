@@ -119,6 +119,40 @@ class BuffersDesc(C.Structure):
     ]
 
 
+# What the operators over an 8-bit cache take (include/swlm.h); device pointers as integers, 0 for none.
+KV8_INT8, KV8_E4M3 = 0, 1   # codes
+KV8_BF16, KV8_FP16 = 0, 1   # keys, values, queries and results
+
+
+class Kv8Cache(C.Structure):
+    """Mirror of `swlm_kv8_cache`."""
+
+    _fields_ = [(f, C.c_void_p) for f in ("k", "v", "k_scale", "v_scale", "weight", "slot_pos")] + [
+        (f, C.c_int32) for f in ("batch", "kv_heads", "head_dim", "capacity", "block", "code")]
+
+
+class Kv8Append(C.Structure):
+    """Mirror of `swlm_kv8_append`."""
+
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_stride", C.c_int64), ("v_stride", C.c_int64)] + [
+        (f, C.c_void_p) for f in ("lengths", "counts", "starts", "seen", "refused")] + [(f, C.c_int32) for f in ("dtype", "n", "rows")]
+
+
+class Kv8Attend(C.Structure):
+    """Mirror of `swlm_kv8_attend`."""
+
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_int64), ("out_stride", C.c_int64)] + [
+        (f, C.c_void_p) for f in ("lengths", "counts", "starts", "scratch")] + [("scratch_bytes", C.c_uint64), ("scale", C.c_float)] + [
+        (f, C.c_int32) for f in ("dtype", "heads", "n", "rows", "max_len", "accumulate")]
+
+
+class Kv8Evict(C.Structure):
+    """Mirror of `swlm_kv8_evict`."""
+
+    _fields_ = [(f, C.c_void_p) for f in ("lengths", "seen", "scratch")] + [("scratch_bytes", C.c_uint64)] + [
+        (f, C.c_int32) for f in ("keep", "sink", "recent", "max_len")]
+
+
 # name -> (restype, argtypes); every symbol include/swlm.h declares
 _P = C.c_void_p
 _I = C.c_int
@@ -197,6 +231,12 @@ SIGNATURES = {
     "swlm_op_flash_decode_dev": (_I, [_P, _I, _I, _I, _I, _I, _I, C.c_float, _P, _P, _P, _P, _P, _P]),
     "swlm_op_flash_decode_noalloc_capacity": (C.c_size_t, []),
     "swlm_op_flash_decode_noalloc_dev": (_I, [_P, _I, _I, _I, _I, _I, _I, C.c_float, _P, _P, _P, _P, _P]),
+    "swlm_op_kv8_append_dev": (_I, [_P, C.POINTER(Kv8Cache), C.POINTER(Kv8Append), _P]),
+    "swlm_op_kv8_attend_scratch_bytes": (C.c_size_t, [C.POINTER(Kv8Cache), C.POINTER(Kv8Attend)]),
+    "swlm_op_kv8_attend_dev": (_I, [_P, C.POINTER(Kv8Cache), C.POINTER(Kv8Attend), _P]),
+    "swlm_op_kv8_evict_scratch_bytes": (C.c_size_t, [C.POINTER(Kv8Cache), C.POINTER(Kv8Evict)]),
+    "swlm_op_kv8_evict_dev": (_I, [_P, C.POINTER(Kv8Cache), C.POINTER(Kv8Cache), C.POINTER(Kv8Evict), _P]),
+    "swlm_op_kv8_lengths_dev": (_I, [_P, _I, _P, _P, _I, _I, _P, _P, _P]),
 }
 
 
