@@ -2,7 +2,7 @@
 //
 //   s_ij = scale * ks[j / T] * (q_i . ck_j),  p = softmax over the slots that query i attends,  out_i = sum_j p_ij vs[j / T] cv_j
 //
-// Codes are exact as fp16 numbers (e4m3 ones times 2^-8), and so are bf16 and fp16 queries after a shift of the row's exponent that brings its
+// Codes are exact as fp16 numbers, and so are bf16 and fp16 queries after a shift of the row's exponent that brings its
 // largest value to 2^12, but for values 2^-26 and less of the largest. So q . ck is an fp16 product with fp32 sums on the tensor cores, and
 // a step of 16 tokens, which never crosses a block, takes its scale as one number behind it.
 //
@@ -19,9 +19,11 @@
 namespace swlm {
 namespace {
 
-constexpr int kWarps = 8, kThreads = kWarps * 32;
-constexpr int kStep = 16;                       // tokens of a warp's step
-constexpr int kSpanStep = kWarps * kStep;       // runs of slots are multiples of it
+constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr int kSub = 2, kStep = 16 * kSub;        // tokens of a warp's step: two tiles of 16
+constexpr int kUnit = kWarps * kStep;           // slots of a step of all warps: work is dealt in these
+constexpr int kStreamBatch = 512;               // sequences whose units a CTA adds up
+constexpr int kSms = 148;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.f;                   // log2 of what a probability may exceed 1 by
 constexpr float kValueUnit = 128.f;             // 2^7: probabilities up to 2^8 stay within fp16
@@ -29,14 +31,17 @@ constexpr int kSaveRows = 64;                   // up to so many rows of a KV he
 
 struct RowsPlan {
     int tiles;      // 8-row tiles per CTA
-    int row_tiles;  // CTAs along the rows
+    int row_tiles;  // of a KV head at most, of 8 * tiles rows each
     int rows;       // n * group
-    int chunk, splits;
+    int stream, ctas;   // CTAs over equal shares of all units (stream), or one per (sequence, KV head, tile)
     int span;       // slots that can be attended, rounded up to kStep
     int pitch;      // rows of a slot's kept scores (0: not kept)
-    float* part_o;  // [batch][kv_heads][rows][splits][head_dim], not normalised
-    float* part_ml; // [batch][kv_heads][rows][splits][2]: reference maximum (log2), sum
+    int join_groups;   // groups of lanes that share a row's parts
+    int ml_always;  // maximum and sum are wanted of rows in one part too
+    float* part_o;  // [places][8 * tiles][head_dim], not normalised; places: (sequence, KV head, tile) + CTA
+    float* part_ml; // [places][8 * tiles][2]: reference maximum (log2), sum
     float* scores;  // [batch][kv_heads][span][pitch], log2
+    int* table;     // [batch + 1]: units before each sequence, and of all
 };
 
 __device__ __forceinline__ unsigned smem_addr(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
@@ -54,19 +59,19 @@ __device__ __forceinline__ uint2 lds64(unsigned a) {
     asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
     return v;
 }
-__device__ __forceinline__ float lds_f32(unsigned a) {
-    float v;
-    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+__device__ __forceinline__ float2 lds_f32x2(unsigned a) {
+    float2 v;
+    asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
     return v;
 }
 __device__ __forceinline__ float exp2_of(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ void mma(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ unsigned transpose8x8(unsigned v) {
     unsigned r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
 __device__ __forceinline__ unsigned pack_half(float a, float b) {
@@ -74,8 +79,7 @@ __device__ __forceinline__ unsigned pack_half(float a, float b) {
     return *reinterpret_cast<const unsigned*>(&v);
 }
 
-// Codes to fp16. int8: with the sign bit turned a byte u = c + 128 is the low byte of 1024 + u. e4m3: sign, exponent and mantissa in their places
-// are the number times 2^-8, subnormal ones too (and 0x7F, which no block holds, a finite number: a stale slot's codes meet the weight 0).
+// Codes to fp16, exactly. int8: with the sign bit turned a byte u = c + 128 is the low byte of 1024 + u.
 template <int CODE> __device__ __forceinline__ unsigned prepared(unsigned word) { return CODE == SWLM_KV8_INT8 ? word ^ 0x80808080u : word; }
 // bytes 2 * HIGH and 2 * HIGH + 1 of a prepared word
 template <int CODE, int HIGH> __device__ __forceinline__ unsigned pair_of(unsigned word) {
@@ -84,10 +88,24 @@ template <int CODE, int HIGH> __device__ __forceinline__ unsigned pair_of(unsign
         const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&biased), __half2half2(__ushort_as_half(0x6480)));   // 1024 + 128
         return *reinterpret_cast<const unsigned*>(&v);
     }
-    const unsigned high = __byte_perm(word, 0u, HIGH ? 0x3424 : 0x1404);   // (0, byte, 0, byte)
-    return (high & 0x80008000u) | ((high >> 1) & 0x3F803F80u);
+    unsigned v;
+    if (HIGH) asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(v) : "r"(word));
+    else asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(v) : "r"(word));
+    return v;
 }
-template <int CODE> __device__ __forceinline__ constexpr float code_unit() { return CODE == SWLM_KV8_INT8 ? 1.f : 256.f; }
+
+// Four results of a row with sum l.
+__device__ __forceinline__ void store_out(unsigned short* dst, const float4& o, float l, bool f16) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    unsigned v[2];
+    if (f16) {
+        v[0] = pack_half(o.x * inv, o.y * inv); v[1] = pack_half(o.z * inv, o.w * inv);
+    } else {
+        const __nv_bfloat162 x = __floats2bfloat162_rn(o.x * inv, o.y * inv), y = __floats2bfloat162_rn(o.z * inv, o.w * inv);
+        v[0] = *reinterpret_cast<const unsigned*>(&x); v[1] = *reinterpret_cast<const unsigned*>(&y);
+    }
+    *reinterpret_cast<uint2*>(dst) = make_uint2(v[0], v[1]);
+}
 
 // Eight 16-bit values as floats.
 __device__ __forceinline__ void widen(const uint4& r, bool f16, float (&x)[8]) {
@@ -113,9 +131,10 @@ __device__ __forceinline__ void row_shift(float top, float& up, float& down) {
 // The slots that query i of a sequence attends are those below this.
 __device__ __forceinline__ int visible(const Kv8Part& part, int i, int span) { return (int)min((long long)part.len + i + 1, (long long)span); }
 
-template <int HD> __host__ __device__ constexpr int stages() { return HD == 128 ? 3 : 5; }
-template <int HD> __host__ __device__ constexpr int stage_bytes() { return 2 * kStep * HD + 16; }   // keys, values, their scales
-template <int HD> constexpr size_t rows_smem() { return (size_t)kWarps * stages<HD>() * stage_bytes<HD>(); }
+template <int HD> __host__ __device__ constexpr int stages() { return HD == 128 ? 2 : 3; }
+template <int HD> __host__ __device__ constexpr int rows_ctas() { return HD == 128 ? 3 : 4; }   // CTAs of one tile per SM
+template <int HD> __host__ __device__ constexpr int stage_bytes() { return 2 * kStep * HD + 16; }   // keys, values, (key, value) scale of either tile
+template <int HD> __host__ __device__ constexpr size_t rows_smem() { return (size_t)kWarps * stages<HD>() * stage_bytes<HD>(); }
 
 // Byte of 16-byte piece c of token r in a step's keys or values. Pieces lie so that the eight lanes of a phase meet different banks: keys are read
 // with the token in the lane's upper bits (two tokens x four pieces), values with it in the lower ones (tokens 0, 2, 4, 6 x two pieces).
@@ -155,336 +174,516 @@ __device__ __forceinline__ void load_query(const unsigned short* src, bool valid
     }
 }
 
-template <int HD, int CODE, int NT>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv8_rows_kernel(const swlm_kv8_cache c, const swlm_kv8_attend a, const RowsPlan p) {
+// Where a CTA's share of the work lies. Stream order: sequences, their KV heads, their tiles of rows, units of kUnit slots. CTA c of C takes U / C
+// units, the first U % C CTAs one more, of one (sequence, KV head, tile) or of several, so that all CTAs have the same work whatever the lengths are.
+struct Shares {
+    int ctas, each, more;   // each CTA has a unit at least, so that the parts of one tile lie one behind the other
+    __device__ __forceinline__ Shares(int units, int launched) {
+        ctas = min(launched, units);
+        each = ctas ? units / ctas : 0;
+        more = units - each * ctas;
+    }
+    __device__ __forceinline__ int first(int cta) const { return cta * each + min(cta, more); }
+    __device__ __forceinline__ int cta_of(int unit) const { return unit < more * (each + 1) ? unit / (each + 1) : more + (unit - more * (each + 1)) / each; }
+};
+__device__ __forceinline__ int sequence_units(const Kv8Part& part, int span) { return (max(visible(part, part.count - 1, span), 1) + kUnit - 1) / kUnit; }
+__device__ __forceinline__ int sequence_tiles(const Kv8Part& part, int G, int TR) { return (part.count * G + TR - 1) / TR; }
+
+template <int HD, int CODE, int NT, bool SAVE>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_rows_kernel(const swlm_kv8_cache c, const swlm_kv8_attend a, const RowsPlan p) {
     constexpr int KS = HD / 16, MT = HD / 16, NS = stages<HD>(), SB = stage_bytes<HD>(), TR = 8 * NT;
     extern __shared__ __align__(16) unsigned char sm[];
     __shared__ float warp_m[kWarps][TR], warp_l[kWarps][TR];
+    __shared__ int scan[kWarps + 1];
+    int4* const info = reinterpret_cast<int4*>(sm + rows_smem<HD>());   // [batch + 1]: units before the sequence, its length, count, first row
     pdl_launch_dependents();
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int b = blockIdx.z, h = blockIdx.y, G = a.heads / c.kv_heads;
-    const int tile = blockIdx.x / p.splits, split = blockIdx.x - tile * p.splits;
-    const Kv8Part part = kv8_part(b, a.lengths, a.counts, a.starts, a.n, a.rows);
-    const int rows = part.count * G, row0 = tile * TR;
-    if (row0 >= rows) return;
-    const int span = min(a.max_len, c.capacity);
-    const int end = visible(part, min((row0 + TR - 1) / G, part.count - 1), span);   // of the tile's last query: it sees most
-    const int from = split * p.chunk, to = min(from + p.chunk, end);
-    if (from >= end && split > 0) return;
-    const size_t head = (size_t)b * c.kv_heads + h;
-    const unsigned char* keys = static_cast<const unsigned char*>(c.k) + head * c.capacity * HD;
-    const unsigned char* values = static_cast<const unsigned char*>(c.v) + head * c.capacity * HD;
-    const float* ks = c.k_scale + head * (c.capacity / c.block);
-    const float* vs = c.v_scale + head * (c.capacity / c.block);
+    const int G = a.heads / c.kv_heads, span = min(a.max_len, c.capacity);
+    const bool f16 = a.dtype == SWLM_KV8_FP16;
     const int block_shift = 31 - __clz(c.block);
 
-    // ring of this warp: step number i covers the 16 slots from `from` + (warp + 8 i) * 16 on. Whole steps are read: they lie within the capacity,
-    // a multiple of 16; what is beyond the last token is masked.
-    const unsigned ring = smem_addr(sm) + warp * NS * SB;
-    const int first = from + warp * kStep, steps = first < to ? (to - first + kSpanStep - 1) / kSpanStep : 0;
-    auto request = [&](int i) {
-        if (i < steps) {
-            const unsigned dst = ring + i % NS * SB;
-            const int base = first + i * kSpanStep;
-            const unsigned char *k = keys + (size_t)base * HD, *v = values + (size_t)base * HD;
-#pragma unroll
-            for (int u = 0; u < HD / 32; ++u) {
-                const int piece = lane + 32 * u, r = piece / (HD / 16), q = piece % (HD / 16);
-                copy16(dst + key_at<HD>(r, q), k + piece * 16);
-                copy16(dst + kStep * HD + value_at<HD>(r, q), v + piece * 16);
+    // ---- this CTA's units ----
+    int u = 0, u_end = 1, b = 0;
+    if (p.stream) {
+        int before = 0;   // units of the sequences before the ones of this turn
+        for (int b0 = 0; b0 < c.batch; b0 += kThreads) {
+            int mine = 0;
+            Kv8Part q{};
+            if (b0 + tid < c.batch) {
+                q = kv8_part(b0 + tid, a.lengths, a.counts, a.starts, a.n, a.rows);
+                if (q.count) mine = sequence_units(q, span) * sequence_tiles(q, G, TR) * c.kv_heads;
             }
-            if (lane < 2) copy4(dst + 2 * kStep * HD + lane * 4, (lane ? vs : ks) + (base >> block_shift));
-        }
-        commit();
-    };
+            int sum = mine;
 #pragma unroll
-    for (int i = 0; i < NS - 1; ++i) request(i);
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += v;
+            }
+            if (lane == 31) scan[warp] = sum;
+            __syncthreads();
+            int all = 0;
+            for (int w = 0; w < kWarps; ++w) {
+                if (w == warp) sum += all;
+                all += scan[w];
+            }
+            if (b0 + tid < c.batch) info[b0 + tid] = make_int4(before + sum - mine, q.len, q.count, q.start);
+            before += all;
+            if (b0 + kThreads < c.batch) __syncthreads();
+        }
+        const int total = before;
+        if (tid == 0) info[c.batch].x = total;
+        __syncthreads();
+        if (blockIdx.x == 0 && p.table)   // for the launch that joins the parts
+            for (int i = tid; i <= c.batch; i += kThreads) p.table[i] = info[i].x;
+        const Shares shares(total, (int)gridDim.x);
+        if ((int)blockIdx.x >= shares.ctas) return;
+        u = shares.first((int)blockIdx.x);
+        u_end = shares.first((int)blockIdx.x + 1);
+    } else {
+        b = blockIdx.z;
+    }
 
-    unsigned qf[NT][KS][2];
-    float factor[NT][2];     // of columns 2 t and 2 t + 1 (rows of the tile): score in log2 per unit of the product
-    int limit[NT][2];
-    {
-        const unsigned short* q = static_cast<const unsigned short*>(a.q);
-        const bool f16 = a.dtype == SWLM_KV8_FP16;
+    // what lies where: offsets of this lane within a step's stage. Copies: piece lane + 32 i, that is row lane / (HD / 16) + i * (512 / HD)
+    const int cp_r = lane / (HD / 16), cp_q = lane % (HD / 16);
+    const unsigned ring = smem_addr(sm) + warp * NS * SB;
+
+    while (u < u_end) {
+        // ---- the next (sequence, KV head, tile) and the slots of it that this CTA has ----
+        int h, tile, unit0, unit1;
+        Kv8Part part;
+        if (p.stream) {
+            for (int hi = c.batch - 1; b < hi;) {   // the sequence that has unit u
+                const int mid = (b + hi) >> 1;
+                if (info[mid + 1].x <= u) b = mid + 1;
+                else hi = mid;
+            }
+            const int4 q = info[b];
+            part = {q.y, q.z, q.w, true};
+            const int per = sequence_units(part, span), tiles = sequence_tiles(part, G, TR), rem = u - q.x, pair = rem / per;
+            h = pair / tiles;
+            tile = pair - h * tiles;
+            unit0 = rem - pair * per;
+            unit1 = min(per, unit0 + u_end - u);
+            u += unit1 - unit0;
+        } else {
+            part = kv8_part(b, a.lengths, a.counts, a.starts, a.n, a.rows);
+            h = blockIdx.y; tile = blockIdx.x; unit0 = 0; unit1 = sequence_units(part, span);
+            u = u_end;
+            if (tile * TR >= part.count * G) break;
+        }
+        const bool whole = unit0 == 0 && unit1 == sequence_units(part, span);   // this CTA has all of it
+        const int rows = part.count * G, row0 = tile * TR;
+        const int end = visible(part, min((row0 + TR - 1) / G, part.count - 1), span);   // of the tile's last query: it sees most
+        const int from = unit0 * kUnit, to = min(unit1 * kUnit, end);
+        const size_t head = (size_t)b * c.kv_heads + h;
+
+        // ring of this warp: its step number i covers the 32 slots from `first` + i * kUnit on. Whole tiles of 16 are read: they lie within the
+        // capacity, a multiple of 16; what is beyond a row's last slot is masked.
+        const int first = from + warp * kStep, steps = first < to ? (to - first + kUnit - 1) / kUnit : 0;
+        const unsigned char* kp = static_cast<const unsigned char*>(c.k) + (head * c.capacity + first) * HD + lane * 16;
+        const unsigned char* vp = static_cast<const unsigned char*>(c.v) + (head * c.capacity + first) * HD + lane * 16;
+        const float* sp = (lane & 1 ? c.v_scale : c.k_scale) + head * (c.capacity >> block_shift);
+        int asked = 0;
+        unsigned ask = ring;
+        auto request = [&]() {
+            if (asked < steps) {
+                const int base = first + asked * kUnit;
+                const bool both = base + 16 < to;   // (else the second tile's memory may not be there)
+#pragma unroll
+                for (int i = 0; i < kStep * HD / 512; ++i) {
+                    if (i < 16 * HD / 512 || both) {
+                        copy16(ask + key_at<HD>(cp_r + i * (512 / HD), cp_q), kp + i * 512);
+                        copy16(ask + kStep * HD + value_at<HD>(cp_r + i * (512 / HD), cp_q), vp + i * 512);
+                    }
+                }
+                if (lane < (both ? 4 : 2)) copy4(ask + 2 * kStep * HD + lane * 4, sp + ((base + (lane >> 1) * 16) >> block_shift));
+                kp += kUnit * HD;
+                vp += kUnit * HD;
+            }
+            commit();
+            ++asked;
+            ask = ask == ring + (NS - 1) * SB ? ring : ask + SB;
+        };
+#pragma unroll
+        for (int i = 0; i < NS - 1; ++i) request();
+
+        unsigned qf[NT][KS][2];
+        float factor[NT][2];     // of columns 2 t and 2 t + 1 (rows of the tile): score in log2 per unit of the product
+        int limit[NT][2], all_see = 0x7FFFFFFF;   // the tile's rows all attend the slots below
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int r = row0 + nt * 8 + g, i = min(r, rows - 1) / G;
             float down;
-            load_query<HD>(q + (int64_t)(part.start + i) * a.q_stride + (size_t)(h * G + min(r, rows - 1) - i * G) * HD, r < rows, f16, t, qf[nt], down);
-            down *= a.scale * kLog2e * code_unit<CODE>();
+            load_query<HD>(static_cast<const unsigned short*>(a.q) + (int64_t)(part.start + i) * a.q_stride + (size_t)(h * G + min(r, rows - 1) - i * G) * HD, r < rows, f16, t,
+                           qf[nt], down);
+            down *= a.scale * kLog2e;
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 factor[nt][e] = __shfl_sync(0xffffffffu, down, (2 * t + e) * 4);
-                const int rc = row0 + nt * 8 + 2 * t + e;
-                limit[nt][e] = rc < rows ? visible(part, rc / G, span) : 0;
+                // (rows behind the last one attend what the last one does: their results are not stored)
+                limit[nt][e] = visible(part, min(row0 + nt * 8 + 2 * t + e, rows - 1) / G, span);
+                all_see = min(all_see, limit[nt][e]);
             }
         }
-    }
-    float acc[NT][MT][4], m_ref[NT][2], l_run[NT][2], v_ref = 0x1p-100f, v_inv = 0x1p100f * kValueUnit;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int j = 0; j < MT; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[nt][j][e] = 0.f;
-        m_ref[nt][0] = m_ref[nt][1] = -INFINITY;
-        l_run[nt][0] = l_run[nt][1] = 0.f;
-    }
-    for (int i = 0; i < steps; ++i) {
-        wait_groups<NS - 2>();
-        __syncwarp();          // this step's copies of all lanes are there, and all lanes have read the step before
-        request(i + NS - 1);
-        const unsigned at = ring + i % NS * SB;
-        const int base = first + i * kSpanStep;
-        // ---- scores ----
-        float s[NT][4] = {};
-#pragma unroll
-        for (int u = 0; u < HD / 64; ++u) {
-            const uint4 lo = lds128(at + key_at<HD>(g, t + 4 * u)), hi = lds128(at + key_at<HD>(g + 8, t + 4 * u));
-            const unsigned lw[4] = {lo.x, lo.y, lo.z, lo.w}, hw[4] = {hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const unsigned x = prepared<CODE>(lw[w]), y = prepared<CODE>(hw[w]);
-                const unsigned a0 = pair_of<CODE, 0>(x), a1 = pair_of<CODE, 0>(y), a2 = pair_of<CODE, 1>(x), a3 = pair_of<CODE, 1>(y);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma(s[nt], a0, a1, a2, a3, qf[nt][u * 4 + w][0], qf[nt][u * 4 + w][1]);
-            }
-        }
-        const float k_scale = lds_f32(at + 2 * kStep * HD), v_scale = lds_f32(at + 2 * kStep * HD + 4);
-        bool moves = false;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int slot = base + g + 8 * (e >> 1);
-                s[nt][e] = slot < limit[nt][e & 1] ? s[nt][e] * (factor[nt][e & 1] * k_scale) : -INFINITY;
-                moves = moves || s[nt][e] > m_ref[nt][e & 1] + kSlack;
-            }
-        if (p.pitch) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const int r = row0 + nt * 8 + 2 * t;
-                if (r < p.pitch) {   // (the pitch is even)
-                    float* dst = p.scores + (head * p.span + base + g) * p.pitch + r;
-                    *reinterpret_cast<float2*>(dst) = make_float2(s[nt][0], s[nt][1]);
-                    *reinterpret_cast<float2*>(dst + 8 * p.pitch) = make_float2(s[nt][2], s[nt][3]);
-                }
-            }
-        }
-        // ---- softmax ----
-        if (__any_sync(0xffffffffu, moves)) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float top = fmaxf(s[nt][e], s[nt][e + 2]);
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                    if (top > m_ref[nt][e] + kSlack) {
-                        const float corr = exp2_of(m_ref[nt][e] - top);   // 0 for a row's first slots
-                        m_ref[nt][e] = top;
-                        l_run[nt][e] *= corr;
-#pragma unroll
-                        for (int j = 0; j < MT; ++j) { acc[nt][j][e] *= corr; acc[nt][j][e + 2] *= corr; }
-                    }
-                }
-        }
-        if (v_scale > v_ref) {
-            const float corr = v_ref / v_scale;
-            v_ref = v_scale;
-            v_inv = kValueUnit / v_scale;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int j = 0; j < MT; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[nt][j][e] *= corr;
-        }
-        const float unit = v_scale * v_inv;
-        unsigned pf[NT][2];
+        all_see = min(all_see, __shfl_xor_sync(0xffffffffu, all_see, 1));
+        all_see = min(all_see, __shfl_xor_sync(0xffffffffu, all_see, 2));
+        float acc[NT][MT][4], m_ref[NT][2], top_ok[NT][2], l_run[NT][2], v_ref = 0x1p-100f, v_inv = 0x1p100f * kValueUnit;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            float w[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float x = s[nt][e], m = m_ref[nt][e & 1];
-                const float pr = exp2_of(x - (m == -INFINITY ? 0.f : m));
-                l_run[nt][e & 1] += pr;
-                w[e] = x == -INFINITY ? 0.f : pr * unit;   // (a slot that the row does not attend may lie in a block that is NaN)
-            }
-            pf[nt][0] = transpose8x8(pack_half(w[0], w[1]));
-            pf[nt][1] = transpose8x8(pack_half(w[2], w[3]));
+            for (int j = 0; j < MT; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[nt][j][e] = 0.f;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) { m_ref[nt][e] = 0.f; top_ok[nt][e] = -INFINITY; l_run[nt][e] = 0.f; }
         }
-        // ---- values: this lane has HD / 8 dimensions of tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 ----
-        const unsigned va = at + kStep * HD;
-        unsigned vw[4][HD / 32];
+        float* save = SAVE ? p.scores + (head * p.span + first + g) * p.pitch + row0 + 2 * t : nullptr;
+        unsigned at = ring;
+        const int k_off = key_at<HD>(g, t), v_off = kStep * HD + (HD == 128 ? value_at<HD>(2 * t, g) : value_at<HD>(2 * t, g >> 1) + (g & 1) * 8);
+        for (int i = 0, base = first; i < steps; ++i, base += kUnit) {
+            wait_groups<NS - 2>();
+            __syncwarp();          // this step's copies of all lanes are there, and all lanes have read the step before
+            request();
+            // ---- scores ----
+            float s[kSub][NT][4] = {};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int r = 2 * t + (k & 1) + 8 * (k >> 1);
-            if (HD == 128) {
-                const uint4 v = lds128(va + value_at<HD>(r, g));
-                vw[k][0] = v.x; vw[k][1] = v.y; vw[k][HD / 32 - 2] = v.z; vw[k][HD / 32 - 1] = v.w;
-            } else {
-                const uint2 v = lds64(va + value_at<HD>(r, g >> 1) + (g & 1) * 8);
-                vw[k][0] = v.x; vw[k][1] = v.y;
+            for (int sub = 0; sub < kSub; ++sub)
+#pragma unroll
+                for (int q = 0; q < HD / 64; ++q) {
+                    const uint4 lo = lds128(at + (k_off ^ (q << 6)) + sub * 16 * HD), hi = lds128(at + (k_off ^ (q << 6)) + sub * 16 * HD + 8 * HD);
+                    const unsigned lw[4] = {lo.x, lo.y, lo.z, lo.w}, hw[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const unsigned x = prepared<CODE>(lw[w]), y = prepared<CODE>(hw[w]);
+                        const unsigned a0 = pair_of<CODE, 0>(x), a1 = pair_of<CODE, 0>(y), a2 = pair_of<CODE, 1>(x), a3 = pair_of<CODE, 1>(y);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) mma(s[sub][nt], a0, a1, a2, a3, qf[nt][q * 4 + w][0], qf[nt][q * 4 + w][1]);
+                    }
+                }
+            const uint4 sc = lds128(at + 2 * kStep * HD);
+            // values: this lane has HD / 8 dimensions of tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of either tile. The first tile's are on their way now
+            unsigned vw[4][HD / 32];
+            auto load_values = [&](int sub) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if (HD == 128) {   // (rows 2 t + 1 and 8 on share the swizzle)
+                        const uint4 v = lds128(at + v_off + sub * 2048 + (k & 1) * 128 + (k >> 1) * 1024);
+                        vw[k][0] = v.x; vw[k][1] = v.y; vw[k][HD / 32 - 2] = v.z; vw[k][HD / 32 - 1] = v.w;
+                    } else {           // (the odd token of a pair lies four pieces further on in their common line)
+                        const uint2 v = lds64(at + (v_off ^ ((k & 1) << 6)) + sub * 1024 + (k >> 1) * 512);
+                        vw[k][0] = v.x; vw[k][1] = v.y;
+                    }
+                }
+            };
+            load_values(0);
+            float k_scale[kSub] = {__uint_as_float(sc.x), __uint_as_float(sc.z)}, v_scale[kSub] = {__uint_as_float(sc.y), __uint_as_float(sc.w)};
+            const bool masked = base + kStep > all_see;
+            if (masked && base + 16 >= to) k_scale[1] = v_scale[1] = 0.f;   // (of a block that may hold nothing yet)
+            bool moves = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int sub = 0; sub < kSub; ++sub) {
+                    const float f0 = factor[nt][0] * k_scale[sub], f1 = factor[nt][1] * k_scale[sub];
+                    s[sub][nt][0] *= f0; s[sub][nt][1] *= f1; s[sub][nt][2] *= f0; s[sub][nt][3] *= f1;
+                    if (masked)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (base + sub * 16 + g + 8 * (e >> 1) >= limit[nt][e & 1]) s[sub][nt][e] = -INFINITY;
+                }
+                moves = moves || fmaxf(fmaxf(s[0][nt][0], s[0][nt][2]), fmaxf(s[1][nt][0], s[1][nt][2])) > top_ok[nt][0] ||
+                        fmaxf(fmaxf(s[0][nt][1], s[0][nt][3]), fmaxf(s[1][nt][1], s[1][nt][3])) > top_ok[nt][1];
             }
-        }
+            if (SAVE) {
 #pragma unroll
-        for (int w = 0; w < HD / 32; ++w) {
-            const unsigned v0 = prepared<CODE>(vw[0][w]), v1 = prepared<CODE>(vw[1][w]), v2 = prepared<CODE>(vw[2][w]), v3 = prepared<CODE>(vw[3][w]);
+                for (int nt = 0; nt < NT; ++nt)
+                    if (row0 + nt * 8 + 2 * t < p.pitch) {   // (the pitch is even)
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {   // dimensions 4 w + 2 half and the next one
-                const unsigned lo = __byte_perm(v0, v1, half ? 0x7362 : 0x5140), hi = __byte_perm(v2, v3, half ? 0x7362 : 0x5140);
-                const unsigned a0 = pair_of<CODE, 0>(lo), a1 = pair_of<CODE, 1>(lo), a2 = pair_of<CODE, 0>(hi), a3 = pair_of<CODE, 1>(hi);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma(acc[nt][2 * w + half], a0, a1, a2, a3, pf[nt][0], pf[nt][1]);
+                        for (int sub = 0; sub < kSub; ++sub) {
+                            *reinterpret_cast<float2*>(save + nt * 8 + sub * 16 * p.pitch) = make_float2(s[sub][nt][0], s[sub][nt][1]);
+                            *reinterpret_cast<float2*>(save + nt * 8 + (sub * 16 + 8) * p.pitch) = make_float2(s[sub][nt][2], s[sub][nt][3]);
+                        }
+                    }
+                save += kUnit * p.pitch;
             }
+            // ---- softmax ----
+            if (__any_sync(0xffffffffu, moves)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float top = fmaxf(fmaxf(s[0][nt][e], s[0][nt][e + 2]), fmaxf(s[1][nt][e], s[1][nt][e + 2]));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                        if (top > top_ok[nt][e]) {
+                            const float corr = top_ok[nt][e] == -INFINITY ? 0.f : exp2_of(m_ref[nt][e] - top);
+                            m_ref[nt][e] = top;
+                            top_ok[nt][e] = top + kSlack;
+                            l_run[nt][e] *= corr;
+#pragma unroll
+                            for (int j = 0; j < MT; ++j) { acc[nt][j][e] *= corr; acc[nt][j][e + 2] *= corr; }
+                        }
+                    }
+            }
+            const float v_top = fmaxf(v_scale[0], v_scale[1]);
+            if (v_top > v_ref) {
+                const float corr = v_ref / v_top;
+                v_ref = v_top;
+                v_inv = kValueUnit / v_top;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int j = 0; j < MT; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[nt][j][e] *= corr;
+            }
+            unsigned pf[kSub][NT][2];
+#pragma unroll
+            for (int sub = 0; sub < kSub; ++sub) {
+                const float unit = v_scale[sub] * v_inv;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float pr = exp2_of(s[sub][nt][e] - m_ref[nt][e & 1]);
+                        l_run[nt][e & 1] += pr;
+                        w[e] = pr * unit;
+                        if (masked && s[sub][nt][e] == -INFINITY) w[e] = 0.f;   // (a slot that the row does not attend may lie in a block that is NaN)
+                    }
+                    pf[sub][nt][0] = transpose8x8(pack_half(w[0], w[1]));
+                    pf[sub][nt][1] = transpose8x8(pack_half(w[2], w[3]));
+                }
+            }
+            // ---- values ----
+#pragma unroll
+            for (int sub = 0; sub < kSub; ++sub) {
+                if (sub) load_values(sub);
+                // what lies behind the last token may be an e4m3 NaN, which the weight 0 would not hide
+                if (CODE == SWLM_KV8_E4M3 && masked)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (base + sub * 16 + 2 * t + (k & 1) + 8 * (k >> 1) >= end)
+#pragma unroll
+                            for (int w = 0; w < HD / 32; ++w) vw[k][w] = 0;
+#pragma unroll
+                for (int w = 0; w < HD / 32; ++w) {
+                    const unsigned v0 = prepared<CODE>(vw[0][w]), v1 = prepared<CODE>(vw[1][w]), v2 = prepared<CODE>(vw[2][w]), v3 = prepared<CODE>(vw[3][w]);
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {   // dimensions 4 w + 2 half and the next one
+                        const unsigned lo = __byte_perm(v0, v1, half ? 0x7362 : 0x5140), hi = __byte_perm(v2, v3, half ? 0x7362 : 0x5140);
+                        const unsigned a0 = pair_of<CODE, 0>(lo), a1 = pair_of<CODE, 1>(lo), a2 = pair_of<CODE, 0>(hi), a3 = pair_of<CODE, 1>(hi);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) mma(acc[nt][2 * w + half], a0, a1, a2, a3, pf[sub][nt][0], pf[sub][nt][1]);
+                    }
+                }
+            }
+            at = at == ring + (NS - 1) * SB ? ring : at + SB;
         }
-    }
 
-    // ---- the warps' results together ----
-    __syncthreads();   // every warp is done with its ring
-    float* const outs = reinterpret_cast<float*>(sm);   // [warp][TR][HD]
-    const float unit = v_ref * (code_unit<CODE>() / kValueUnit);
+        // ---- the warps' results together ----
+        __syncthreads();   // every warp is done with its ring (only empty groups are outstanding)
+        float* const outs = reinterpret_cast<float*>(sm);   // [warp][TR][HD]
+        const float unit = v_ref * (1.f / kValueUnit);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+        for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            float l = l_run[nt][e];
-            l += __shfl_xor_sync(0xffffffffu, l, 4);
-            l += __shfl_xor_sync(0xffffffffu, l, 8);
-            l += __shfl_xor_sync(0xffffffffu, l, 16);
-            if (g == 0) { warp_m[warp][nt * 8 + 2 * t + e] = m_ref[nt][e]; warp_l[warp][nt * 8 + 2 * t + e] = l; }
-        }
-#pragma unroll
-        for (int j = 0; j < MT; ++j)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)   // row 2 t + e, dimensions g * HD / 8 + 2 j and the next one
-                *reinterpret_cast<float2*>(outs + (size_t)(warp * TR + nt * 8 + 2 * t + e) * HD + g * (HD / 8) + 2 * j) = make_float2(acc[nt][j][e] * unit, acc[nt][j][e + 2] * unit);
-    }
-    __syncthreads();
-    const bool f16 = a.dtype == SWLM_KV8_FP16;
-    for (int item = tid; item < TR * (HD / 4); item += kThreads) {
-        const int r = item / (HD / 4), d = item % (HD / 4) * 4, row = row0 + r;
-        if (row >= rows) continue;
-        float m = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, warp_m[w][r]);
-        float l = 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            // (a row whose scores are all NaN has no maximum and a sum that is NaN)
-            const float f = warp_m[w][r] == -INFINITY ? (warp_l[w][r] == 0.f ? 0.f : 1.f) : exp2_of(warp_m[w][r] - m);
-            const float4 v = *reinterpret_cast<const float4*>(outs + (size_t)(w * TR + r) * HD + d);
-            l += f * warp_l[w][r];
-            o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
-        }
-        const size_t at = (head * p.rows + row) * p.splits + split;
-        if (d == 0 && p.part_ml) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m, l);
-        if (p.splits > 1) {
-            *reinterpret_cast<float4*>(p.part_o + at * HD + d) = o;
-        } else {
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-            const int i = row / G;
-            unsigned short* dst = static_cast<unsigned short*>(a.out) + (int64_t)(part.start + i) * a.out_stride + (size_t)(h * G + row - i * G) * HD + d;
-            unsigned v[2];
-            if (f16) {
-                v[0] = pack_half(o.x * inv, o.y * inv); v[1] = pack_half(o.z * inv, o.w * inv);
-            } else {
-                const __nv_bfloat162 x = __floats2bfloat162_rn(o.x * inv, o.y * inv), y = __floats2bfloat162_rn(o.z * inv, o.w * inv);
-                v[0] = *reinterpret_cast<const unsigned*>(&x); v[1] = *reinterpret_cast<const unsigned*>(&y);
+            for (int e = 0; e < 2; ++e) {
+                float l = l_run[nt][e];
+                l += __shfl_xor_sync(0xffffffffu, l, 4);
+                l += __shfl_xor_sync(0xffffffffu, l, 8);
+                l += __shfl_xor_sync(0xffffffffu, l, 16);
+                if (g == 0) {
+                    warp_m[warp][nt * 8 + 2 * t + e] = top_ok[nt][e] == -INFINITY ? -INFINITY : m_ref[nt][e];
+                    warp_l[warp][nt * 8 + 2 * t + e] = l;
+                }
             }
-            *reinterpret_cast<uint2*>(dst) = make_uint2(v[0], v[1]);
+#pragma unroll
+            for (int j = 0; j < MT; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)   // row 2 t + e, dimensions g * HD / 8 + 2 j and the next one
+                    *reinterpret_cast<float2*>(outs + (size_t)(warp * TR + nt * 8 + 2 * t + e) * HD + g * (HD / 8) + 2 * j) =
+                        make_float2(acc[nt][j][e] * unit, acc[nt][j][e + 2] * unit);
         }
+        __syncthreads();
+        // parts of a (sequence, KV head, tile): its number plus the CTA's, which both grow along the stream
+        const size_t slot = (size_t)(head * p.row_tiles + tile) + (p.stream ? blockIdx.x : 0);
+        for (int item = tid; item < TR * (HD / 4); item += kThreads) {
+            const int r = item / (HD / 4), d = item % (HD / 4) * 4, row = row0 + r;
+            if (row >= rows) continue;
+            float m = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) m = fmaxf(m, warp_m[w][r]);
+            float l = 0.f;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                // (a row whose scores are all NaN has no maximum and a sum that is NaN)
+                const float f = warp_m[w][r] == -INFINITY ? (warp_l[w][r] == 0.f ? 0.f : 1.f) : exp2_of(warp_m[w][r] - m);
+                const float4 v = *reinterpret_cast<const float4*>(outs + (size_t)(w * TR + r) * HD + d);
+                l += f * warp_l[w][r];
+                o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
+            }
+            if (d == 0 && (SAVE || p.ml_always || !whole)) *reinterpret_cast<float2*>(p.part_ml + (slot * TR + r) * 2) = make_float2(m, l);
+            if (!whole) {
+                *reinterpret_cast<float4*>(p.part_o + (slot * TR + r) * HD + d) = o;
+            } else {
+                const int i = row / G;
+                store_out(static_cast<unsigned short*>(a.out) + (int64_t)(part.start + i) * a.out_stride + (size_t)(h * G + row - i * G) * HD + d, o, l, f16);
+            }
+        }
+        __syncthreads();   // the next one's copies take the results' place
     }
 }
 
-// Maximum and sum of a row over the parts that it has, by a group of LANES lanes; all of them get both.
+// Parts of one (sequence, KV head, tile of rows): the first one's place and their number.
+struct Parts { size_t slot; int count; };
+__device__ __forceinline__ Parts parts_of(const RowsPlan& p, const Kv8Part& part, int b, int batch, size_t head, int h, int tile, int span, int G) {
+    const size_t slot = head * p.row_tiles + tile;
+    if (!p.stream) return {slot, 1};
+    const Shares shares(p.table[batch], p.ctas);
+    const int per = sequence_units(part, span), u = p.table[b] + (h * sequence_tiles(part, G, 8 * p.tiles) + tile) * per, c0 = shares.cta_of(u);
+    return {slot + c0, shares.cta_of(u + per - 1) - c0 + 1};
+}
+
+// Maximum and sum of a row over its parts, `pitch` floats apart, by a group of LANES lanes; all of them get both.
 template <int LANES>
-__device__ __forceinline__ void row_total(const float* ml, int parts, int lane, float& m, float& l) {
+__device__ __forceinline__ void row_total(const float* ml, int pitch, int parts, int lane, float& m, float& l) {
     m = -INFINITY;
-    for (int s = lane; s < parts; s += LANES) m = fmaxf(m, ml[2 * s]);
+    for (int s = lane; s < parts; s += LANES) m = fmaxf(m, ml[(size_t)s * pitch]);
 #pragma unroll
     for (int o = LANES / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     l = 0.f;
     for (int s = lane; s < parts; s += LANES) {
-        const float x = ml[2 * s], v = ml[2 * s + 1];
+        const float x = ml[(size_t)s * pitch], v = ml[(size_t)s * pitch + 1];
         l += x == -INFINITY ? v : exp2_of(x - m) * v;   // (v is 0, or NaN where a part's scores are all NaN)
     }
 #pragma unroll
     for (int o = LANES / 2; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
 }
 
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 256, kJoinTurns = 4, kJoinSlots = kJoinThreads * kJoinTurns;
 
-// CTAs 0 .. join - 1 along x join the parts of the rows, the others add the kept scores' weights, 256 slots each.
+// CTAs 0 .. join - 1 along x join the parts of the rows that have several, the others add the kept scores' weights, kJoinSlots slots each.
 template <int HD>
 __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const swlm_kv8_cache c, const swlm_kv8_attend a, const RowsPlan p, const int join) {
     constexpr int LANES = HD / 4, PER = kJoinThreads / LANES;   // lanes of a row, rows of a CTA
+    constexpr int AHEAD = 8;                                    // parts that are loaded before the first is used
     __shared__ float row_m[kSaveRows], row_inv[kSaveRows];
     __shared__ int row_limit[kSaveRows];
+    __shared__ float group_m[PER], group_l[PER];
+    __shared__ float4 group_o[kJoinThreads];
     pdl_launch_dependents();
     pdl_wait();
-    const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x, G = a.heads / c.kv_heads;
+    const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x, G = a.heads / c.kv_heads, TR = 8 * p.tiles;
     const Kv8Part part = kv8_part(b, a.lengths, a.counts, a.starts, a.n, a.rows);
     const int rows = part.count * G, span = min(a.max_len, c.capacity);
+    if (rows == 0) return;
     const size_t head = (size_t)b * c.kv_heads + h;
-    auto parts_of = [&](int limit) { return max(1, (limit + p.chunk - 1) / p.chunk); };   // (part 0 is always written)
     if ((int)blockIdx.x < join) {
-        const int row = (int)blockIdx.x * PER + tid / LANES, lane = tid % LANES;
-        const bool on = row < rows;
-        const int parts = on ? parts_of(visible(part, row / G, span)) : 0;
-        const size_t at = (head * p.rows + (on ? row : 0)) * p.splits;
-        float m, l;
-        row_total<LANES>(p.part_ml + at * 2, parts, lane, m, l);
-        if (!on) return;
+        // p.join_groups groups of lanes take every so many-th part of a row, the first of them puts their results together
+        const int group = tid / LANES, lane = tid % LANES, d = lane * 4, sub = group % p.join_groups;
+        const int row = (int)blockIdx.x * (PER / p.join_groups) + group / p.join_groups;
+        const int tile = min(row, rows - 1) / TR, r = min(row, rows - 1) - tile * TR;
+        const Parts parts = parts_of(p, part, b, c.batch, head, h, tile, span, G);
+        const bool on = row < rows && parts.count > 1;
+        const float* ml = p.part_ml + (parts.slot * TR + r) * 2;
+        const float* po = p.part_o + (parts.slot * TR + r) * HD + d;
+        float m = -INFINITY, l = 0.f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int s = 0; s < parts; ++s) {
-            const float x = p.part_ml[(at + s) * 2];
-            const float f = x == -INFINITY ? 1.f : exp2_of(x - m);   // (a part without slots has zeros)
-            const float4 v = *reinterpret_cast<const float4*>(p.part_o + (at + s) * HD + lane * 4);
-            o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
+        if (on)
+            for (int s0 = sub; s0 < parts.count; s0 += AHEAD * p.join_groups) {
+                float2 x[AHEAD];
+                float4 v[AHEAD];
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) {
+                    const int s = min(s0 + i * p.join_groups, parts.count - 1);
+                    x[i] = *reinterpret_cast<const float2*>(ml + (size_t)s * TR * 2);
+                    v[i] = *reinterpret_cast<const float4*>(po + (size_t)s * TR * HD);
+                }
+                float top = m;
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) top = fmaxf(top, x[i].x);   // (the last part may come several times)
+                const float corr = m == -INFINITY ? 1.f : exp2_of(m - top);   // (no maximum so far: zeros, or NaN)
+                o.x *= corr; o.y *= corr; o.z *= corr; o.w *= corr; l *= corr;
+                m = top;
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) {
+                    const float f = s0 + i * p.join_groups >= parts.count ? 0.f : x[i].x == -INFINITY ? 1.f : exp2_of(x[i].x - m);   // (a part without slots has zeros, or NaN)
+                    if (f == 0.f) continue;
+                    l += f * x[i].y;
+                    o.x += f * v[i].x; o.y += f * v[i].y; o.z += f * v[i].z; o.w += f * v[i].w;
+                }
+            }
+        if (p.join_groups > 1) {
+            if (lane == 0) { group_m[group] = m; group_l[group] = l; }
+            group_o[tid] = o;
+            __syncthreads();
+            if (sub) return;
+            float top = m;
+            for (int i = 1; i < p.join_groups; ++i) top = fmaxf(top, group_m[group + i]);
+            float sum = 0.f;
+            float4 all = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int i = 0; i < p.join_groups; ++i) {
+                const float x = group_m[group + i], f = x == -INFINITY ? 1.f : exp2_of(x - top);
+                const float4 v = group_o[tid + i * LANES];
+                sum += f * group_l[group + i];
+                all.x += f * v.x; all.y += f * v.y; all.z += f * v.z; all.w += f * v.w;
+            }
+            l = sum;
+            o = all;
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        if (!on) return;
         const int i = row / G;
-        unsigned short* dst = static_cast<unsigned short*>(a.out) + (int64_t)(part.start + i) * a.out_stride + (size_t)(h * G + row - i * G) * HD + lane * 4;
-        unsigned v[2];
-        if (a.dtype == SWLM_KV8_FP16) {
-            v[0] = pack_half(o.x * inv, o.y * inv); v[1] = pack_half(o.z * inv, o.w * inv);
-        } else {
-            const __nv_bfloat162 x = __floats2bfloat162_rn(o.x * inv, o.y * inv), y = __floats2bfloat162_rn(o.z * inv, o.w * inv);
-            v[0] = *reinterpret_cast<const unsigned*>(&x); v[1] = *reinterpret_cast<const unsigned*>(&y);
-        }
-        *reinterpret_cast<uint2*>(dst) = make_uint2(v[0], v[1]);
+        store_out(static_cast<unsigned short*>(a.out) + (int64_t)(part.start + i) * a.out_stride + (size_t)(h * G + row - i * G) * HD + d, o, l, a.dtype == SWLM_KV8_FP16);
         return;
     }
-    if (rows == 0) return;
-    const int end = visible(part, part.count - 1, span), slot = ((int)blockIdx.x - join) * kJoinThreads + tid;
-    if (slot - tid >= end) return;
+    // the scores of this thread's slots and what they had so far are on their way while the rows' totals are worked out
+    const int end = visible(part, part.count - 1, span), slot0 = ((int)blockIdx.x - join) * kJoinSlots + tid;
+    if (slot0 - tid >= end) return;
+    float* const w = c.weight + head * c.capacity;
+    const float* const sc = p.scores + head * p.span * p.pitch;
+    float had[kJoinTurns];
+    float4 x[kJoinTurns];
+#pragma unroll
+    for (int i = 0; i < kJoinTurns; ++i) {
+        const int slot = min(slot0 + i * kJoinThreads, end - 1);
+        had[i] = w[slot];
+        if (p.pitch == 2) {
+            const float2 v = *reinterpret_cast<const float2*>(sc + (size_t)slot * 2);
+            x[i] = make_float4(v.x, v.y, 0.f, 0.f);
+        } else {
+            x[i] = *reinterpret_cast<const float4*>(sc + (size_t)slot * p.pitch);
+        }
+    }
     for (int row = tid >> 5; row < rows; row += kJoinThreads / 32) {
-        const int limit = visible(part, row / G, span);
+        const int tile = row / TR, r = row - tile * TR;
+        const Parts parts = parts_of(p, part, b, c.batch, head, h, tile, span, G);
         float m, l;
-        row_total<32>(p.part_ml + (head * p.rows + row) * p.splits * 2, parts_of(limit), tid & 31, m, l);
+        row_total<32>(p.part_ml + (parts.slot * TR + r) * 2, TR * 2, parts.count, tid & 31, m, l);
         if ((tid & 31) == 0) {
             row_m[row] = m == -INFINITY ? 0.f : m;
             row_inv[row] = l == 0.f ? 0.f : 1.f / l;
-            row_limit[row] = limit;
+            row_limit[row] = visible(part, row / G, span);
         }
     }
     __syncthreads();
-    if (slot >= end) return;
-    const float* sc = p.scores + (head * p.span + slot) * p.pitch;
-    float sum = 0.f;
-    for (int row = 0; row < rows; row += 2) {
-        const float2 x = *reinterpret_cast<const float2*>(sc + row);
-        if (slot < row_limit[row]) sum += exp2_of(x.x - row_m[row]) * row_inv[row];
-        if (row + 1 < rows && slot < row_limit[row + 1]) sum += exp2_of(x.y - row_m[row + 1]) * row_inv[row + 1];
+#pragma unroll
+    for (int i = 0; i < kJoinTurns; ++i) {
+        const int slot = slot0 + i * kJoinThreads;
+        if (slot >= end) break;
+        float sum = 0.f;
+        for (int row = 0; row < rows; row += 4) {
+            if (row) x[i] = *reinterpret_cast<const float4*>(sc + (size_t)slot * p.pitch + row);
+            const float v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (row + e < rows && slot < row_limit[row + e]) sum += exp2_of(v[e] - row_m[row + e]) * row_inv[row + e];
+        }
+        w[slot] = had[i] + sum;
     }
-    c.weight[head * c.capacity + slot] += sum;
 }
 
 // The weights of many rows: the scores are worked out again with the rows' totals known. A warp keeps the fragments of 16 tokens' keys in registers and
@@ -501,10 +700,10 @@ __global__ void __launch_bounds__(kAgainWarps * 32) kv8_weights_kernel(const swl
     const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, G = a.heads / c.kv_heads;
     const Kv8Part part = kv8_part(b, a.lengths, a.counts, a.starts, a.n, a.rows);
     const int rows = part.count * G, span = min(a.max_len, c.capacity);
-    const int end = rows ? visible(part, part.count - 1, span) : 0, cta0 = (int)blockIdx.x * kAgainWarps * kStep;
+    const int end = rows ? visible(part, part.count - 1, span) : 0, cta0 = (int)blockIdx.x * kAgainWarps * 16;
     if (cta0 >= end) return;
     const size_t head = (size_t)b * c.kv_heads + h;
-    const int base = cta0 + warp * kStep;
+    const int base = cta0 + warp * 16;
     const bool on = base < end;
     unsigned kf[KS][4];
     float k_scale = 0.f;
@@ -544,12 +743,13 @@ __global__ void __launch_bounds__(kAgainWarps * 32) kv8_weights_kernel(const swl
             float m = -INFINITY, l = 0.f;
             if (t == 0) {
                 if (row < rows) {
-                    const float* ml = p.part_ml + (head * p.rows + row) * p.splits * 2;
-                    const int parts = max(1, (limit + p.chunk - 1) / p.chunk);
-                    for (int s = 0; s < parts; ++s) m = fmaxf(m, ml[2 * s]);
-                    for (int s = 0; s < parts; ++s) l += ml[2 * s] == -INFINITY ? ml[2 * s + 1] : exp2_of(ml[2 * s] - m) * ml[2 * s + 1];
+                    const int TR = 8 * p.tiles, tile = row / TR;
+                    const Parts parts = parts_of(p, part, b, c.batch, head, h, tile, span, G);
+                    const float* ml = p.part_ml + (parts.slot * TR + row - tile * TR) * 2;
+                    for (int s = 0; s < parts.count; ++s) m = fmaxf(m, ml[2 * TR * s]);
+                    for (int s = 0; s < parts.count; ++s) l += ml[2 * TR * s] == -INFINITY ? ml[2 * TR * s + 1] : exp2_of(ml[2 * TR * s] - m) * ml[2 * TR * s + 1];
                 }
-                row_factor[r] = down * (a.scale * kLog2e * code_unit<CODE>());
+                row_factor[r] = down * (a.scale * kLog2e);
                 row_m[r] = m == -INFINITY ? 0.f : m;
                 row_inv[r] = l == 0.f ? 0.f : 1.f / l;
                 row_limit[r] = limit;
@@ -591,53 +791,72 @@ RowsPlan rows_plan(const swlm_kv8_cache& c, const swlm_kv8_attend& a, size_t* by
     p.tiles = p.rows <= 8 ? 1 : 2;
     p.row_tiles = (p.rows + 8 * p.tiles - 1) / (8 * p.tiles);
     p.span = (span + kStep - 1) / kStep * kStep;
-    // runs of slots so that the CTAs fill the GPU: two per SM with one tile, one with two
-    const long long ctas = (long long)c.batch * c.kv_heads * p.row_tiles;
-    const int want = p.tiles == 1 ? 296 : 148;
-    const int most = std::max(1, (span + kSpanStep - 1) / kSpanStep);
-    const int splits = (int)std::min<long long>(std::min(most, 64), std::max<long long>(1, want / ctas));
-    p.chunk = ((span + splits - 1) / splits + kSpanStep - 1) / kSpanStep * kSpanStep;
-    p.splits = std::max(1, (span + p.chunk - 1) / p.chunk);
-    const size_t parts = (size_t)c.batch * c.kv_heads * p.rows * p.splits;
+    const long long groups = (long long)c.batch * c.kv_heads * p.row_tiles, units = groups * ((span + kUnit - 1) / kUnit);
+    // CTAs that fill the GPU once, or one per unit where there are fewer
+    const int fill = kSms * (p.tiles > 1 ? 2 : c.head_dim == 128 ? rows_ctas<128>() : rows_ctas<64>());
+    p.stream = c.batch <= kStreamBatch && units < (1LL << 30) && groups < 16 * fill;
+    p.ctas = p.stream ? (int)std::min<long long>(fill, units) : 0;
+    const bool several = p.stream && units > groups;   // parts that have to be joined
+    const size_t places = (size_t)groups + p.ctas;
+    p.ml_always = a.accumulate != 0;
+    // a group of lanes takes up to eight parts at once: as many groups as a row with the most parts has such turns
+    const long long most = std::min<long long>(units / groups, p.ctas / groups + 2);
+    p.join_groups = most > 32 ? 8 : most > 16 ? 4 : most > 8 ? 2 : 1;
     size_t at = 0;
     char* base = static_cast<char*>(a.scratch);
-    if (p.splits > 1) { p.part_o = reinterpret_cast<float*>(base); at += align16(parts * c.head_dim * 4); }
-    if (p.splits > 1 || a.accumulate) { p.part_ml = reinterpret_cast<float*>(base + at); at += align16(parts * 8); }
+    auto take = [&](size_t n) { char* q = base + at; at += align16(n); return q; };
+    if (several) p.part_o = reinterpret_cast<float*>(take(places * 8 * p.tiles * c.head_dim * 4));
+    if (several || a.accumulate) {
+        p.part_ml = reinterpret_cast<float*>(take(places * 8 * p.tiles * 8));
+        if (p.stream) p.table = reinterpret_cast<int*>(take(((size_t)c.batch + 1) * 4));
+    }
     if (a.accumulate && p.rows <= kSaveRows) {
-        p.pitch = (p.rows + 1) / 2 * 2;
-        p.scores = reinterpret_cast<float*>(base + at);
-        at += align16((size_t)c.batch * c.kv_heads * p.span * p.pitch * 4);
+        p.pitch = p.rows <= 2 ? 2 : (p.rows + 3) / 4 * 4;
+        p.scores = reinterpret_cast<float*>(take((size_t)c.batch * c.kv_heads * p.span * p.pitch * 4));
     }
     *bytes = at;
     return p;
 }
 
+template <int HD, int CODE, int NT>
+cudaError_t launch_tiles(const dim3& grid, size_t smem, const swlm_kv8_cache& c, const swlm_kv8_attend& a, const RowsPlan& p, cudaStream_t s) {
+    return p.pitch ? launch_k(kv8_rows_kernel<HD, CODE, NT, true>, grid, dim3(kThreads), smem, s, c, a, p)
+                   : launch_k(kv8_rows_kernel<HD, CODE, NT, false>, grid, dim3(kThreads), smem, s, c, a, p);
+}
+
 template <int HD, int CODE>
 int launch_rows(const swlm_kv8_cache& c, const swlm_kv8_attend& a, const RowsPlan& p, cudaStream_t s) {
-    const dim3 grid((unsigned)(p.row_tiles * p.splits), (unsigned)c.kv_heads, (unsigned)c.batch);
-    const cudaError_t e = p.tiles == 1 ? launch_k(kv8_rows_kernel<HD, CODE, 1>, grid, dim3(kThreads), rows_smem<HD>(), s, c, a, p)
-                                       : launch_k(kv8_rows_kernel<HD, CODE, 2>, grid, dim3(kThreads), rows_smem<HD>(), s, c, a, p);
+    const dim3 grid = p.stream ? dim3((unsigned)p.ctas) : dim3((unsigned)p.row_tiles, (unsigned)c.kv_heads, (unsigned)c.batch);
+    const size_t smem = rows_smem<HD>() + (p.stream ? ((size_t)c.batch + 1) * sizeof(int4) : 0);
+    const cudaError_t e = p.tiles == 1 ? launch_tiles<HD, CODE, 1>(grid, smem, c, a, p, s) : launch_tiles<HD, CODE, 2>(grid, smem, c, a, p, s);
     if (e != cudaSuccess) return cuda_fail(e, "kv8 attention launch");
     const int span = std::min(a.max_len, c.capacity);
-    const int join = p.splits > 1 ? (p.rows + kJoinThreads / (HD / 4) - 1) / (kJoinThreads / (HD / 4)) : 0;
-    const int slots = p.pitch ? (span + kJoinThreads - 1) / kJoinThreads : 0;
+    const int per = kJoinThreads / (HD / 4) / p.join_groups, join = p.part_o ? (p.rows + per - 1) / per : 0;
+    const int slots = p.pitch ? (span + kJoinSlots - 1) / kJoinSlots : 0;
     if (join + slots) {
         const cudaError_t j = launch_k(kv8_join_kernel<HD>, dim3((unsigned)(join + slots), (unsigned)c.kv_heads, (unsigned)c.batch), dim3(kJoinThreads), 0, s, c, a, p, join);
         if (j != cudaSuccess) return cuda_fail(j, "kv8 join launch");
     }
     if (a.accumulate && !p.pitch) {
-        constexpr int per = kAgainWarps * kStep;
+        constexpr int per = kAgainWarps * 16;
         const cudaError_t w = launch_k(kv8_weights_kernel<HD, CODE>, dim3((unsigned)((span + per - 1) / per), (unsigned)c.kv_heads, (unsigned)c.batch), dim3(kAgainWarps * 32), 0, s, c, a, p);
         if (w != cudaSuccess) return cuda_fail(w, "kv8 weights launch");
     }
     return SWLM_OK;
 }
 
+template <int HD, int CODE, int NT, bool SAVE>
+int init_one() {
+    SWLM_CUDA(cudaFuncSetAttribute(kv8_rows_kernel<HD, CODE, NT, SAVE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(rows_smem<HD>() + (kStreamBatch + 1) * sizeof(int4))));
+    return SWLM_OK;
+}
 template <int HD, int CODE>
 int init_rows() {
-    SWLM_CUDA(cudaFuncSetAttribute(kv8_rows_kernel<HD, CODE, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rows_smem<HD>()));
-    SWLM_CUDA(cudaFuncSetAttribute(kv8_rows_kernel<HD, CODE, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rows_smem<HD>()));
-    return SWLM_OK;
+    int rc = init_one<HD, CODE, 1, false>();
+    if (!rc) rc = init_one<HD, CODE, 1, true>();
+    if (!rc) rc = init_one<HD, CODE, 2, false>();
+    if (!rc) rc = init_one<HD, CODE, 2, true>();
+    return rc;
 }
 // the warps' results (at most two tiles) take the rings' place
 static_assert((size_t)kWarps * 16 * 128 * 4 <= rows_smem<128>() && (size_t)kWarps * 16 * 64 * 4 <= rows_smem<64>(), "results fit the rings");
