@@ -16,13 +16,12 @@
 // of their scores in tensor memory and are read there as the A operand. The reference maximum of a row moves only when it would grow
 // by more than 2^8 (probabilities stay below 256, exactly undone by the sum at the end), so that the output is rarely rescaled.
 // Every mbarrier wait is bounded (see qgemm_tc.cu).
-#include "swlm_internal.h"
-#include "tc_device.cuh"
+#include "tc_attention.cuh"
 
 namespace swlm {
 namespace {
 
-constexpr int kPaRows = 128, kPaKeys = 64, kPaThreads = 192;
+constexpr int kPaThreads = 192;
 constexpr float kPaLog2e = 1.4426950408889634f;
 constexpr float kPaSlack = 8.f;   // log2 of what a row's probabilities may exceed 1 by
 
@@ -34,48 +33,6 @@ struct PromptAttnParams {
     __nv_bfloat16* out; int out_stride;
     int* status;
 };
-
-// (descriptors by their low words; `b_hi`: the high word of B's)
-__device__ __forceinline__ void pa_mma_ss(unsigned d, unsigned a_lo, unsigned b_lo, unsigned idesc, unsigned acc) {
-    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}"
-                 ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(kUmmaDescHi), "r"(idesc), "r"(acc) : "memory");
-}
-__device__ __forceinline__ void pa_mma_ts(unsigned d, unsigned a, unsigned b_lo, unsigned idesc, unsigned acc) {
-    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 b, {%2, %3};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}"
-                 ::"r"(d), "r"(a), "r"(b_lo), "r"(kUmmaDescHi), "r"(idesc), "r"(acc) : "memory");
-}
-// D fp32, A = B = bf16, M = 128, N = n; `b_mn`: B's rows lie along K (its N index is the contiguous one)
-__host__ __device__ constexpr unsigned pa_idesc(int n, bool b_mn) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? 1u << 16 : 0u) | ((unsigned)(n >> 3) << 17) | ((unsigned)(kPaRows >> 4) << 24);
-}
-// Descriptor (low word) of a tile whose contiguous index is N: blocks of 64 elements (128 bytes) `block` bytes apart, eight rows of K
-// per 1024 bytes
-__device__ __forceinline__ unsigned pa_desc_mn_lo(unsigned addr, unsigned block) { return umma_desc_lo(addr) | (block >> 4) << 16; }
-#define PA_R8(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]), "=r"(v[o + 7])
-#define PA_I8(v, o) "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), "r"(v[o + 5]), "r"(v[o + 6]), "r"(v[o + 7])
-__device__ __forceinline__ void pa_ld32(unsigned addr, unsigned* v) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-                 : PA_R8(v, 0), PA_R8(v, 8), PA_R8(v, 16), PA_R8(v, 24) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void pa_st32(unsigned addr, const unsigned* v) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
-                 ::"r"(addr), PA_I8(v, 0), PA_I8(v, 8), PA_I8(v, 16), PA_I8(v, 24) : "memory");
-}
-__device__ __forceinline__ void pa_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void pa_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void pa_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void pa_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void pa_arrive(unsigned long long* bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory"); }
-__device__ __forceinline__ float pa_exp2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-__device__ __forceinline__ unsigned pa_pack(float a, float b) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const unsigned*>(&v);
-}
-// (a, b) as bf16 pairs hi + lo
-__device__ __forceinline__ void pa_split(float a, float b, unsigned& hi, unsigned& lo) {
-    hi = pa_pack(a, b);
-    lo = pa_pack(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xFFFF0000u));
-}
 
 // A wait by parity cannot tell a phase from the one two before it, so the phase before the awaited one has to be known to be over:
 //   q_ready, o_done  have one phase;
@@ -165,7 +122,7 @@ __global__ void __launch_bounds__(kPaThreads, 2) attn_prompt_kernel(const Prompt
 #pragma unroll
                     for (int kk = 0; kk < HD / 16; ++kk)
                         pa_mma_ss(d, (part ? ql : qh) + (kk >> 2) * (Q_HALF / 16) + 2 * (kk & 3), kd + (kk >> 2) * (KV_HALF / 16) + 2 * (kk & 3),
-                                  pa_idesc(kPaKeys, false), part > 0 || kk > 0 ? 1u : 0u);
+                                  pa_idesc(kPaKeys, false, true), part > 0 || kk > 0 ? 1u : 0u);
                 umma_commit(&bars.s_full[j & 1]);
             }
             __syncwarp();
@@ -186,7 +143,7 @@ __global__ void __launch_bounds__(kPaThreads, 2) attn_prompt_kernel(const Prompt
                 for (int part = 0; part < 2; ++part)
 #pragma unroll
                     for (int kk = 0; kk < kPaKeys / 16; ++kk)
-                        pa_mma_ts(tm + O_COL, tm + (unsigned)(j & 1) * 64u + part * 32u + 8u * kk, vd + kk * (2048 / 16), pa_idesc(HD, true),
+                        pa_mma_ts(tm + O_COL, tm + (unsigned)(j & 1) * 64u + part * 32u + 8u * kk, vd + kk * (2048 / 16), pa_idesc(HD, true, true),
                                   part > 0 || kk > 0 ? 1u : j > 0 ? 1u : 0u);
                 umma_commit(&bars.pv_done);
             }

@@ -507,7 +507,12 @@ int swlm_op_kv8_attend_dev(swlm_ctx* ctx, const swlm_kv8_cache* cache, const swl
     const size_t need = kv8_attend_scratch(c, a);
     if (need && (!a.scratch || !aligned(a.scratch, 16) || a.scratch_bytes < need)) { set_error("kv8: %zu bytes of 16-byte aligned scratch are needed", need); return SWLM_ERR_INVALID; }
     SWLM_CUDA(cudaSetDevice(ctx->device));
-    return launch_kv8_attend(c, a, stream_of(ctx, cuda_stream));
+    if (*static_cast<volatile int*>(ctx->kv8_status)) {
+        set_error("kv8: a bounded device-side wait of an earlier call expired (code %d): its results are not valid", *ctx->kv8_status);
+        *ctx->kv8_status = 0;
+        return SWLM_ERR_TIMEOUT;
+    }
+    return launch_kv8_attend(c, a, ctx->kv8_status, stream_of(ctx, cuda_stream));
 }
 
 size_t swlm_op_kv8_evict_scratch_bytes(const swlm_kv8_cache* cache, const swlm_kv8_evict* how) {

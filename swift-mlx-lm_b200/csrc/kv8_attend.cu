@@ -14,35 +14,14 @@
 // the largest scale keep that precision. Partial results of several runs are joined by a second launch, which also adds the weights.
 #include <algorithm>
 
-#include "kv8.h"
+#include "kv8_device.cuh"
 
 namespace swlm {
+using namespace kv8;
 namespace {
 
-constexpr int kWarps = 4, kThreads = kWarps * 32;
-constexpr int kSub = 2, kStep = 16 * kSub;        // tokens of a warp's step: two tiles of 16
-constexpr int kUnit = kWarps * kStep;           // slots of a step of all warps: work is dealt in these
 constexpr int kStreamBatch = 512;               // sequences whose units a CTA adds up
-constexpr int kSms = 148;
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kSlack = 8.f;                   // log2 of what a probability may exceed 1 by
-constexpr float kValueUnit = 128.f;             // 2^7: probabilities up to 2^8 stay within fp16
 constexpr int kSaveRows = 64;                   // up to so many rows of a KV head the scores are kept for the weights, beyond they are worked out again
-
-struct RowsPlan {
-    int tiles;      // 8-row tiles per CTA
-    int row_tiles;  // of a KV head at most, of 8 * tiles rows each
-    int rows;       // n * group
-    int stream, ctas;   // CTAs over equal shares of all units (stream), or one per (sequence, KV head, tile)
-    int span;       // slots that can be attended, rounded up to kStep
-    int pitch;      // rows of a slot's kept scores (0: not kept)
-    int join_groups;   // groups of lanes that share a row's parts
-    int ml_always;  // maximum and sum are wanted of rows in one part too
-    float* part_o;  // [places][8 * tiles][head_dim], not normalised; places: (sequence, KV head, tile) + CTA
-    float* part_ml; // [places][8 * tiles][2]: reference maximum (log2), sum
-    float* scores;  // [batch][kv_heads][span][pitch], log2
-    int* table;     // [batch + 1]: units before each sequence, and of all
-};
 
 __device__ __forceinline__ unsigned smem_addr(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void copy16(unsigned dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
@@ -64,7 +43,6 @@ __device__ __forceinline__ float2 lds_f32x2(unsigned a) {
     asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
     return v;
 }
-__device__ __forceinline__ float exp2_of(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ void mma(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -74,63 +52,6 @@ __device__ __forceinline__ unsigned transpose8x8(unsigned v) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
-__device__ __forceinline__ unsigned pack_half(float a, float b) {
-    const __half2 v = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const unsigned*>(&v);
-}
-
-// Codes to fp16, exactly. int8: with the sign bit turned a byte u = c + 128 is the low byte of 1024 + u.
-template <int CODE> __device__ __forceinline__ unsigned prepared(unsigned word) { return CODE == SWLM_KV8_INT8 ? word ^ 0x80808080u : word; }
-// bytes 2 * HIGH and 2 * HIGH + 1 of a prepared word
-template <int CODE, int HIGH> __device__ __forceinline__ unsigned pair_of(unsigned word) {
-    if (CODE == SWLM_KV8_INT8) {
-        const unsigned biased = __byte_perm(word, 0x64646464u, HIGH ? 0x4342 : 0x4140);
-        const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&biased), __half2half2(__ushort_as_half(0x6480)));   // 1024 + 128
-        return *reinterpret_cast<const unsigned*>(&v);
-    }
-    unsigned v;
-    if (HIGH) asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(v) : "r"(word));
-    else asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(v) : "r"(word));
-    return v;
-}
-
-// Four results of a row with sum l.
-__device__ __forceinline__ void store_out(unsigned short* dst, const float4& o, float l, bool f16) {
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    unsigned v[2];
-    if (f16) {
-        v[0] = pack_half(o.x * inv, o.y * inv); v[1] = pack_half(o.z * inv, o.w * inv);
-    } else {
-        const __nv_bfloat162 x = __floats2bfloat162_rn(o.x * inv, o.y * inv), y = __floats2bfloat162_rn(o.z * inv, o.w * inv);
-        v[0] = *reinterpret_cast<const unsigned*>(&x); v[1] = *reinterpret_cast<const unsigned*>(&y);
-    }
-    *reinterpret_cast<uint2*>(dst) = make_uint2(v[0], v[1]);
-}
-
-// Eight 16-bit values as floats.
-__device__ __forceinline__ void widen(const uint4& r, bool f16, float (&x)[8]) {
-    const unsigned w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (f16) {
-            const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-            x[2 * i] = v.x; x[2 * i + 1] = v.y;
-        } else {
-            x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-        }
-    }
-}
-// The power of two that brings `top`, a row's largest |value|, to 2^12 or a little more (NaN for a row that is not finite), and its inverse.
-__device__ __forceinline__ void row_shift(float top, float& up, float& down) {
-    const int e = (int)(__float_as_uint(top) >> 23);   // 0 for zero and subnormal ones
-    const int shift = top > 0.f ? min(12 + 127 - e, 126) : 0;
-    up = e == 255 ? kKv8NaN : __uint_as_float((unsigned)(127 + shift) << 23);
-    down = e == 255 ? kKv8NaN : __uint_as_float((unsigned)(127 - shift) << 23);
-}
-
-// The slots that query i of a sequence attends are those below this.
-__device__ __forceinline__ int visible(const Kv8Part& part, int i, int span) { return (int)min((long long)part.len + i + 1, (long long)span); }
-
 template <int HD> __host__ __device__ constexpr int stages() { return HD == 128 ? 2 : 3; }
 template <int HD> __host__ __device__ constexpr int rows_ctas() { return HD == 128 ? 3 : 4; }   // CTAs of one tile per SM
 template <int HD> __host__ __device__ constexpr int stage_bytes() { return 2 * kStep * HD + 16; }   // keys, values, (key, value) scale of either tile
@@ -173,21 +94,6 @@ __device__ __forceinline__ void load_query(const unsigned short* src, bool valid
         frag[k][1] = pack_half(x[4 * k + 2] * up, x[4 * k + 3] * up);
     }
 }
-
-// Where a CTA's share of the work lies. Stream order: sequences, their KV heads, their tiles of rows, units of kUnit slots. CTA c of C takes U / C
-// units, the first U % C CTAs one more, of one (sequence, KV head, tile) or of several, so that all CTAs have the same work whatever the lengths are.
-struct Shares {
-    int ctas, each, more;   // each CTA has a unit at least, so that the parts of one tile lie one behind the other
-    __device__ __forceinline__ Shares(int units, int launched) {
-        ctas = min(launched, units);
-        each = ctas ? units / ctas : 0;
-        more = units - each * ctas;
-    }
-    __device__ __forceinline__ int first(int cta) const { return cta * each + min(cta, more); }
-    __device__ __forceinline__ int cta_of(int unit) const { return unit < more * (each + 1) ? unit / (each + 1) : more + (unit - more * (each + 1)) / each; }
-};
-__device__ __forceinline__ int sequence_units(const Kv8Part& part, int span) { return (max(visible(part, part.count - 1, span), 1) + kUnit - 1) / kUnit; }
-__device__ __forceinline__ int sequence_tiles(const Kv8Part& part, int G, int TR) { return (part.count * G + TR - 1) / TR; }
 
 template <int HD, int CODE, int NT, bool SAVE>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_rows_kernel(const swlm_kv8_cache c, const swlm_kv8_attend a, const RowsPlan p) {
@@ -538,16 +444,6 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_r
     }
 }
 
-// Parts of one (sequence, KV head, tile of rows): the first one's place and their number.
-struct Parts { size_t slot; int count; };
-__device__ __forceinline__ Parts parts_of(const RowsPlan& p, const Kv8Part& part, int b, int batch, size_t head, int h, int tile, int span, int G) {
-    const size_t slot = head * p.row_tiles + tile;
-    if (!p.stream) return {slot, 1};
-    const Shares shares(p.table[batch], p.ctas);
-    const int per = sequence_units(part, span), u = p.table[b] + (h * sequence_tiles(part, G, 8 * p.tiles) + tile) * per, c0 = shares.cta_of(u);
-    return {slot + c0, shares.cta_of(u + per - 1) - c0 + 1};
-}
-
 // Maximum and sum of a row over its parts, `pitch` floats apart, by a group of LANES lanes; all of them get both.
 template <int LANES>
 __device__ __forceinline__ void row_total(const float* ml, int pitch, int parts, int lane, float& m, float& l) {
@@ -788,19 +684,29 @@ RowsPlan rows_plan(const swlm_kv8_cache& c, const swlm_kv8_attend& a, size_t* by
     RowsPlan p{};
     const int span = std::min(a.max_len, c.capacity), G = a.heads / c.kv_heads;
     p.rows = a.n * G;
-    p.tiles = p.rows <= 8 ? 1 : 2;
+    p.tiles = p.rows <= 8 ? 1 : p.rows <= kSaveRows ? 2 : kPromptRows / 8;
     p.row_tiles = (p.rows + 8 * p.tiles - 1) / (8 * p.tiles);
     p.span = (span + kStep - 1) / kStep * kStep;
     const long long groups = (long long)c.batch * c.kv_heads * p.row_tiles, units = groups * ((span + kUnit - 1) / kUnit);
-    // CTAs that fill the GPU once, or one per unit where there are fewer
-    const int fill = kSms * (p.tiles > 1 ? 2 : c.head_dim == 128 ? rows_ctas<128>() : rows_ctas<64>());
-    p.stream = c.batch <= kStreamBatch && units < (1LL << 30) && groups < 16 * fill;
-    p.ctas = p.stream ? (int)std::min<long long>(fill, units) : 0;
-    const bool several = p.stream && units > groups;   // parts that have to be joined
-    const size_t places = (size_t)groups + p.ctas;
+    bool several;   // parts that have to be joined
+    if (p.tiles > 2) {
+        // runs of at least eight key tiles, as many as make two CTAs per SM
+        const long long want = std::max<long long>(1, 2 * kSms / groups), most = (span + 8 * kPromptKeys - 1) / (8 * kPromptKeys);
+        const int runs = (int)std::min(want, most);
+        p.chunk = ((span + runs - 1) / runs + kPromptKeys - 1) / kPromptKeys * kPromptKeys;
+        p.splits = (span + p.chunk - 1) / p.chunk;
+        several = p.splits > 1;
+    } else {
+        // CTAs that fill the GPU once, or one per unit where there are fewer
+        const int fill = kSms * (p.tiles > 1 ? 2 : c.head_dim == 128 ? rows_ctas<128>() : rows_ctas<64>());
+        p.stream = c.batch <= kStreamBatch && units < (1LL << 30) && groups < 16 * fill;
+        p.ctas = p.stream ? (int)std::min<long long>(fill, units) : 0;
+        several = p.stream && units > groups;
+    }
+    const size_t places = p.splits ? (size_t)groups * p.splits : (size_t)groups + p.ctas;
     p.ml_always = a.accumulate != 0;
     // a group of lanes takes up to eight parts at once: as many groups as a row with the most parts has such turns
-    const long long most = std::min<long long>(units / groups, p.ctas / groups + 2);
+    const long long most = p.splits ? p.splits : std::min<long long>(units / groups, p.ctas / groups + 2);
     p.join_groups = most > 32 ? 8 : most > 16 ? 4 : most > 8 ? 2 : 1;
     size_t at = 0;
     char* base = static_cast<char*>(a.scratch);
@@ -825,11 +731,16 @@ cudaError_t launch_tiles(const dim3& grid, size_t smem, const swlm_kv8_cache& c,
 }
 
 template <int HD, int CODE>
-int launch_rows(const swlm_kv8_cache& c, const swlm_kv8_attend& a, const RowsPlan& p, cudaStream_t s) {
-    const dim3 grid = p.stream ? dim3((unsigned)p.ctas) : dim3((unsigned)p.row_tiles, (unsigned)c.kv_heads, (unsigned)c.batch);
-    const size_t smem = rows_smem<HD>() + (p.stream ? ((size_t)c.batch + 1) * sizeof(int4) : 0);
-    const cudaError_t e = p.tiles == 1 ? launch_tiles<HD, CODE, 1>(grid, smem, c, a, p, s) : launch_tiles<HD, CODE, 2>(grid, smem, c, a, p, s);
-    if (e != cudaSuccess) return cuda_fail(e, "kv8 attention launch");
+int launch_rows(const swlm_kv8_cache& c, const swlm_kv8_attend& a, const RowsPlan& p, int* status, cudaStream_t s) {
+    if (p.splits) {
+        const int rc = launch_kv8_prompt(c, a, p, status, s);
+        if (rc) return rc;
+    } else {
+        const dim3 grid = p.stream ? dim3((unsigned)p.ctas) : dim3((unsigned)p.row_tiles, (unsigned)c.kv_heads, (unsigned)c.batch);
+        const size_t smem = rows_smem<HD>() + (p.stream ? ((size_t)c.batch + 1) * sizeof(int4) : 0);
+        const cudaError_t e = p.tiles == 1 ? launch_tiles<HD, CODE, 1>(grid, smem, c, a, p, s) : launch_tiles<HD, CODE, 2>(grid, smem, c, a, p, s);
+        if (e != cudaSuccess) return cuda_fail(e, "kv8 attention launch");
+    }
     const int span = std::min(a.max_len, c.capacity);
     const int per = kJoinThreads / (HD / 4) / p.join_groups, join = p.part_o ? (p.rows + per - 1) / per : 0;
     const int slots = p.pitch ? (span + kJoinSlots - 1) / kJoinSlots : 0;
@@ -868,6 +779,7 @@ int kv8_attend_init() {
     if (!rc) rc = init_rows<128, SWLM_KV8_E4M3>();
     if (!rc) rc = init_rows<64, SWLM_KV8_INT8>();
     if (!rc) rc = init_rows<64, SWLM_KV8_E4M3>();
+    if (!rc) rc = kv8_prompt_init();
     return rc;
 }
 
@@ -877,11 +789,11 @@ size_t kv8_attend_scratch(const swlm_kv8_cache& c, const swlm_kv8_attend& a) {
     return bytes;
 }
 
-int launch_kv8_attend(const swlm_kv8_cache& c, const swlm_kv8_attend& a, cudaStream_t s) {
+int launch_kv8_attend(const swlm_kv8_cache& c, const swlm_kv8_attend& a, int* status, cudaStream_t s) {
     size_t bytes;
     const RowsPlan p = rows_plan(c, a, &bytes);
-    if (c.head_dim == 128) return c.code == SWLM_KV8_INT8 ? launch_rows<128, SWLM_KV8_INT8>(c, a, p, s) : launch_rows<128, SWLM_KV8_E4M3>(c, a, p, s);
-    return c.code == SWLM_KV8_INT8 ? launch_rows<64, SWLM_KV8_INT8>(c, a, p, s) : launch_rows<64, SWLM_KV8_E4M3>(c, a, p, s);
+    if (c.head_dim == 128) return c.code == SWLM_KV8_INT8 ? launch_rows<128, SWLM_KV8_INT8>(c, a, p, status, s) : launch_rows<128, SWLM_KV8_E4M3>(c, a, p, status, s);
+    return c.code == SWLM_KV8_INT8 ? launch_rows<64, SWLM_KV8_INT8>(c, a, p, status, s) : launch_rows<64, SWLM_KV8_E4M3>(c, a, p, status, s);
 }
 
 }  // namespace swlm

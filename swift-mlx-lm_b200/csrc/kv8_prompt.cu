@@ -1,0 +1,372 @@
+// Attention of many query rows over a cache of 8-bit codes (prompt portions), on the 5th-generation tensor cores (tcgen05 / TMEM).
+//
+// A CTA has 128 rows, rows being the queries of a sequence times the heads of a group, and a run of its slots. Codes become fp16 numbers on their
+// way to shared memory, queries are shifted to fp16 (both exact, see kv8_attend.cu), so that scores are one product with fp32 sums; a tile's
+// scores take the factor of their block, probabilities that of the values' block over the largest so far (2^7 times, as fp16).
+//
+// Roles: four warps bring keys and values from the cache, convert them and store them in the swizzled layout of the products' operands (two
+// slots each); a warp issues the MMAs (S = Q K^T of tile j + 1 while tile j is in its softmax: two score regions); four warps do
+// the softmax, a thread per row. Probabilities take the place of their scores in tensor memory and are read there as the A operand. The
+// reference maximum of a row moves only when it would grow by more than 2^8. Two CTAs share an SM.
+//
+// What bounds it, with heads of 128: 512 clocks of the tensor pipe per tile of 64 keys, 512 of the exponential unit (8192 of 16 per clock).
+#include <algorithm>
+
+#include "kv8_device.cuh"
+#include "tc_attention.cuh"
+
+namespace swlm {
+using namespace kv8;
+namespace {
+
+static_assert(kPromptRows == kPaRows && kPromptKeys == kPaKeys, "the shared helpers' tiles");
+constexpr int kSoftmaxThreads = 128, kMmaWarp = 4, kLoadThreads = 128, kPromptThreads = kSoftmaxThreads + 32 + kLoadThreads;
+constexpr float kFoldUnit = 0x1p-20f;   // value scales down to this part of the largest go into the exponent
+
+// Phases (a wait by parity cannot tell a phase from the one two before it): for tile j
+//   k_full[j & 1], v_full[j & 1], p_ready[j & 1]   waited for phase by phase by the MMA warp
+//   s_full[j & 1]    phase by phase by the softmax warps; by the loaders before tile j + 2, whose scores cannot be there yet
+//   pv_done[j & 1]   by the loaders before tile j + 2, whose product cannot be there yet; by the MMA warp in the round behind; by a softmax warp for
+//                    tile j - 1 behind s_full(j): the scores of tile j are issued behind pv_done(j - 2), and tile j + 1's product waits for this warp
+//   q_ready, o_done  have one phase
+struct PromptBars {
+    unsigned long long q_ready, k_full[2], v_full[2], s_full[2], p_ready[2], pv_done[2], o_done;
+    unsigned tmem;
+    int failed;
+};
+
+template <int HD> __host__ __device__ constexpr size_t prompt_smem() { return (size_t)kPaRows * HD * 2 + 4 * kPaKeys * HD * 2 + 1024; }
+
+template <int HD, int CODE>
+__global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const swlm_kv8_cache c, const swlm_kv8_attend a, const RowsPlan p, int* status) {
+    constexpr int HALVES = HD / 64;                        // 128-byte halves of a row
+    constexpr unsigned Q_HALF = kPaRows * 128, Q_BYTES = HALVES * Q_HALF, KV_HALF = kPaKeys * 128, KV_BYTES = HALVES * KV_HALF;
+    constexpr unsigned kTmemCols = 256, O_COL = 128;       // scores / probabilities 0..63 and 64..127, output from 128 on
+    extern __shared__ __align__(1024) unsigned char prompt_raw[];
+    unsigned char* const sm = prompt_raw + ((1024 - (smem_u32(prompt_raw) & 1023)) & 1023);
+    unsigned char *const q_sm = sm, *const k_sm = sm + Q_BYTES, *const v_sm = k_sm + 2 * KV_BYTES;
+    __shared__ __align__(8) PromptBars bars;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int b = blockIdx.z, h = blockIdx.y, G = a.heads / c.kv_heads, span = min(a.max_len, c.capacity);
+    const int tile = p.row_tiles - 1 - (int)blockIdx.x / p.splits, split = (int)blockIdx.x % p.splits;   // the longest rows first
+    const Kv8Part part = kv8_part(b, a.lengths, a.counts, a.starts, a.n, a.rows);
+    const int rows = part.count * G, row0 = tile * kPaRows;
+    if (row0 >= rows) return;
+    const int end = visible(part, min(row0 + kPaRows - 1, rows - 1) / G, span);   // of the tile's last query: it sees most
+    const int key_lo = split * p.chunk;
+    if (split > 0 && key_lo >= end) return;
+    const int n_tiles = (max(min(end - key_lo, p.chunk), 0) + kPaKeys - 1) / kPaKeys;
+    const size_t head = (size_t)b * c.kv_heads + h;
+    const int block_shift = 31 - __clz(c.block);
+    volatile int* const failed = &bars.failed;
+    auto fail = [&](int code) { atomicExch_system(status, code); *failed = 1; };
+
+    if (tid == 0) {
+        mbar_init(&bars.q_ready, 4);
+        mbar_init(&bars.o_done, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bars.k_full[i], kLoadThreads / 32);
+            mbar_init(&bars.v_full[i], kLoadThreads / 32);
+            mbar_init(&bars.s_full[i], 1);
+            mbar_init(&bars.p_ready[i], 4);
+            mbar_init(&bars.pv_done[i], 1);
+        }
+        bars.failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        __syncwarp();
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem)), "r"(kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pa_before();
+    __syncthreads();
+    pa_after();
+    const unsigned tm = bars.tmem;
+
+    if (warp > kMmaWarp) {
+        // ---- keys and values: codes in, fp16 out --------------------------------------------------------------------------------------
+        constexpr int PIECES = HD / 16, PER = kPaKeys * PIECES / kLoadThreads;   // 16-byte pieces of a token, of this thread in a tile
+        const int lt = tid - kSoftmaxThreads - 32, piece = lt % PIECES, key = lt / PIECES;
+        const unsigned char* kg = static_cast<const unsigned char*>(c.k) + head * c.capacity * HD + piece * 16;
+        const unsigned char* vg = static_cast<const unsigned char*>(c.v) + head * c.capacity * HD + piece * 16;
+        uint4 kr[PER], vr[PER];
+        auto load = [&](const unsigned char* src, uint4 (&r)[PER], int j) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int slot = key_lo + j * kPaKeys + key + i * (kPaKeys / PER);
+                r[i] = slot < end ? __ldg(reinterpret_cast<const uint4*>(src + (size_t)slot * HD)) : make_uint4(0, 0, 0, 0);   // (nothing that may be NaN)
+            }
+        };
+        auto store = [&](unsigned char* dst, const uint4 (&r)[PER]) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int row = key + i * (kPaKeys / PER), chunk = piece * 2 & 7;
+                const unsigned w[4] = {prepared<CODE>(r[i].x), prepared<CODE>(r[i].y), prepared<CODE>(r[i].z), prepared<CODE>(r[i].w)};
+                const uint4 lo = make_uint4(pair_of<CODE, 0>(w[0]), pair_of<CODE, 1>(w[0]), pair_of<CODE, 0>(w[1]), pair_of<CODE, 1>(w[1]));
+                const uint4 hi = make_uint4(pair_of<CODE, 0>(w[2]), pair_of<CODE, 1>(w[2]), pair_of<CODE, 0>(w[3]), pair_of<CODE, 1>(w[3]));
+                unsigned char* const at = dst + (piece >> 2) * KV_HALF + row * 128;
+                // (the second half's pieces go the other way round: the eight lanes of a phase meet different banks)
+                const bool other = piece >= 4;
+                *reinterpret_cast<uint4*>(at + (((chunk + other) ^ (row & 7)) << 4)) = other ? hi : lo;
+                *reinterpret_cast<uint4*>(at + (((chunk + !other) ^ (row & 7)) << 4)) = other ? lo : hi;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+        };
+        bool ok = true;
+        if (n_tiles) { load(kg, kr, 0); load(vg, vr, 0); }
+        for (int j = 0; j < n_tiles; ++j) {
+            if (*failed || (j >= 2 && !mbar_wait_warp(&bars.s_full[j & 1], (unsigned)(((j - 2) >> 1) & 1)))) { ok = false; break; }
+            store(k_sm + (j & 1) * KV_BYTES, kr);
+            if (lane == 0) pa_arrive(&bars.k_full[j & 1]);
+            if (j + 1 < n_tiles) load(kg, kr, j + 1);
+            if (j >= 2 && !mbar_wait_warp(&bars.pv_done[j & 1], (unsigned)(((j - 2) >> 1) & 1))) { ok = false; break; }
+            store(v_sm + (j & 1) * KV_BYTES, vr);
+            if (lane == 0) pa_arrive(&bars.v_full[j & 1]);
+            if (j + 1 < n_tiles) load(vg, vr, j + 1);
+        }
+        if (!ok && lane == 0) fail(31);
+        __syncwarp();
+    } else if (warp == kMmaWarp) {
+        const bool el = elect_one();
+        const unsigned qd = umma_desc_lo(smem_u32(q_sm)), kd = umma_desc_lo(smem_u32(k_sm)), vd = pa_desc_mn_lo(smem_u32(v_sm), KV_HALF);
+        auto scores = [&](int j) {
+            if (el) {
+#pragma unroll
+                for (int kk = 0; kk < HD / 16; ++kk)
+                    pa_mma_ss(tm + (unsigned)(j & 1) * 64u, qd + (kk >> 2) * (Q_HALF / 16) + 2 * (kk & 3), kd + (j & 1) * (KV_BYTES / 16) + (kk >> 2) * (KV_HALF / 16) + 2 * (kk & 3),
+                              pa_idesc(kPaKeys, false, false), kk > 0 ? 1u : 0u);
+                umma_commit(&bars.s_full[j & 1]);
+            }
+            __syncwarp();
+        };
+        bool ok = true;
+        if (n_tiles) {
+            ok = mbar_wait_warp(&bars.q_ready, 0u) && mbar_wait_warp(&bars.k_full[0], 0u);
+            if (ok) { pa_after(); scores(0); }
+        }
+        for (int j = 0; j < n_tiles && ok; ++j) {
+            if (j + 1 < n_tiles) {
+                // the region of tile j + 1 held the probabilities of tile j - 1
+                if (!mbar_wait_warp(&bars.k_full[(j + 1) & 1], (unsigned)(((j + 1) >> 1) & 1)) || (j > 0 && !mbar_wait_warp(&bars.pv_done[(j - 1) & 1], (unsigned)(((j - 1) >> 1) & 1)))) { ok = false; break; }
+                pa_after();
+                scores(j + 1);
+            }
+            if (!mbar_wait_warp(&bars.p_ready[j & 1], (unsigned)((j >> 1) & 1)) || !mbar_wait_warp(&bars.v_full[j & 1], (unsigned)((j >> 1) & 1))) { ok = false; break; }
+            pa_after();
+            if (el) {
+#pragma unroll
+                for (int kk = 0; kk < kPaKeys / 16; ++kk)
+                    pa_mma_ts(tm + O_COL, tm + (unsigned)(j & 1) * 64u + 8u * kk, vd + (j & 1) * (KV_BYTES / 16) + kk * (2048 / 16), pa_idesc(HD, true, false), kk > 0 || j > 0 ? 1u : 0u);
+                umma_commit(&bars.pv_done[j & 1]);
+            }
+            __syncwarp();
+        }
+        if (el) {
+            if (!ok) fail(32);
+            umma_commit(&bars.o_done);   // also behind whatever was issued before a failure
+        }
+        __syncwarp();
+        if (!mbar_wait_warp(&bars.o_done, 0u) && el) fail(32);   // tensor memory is not freed under MMAs in flight
+    } else {
+        const int r = tid, row = row0 + r, i = min(row, rows - 1) / G;
+        const bool row_ok = row < rows, f16 = a.dtype == SWLM_KV8_FP16;
+        const int limit = visible(part, i, span);   // (rows past the last one attend what it does; they are not stored)
+        float factor;
+        // ---- q: this thread's row, shifted to fp16 ----------------------------------------------------------------------------------------
+        {
+            const unsigned short* src = static_cast<const unsigned short*>(a.q) + (int64_t)(part.start + i) * a.q_stride + (size_t)(h * G + min(row, rows - 1) - i * G) * HD;
+            unsigned top = 0;   // largest |value| as its 15 bits
+#pragma unroll 4
+            for (int d = 0; d < HD; d += 8) {
+                const uint4 v = *reinterpret_cast<const uint4*>(src + d);
+                const unsigned m = __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
+                top = max(top, max(m & 0xFFFFu, m >> 16));
+            }
+            float up;
+            row_shift(f16 ? __half2float(__ushort_as_half((unsigned short)top)) : __uint_as_float(top << 16), up, factor);
+            factor *= a.scale * kLog2e;
+#pragma unroll 4
+            for (int d = 0; d < HD; d += 8) {
+                float x[8];
+                widen(*reinterpret_cast<const uint4*>(src + d), f16, x);
+                uint4 v;
+                v.x = pack_half(x[0] * up, x[1] * up); v.y = pack_half(x[2] * up, x[3] * up);
+                v.z = pack_half(x[4] * up, x[5] * up); v.w = pack_half(x[6] * up, x[7] * up);
+                *reinterpret_cast<uint4*>(q_sm + (d >> 6) * Q_HALF + r * 128 + ((((d >> 3) & 7) ^ (r & 7)) << 4)) = v;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) pa_arrive(&bars.q_ready);
+        }
+        // ---- softmax, a thread per row -------------------------------------------------------------------------------------------------------
+        const unsigned lanes = (unsigned)(warp * 32) << 16;
+        const float* ks = c.k_scale + head * (c.capacity >> block_shift);
+        const float* vs = c.v_scale + head * (c.capacity >> block_shift);
+        float m_ref = -INFINITY, l_run = 0.f, v_ref = 0x1p-100f;
+        float kn[4], vn[4];   // the next tile's scales, of 16 keys each; 0 behind the last token
+        auto scales = [&](int j) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int slot = key_lo + j * kPaKeys + g * 16;
+                kn[g] = slot < end ? __ldg(ks + (slot >> block_shift)) : 0.f;
+                vn[g] = slot < end ? __ldg(vs + (slot >> block_shift)) : 0.f;
+            }
+        };
+        if (n_tiles) scales(0);
+        bool ok = true;
+        for (int j = 0; j < n_tiles; ++j) {
+            const unsigned region = tm + lanes + (unsigned)(j & 1) * 64u;
+            float fk[4], vt[4];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) { fk[g] = factor * kn[g]; vt[g] = vn[g]; }
+            if (j + 1 < n_tiles) scales(j + 1);
+            if (!mbar_wait_warp(&bars.s_full[j & 1], (unsigned)((j >> 1) & 1))) { ok = false; break; }
+            pa_after();
+            unsigned v[64];
+            pa_ld32(region, v);
+            pa_ld32(region + 32u, v + 32);
+            pa_wait_ld();
+            const int key0 = key_lo + j * kPaKeys;
+            const bool masked = !__all_sync(0xffffffffu, key0 + kPaKeys <= limit);
+            float top = -INFINITY;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                float t = -INFINITY;
+                if (masked)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) t = fmaxf(t, key0 + g * 16 + e < limit ? __uint_as_float(v[g * 16 + e]) : -INFINITY);
+                else
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) t = fmaxf(t, __uint_as_float(v[g * 16 + e]));
+                if (t > -INFINITY) top = fmaxf(top, t * fk[g]);   // (factors are not negative: the largest score stays the largest)
+            }
+            const bool moves = top > m_ref + kSlack;
+            const float v_top = fmaxf(fmaxf(vt[0], vt[1]), fmaxf(vt[2], vt[3]));
+            if (__any_sync(0xffffffffu, moves || v_top > v_ref)) {
+                float corr = moves ? pa_exp2(m_ref - top) : 1.f;   // 0 for a row's first keys
+                if (moves) { m_ref = top; l_run *= corr; }
+                if (v_top > v_ref) { corr *= v_ref / v_top; v_ref = v_top; }
+                if (j > 0) {   // the output so far: complete, and the next product waits for this warp
+                    if (!mbar_wait_warp(&bars.pv_done[(j - 1) & 1], (unsigned)(((j - 1) >> 1) & 1))) { ok = false; break; }
+                    pa_after();
+#pragma unroll 1
+                    for (int d = 0; d < HD; d += 16) {
+                        unsigned o[16];
+                        pa_ld16(tm + lanes + O_COL + d, o);
+                        pa_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+                        pa_st16(tm + lanes + O_COL + d, o);
+                    }
+                    pa_wait_st();
+                }
+            }
+            const float base = m_ref == -INFINITY ? 0.f : m_ref;   // nothing attended so far: all probabilities 0
+            float unit[4];
+            bool folds = !masked;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                unit[g] = vt[g] / v_ref * kValueUnit;
+                folds = folds && unit[g] >= kFoldUnit * kValueUnit;
+            }
+            if (folds) {
+                // the unit goes into the exponent, and out of the sum again
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const float shift = __log2f(unit[g]) - base;
+                    float sum = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        const float x = pa_exp2(fmaf(__uint_as_float(v[g * 16 + e]), fk[g], shift)), y = pa_exp2(fmaf(__uint_as_float(v[g * 16 + e + 1]), fk[g], shift));
+                        sum += x + y;
+                        v[g * 8 + e / 2] = pack_half(x, y);
+                    }
+                    l_run += sum / unit[g];
+                }
+            } else {
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        float w[2];
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const bool sees = key0 + g * 16 + e + k < limit;   // (what a row does not attend may lie in a block that is NaN)
+                            const float x = sees ? pa_exp2(fmaf(__uint_as_float(v[g * 16 + e + k]), fk[g], -base)) : 0.f;
+                            l_run += x;
+                            w[k] = sees ? x * unit[g] : 0.f;
+                        }
+                        v[g * 8 + e / 2] = pack_half(w[0], w[1]);
+                    }
+                }
+            }
+            pa_st32(region, v);
+            pa_wait_st();
+            pa_before();
+            __syncwarp();
+            if (lane == 0) pa_arrive(&bars.p_ready[j & 1]);
+        }
+        if (ok && (!mbar_wait_warp(&bars.o_done, 0u) || *failed)) ok = false;
+        if (!ok) fail(33);
+        __syncwarp();
+        pa_after();
+        if (ok) {
+            const bool whole = end <= p.chunk;   // this CTA has all of the tile's slots
+            const size_t at = ((head * p.row_tiles + tile) * p.splits + split) * kPaRows + r;
+            const float unit = v_ref * (1.f / kValueUnit);
+            if (row_ok && (!whole || p.ml_always)) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m_ref, l_run);
+            unsigned short* dst = static_cast<unsigned short*>(a.out) + (int64_t)(part.start + i) * a.out_stride + (size_t)(h * G + min(row, rows - 1) - i * G) * HD;
+#pragma unroll 1
+            for (int d = 0; d < HD; d += 16) {
+                unsigned o[16] = {};
+                if (n_tiles) {
+                    pa_ld16(tm + lanes + O_COL + d, o);
+                    pa_wait_ld();
+                }
+                if (row_ok)
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        const float4 x = make_float4(__uint_as_float(o[e]) * unit, __uint_as_float(o[e + 1]) * unit, __uint_as_float(o[e + 2]) * unit, __uint_as_float(o[e + 3]) * unit);
+                        if (whole) store_out(dst + d + e, x, l_run, f16);
+                        else *reinterpret_cast<float4*>(p.part_o + at * HD + d + e) = x;
+                    }
+            }
+        }
+    }
+    pa_before();
+    __syncthreads();
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(kTmemCols) : "memory");
+}
+
+template <int HD, int CODE>
+int launch_prompt(const swlm_kv8_cache& c, const swlm_kv8_attend& a, const RowsPlan& p, int* status, cudaStream_t s) {
+    const cudaError_t e = launch_k(kv8_prompt_kernel<HD, CODE>, dim3((unsigned)(p.row_tiles * p.splits), (unsigned)c.kv_heads, (unsigned)c.batch), dim3(kPromptThreads),
+                                   prompt_smem<HD>(), s, c, a, p, status);
+    return e == cudaSuccess ? SWLM_OK : cuda_fail(e, "kv8 prompt attention launch");
+}
+template <int HD, int CODE>
+int init_prompt() {
+    SWLM_CUDA(cudaFuncSetAttribute(kv8_prompt_kernel<HD, CODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prompt_smem<HD>()));
+    return SWLM_OK;
+}
+
+}  // namespace
+
+int kv8_prompt_init() {
+    int rc = init_prompt<128, SWLM_KV8_INT8>();
+    if (!rc) rc = init_prompt<128, SWLM_KV8_E4M3>();
+    if (!rc) rc = init_prompt<64, SWLM_KV8_INT8>();
+    if (!rc) rc = init_prompt<64, SWLM_KV8_E4M3>();
+    return rc;
+}
+
+int launch_kv8_prompt(const swlm_kv8_cache& c, const swlm_kv8_attend& a, const RowsPlan& p, int* status, cudaStream_t s) {
+    if (c.head_dim == 128) return c.code == SWLM_KV8_INT8 ? launch_prompt<128, SWLM_KV8_INT8>(c, a, p, status, s) : launch_prompt<128, SWLM_KV8_E4M3>(c, a, p, status, s);
+    return c.code == SWLM_KV8_INT8 ? launch_prompt<64, SWLM_KV8_INT8>(c, a, p, status, s) : launch_prompt<64, SWLM_KV8_E4M3>(c, a, p, status, s);
+}
+
+}  // namespace swlm

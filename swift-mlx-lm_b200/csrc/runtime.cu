@@ -1397,7 +1397,9 @@ int swlm_ctx_create(int device_id, int tp_rank, int tp_size, swlm_ctx** out) {
     if (!rc) rc = grouped_init();
     if (!rc) rc = retention_init();
     if (!rc) rc = kv8_init();
+    if (!rc && (e = cudaHostAlloc((void**)&ctx->kv8_status, sizeof(int), cudaHostAllocMapped)) != cudaSuccess) rc = cuda_fail(e, "status word");
     if (rc) { cudaStreamDestroy(ctx->stream); delete ctx; return rc; }
+    *ctx->kv8_status = 0;
     *out = ctx;
     return SWLM_OK;
 }
@@ -1415,6 +1417,7 @@ void swlm_ctx_destroy(swlm_ctx* ctx) {
     for (auto& kv : ctx->matrix_cat) cudaFree(kv.second.data);
     cudaFree(ctx->op_partial);
     cudaFree(ctx->tc_status);
+    if (ctx->kv8_status) cudaFreeHost(ctx->kv8_status);
     cudaFree(ctx->op_xh);
     cudaFree(ctx->op_counters);
     cudaFree(ctx->op_attn_counters);
