@@ -5,8 +5,8 @@
 // scores take the factor of their block, probabilities that of the values' block over the largest so far (2^7 times, as fp16).
 //
 // Roles: four warps bring keys and values from the cache, convert them and store them in the swizzled layout of the products' operands (two
-// slots each); a warp issues the MMAs (S = Q K^T of tile j + 1 while tile j is in its softmax: two score regions); four warps do
-// the softmax, a thread per row. Probabilities take the place of their scores in tensor memory and are read there as the A operand. The
+// slots each); the first of them also issues the MMAs (S = Q K^T of tile j + 1 while tile j is in its softmax: two score regions); four warps
+// do the softmax, a thread per row. Probabilities take the place of their scores in tensor memory and are read there as the A operand. The
 // reference maximum of a row moves only when it would grow by more than 2^8. Two CTAs share an SM.
 //
 // What bounds it, with heads of 128: 512 clocks of the tensor pipe per tile of 64 keys, 512 of the exponential unit (8192 of 16 per clock).
@@ -20,20 +20,42 @@ using namespace kv8;
 namespace {
 
 static_assert(kPromptRows == kPaRows && kPromptKeys == kPaKeys, "the shared helpers' tiles");
-constexpr int kSoftmaxThreads = 128, kMmaWarp = 4, kLoadThreads = 128, kPromptThreads = kSoftmaxThreads + 32 + kLoadThreads;
+constexpr int kSoftmaxThreads = 128, kMmaWarp = 4, kLoadThreads = 128, kPromptThreads = kSoftmaxThreads + kLoadThreads;
 constexpr float kFoldUnit = 0x1p-20f;   // value scales down to this part of the largest go into the exponent
 
 // Phases (a wait by parity cannot tell a phase from the one two before it): for tile j
-//   k_full[j & 1], v_full[j & 1], p_ready[j & 1]   waited for phase by phase by the MMA warp
+//   k_full[j & 1], v_full[j & 1], p_ready[j & 1]   waited for phase by phase by the warp that issues the MMAs
 //   s_full[j & 1]    phase by phase by the softmax warps; by the loaders before tile j + 2, whose scores cannot be there yet
-//   pv_done[j & 1]   by the loaders before tile j + 2, whose product cannot be there yet; by the MMA warp in the round behind; by a softmax warp for
-//                    tile j - 1 behind s_full(j): the scores of tile j are issued behind pv_done(j - 2), and tile j + 1's product waits for this warp
+//   pv_done[j & 1]   by the loaders before tile j + 2, whose product cannot be there yet; by a softmax warp for tile j - 1 behind s_full(j): the scores of tile j are issued behind pv_done(j - 2), and tile j + 1's product waits for this warp
 //   q_ready, o_done  have one phase
 struct PromptBars {
     unsigned long long q_ready, k_full[2], v_full[2], s_full[2], p_ready[2], pv_done[2], o_done;
     unsigned tmem;
     int failed;
 };
+
+// Two fp32 operations as one instruction.
+__device__ __forceinline__ unsigned long long pair_bits(const float2& v) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+    return r;
+}
+__device__ __forceinline__ float2 bits_pair(unsigned long long v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(const float2& a, const float2& b, const float2& c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)), "l"(pair_bits(c)));
+    return bits_pair(r);
+}
+__device__ __forceinline__ float2 add2(const float2& a, const float2& b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)));
+    return bits_pair(r);
+}
+__device__ __forceinline__ float log2_of(float x) { float y; asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
 template <int HD> __host__ __device__ constexpr size_t prompt_smem() { return (size_t)kPaRows * HD * 2 + 4 * kPaKeys * HD * 2 + 1024; }
 
@@ -86,54 +108,41 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const swl
     pa_after();
     const unsigned tm = bars.tmem;
 
-    if (warp > kMmaWarp) {
-        // ---- keys and values: codes in, fp16 out --------------------------------------------------------------------------------------
-        constexpr int PIECES = HD / 16, PER = kPaKeys * PIECES / kLoadThreads;   // 16-byte pieces of a token, of this thread in a tile
-        const int lt = tid - kSoftmaxThreads - 32, piece = lt % PIECES, key = lt / PIECES;
-        const unsigned char* kg = static_cast<const unsigned char*>(c.k) + head * c.capacity * HD + piece * 16;
-        const unsigned char* vg = static_cast<const unsigned char*>(c.v) + head * c.capacity * HD + piece * 16;
+    if (warp >= kMmaWarp) {
+        // ---- keys and values: codes in, fp16 out; warp kMmaWarp issues the products ------------------------------------------------------------
+        constexpr int PIECES = HD / 16, PER = kPaKeys * PIECES / kLoadThreads, STEP = kPaKeys / PER;   // 16-byte pieces of a token, of this thread in a tile
+        const int lt = tid - kSoftmaxThreads, piece = lt % PIECES, key = lt / PIECES;                  // (keys key, key + STEP, ...)
+        const size_t at = (head * c.capacity + key_lo + key) * HD + piece * 16;
+        const unsigned char* kg = static_cast<const unsigned char*>(c.k) + at;
+        const unsigned char* vg = static_cast<const unsigned char*>(c.v) + at;
         uint4 kr[PER], vr[PER];
         auto load = [&](const unsigned char* src, uint4 (&r)[PER], int j) {
+            const int slot = key_lo + j * kPaKeys + key;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                const int slot = key_lo + j * kPaKeys + key + i * (kPaKeys / PER);
-                r[i] = slot < end ? __ldg(reinterpret_cast<const uint4*>(src + (size_t)slot * HD)) : make_uint4(0, 0, 0, 0);   // (nothing that may be NaN)
-            }
+            for (int i = 0; i < PER; ++i)
+                r[i] = slot + i * STEP < end ? __ldg(reinterpret_cast<const uint4*>(src + i * STEP * HD)) : make_uint4(0, 0, 0, 0);   // (nothing that may be NaN)
         };
+        // Two chunks of eight values per piece. The pieces of a row's second half go the other way round, so that the eight lanes of a phase meet
+        // different banks; STEP is a multiple of 8, so that all of this thread's rows have the same swizzle
+        static_assert(STEP % 8 == 0, "one swizzle");
+        const int chunk = piece * 2 & 7;
+        const bool other = piece >= 4;
+        const unsigned off = (piece >> 2) * KV_HALF + key * 128, off0 = off + (((chunk + other) ^ (key & 7)) << 4), off1 = off + (((chunk + !other) ^ (key & 7)) << 4);
         auto store = [&](unsigned char* dst, const uint4 (&r)[PER]) {
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
-                const int row = key + i * (kPaKeys / PER), chunk = piece * 2 & 7;
-                const unsigned w[4] = {prepared<CODE>(r[i].x), prepared<CODE>(r[i].y), prepared<CODE>(r[i].z), prepared<CODE>(r[i].w)};
-                const uint4 lo = make_uint4(pair_of<CODE, 0>(w[0]), pair_of<CODE, 1>(w[0]), pair_of<CODE, 0>(w[1]), pair_of<CODE, 1>(w[1]));
-                const uint4 hi = make_uint4(pair_of<CODE, 0>(w[2]), pair_of<CODE, 1>(w[2]), pair_of<CODE, 0>(w[3]), pair_of<CODE, 1>(w[3]));
-                unsigned char* const at = dst + (piece >> 2) * KV_HALF + row * 128;
-                // (the second half's pieces go the other way round: the eight lanes of a phase meet different banks)
-                const bool other = piece >= 4;
-                *reinterpret_cast<uint4*>(at + (((chunk + other) ^ (row & 7)) << 4)) = other ? hi : lo;
-                *reinterpret_cast<uint4*>(at + (((chunk + !other) ^ (row & 7)) << 4)) = other ? lo : hi;
+                const unsigned w[4] = {prepared<CODE>(other ? r[i].z : r[i].x), prepared<CODE>(other ? r[i].w : r[i].y), prepared<CODE>(other ? r[i].x : r[i].z),
+                                       prepared<CODE>(other ? r[i].y : r[i].w)};
+                *reinterpret_cast<uint4*>(dst + off0 + i * STEP * 128) = make_uint4(pair_of<CODE, 0>(w[0]), pair_of<CODE, 1>(w[0]), pair_of<CODE, 0>(w[1]), pair_of<CODE, 1>(w[1]));
+                *reinterpret_cast<uint4*>(dst + off1 + i * STEP * 128) = make_uint4(pair_of<CODE, 0>(w[2]), pair_of<CODE, 1>(w[2]), pair_of<CODE, 0>(w[3]), pair_of<CODE, 1>(w[3]));
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
         };
-        bool ok = true;
-        if (n_tiles) { load(kg, kr, 0); load(vg, vr, 0); }
-        for (int j = 0; j < n_tiles; ++j) {
-            if (*failed || (j >= 2 && !mbar_wait_warp(&bars.s_full[j & 1], (unsigned)(((j - 2) >> 1) & 1)))) { ok = false; break; }
-            store(k_sm + (j & 1) * KV_BYTES, kr);
-            if (lane == 0) pa_arrive(&bars.k_full[j & 1]);
-            if (j + 1 < n_tiles) load(kg, kr, j + 1);
-            if (j >= 2 && !mbar_wait_warp(&bars.pv_done[j & 1], (unsigned)(((j - 2) >> 1) & 1))) { ok = false; break; }
-            store(v_sm + (j & 1) * KV_BYTES, vr);
-            if (lane == 0) pa_arrive(&bars.v_full[j & 1]);
-            if (j + 1 < n_tiles) load(vg, vr, j + 1);
-        }
-        if (!ok && lane == 0) fail(31);
-        __syncwarp();
-    } else if (warp == kMmaWarp) {
-        const bool el = elect_one();
+        const bool issues = warp == kMmaWarp, el = elect_one();
         const unsigned qd = umma_desc_lo(smem_u32(q_sm)), kd = umma_desc_lo(smem_u32(k_sm)), vd = pa_desc_mn_lo(smem_u32(v_sm), KV_HALF);
         auto scores = [&](int j) {
+            pa_after();
             if (el) {
 #pragma unroll
                 for (int kk = 0; kk < HD / 16; ++kk)
@@ -143,19 +152,8 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const swl
             }
             __syncwarp();
         };
-        bool ok = true;
-        if (n_tiles) {
-            ok = mbar_wait_warp(&bars.q_ready, 0u) && mbar_wait_warp(&bars.k_full[0], 0u);
-            if (ok) { pa_after(); scores(0); }
-        }
-        for (int j = 0; j < n_tiles && ok; ++j) {
-            if (j + 1 < n_tiles) {
-                // the region of tile j + 1 held the probabilities of tile j - 1
-                if (!mbar_wait_warp(&bars.k_full[(j + 1) & 1], (unsigned)(((j + 1) >> 1) & 1)) || (j > 0 && !mbar_wait_warp(&bars.pv_done[(j - 1) & 1], (unsigned)(((j - 1) >> 1) & 1)))) { ok = false; break; }
-                pa_after();
-                scores(j + 1);
-            }
-            if (!mbar_wait_warp(&bars.p_ready[j & 1], (unsigned)((j >> 1) & 1)) || !mbar_wait_warp(&bars.v_full[j & 1], (unsigned)((j >> 1) & 1))) { ok = false; break; }
+        auto product = [&](int j) {   // false: a wait expired
+            if (!mbar_wait_warp(&bars.p_ready[j & 1], (unsigned)((j >> 1) & 1)) || !mbar_wait_warp(&bars.v_full[j & 1], (unsigned)((j >> 1) & 1))) return false;
             pa_after();
             if (el) {
 #pragma unroll
@@ -164,13 +162,36 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const swl
                 umma_commit(&bars.pv_done[j & 1]);
             }
             __syncwarp();
+            return true;
+        };
+        bool ok = true;
+        if (n_tiles) { load(kg, kr, 0); load(vg, vr, 0); }
+        for (int j = 0; j < n_tiles; ++j) {
+            kg += kPaKeys * HD;
+            vg += kPaKeys * HD;
+            if (*failed || (j >= 2 && !mbar_wait_warp(&bars.s_full[j & 1], (unsigned)(((j - 2) >> 1) & 1)))) { ok = false; break; }
+            store(k_sm + (j & 1) * KV_BYTES, kr);
+            if (lane == 0) pa_arrive(&bars.k_full[j & 1]);
+            if (j + 1 < n_tiles) load(kg, kr, j + 1);
+            // (the product of tile j - 2 has read its values, and its probabilities in the region of tile j's scores)
+            if (j >= 2 && !mbar_wait_warp(&bars.pv_done[j & 1], (unsigned)(((j - 2) >> 1) & 1))) { ok = false; break; }
+            if (issues) {
+                if ((j == 0 && !mbar_wait_warp(&bars.q_ready, 0u)) || !mbar_wait_warp(&bars.k_full[j & 1], (unsigned)((j >> 1) & 1))) { ok = false; break; }
+                scores(j);
+            }
+            store(v_sm + (j & 1) * KV_BYTES, vr);
+            if (lane == 0) pa_arrive(&bars.v_full[j & 1]);
+            if (j + 1 < n_tiles) load(vg, vr, j + 1);
+            if (issues && j > 0 && !product(j - 1)) { ok = false; break; }
         }
-        if (el) {
-            if (!ok) fail(32);
-            umma_commit(&bars.o_done);   // also behind whatever was issued before a failure
+        if (issues) {
+            if (ok && n_tiles) ok = product(n_tiles - 1);
+            if (el) umma_commit(&bars.o_done);   // also behind whatever was issued before a failure
+            __syncwarp();
+            ok = mbar_wait_warp(&bars.o_done, 0u) && ok;   // tensor memory is not freed under MMAs in flight
         }
+        if (!ok && lane == 0) fail(31);
         __syncwarp();
-        if (!mbar_wait_warp(&bars.o_done, 0u) && el) fail(32);   // tensor memory is not freed under MMAs in flight
     } else {
         const int r = tid, row = row0 + r, i = min(row, rows - 1) / G;
         const bool row_ok = row < rows, f16 = a.dtype == SWLM_KV8_FP16;
@@ -206,7 +227,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const swl
         const unsigned lanes = (unsigned)(warp * 32) << 16;
         const float* ks = c.k_scale + head * (c.capacity >> block_shift);
         const float* vs = c.v_scale + head * (c.capacity >> block_shift);
-        float m_ref = -INFINITY, l_run = 0.f, v_ref = 0x1p-100f;
+        float m_ref = -INFINITY, l_run = 0.f, v_ref = 0x1p-100f, v_inv = 0x1p100f * kValueUnit;
         float kn[4], vn[4];   // the next tile's scales, of 16 keys each; 0 behind the last token
         auto scales = [&](int j) {
 #pragma unroll
@@ -249,7 +270,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const swl
             if (__any_sync(0xffffffffu, moves || v_top > v_ref)) {
                 float corr = moves ? pa_exp2(m_ref - top) : 1.f;   // 0 for a row's first keys
                 if (moves) { m_ref = top; l_run *= corr; }
-                if (v_top > v_ref) { corr *= v_ref / v_top; v_ref = v_top; }
+                if (v_top > v_ref) { corr *= v_ref / v_top; v_ref = v_top; v_inv = kValueUnit / v_top; }
                 if (j > 0) {   // the output so far: complete, and the next product waits for this warp
                     if (!mbar_wait_warp(&bars.pv_done[(j - 1) & 1], (unsigned)(((j - 1) >> 1) & 1))) { ok = false; break; }
                     pa_after();
@@ -270,22 +291,24 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const swl
             bool folds = !masked;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                unit[g] = vt[g] / v_ref * kValueUnit;
+                unit[g] = vt[g] * v_inv;
                 folds = folds && unit[g] >= kFoldUnit * kValueUnit;
             }
             if (folds) {
                 // the unit goes into the exponent, and out of the sum again
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    const float shift = __log2f(unit[g]) - base;
-                    float sum = 0.f;
+                    const float shift = log2_of(unit[g]) - base;
+                    const float2 fk2 = make_float2(fk[g], fk[g]), shift2 = make_float2(shift, shift);
+                    float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
-                        const float x = pa_exp2(fmaf(__uint_as_float(v[g * 16 + e]), fk[g], shift)), y = pa_exp2(fmaf(__uint_as_float(v[g * 16 + e + 1]), fk[g], shift));
-                        sum += x + y;
-                        v[g * 8 + e / 2] = pack_half(x, y);
+                        float2 x = fma2(make_float2(__uint_as_float(v[g * 16 + e]), __uint_as_float(v[g * 16 + e + 1])), fk2, shift2);
+                        x = make_float2(pa_exp2(x.x), pa_exp2(x.y));
+                        sum = add2(sum, x);
+                        v[g * 8 + e / 2] = pack_half(x.x, x.y);
                     }
-                    l_run += sum / unit[g];
+                    l_run += __fdividef(sum.x + sum.y, unit[g]);
                 }
             } else {
 #pragma unroll
