@@ -528,10 +528,12 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const swlm_kv8_c
                 sum += f * group_l[group + i];
                 all.x += f * v.x; all.y += f * v.y; all.z += f * v.z; all.w += f * v.w;
             }
+            m = top;
             l = sum;
             o = all;
         }
         if (!on) return;
+        if (p.q_shift && lane == 0) p.q_shift[head * p.row_tiles * TR + row] = row_shift_of(m, l);
         const int i = row / G;
         store_out(static_cast<unsigned short*>(a.out) + (int64_t)(part.start + i) * a.out_stride + (size_t)(h * G + row - i * G) * HD + d, o, l, a.dtype == SWLM_KV8_FP16);
         return;
@@ -582,102 +584,6 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const swlm_kv8_c
     }
 }
 
-// The weights of many rows: the scores are worked out again with the rows' totals known. A warp keeps the fragments of 16 tokens' keys in registers and
-// walks the rows that attend them; a CTA's rows go through shared memory as fp16, 32 at a time. Nothing is added across warps.
-constexpr int kAgainWarps = 4, kAgainRows = 32;
-template <int HD, int CODE>
-__global__ void __launch_bounds__(kAgainWarps * 32) kv8_weights_kernel(const swlm_kv8_cache c, const swlm_kv8_attend a, const RowsPlan p) {
-    constexpr int KS = HD / 16, PITCH = HD + 16;   // (rows 32 bytes further on than their length: the four rows of a phase meet different banks)
-    __shared__ __align__(16) __half qs[kAgainRows][PITCH];
-    __shared__ float row_factor[kAgainRows], row_m[kAgainRows], row_inv[kAgainRows];
-    __shared__ int row_limit[kAgainRows];
-    pdl_launch_dependents();
-    pdl_wait();
-    const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, G = a.heads / c.kv_heads;
-    const Kv8Part part = kv8_part(b, a.lengths, a.counts, a.starts, a.n, a.rows);
-    const int rows = part.count * G, span = min(a.max_len, c.capacity);
-    const int end = rows ? visible(part, part.count - 1, span) : 0, cta0 = (int)blockIdx.x * kAgainWarps * 16;
-    if (cta0 >= end) return;
-    const size_t head = (size_t)b * c.kv_heads + h;
-    const int base = cta0 + warp * 16;
-    const bool on = base < end;
-    unsigned kf[KS][4];
-    float k_scale = 0.f;
-    if (on) {
-        const unsigned char* keys = static_cast<const unsigned char*>(c.k) + (head * c.capacity + base) * HD;
-        k_scale = c.k_scale[head * (c.capacity / c.block) + base / c.block];
-#pragma unroll
-        for (int u = 0; u < HD / 64; ++u) {
-            const uint4 lo = *reinterpret_cast<const uint4*>(keys + g * HD + (t + 4 * u) * 16), hi = *reinterpret_cast<const uint4*>(keys + (g + 8) * HD + (t + 4 * u) * 16);
-            const unsigned lw[4] = {lo.x, lo.y, lo.z, lo.w}, hw[4] = {hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const unsigned x = prepared<CODE>(lw[w]), y = prepared<CODE>(hw[w]);
-                kf[u * 4 + w][0] = pair_of<CODE, 0>(x); kf[u * 4 + w][1] = pair_of<CODE, 0>(y);
-                kf[u * 4 + w][2] = pair_of<CODE, 1>(x); kf[u * 4 + w][3] = pair_of<CODE, 1>(y);
-            }
-        }
-    }
-    float sum[2] = {0.f, 0.f};   // of tokens g and g + 8, over this lane's columns
-    // the first query that attends the CTA's first slot
-    const int row_from = (int)min((long long)max((long long)cta0 - part.len, 0LL) * G, (long long)rows) / 8 * 8;
-    const unsigned short* q = static_cast<const unsigned short*>(a.q);
-    const bool f16 = a.dtype == SWLM_KV8_FP16;
-    for (int r0 = row_from; r0 < rows; r0 += kAgainRows) {
-        __syncthreads();
-        // four lanes per row, a quarter of it each
-#pragma unroll 1
-        for (int k = 0; k < kAgainRows / (kAgainWarps * 8); ++k) {
-            const int r = k * kAgainWarps * 8 + warp * 8 + g, row = r0 + r, i = min(row, rows - 1) / G;
-            unsigned frag[KS][2];
-            float down;
-            load_query<HD>(q + (int64_t)(part.start + i) * a.q_stride + (size_t)(h * G + min(row, rows - 1) - i * G) * HD, row < rows, f16, t, frag, down);
-            // kept in the order of the fragments: lane t's pairs of k-step s at s * 16 + 4 t
-#pragma unroll
-            for (int s = 0; s < KS; ++s) *reinterpret_cast<uint2*>(&qs[r][s * 16 + 4 * t]) = make_uint2(frag[s][0], frag[s][1]);
-            const int limit = row < rows ? visible(part, i, span) : 0;
-            float m = -INFINITY, l = 0.f;
-            if (t == 0) {
-                if (row < rows) {
-                    const int TR = 8 * p.tiles, tile = row / TR;
-                    const Parts parts = parts_of(p, part, b, c.batch, head, h, tile, span, G);
-                    const float* ml = p.part_ml + (parts.slot * TR + row - tile * TR) * 2;
-                    for (int s = 0; s < parts.count; ++s) m = fmaxf(m, ml[2 * TR * s]);
-                    for (int s = 0; s < parts.count; ++s) l += ml[2 * TR * s] == -INFINITY ? ml[2 * TR * s + 1] : exp2_of(ml[2 * TR * s] - m) * ml[2 * TR * s + 1];
-                }
-                row_factor[r] = down * (a.scale * kLog2e);
-                row_m[r] = m == -INFINITY ? 0.f : m;
-                row_inv[r] = l == 0.f ? 0.f : 1.f / l;
-                row_limit[r] = limit;
-            }
-        }
-        __syncthreads();
-        if (!on) continue;
-        for (int rt = 0; rt < min(kAgainRows, rows - r0); rt += 8) {
-            float s[4] = {};
-#pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                const uint2 v = *reinterpret_cast<const uint2*>(&qs[rt + g][k * 16 + 4 * t]);
-                mma(s, kf[k][0], kf[k][1], kf[k][2], kf[k][3], v.x, v.y);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int r = rt + 2 * t + (e & 1), slot = base + g + 8 * (e >> 1);
-                if (slot < row_limit[r]) sum[e >> 1] += exp2_of(s[e] * (row_factor[r] * k_scale) - row_m[r]) * row_inv[r];
-            }
-        }
-    }
-    if (!on) return;
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        float v = sum[e];
-        v += __shfl_xor_sync(0xffffffffu, v, 1);
-        v += __shfl_xor_sync(0xffffffffu, v, 2);
-        const int slot = base + g + 8 * e;
-        if (t == 0 && slot < end) c.weight[head * c.capacity + slot] += v;
-    }
-}
-
 constexpr size_t align16(size_t v) { return (v + 15) & ~(size_t)15; }
 
 RowsPlan rows_plan(const swlm_kv8_cache& c, const swlm_kv8_attend& a, size_t* bytes) {
@@ -704,7 +610,7 @@ RowsPlan rows_plan(const swlm_kv8_cache& c, const swlm_kv8_attend& a, size_t* by
         several = p.stream && units > groups;
     }
     const size_t places = p.splits ? (size_t)groups * p.splits : (size_t)groups + p.ctas;
-    p.ml_always = a.accumulate != 0;
+    p.ml_always = a.accumulate && p.rows <= kSaveRows;
     // a group of lanes takes up to eight parts at once: as many groups as a row with the most parts has such turns
     const long long most = p.splits ? p.splits : std::min<long long>(units / groups, p.ctas / groups + 2);
     p.join_groups = most > 32 ? 8 : most > 16 ? 4 : most > 8 ? 2 : 1;
@@ -712,13 +618,18 @@ RowsPlan rows_plan(const swlm_kv8_cache& c, const swlm_kv8_attend& a, size_t* by
     char* base = static_cast<char*>(a.scratch);
     auto take = [&](size_t n) { char* q = base + at; at += align16(n); return q; };
     if (several) p.part_o = reinterpret_cast<float*>(take(places * 8 * p.tiles * c.head_dim * 4));
-    if (several || a.accumulate) {
+    if (several || p.ml_always) {
         p.part_ml = reinterpret_cast<float*>(take(places * 8 * p.tiles * 8));
         if (p.stream) p.table = reinterpret_cast<int*>(take(((size_t)c.batch + 1) * 4));
     }
     if (a.accumulate && p.rows <= kSaveRows) {
         p.pitch = p.rows <= 2 ? 2 : (p.rows + 3) / 4 * 4;
         p.scores = reinterpret_cast<float*>(take((size_t)c.batch * c.kv_heads * p.span * p.pitch * 4));
+    } else if (a.accumulate) {
+        const size_t rows = (size_t)groups * kPromptRows;
+        p.q16 = reinterpret_cast<__half*>(take(rows * c.head_dim * 2));
+        p.q_factor = reinterpret_cast<float*>(take(rows * 4));
+        p.q_shift = reinterpret_cast<float*>(take(rows * 4));
     }
     *bytes = at;
     return p;
@@ -748,11 +659,7 @@ int launch_rows(const swlm_kv8_cache& c, const swlm_kv8_attend& a, const RowsPla
         const cudaError_t j = launch_k(kv8_join_kernel<HD>, dim3((unsigned)(join + slots), (unsigned)c.kv_heads, (unsigned)c.batch), dim3(kJoinThreads), 0, s, c, a, p, join);
         if (j != cudaSuccess) return cuda_fail(j, "kv8 join launch");
     }
-    if (a.accumulate && !p.pitch) {
-        constexpr int per = kAgainWarps * 16;
-        const cudaError_t w = launch_k(kv8_weights_kernel<HD, CODE>, dim3((unsigned)((span + per - 1) / per), (unsigned)c.kv_heads, (unsigned)c.batch), dim3(kAgainWarps * 32), 0, s, c, a, p);
-        if (w != cudaSuccess) return cuda_fail(w, "kv8 weights launch");
-    }
+    if (p.q16) return launch_kv8_prompt_weights(c, a, p, status, s);
     return SWLM_OK;
 }
 

@@ -29,6 +29,11 @@ struct RowsPlan {
     float* part_o;  // [places][8 * tiles][head_dim], not normalised; places: (sequence, KV head, tile) + CTA, or of many rows * splits + run
     float* part_ml; // [places][8 * tiles][2]: reference maximum (log2), sum
     float* scores;  // [batch][kv_heads][span][pitch], log2
+    // many rows whose weights are added: the shifted queries as fp16 in tiles of 64 rows, [batch][kv_heads][tiles][head_dim / 64][64][64], swizzled as the
+    // products read them, and per row what turns a product into log2 of a weight: times the factor, times the key's scale, plus the shift
+    __half* q16;
+    float* q_factor;  // [batch][kv_heads][row_tiles * 128]
+    float* q_shift;
     int* table;     // [batch + 1]: units before each sequence, and of all
 };
 
@@ -53,6 +58,10 @@ template <int CODE, int HIGH> __device__ __forceinline__ unsigned pair_of(unsign
     else asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(v) : "r"(word));
     return v;
 }
+
+// What is added to a score (log2) to make it log2 of a weight: minus the row's maximum and the logarithm of its sum. A row that attends
+// nothing has no weights.
+__device__ __forceinline__ float row_shift_of(float m, float l) { return l == 0.f ? -INFINITY : -((m == -INFINITY ? 0.f : m) + log2f(l)); }
 
 // Four results of a row with sum l.
 __device__ __forceinline__ void store_out(unsigned short* dst, const float4& o, float l, bool f16) {
@@ -126,5 +135,6 @@ constexpr int kPromptRows = 128, kPromptKeys = 64;
 }  // namespace kv8
 
 int kv8_prompt_init();
+int launch_kv8_prompt_weights(const swlm_kv8_cache& c, const swlm_kv8_attend& a, const kv8::RowsPlan& p, int* status, cudaStream_t s);
 int launch_kv8_prompt(const swlm_kv8_cache& c, const swlm_kv8_attend& a, const kv8::RowsPlan& p, int* status, cudaStream_t s);
 }  // namespace swlm

@@ -55,6 +55,11 @@ __device__ __forceinline__ float2 add2(const float2& a, const float2& b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)));
     return bits_pair(r);
 }
+__device__ __forceinline__ float2 mul2(const float2& a, const float2& b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)));
+    return bits_pair(r);
+}
 __device__ __forceinline__ float log2_of(float x) { float y; asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
 template <int HD> __host__ __device__ constexpr size_t prompt_smem() { return (size_t)kPaRows * HD * 2 + 4 * kPaKeys * HD * 2 + 1024; }
@@ -207,6 +212,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const swl
                 const unsigned m = __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
                 top = max(top, max(m & 0xFFFFu, m >> 16));
             }
+            const bool keeps = p.q16 && split == 0;   // for the launch that adds the weights
             float up;
             row_shift(f16 ? __half2float(__ushort_as_half((unsigned short)top)) : __uint_as_float(top << 16), up, factor);
             factor *= a.scale * kLog2e;
@@ -217,8 +223,11 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const swl
                 uint4 v;
                 v.x = pack_half(x[0] * up, x[1] * up); v.y = pack_half(x[2] * up, x[3] * up);
                 v.z = pack_half(x[4] * up, x[5] * up); v.w = pack_half(x[6] * up, x[7] * up);
-                *reinterpret_cast<uint4*>(q_sm + (d >> 6) * Q_HALF + r * 128 + ((((d >> 3) & 7) ^ (r & 7)) << 4)) = v;
+                const int at = r * 128 + ((((d >> 3) & 7) ^ (r & 7)) << 4);
+                *reinterpret_cast<uint4*>(q_sm + (d >> 6) * Q_HALF + at) = v;
+                if (keeps) *reinterpret_cast<uint4*>(reinterpret_cast<unsigned char*>(p.q16) + (((head * p.row_tiles + tile) * 2 + (r >> 6)) * HALVES + (d >> 6)) * 8192 + (at & 8191)) = v;
             }
+            if (keeps) p.q_factor[(head * p.row_tiles + tile) * kPaRows + r] = row_ok ? factor : 0.f;
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) pa_arrive(&bars.q_ready);
@@ -342,6 +351,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const swl
             const size_t at = ((head * p.row_tiles + tile) * p.splits + split) * kPaRows + r;
             const float unit = v_ref * (1.f / kValueUnit);
             if (row_ok && (!whole || p.ml_always)) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m_ref, l_run);
+            if (p.q_shift && (whole || !row_ok)) p.q_shift[(head * p.row_tiles + tile) * kPaRows + r] = row_ok ? row_shift_of(m_ref, l_run) : -INFINITY;
             unsigned short* dst = static_cast<unsigned short*>(a.out) + (int64_t)(part.start + i) * a.out_stride + (size_t)(h * G + min(row, rows - 1) - i * G) * HD;
 #pragma unroll 1
             for (int d = 0; d < HD; d += 16) {
@@ -365,6 +375,164 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const swl
     if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(kTmemCols) : "memory");
 }
 
+// The weights of many rows: weight_j += sum over rows i of exp2(s_ij + shift_i), with the rows' totals known. A CTA has 128 keys, the rows of the products
+// (S^T = K Q^T: a thread per key, so that nothing is added across threads), and walks the row tiles that attend them. Four slots: the
+// queries of a tile, their factors and shifts come as bulk copies while the tiles before are multiplied and summed.
+constexpr int kWeightKeys = 128, kWeightRows = 64, kWeightSlots = 4, kWeightThreads = kWeightKeys + 32;
+struct WeightBars {
+    unsigned long long k_ready, o_done, q_full[kWeightSlots], s_full[kWeightSlots], s_free[kWeightSlots];
+    unsigned tmem;
+    int failed;
+};
+template <int HD> __host__ __device__ constexpr size_t weights_smem() { return (size_t)kWeightKeys * HD * 2 + (size_t)kWeightSlots * kWeightRows * HD * 2 + 1024; }
+
+template <int HD, int CODE>
+__global__ void __launch_bounds__(kWeightThreads, 2) kv8_weights_kernel(const swlm_kv8_cache c, const swlm_kv8_attend a, const RowsPlan p, int* status) {
+    constexpr int HALVES = HD / 64;
+    constexpr unsigned K_HALF = kWeightKeys * 128, Q_HALF = kWeightRows * 128, Q_BYTES = HALVES * Q_HALF;
+    constexpr unsigned kTmemCols = kWeightSlots * 64;
+    extern __shared__ __align__(1024) unsigned char weights_raw[];
+    unsigned char* const k_sm = weights_raw + ((1024 - (smem_u32(weights_raw) & 1023)) & 1023);
+    unsigned char* const q_sm = k_sm + HALVES * K_HALF;
+    __shared__ __align__(16) float rows_sm[kWeightSlots][2][kWeightRows];   // factors, shifts
+    __shared__ __align__(8) WeightBars bars;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int b = blockIdx.z, h = blockIdx.y, G = a.heads / c.kv_heads, span = min(a.max_len, c.capacity);
+    const Kv8Part part = kv8_part(b, a.lengths, a.counts, a.starts, a.n, a.rows);
+    const int rows = part.count * G, end = rows ? visible(part, part.count - 1, span) : 0, key0 = (int)blockIdx.x * kWeightKeys;
+    if (key0 >= end) return;
+    const size_t head = (size_t)b * c.kv_heads + h;
+    // rows from (key - length) * G on attend a key; the first tile with one that attends this CTA's first key
+    const int tile0 = (int)(max((long long)key0 - part.len, 0LL) * G / kWeightRows), tiles = (rows + kWeightRows - 1) / kWeightRows - tile0;
+    volatile int* const failed = &bars.failed;
+    auto fail = [&](int code) { atomicExch_system(status, code); *failed = 1; };
+    if (tid == 0) {
+        mbar_init(&bars.k_ready, 4);
+        mbar_init(&bars.o_done, 1);
+        for (int i = 0; i < kWeightSlots; ++i) { mbar_init(&bars.q_full[i], 1); mbar_init(&bars.s_full[i], 1); mbar_init(&bars.s_free[i], 4); }
+        bars.failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        __syncwarp();
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem)), "r"(kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pa_before();
+    __syncthreads();
+    pa_after();
+    const unsigned tm = bars.tmem;
+
+    if (warp == 4) {
+        // Tile t of this CTA (slot t & 3): its copies are asked for behind s_free(t - 4), so its slot, rows and scores' region are free then
+        const bool el = elect_one();
+        const unsigned kd = umma_desc_lo(smem_u32(k_sm)), qd = umma_desc_lo(smem_u32(q_sm));
+        const unsigned char* q = reinterpret_cast<const unsigned char*>(p.q16) + (head * p.row_tiles * 2 + tile0) * Q_BYTES;
+        const float* factor = p.q_factor + head * p.row_tiles * kPaRows + (size_t)tile0 * kWeightRows;
+        const float* shift = p.q_shift + head * p.row_tiles * kPaRows + (size_t)tile0 * kWeightRows;
+        int asked = 0;
+        auto ask = [&]() {
+            if (el) {
+                const int slot = asked & (kWeightSlots - 1);
+                const unsigned bar = smem_u32(&bars.q_full[slot]);
+                mbar_expect(bar, Q_BYTES + 2 * kWeightRows * 4);
+                bulk_load(smem_u32(q_sm) + slot * Q_BYTES, q + (size_t)asked * Q_BYTES, Q_BYTES, bar);
+                bulk_load(smem_u32(rows_sm[slot][0]), factor + asked * kWeightRows, kWeightRows * 4, bar);
+                bulk_load(smem_u32(rows_sm[slot][1]), shift + asked * kWeightRows, kWeightRows * 4, bar);
+            }
+            __syncwarp();
+            ++asked;
+        };
+        while (asked < tiles && asked < kWeightSlots - 1) ask();
+        bool ok = mbar_wait_warp(&bars.k_ready, 0u);
+        for (int t = 0; t < tiles && ok; ++t) {
+            const int slot = t & (kWeightSlots - 1);
+            if (*failed || !mbar_wait_warp(&bars.q_full[slot], (unsigned)((t / kWeightSlots) & 1))) { ok = false; break; }
+            pa_after();
+            if (el) {
+#pragma unroll
+                for (int kk = 0; kk < HD / 16; ++kk)
+                    pa_mma_ss(tm + slot * 64u, kd + (kk >> 2) * (K_HALF / 16) + 2 * (kk & 3), qd + slot * (Q_BYTES / 16) + (kk >> 2) * (Q_HALF / 16) + 2 * (kk & 3),
+                              pa_idesc(kWeightRows, false, false), kk > 0 ? 1u : 0u);
+                umma_commit(&bars.s_full[slot]);
+            }
+            __syncwarp();
+            if (asked < tiles) {
+                // the slot of tile t + 3, which tile t - 1 had
+                if (t > 0 && !mbar_wait_warp(&bars.s_free[(t - 1) & (kWeightSlots - 1)], (unsigned)(((t - 1) / kWeightSlots) & 1))) { ok = false; break; }
+                ask();
+            }
+        }
+        if (el) umma_commit(&bars.o_done);
+        __syncwarp();
+        ok = mbar_wait_warp(&bars.o_done, 0u) && ok;   // tensor memory is not freed under MMAs in flight, nor shared memory left under copies
+        for (int t = max(0, asked - kWeightSlots); t < asked; ++t) ok = mbar_wait_warp(&bars.q_full[t & (kWeightSlots - 1)], (unsigned)((t / kWeightSlots) & 1)) && ok;
+        if (!ok && lane == 0) fail(34);
+        __syncwarp();
+    } else {
+        // ---- this CTA's keys ----
+        constexpr int PIECES = HD / 16, STEP = kWeightKeys / PIECES;   // (threads of a token, tokens of a turn)
+        const int piece = tid % PIECES, row = tid / PIECES, chunk = piece * 2 & 7;
+        const unsigned char* src = static_cast<const unsigned char*>(c.k) + (head * c.capacity + key0) * HD + piece * 16;
+        const unsigned off = (piece >> 2) * K_HALF;
+#pragma unroll 4
+        for (int r = row; r < kWeightKeys; r += STEP) {
+            const uint4 v = key0 + r < end ? __ldg(reinterpret_cast<const uint4*>(src + (size_t)r * HD)) : make_uint4(0, 0, 0, 0);
+            const unsigned w[4] = {prepared<CODE>(v.x), prepared<CODE>(v.y), prepared<CODE>(v.z), prepared<CODE>(v.w)};
+            *reinterpret_cast<uint4*>(k_sm + off + r * 128 + ((chunk ^ (r & 7)) << 4)) = make_uint4(pair_of<CODE, 0>(w[0]), pair_of<CODE, 1>(w[0]), pair_of<CODE, 0>(w[1]), pair_of<CODE, 1>(w[1]));
+            *reinterpret_cast<uint4*>(k_sm + off + r * 128 + (((chunk + 1) ^ (r & 7)) << 4)) = make_uint4(pair_of<CODE, 0>(w[2]), pair_of<CODE, 1>(w[2]), pair_of<CODE, 0>(w[3]), pair_of<CODE, 1>(w[3]));
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) pa_arrive(&bars.k_ready);
+        // ---- a thread per key ----
+        const int key = key0 + tid;
+        const float scale = key < end ? c.k_scale[head * (c.capacity / c.block) + key / c.block] : 0.f;
+        const float2 scale2 = make_float2(scale, scale);
+        const long long first = ((long long)key - part.len) * G - (long long)tile0 * kWeightRows;   // the first row, from tile0 on, that attends it
+        const unsigned lanes = (unsigned)(warp * 32) << 16;
+        float2 sum = make_float2(0.f, 0.f);
+        bool ok = true;
+        for (int t = 0; t < tiles; ++t) {
+            const int slot = t & (kWeightSlots - 1);
+            const unsigned phase = (unsigned)((t / kWeightSlots) & 1);
+            if (!mbar_wait_warp(&bars.q_full[slot], phase) || !mbar_wait_warp(&bars.s_full[slot], phase)) { ok = false; break; }
+            pa_after();
+            unsigned v[64];
+            pa_ld32(tm + lanes + slot * 64u, v);
+            pa_ld32(tm + lanes + slot * 64u + 32u, v + 32);
+            pa_wait_ld();
+            const bool masked = !__all_sync(0xffffffffu, first <= (long long)t * kWeightRows);
+#pragma unroll
+            for (int e = 0; e < kWeightRows; e += 4) {
+                const float4 f = *reinterpret_cast<const float4*>(&rows_sm[slot][0][e]), m = *reinterpret_cast<const float4*>(&rows_sm[slot][1][e]);
+                float2 x = fma2(mul2(make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), scale2), make_float2(f.x, f.y), make_float2(m.x, m.y));
+                float2 y = fma2(mul2(make_float2(__uint_as_float(v[e + 2]), __uint_as_float(v[e + 3])), scale2), make_float2(f.z, f.w), make_float2(m.z, m.w));
+                x = make_float2(pa_exp2(x.x), pa_exp2(x.y));
+                y = make_float2(pa_exp2(y.x), pa_exp2(y.y));
+                if (masked) {
+                    const long long at = (long long)t * kWeightRows + e;
+                    if (at < first) x.x = 0.f;
+                    if (at + 1 < first) x.y = 0.f;
+                    if (at + 2 < first) y.x = 0.f;
+                    if (at + 3 < first) y.y = 0.f;
+                }
+                sum = add2(sum, add2(x, y));
+            }
+            pa_before();
+            __syncwarp();
+            if (lane == 0) pa_arrive(&bars.s_free[slot]);
+        }
+        if (!ok) fail(35);
+        else if (key < end) c.weight[head * c.capacity + key] += sum.x + sum.y;
+    }
+    pa_before();
+    __syncthreads();
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(kTmemCols) : "memory");
+}
+
 template <int HD, int CODE>
 int launch_prompt(const swlm_kv8_cache& c, const swlm_kv8_attend& a, const RowsPlan& p, int* status, cudaStream_t s) {
     const cudaError_t e = launch_k(kv8_prompt_kernel<HD, CODE>, dim3((unsigned)(p.row_tiles * p.splits), (unsigned)c.kv_heads, (unsigned)c.batch), dim3(kPromptThreads),
@@ -372,7 +540,15 @@ int launch_prompt(const swlm_kv8_cache& c, const swlm_kv8_attend& a, const RowsP
     return e == cudaSuccess ? SWLM_OK : cuda_fail(e, "kv8 prompt attention launch");
 }
 template <int HD, int CODE>
+int launch_weights(const swlm_kv8_cache& c, const swlm_kv8_attend& a, const RowsPlan& p, int* status, cudaStream_t s) {
+    const int span = std::min(a.max_len, c.capacity);
+    const cudaError_t e = launch_k(kv8_weights_kernel<HD, CODE>, dim3((unsigned)((span + kWeightKeys - 1) / kWeightKeys), (unsigned)c.kv_heads, (unsigned)c.batch), dim3(kWeightThreads),
+                                   weights_smem<HD>(), s, c, a, p, status);
+    return e == cudaSuccess ? SWLM_OK : cuda_fail(e, "kv8 prompt weights launch");
+}
+template <int HD, int CODE>
 int init_prompt() {
+    SWLM_CUDA(cudaFuncSetAttribute(kv8_weights_kernel<HD, CODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)weights_smem<HD>()));
     SWLM_CUDA(cudaFuncSetAttribute(kv8_prompt_kernel<HD, CODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prompt_smem<HD>()));
     return SWLM_OK;
 }
@@ -385,6 +561,11 @@ int kv8_prompt_init() {
     if (!rc) rc = init_prompt<64, SWLM_KV8_INT8>();
     if (!rc) rc = init_prompt<64, SWLM_KV8_E4M3>();
     return rc;
+}
+
+int launch_kv8_prompt_weights(const swlm_kv8_cache& c, const swlm_kv8_attend& a, const RowsPlan& p, int* status, cudaStream_t s) {
+    if (c.head_dim == 128) return c.code == SWLM_KV8_INT8 ? launch_weights<128, SWLM_KV8_INT8>(c, a, p, status, s) : launch_weights<128, SWLM_KV8_E4M3>(c, a, p, status, s);
+    return c.code == SWLM_KV8_INT8 ? launch_weights<64, SWLM_KV8_INT8>(c, a, p, status, s) : launch_weights<64, SWLM_KV8_E4M3>(c, a, p, status, s);
 }
 
 int launch_kv8_prompt(const swlm_kv8_cache& c, const swlm_kv8_attend& a, const RowsPlan& p, int* status, cudaStream_t s) {
