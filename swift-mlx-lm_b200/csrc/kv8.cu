@@ -3,34 +3,91 @@
 // append   s = max(s0, max |x| / top), c = round(x / s) with IEEE quotients, so that a code is the same whatever the launch. One CTA per
 //          (block of tokens, KV head, keys or values): the new values of the block stay in registers between the search for the largest and
 //          the rounding, each is read once.
-// evict    select: one CTA per (sequence, KV head) finds the `keep` largest keys by radix selection and pairs the free slots below `keep`
+// evict    select: one cluster of CTAs per (sequence, KV head) finds the `keep` largest keys by radix selection and pairs the free slots below `keep`
 //          with the tokens that stay from behind. move: one CTA per (block below `keep`, KV head, keys or values) gathers what the
 //          block takes, scales it anew and stores it. Only slots from `keep` on are sources of another block's slots and only slots below
 //          `keep` are written, so that the blocks need no order among them, also in place; the scales of the sources, which the last block
 //          may share with slots that are written, are taken along by the first kernel.
+#include <cooperative_groups.h>
 #include <cuda_fp8.h>
 
 #include <algorithm>
 #include <climits>
 
-#include "kv8.h"
+#include "kv8_device.cuh"
 #include "swlm_runtime.h"
 
+namespace cg = cooperative_groups;
+
 namespace swlm {
+using namespace kv8;
 namespace {
 
 constexpr float kTopInt8 = 127.f, kTopE4m3 = 448.f;
 
 template <int CODE> __device__ __forceinline__ constexpr float kv8_top() { return CODE == SWLM_KV8_INT8 ? kTopInt8 : kTopE4m3; }
 
-// the nearest code of y = x / s, as a byte (|y| <= top but for the last place; the clamp is for scales that are subnormal)
+// A code is round(x / s) of the IEEE quotient, which costs some twenty instructions. The product with 1 / s is off by 2^-21 of itself at most (also with the
+// factor of an old scale in it), so that only a value within that of a border between two codes needs the quotient.
+
+// the code of the quotient y, as a byte (|y| <= top but for the last place; the clamp is for scales that are subnormal)
 template <int CODE> __device__ __forceinline__ unsigned kv8_code(float y) {
     if (CODE == SWLM_KV8_INT8) return (unsigned)__float2int_rn(fminf(fmaxf(y, -kTopInt8), kTopInt8)) & 0xFFu;
     return (unsigned)__nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
 }
-template <int CODE> __device__ __forceinline__ float kv8_number(unsigned byte) {
-    if (CODE == SWLM_KV8_INT8) return (float)(int)(signed char)byte;
-    return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)));
+// The codes of four values whose quotients are about y, as a word; `sure`: none of them is next to a border.
+template <int CODE> __device__ __forceinline__ unsigned kv8_codes4(const float (&y)[4], bool& sure) {
+    if (CODE == SWLM_KV8_INT8) {
+        // the low byte of 1.5 * 2^23 + y is y rounded to an integer, ties to even
+        float far = 0.f;
+        unsigned k[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float m = y[e] + 12582912.f;
+            k[e] = __float_as_uint(m);
+            far = fmaxf(far, fabsf(y[e] - (m - 12582912.f)));
+        }
+        sure = sure && far < 0.4998f;   // 127 * 2^-21 = 0.00006 from the border
+        return __byte_perm(__byte_perm(k[0], k[1], 0x0040), __byte_perm(k[2], k[3], 0x0040), 0x5410);
+    }
+    unsigned lo, hi;
+    constexpr float down = 1.f - 0x1p-20f, up = 1.f + 0x1p-20f;
+    asm("{\n\t.reg .b16 a, b;\n\tcvt.rn.satfinite.e4m3x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 b, %4, %3;\n\tmov.b32 %0, {a, b};\n\t}"
+        : "=r"(lo) : "f"(y[0] * down), "f"(y[1] * down), "f"(y[2] * down), "f"(y[3] * down));
+    asm("{\n\t.reg .b16 a, b;\n\tcvt.rn.satfinite.e4m3x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 b, %4, %3;\n\tmov.b32 %0, {a, b};\n\t}"
+        : "=r"(hi) : "f"(y[0] * up), "f"(y[1] * up), "f"(y[2] * up), "f"(y[3] * up));
+    sure = sure && lo == hi;
+    return lo;
+}
+// Scales whose inverse and products are normal numbers.
+__device__ __forceinline__ bool kv8_ordinary(float s) { return s > 0x1p-100f && s < 0x1p100f; }
+
+// a word's codes as numbers
+template <int CODE> __device__ __forceinline__ void kv8_numbers4(unsigned word, float (&x)[4]) {
+    if (CODE == SWLM_KV8_INT8) {
+        const unsigned u = word ^ 0x80808080u;   // c + 128, the low byte of 2^23 + u
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7650 + e)) - (8388608.f + 128.f);
+    } else {
+        const __half2 a = __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(word & 0xFFFFu), __NV_E4M3)), b = __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(word >> 16), __NV_E4M3));
+        const float2 p = __half22float2(a), q = __half22float2(b);
+        x[0] = p.x; x[1] = p.y; x[2] = q.x; x[3] = q.y;
+    }
+}
+// The word's codes, held at scale `from`, at scale s (inv: 1 / s; ordinary: both scales are).
+template <int CODE> __device__ __forceinline__ unsigned kv8_again(unsigned word, float from, float s, float factor, bool ordinary) {
+    float x[4], y[4];
+    kv8_numbers4<CODE>(word, x);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = x[e] * factor;
+    bool sure = ordinary;
+    unsigned out = kv8_codes4<CODE>(y, sure);
+    if (!sure) {
+        out = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out |= kv8_code<CODE>(__fdiv_rn(x[e] * from, s)) << (8 * e);
+    }
+    return out;
 }
 
 // Largest of a CTA's unsigned numbers, to all of its threads.
@@ -93,7 +150,8 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const swlm_k
     const float s = finite ? fmaxf(s0, __fdiv_rn(half_bits(top, f16), kv8_top<CODE>())) : kKv8NaN;
     if (blockDim.x == 32) __syncwarp();
     if (tid == 0) *scale = s;
-    const bool grows = old && finite && s > s0;
+    const bool grows = old && finite && s > s0, ordinary = kv8_ordinary(s);
+    const float inv = 1.f / s;
 #pragma unroll
     for (int u = 0; u < kAppendUnits; ++u) {
         const int i = tid + u * (int)blockDim.x;
@@ -102,7 +160,21 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const swlm_k
             unsigned out[2] = {0, 0};
             if (finite && s > 0.f)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) out[e >> 2] |= kv8_code<CODE>(__fdiv_rn(half_bits((w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu, f16), s)) << (8 * (e & 3));
+                for (int k = 0; k < 2; ++k) {
+                    float v[4], y[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        v[e] = half_bits((w[2 * k + (e >> 1)] >> (16 * (e & 1))) & 0xFFFFu, f16);
+                        y[e] = v[e] * inv;
+                    }
+                    bool sure = ordinary;
+                    out[k] = kv8_codes4<CODE>(y, sure);
+                    if (!sure) {
+                        out[k] = 0;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) out[k] |= kv8_code<CODE>(__fdiv_rn(v[e], s)) << (8 * e);
+                    }
+                }
             *reinterpret_cast<uint2*>(codes + (size_t)(low - base + i / per) * c.head_dim + i % per * 8) = make_uint2(out[0], out[1]);
         }
     }
@@ -110,12 +182,8 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const swlm_k
         for (int i = tid; i < old * per; i += blockDim.x) {
             uint2* at = reinterpret_cast<uint2*>(codes + (size_t)i * 8);
             const uint2 was = *at;
-            const unsigned w[2] = {was.x, was.y};
-            unsigned out[2] = {0, 0};
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                out[e >> 2] |= kv8_code<CODE>(__fdiv_rn(kv8_number<CODE>((w[e >> 2] >> (8 * (e & 3))) & 0xFFu) * s0, s)) << (8 * (e & 3));
-            *at = make_uint2(out[0], out[1]);
+            const bool both = ordinary && kv8_ordinary(s0);
+            *at = make_uint2(kv8_again<CODE>(was.x, s0, s, s0 * inv, both), kv8_again<CODE>(was.y, s0, s, s0 * inv, both));
         }
     if (which == 0)
         for (int slot = low + tid; slot < high; slot += blockDim.x) {
@@ -136,9 +204,9 @@ __global__ void kv8_lengths_kernel(int batch, const int32_t* in, const int32_t* 
 
 // ---- evict -----------------------------------------------------------------------------------------------------------------
 
-constexpr int kSelectThreads = 1024, kSelectWarps = kSelectThreads / 32;
+constexpr int kSelectCtas = 8, kSelectThreads = 512, kSelectWarps = kSelectThreads / 32;   // CTAs of a cluster
 constexpr int kDigitBits = 11, kDigits = 1 << kDigitBits;
-constexpr int kCachedKeys = 48 * 1024;   // keys that stay in shared memory between the passes (192 KB of 227)
+constexpr int kCachedKeys = 24 * 1024;   // keys of a CTA that stay in shared memory between the passes
 
 // Scratch of one (sequence, KV head): where slot j < keep comes from (j itself, or ~i: the i-th of the tokens that move), the slots of the
 // tokens that move and the scales of their keys and values.
@@ -158,42 +226,58 @@ __device__ __forceinline__ unsigned evict_key(float w, int pos, int sink, long l
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// One cluster per (sequence, KV head); its CTAs have equal runs of slots. The digits' counts of all of them are added up by each.
 template <bool CACHED>
-__global__ void __launch_bounds__(kSelectThreads) kv8_select_kernel(const swlm_kv8_cache c, const swlm_kv8_evict a) {
+__global__ void __cluster_dims__(kSelectCtas, 1, 1) __launch_bounds__(kSelectThreads) kv8_select_kernel(const swlm_kv8_cache c, const swlm_kv8_evict a) {
     extern __shared__ unsigned keys[];
-    __shared__ unsigned hist[kDigits];
-    __shared__ int seg[3][kSelectWarps];
+    __shared__ unsigned hist[2][kDigits], all[kDigits];
+    __shared__ int seg[3][kSelectWarps], counted[3];   // ties, free slots, moving tokens: of a warp, of the CTA
     __shared__ unsigned found_digit, found_above;
     pdl_launch_dependents();
     pdl_wait();
-    const int b = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int b = blockIdx.y, h = blockIdx.x / kSelectCtas, rank = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int len = min(min(a.lengths[b], a.max_len), c.capacity), keep = a.keep;
-    if (len <= keep) return;   // nothing leaves: the second kernel does not look at the plan
+    if (len <= keep) return;   // (the whole cluster) nothing leaves: the second kernel does not look at the plan
     const size_t head = (size_t)b * c.kv_heads + h;
     const float* weight = c.weight + head * c.capacity;
     const int32_t* pos = c.slot_pos + head * c.capacity;
     const long long recent_from = (long long)a.seen[b] - a.recent;
+    // this CTA's slots: first .. last - 1
+    const int share = (len + kSelectCtas * 32 - 1) / (kSelectCtas * 32) * 32, first = min(rank * share, len), last = min(first + share, len);
     auto key_of = [&](int i) { return evict_key(weight[i], pos[i], a.sink, recent_from); };
-    if (CACHED)
-        for (int i = tid; i < len; i += kSelectThreads) keys[i] = key_of(i);
-    auto key = [&](int i) { return CACHED ? keys[i] : key_of(i); };
+    for (int i = tid; i < 2 * kDigits; i += kSelectThreads) hist[0][i] = 0;
+    if (CACHED) {
+#pragma unroll 4
+        for (int i = first + tid; i < last; i += kSelectThreads) keys[i - first] = key_of(i);
+    }
+    auto key = [&](int i) { return CACHED ? keys[i - first] : key_of(i); };
+    __syncthreads();
 
     // radix selection of the keep-th largest key, from the top digit down
     unsigned prefix = 0, mask = 0;
-    int want = keep;   // how many keys are still to be found among those that share the prefix
-    for (int shift = 32 - kDigitBits; ; shift = max(shift - kDigitBits, 0)) {
-        for (int i = tid; i < kDigits; i += kSelectThreads) hist[i] = 0;
-        __syncthreads();
-        for (int i = tid; i < len; i += kSelectThreads) {
+    int want = keep, pass = 0;   // how many keys are still to be found among those that share the prefix
+    for (int shift = 32 - kDigitBits; ; shift = max(shift - kDigitBits, 0), ++pass) {
+        unsigned* const mine = hist[pass & 1];
+        for (int i = first + tid; i < last; i += kSelectThreads) {
             const unsigned k = key(i);
-            if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (kDigits - 1)], 1u);
+            if ((k & mask) == prefix) atomicAdd(&mine[(k >> shift) & (kDigits - 1)], 1u);
+        }
+        cluster.sync();   // (what the pass before counted has been read by all)
+        for (int i = tid; i < kDigits; i += kSelectThreads) {
+            unsigned sum = 0;
+#pragma unroll
+            for (int r = 0; r < kSelectCtas; ++r) sum += cluster.map_shared_rank(mine, r)[i];
+            all[i] = sum;
+            hist[(pass + 1) & 1][i] = 0;
         }
         __syncthreads();
         if (warp == 0) {   // lane l has the 64 digits from the (31 - l)-th group on: counts from the top down
             constexpr int PER = kDigits / 32;
-            const int first = (31 - lane) * PER;
+            const int group = (31 - lane) * PER;
             unsigned sum = 0;
-            for (int i = 0; i < PER; ++i) sum += hist[first + i];
+#pragma unroll 8
+            for (int i = 0; i < PER; ++i) sum += all[group + (i + lane) % PER];   // (lanes meet different banks)
             unsigned above = sum;
             for (int o = 1; o < 32; o <<= 1) {
                 const unsigned v = __shfl_up_sync(0xffffffffu, above, o);
@@ -201,8 +285,8 @@ __global__ void __launch_bounds__(kSelectThreads) kv8_select_kernel(const swlm_k
             }
             above -= sum;   // keys of higher groups
             if (above < (unsigned)want && above + sum >= (unsigned)want) {
-                int d = first + PER - 1;
-                while (above + hist[d] < (unsigned)want) above += hist[d--];
+                int d = group + PER - 1;
+                while (above + all[d] < (unsigned)want) above += all[d--];
                 found_digit = (unsigned)d;
                 found_above = above;
             }
@@ -212,26 +296,39 @@ __global__ void __launch_bounds__(kSelectThreads) kv8_select_kernel(const swlm_k
         prefix = (prefix & ~digits) | found_digit << shift;   // (the last digit overlaps the one before it, with the same bits there)
         mask |= digits;
         want -= (int)found_above;
-        __syncthreads();
         if (shift == 0) break;
     }
     const unsigned limit = prefix;   // keys above it stay, and the first `want` of those equal to it
 
     // a run of slots per warp: ties first, then free slots below `keep` and staying ones from it on, each numbered in slot order
-    const int run = (len + kSelectThreads - 1) / kSelectThreads * 32, from = min(warp * run, len), to = min(from + run, len);
+    const int run = (last - first + kSelectThreads - 1) / kSelectThreads * 32, from = min(first + warp * run, last), to = min(from + run, last);
     const unsigned below = (1u << lane) - 1u;
+    auto before = [&](int what, int own) {   // how many there are in the runs before this warp's, of all CTAs
+        if (lane == 0) seg[what][warp] = own;
+        __syncthreads();
+        int sum = 0;
+        for (int w = 0; w < kSelectWarps; ++w) sum += seg[what][w];
+        if (tid == 0) counted[what] = sum;
+        int prior = 0;
+        for (int w = 0; w < warp; ++w) prior += seg[what][w];
+        return prior;
+    };
+    auto of_ranks = [&](int what) {
+        int sum = 0;
+        for (int r = 0; r < rank; ++r) sum += cluster.map_shared_rank(counted, r)[what];
+        return sum;
+    };
     int ties = 0;
-    for (int i = from; i < to; i += 32) ties += __popc(__ballot_sync(0xffffffffu, i + lane < to && key(min(i + lane, len - 1)) == limit));
-    if (lane == 0) seg[0][warp] = ties;
-    __syncthreads();
-    int tie0 = 0;
-    for (int w = 0; w < warp; ++w) tie0 += seg[0][w];
+    for (int i = from; i < to; i += 32) ties += __popc(__ballot_sync(0xffffffffu, i + lane < to && key(min(i + lane, to - 1)) == limit));
+    int tie0 = before(0, ties);
+    cluster.sync();
+    tie0 += of_ranks(0);
     auto walk = [&](auto&& each) {   // each(slot, within, stays)
         int t = tie0;
         for (int i = from; i < to; i += 32) {
             const int slot = i + lane;
             const bool in = slot < to;
-            const unsigned k = key(min(slot, len - 1));
+            const unsigned k = key(min(slot, to - 1));
             const unsigned tied = __ballot_sync(0xffffffffu, in && k == limit);
             const bool stays = in && (k > limit || (k == limit && t + __popc(tied & below) < want));
             t += __popc(tied);
@@ -243,10 +340,10 @@ __global__ void __launch_bounds__(kSelectThreads) kv8_select_kernel(const swlm_k
         free_slots += __popc(__ballot_sync(0xffffffffu, in && slot < keep && !stays));
         moving += __popc(__ballot_sync(0xffffffffu, stays && slot >= keep));
     });
-    if (lane == 0) { seg[1][warp] = free_slots; seg[2][warp] = moving; }
-    __syncthreads();
-    int free0 = 0, move0 = 0;
-    for (int w = 0; w < warp; ++w) { free0 += seg[1][w]; move0 += seg[2][w]; }
+    int free0 = before(1, free_slots), move0 = before(2, moving);
+    cluster.sync();
+    free0 += of_ranks(1);
+    move0 += of_ranks(2);
     const EvictPlan plan(a.scratch, head, keep);
     const float* ks = c.k_scale + head * (c.capacity / c.block);
     const float* vs = c.v_scale + head * (c.capacity / c.block);
@@ -262,6 +359,7 @@ __global__ void __launch_bounds__(kSelectThreads) kv8_select_kernel(const swlm_k
         free0 += __popc(f);
         move0 += __popc(m);
     });
+    cluster.sync();   // no CTA leaves while another may read its counts
 }
 
 constexpr int kMoveThreads = 256, kMoveUnits = 4;   // a unit: 16 codes
@@ -311,12 +409,14 @@ __global__ void __launch_bounds__(kMoveThreads) kv8_move_kernel(const swlm_kv8_c
         raw[u] = *reinterpret_cast<const uint4*>(from + (size_t)source[i / per] * c.head_dim + i % per * 16);
         if (changed) {
             const unsigned w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-            unsigned m = 0;   // of each byte's |code|: an integer, or the seven bits of an e4m3 number
+            __half2 m = __half2half2(__ushort_as_half(0));   // of each pair's |code|
 #pragma unroll
-            for (int e = 0; e < 4; ++e) m = __vmaxu4(m, CODE == SWLM_KV8_INT8 ? __vabsss4(w[e]) : w[e] & 0x7F7F7F7Fu);
-            m = __vmaxu4(m, m >> 16);
-            m = max(m & 0xFFu, (m >> 8) & 0xFFu);
-            top = max(top, __float_as_uint(fabsf(kv8_number<CODE>(m) * scales[i / per])));
+            for (int e = 0; e < 4; ++e) {
+                const unsigned x = prepared<CODE>(w[e]), lo = pair_of<CODE, 0>(x), hi = pair_of<CODE, 1>(x);
+                m = __hmax2_nan(m, __hmax2_nan(__habs2(*reinterpret_cast<const __half2*>(&lo)), __habs2(*reinterpret_cast<const __half2*>(&hi))));
+            }
+            const float2 both = __half22float2(m);
+            top = max(top, max(__float_as_uint(fabsf(both.x * scales[i / per])), __float_as_uint(fabsf(both.y * scales[i / per]))));
         }
     }
     if (!changed) {
@@ -329,7 +429,8 @@ __global__ void __launch_bounds__(kMoveThreads) kv8_move_kernel(const swlm_kv8_c
     } else {
         top = block_max(top, warps);
         const bool finite = top < 0x7F800000u;
-        const float s = finite ? __fdiv_rn(__uint_as_float(top), kv8_top<CODE>()) : kKv8NaN;
+        const float s = finite ? __fdiv_rn(__uint_as_float(top), kv8_top<CODE>()) : kKv8NaN, inv = 1.f / s;
+        const bool ordinary = kv8_ordinary(s);
         if (tid == 0) (which ? to.v_scale : to.k_scale)[head * (to.capacity / T) + blockIdx.x] = s;
 #pragma unroll
         for (int u = 0; u < kMoveUnits; ++u) {
@@ -337,11 +438,11 @@ __global__ void __launch_bounds__(kMoveThreads) kv8_move_kernel(const swlm_kv8_c
             if (i >= units) continue;
             const unsigned w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
             unsigned out[4] = {0, 0, 0, 0};
-            const float mine = scales[i / per];
+            const float mine = scales[i / per], factor = mine * inv;
+            const bool both = ordinary && kv8_ordinary(mine);
             if (finite && s > 0.f)
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    out[e >> 2] |= kv8_code<CODE>(__fdiv_rn(kv8_number<CODE>((w[e >> 2] >> (8 * (e & 3))) & 0xFFu) * mine, s)) << (8 * (e & 3));
+                for (int e = 0; e < 4; ++e) out[e] = kv8_again<CODE>(w[e], mine, s, factor, both);
             *reinterpret_cast<uint4*>(dst + (size_t)i * 16) = make_uint4(out[0], out[1], out[2], out[3]);
         }
     }
@@ -384,9 +485,10 @@ int launch_kv8_evict(const swlm_kv8_cache& c, const swlm_kv8_cache& to, const sw
     const int span = std::min(a.max_len, c.capacity);
     cudaError_t e = cudaSuccess;
     if (span > a.keep) {
-        const dim3 grid((unsigned)c.kv_heads, (unsigned)c.batch);
-        if (span <= kCachedKeys) {
-            e = launch_k(kv8_select_kernel<true>, grid, dim3(kSelectThreads), (size_t)span * 4, s, c, a);
+        const dim3 grid((unsigned)c.kv_heads * kSelectCtas, (unsigned)c.batch);
+        const int share = (span + kSelectCtas * 32 - 1) / (kSelectCtas * 32) * 32;
+        if (share <= kCachedKeys) {
+            e = launch_k(kv8_select_kernel<true>, grid, dim3(kSelectThreads), (size_t)share * 4, s, c, a);
         } else {
             e = launch_k(kv8_select_kernel<false>, grid, dim3(kSelectThreads), 0, s, c, a);
         }

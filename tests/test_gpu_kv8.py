@@ -385,10 +385,10 @@ def test_evict_of_equal_and_special_weights(pkg, store, weights):
         check_evicted(before, before, work, [500], keep, 2, 5, [500])
 
 
-def test_evict_from_a_long_cache(pkg, store):
-    """More keys than fit shared memory."""
-    n = 49152 + 700
-    cache = Cache(pkg, 1, 1, 64, 49920, 128, 1).fill([n])
+@pytest.mark.parametrize("n", [49152 + 700, 8 * 24576 + 700])
+def test_evict_from_a_long_cache(pkg, store, n):
+    """Many keys, and more than fit shared memory."""
+    cache = Cache(pkg, 1, 1, 64, -(-n // 128) * 128, 128, 1).fill([n])
     to = Cache(pkg, 1, 1, 64, 2048, 128, 1)
     to_before = to.clone()
     evict(pkg, store, cache, to, 2000, 4, 64, ints(n), ints(n))
