@@ -27,67 +27,58 @@ constexpr float kTopInt8 = 127.f, kTopE4m3 = 448.f;
 
 template <int CODE> __device__ __forceinline__ constexpr float kv8_top() { return CODE == SWLM_KV8_INT8 ? kTopInt8 : kTopE4m3; }
 
-// A code is round(x / s) of the IEEE quotient, which costs some twenty instructions. The product with 1 / s is off by 2^-21 of itself at most (also with the
-// factor of an old scale in it), so that only a value within that of a border between two codes needs the quotient.
+// A code is round(x / s) of the IEEE quotient. Two of Markstein's steps, q += (x - q s) / s with the rounded inverse and an exact residual, give that
+// quotient from x / s's first approximation, where nothing is subnormal: five operations, two values to an instruction, no branch.
 
 // the code of the quotient y, as a byte (|y| <= top but for the last place; the clamp is for scales that are subnormal)
 template <int CODE> __device__ __forceinline__ unsigned kv8_code(float y) {
     if (CODE == SWLM_KV8_INT8) return (unsigned)__float2int_rn(fminf(fmaxf(y, -kTopInt8), kTopInt8)) & 0xFFu;
     return (unsigned)__nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
 }
-// The codes of four values whose quotients are about y, as a word; `sure`: none of them is next to a border.
-template <int CODE> __device__ __forceinline__ unsigned kv8_codes4(const float (&y)[4], bool& sure) {
-    if (CODE == SWLM_KV8_INT8) {
-        // the low byte of 1.5 * 2^23 + y is y rounded to an integer, ties to even
-        float far = 0.f;
-        unsigned k[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float m = y[e] + 12582912.f;
-            k[e] = __float_as_uint(m);
-            far = fmaxf(far, fabsf(y[e] - (m - 12582912.f)));
-        }
-        sure = sure && far < 0.4998f;   // 127 * 2^-21 = 0.00006 from the border
-        return __byte_perm(__byte_perm(k[0], k[1], 0x0040), __byte_perm(k[2], k[3], 0x0040), 0x5410);
+// A block's scale and its inverse. Scales far from 1 (whose residuals might be subnormal) go by division.
+struct Divisor {
+    float s, inv;
+    bool ordinary;
+    __device__ __forceinline__ explicit Divisor(float scale) : s(scale), inv(1.f / scale), ordinary(scale > 0x1p-60f && scale < 0x1p60f) {}
+    __device__ __forceinline__ float2 quotient(const float2& x) const {
+        const float2 inv2 = make_float2(inv, inv), minus = make_float2(-s, -s);
+        float2 q = mul2(x, inv2);
+        q = fma2(fma2(q, minus, x), inv2, q);
+        return fma2(fma2(q, minus, x), inv2, q);
     }
-    unsigned lo, hi;
-    constexpr float down = 1.f - 0x1p-20f, up = 1.f + 0x1p-20f;
-    asm("{\n\t.reg .b16 a, b;\n\tcvt.rn.satfinite.e4m3x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 b, %4, %3;\n\tmov.b32 %0, {a, b};\n\t}"
-        : "=r"(lo) : "f"(y[0] * down), "f"(y[1] * down), "f"(y[2] * down), "f"(y[3] * down));
-    asm("{\n\t.reg .b16 a, b;\n\tcvt.rn.satfinite.e4m3x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 b, %4, %3;\n\tmov.b32 %0, {a, b};\n\t}"
-        : "=r"(hi) : "f"(y[0] * up), "f"(y[1] * up), "f"(y[2] * up), "f"(y[3] * up));
-    sure = sure && lo == hi;
-    return lo;
+};
+// The codes of four values, as a word.
+template <int CODE> __device__ __forceinline__ unsigned kv8_codes4(const float2& x, const float2& y, const Divisor& d) {
+    if (!d.ordinary)
+        return kv8_code<CODE>(__fdiv_rn(x.x, d.s)) | kv8_code<CODE>(__fdiv_rn(x.y, d.s)) << 8 | kv8_code<CODE>(__fdiv_rn(y.x, d.s)) << 16 | kv8_code<CODE>(__fdiv_rn(y.y, d.s)) << 24;
+    float2 p = d.quotient(x), q = d.quotient(y);
+    if (CODE == SWLM_KV8_INT8) {
+        // the low byte of 1.5 * 2^23 + v is v rounded to an integer, ties to even
+        const float2 magic = make_float2(12582912.f, 12582912.f);
+        p = add2(p, magic);
+        q = add2(q, magic);
+        return __byte_perm(__byte_perm(__float_as_uint(p.x), __float_as_uint(p.y), 0x0040), __byte_perm(__float_as_uint(q.x), __float_as_uint(q.y), 0x0040), 0x5410);
+    }
+    unsigned word;   // (the steps turn -0 into 0; its code has the sign)
+    asm("{\n\t.reg .b16 p, q;\n\tcvt.rn.satfinite.e4m3x2.f32 p, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 q, %4, %3;\n\tmov.b32 %0, {p, q};\n\t}"
+        : "=r"(word) : "f"(copysignf(p.x, x.x)), "f"(copysignf(p.y, x.y)), "f"(copysignf(q.x, y.x)), "f"(copysignf(q.y, y.y)));
+    return word;
 }
-// Scales whose inverse and products are normal numbers.
-__device__ __forceinline__ bool kv8_ordinary(float s) { return s > 0x1p-100f && s < 0x1p100f; }
-
-// a word's codes as numbers
-template <int CODE> __device__ __forceinline__ void kv8_numbers4(unsigned word, float (&x)[4]) {
+// The word's codes, held at scale `from`, at another.
+template <int CODE> __device__ __forceinline__ unsigned kv8_again(unsigned word, float from, const Divisor& d) {
+    float2 x, y;
+    const float2 from2 = make_float2(from, from);
     if (CODE == SWLM_KV8_INT8) {
         const unsigned u = word ^ 0x80808080u;   // c + 128, the low byte of 2^23 + u
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7650 + e)) - (8388608.f + 128.f);
+        const float2 bias = make_float2(-8388736.f, -8388736.f);
+        x = add2(make_float2(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7650)), __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7651))), bias);
+        y = add2(make_float2(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7652)), __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7653))), bias);
     } else {
-        const __half2 a = __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(word & 0xFFFFu), __NV_E4M3)), b = __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(word >> 16), __NV_E4M3));
-        const float2 p = __half22float2(a), q = __half22float2(b);
-        x[0] = p.x; x[1] = p.y; x[2] = q.x; x[3] = q.y;
+        const unsigned lo = pair_of<CODE, 0>(word), hi = pair_of<CODE, 1>(word);
+        x = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+        y = __half22float2(*reinterpret_cast<const __half2*>(&hi));
     }
-}
-// The word's codes, held at scale `from`, at scale s (inv: 1 / s; ordinary: both scales are).
-template <int CODE> __device__ __forceinline__ unsigned kv8_again(unsigned word, float from, float s, float factor, bool ordinary) {
-    float x[4], y[4];
-    kv8_numbers4<CODE>(word, x);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = x[e] * factor;
-    bool sure = ordinary;
-    unsigned out = kv8_codes4<CODE>(y, sure);
-    if (!sure) {
-        out = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) out |= kv8_code<CODE>(__fdiv_rn(x[e] * from, s)) << (8 * e);
-    }
-    return out;
+    return kv8_codes4<CODE>(mul2(x, from2), mul2(y, from2), d);
 }
 
 // Largest of a CTA's unsigned numbers, to all of its threads.
@@ -106,11 +97,15 @@ __device__ __forceinline__ unsigned block_max(unsigned v, unsigned* warps) {
 constexpr int kAppendThreads = 256, kAppendUnits = 8;   // a unit: eight values of a token, at most 128 * 128 / 8 of them in a block
 static_assert(kAppendThreads * kAppendUnits * 8 >= kKv8MaxBlock * 128, "a block fits its CTA");
 
-__device__ __forceinline__ float half_bits(unsigned bits, bool f16) {
-    return f16 ? __half2float(__ushort_as_half((unsigned short)bits)) : __uint_as_float(bits << 16);
+template <bool F16> __device__ __forceinline__ float half_bits(unsigned bits) {
+    return F16 ? __half2float(__ushort_as_half((unsigned short)bits)) : __uint_as_float(bits << 16);
+}
+// the two values of a word
+template <bool F16> __device__ __forceinline__ float2 halves(unsigned word) {
+    return F16 ? __half22float2(*reinterpret_cast<const __half2*>(&word)) : make_float2(__uint_as_float(word << 16), __uint_as_float(word & 0xFFFF0000u));
 }
 
-template <int CODE>
+template <int CODE, bool F16>
 __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const swlm_kv8_cache c, const swlm_kv8_append a) {
     __shared__ unsigned warps[kAppendThreads / 32];
     pdl_launch_dependents();
@@ -124,14 +119,14 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const swlm_k
     const int low = max(part.len, base), high = min(part.len + part.count, base + T);   // new slots of this block
     if (low >= high) return;
     const int old = low - base;   // tokens that it has
-    const bool f16 = a.dtype == SWLM_KV8_FP16;
     const unsigned short* x = static_cast<const unsigned short*>(which ? a.v : a.k);
     const int64_t stride = which ? a.v_stride : a.k_stride;
+    x += part.start * stride + h * c.head_dim;
     unsigned char* codes = static_cast<unsigned char*>(which ? c.v : c.k) + ((size_t)(b * (size_t)c.kv_heads + h) * c.capacity + base) * c.head_dim;
     float* scale = (which ? c.v_scale : c.k_scale) + (size_t)(b * (size_t)c.kv_heads + h) * (c.capacity / T) + blk;
     const float s0 = old ? *scale : 0.f;
 
-    const int per = c.head_dim >> 3, units = (high - low) * per;   // units of a token, new units
+    const int per = c.head_dim == 128 ? 4 : 3, units = (high - low) << per;   // log2 of the units of a token, new units
     uint4 raw[kAppendUnits];
     unsigned top = 0;   // largest |value| as its 15 bits: the order of the numbers, infinity and NaN above all
 #pragma unroll
@@ -139,19 +134,19 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const swlm_k
         const int i = tid + u * (int)blockDim.x;
         raw[u] = make_uint4(0, 0, 0, 0);
         if (i < units) {
-            const int slot = low + i / per, d = i % per * 8;
-            raw[u] = *reinterpret_cast<const uint4*>(x + (int64_t)(part.start + slot - part.len) * stride + (size_t)h * c.head_dim + d);
+            const int row = (i >> per) + low - part.len, d = (i & ((1 << per) - 1)) * 8;
+            raw[u] = *reinterpret_cast<const uint4*>(x + row * stride + d);
         }
         const unsigned m = __vmaxu2(__vmaxu2(raw[u].x & 0x7FFF7FFFu, raw[u].y & 0x7FFF7FFFu), __vmaxu2(raw[u].z & 0x7FFF7FFFu, raw[u].w & 0x7FFF7FFFu));
         top = max(top, max(m & 0xFFFFu, m >> 16));
     }
     top = block_max(top, warps);   // (all have read the old scale when it returns, or are the only warp)
-    const bool finite = top < (f16 ? 0x7C00u : 0x7F80u) && s0 == s0;
-    const float s = finite ? fmaxf(s0, __fdiv_rn(half_bits(top, f16), kv8_top<CODE>())) : kKv8NaN;
+    const bool finite = top < (F16 ? 0x7C00u : 0x7F80u) && s0 == s0;
+    const float s = finite ? fmaxf(s0, __fdiv_rn(half_bits<F16>(top), kv8_top<CODE>())) : kKv8NaN;
     if (blockDim.x == 32) __syncwarp();
     if (tid == 0) *scale = s;
-    const bool grows = old && finite && s > s0, ordinary = kv8_ordinary(s);
-    const float inv = 1.f / s;
+    const bool grows = old && finite && s > s0;
+    const Divisor divisor(s);
 #pragma unroll
     for (int u = 0; u < kAppendUnits; ++u) {
         const int i = tid + u * (int)blockDim.x;
@@ -160,30 +155,15 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const swlm_k
             unsigned out[2] = {0, 0};
             if (finite && s > 0.f)
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    float v[4], y[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        v[e] = half_bits((w[2 * k + (e >> 1)] >> (16 * (e & 1))) & 0xFFFFu, f16);
-                        y[e] = v[e] * inv;
-                    }
-                    bool sure = ordinary;
-                    out[k] = kv8_codes4<CODE>(y, sure);
-                    if (!sure) {
-                        out[k] = 0;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) out[k] |= kv8_code<CODE>(__fdiv_rn(v[e], s)) << (8 * e);
-                    }
-                }
-            *reinterpret_cast<uint2*>(codes + (size_t)(low - base + i / per) * c.head_dim + i % per * 8) = make_uint2(out[0], out[1]);
+                for (int k = 0; k < 2; ++k) out[k] = kv8_codes4<CODE>(halves<F16>(w[2 * k]), halves<F16>(w[2 * k + 1]), divisor);
+            *reinterpret_cast<uint2*>(codes + (old << (per + 3)) + i * 8) = make_uint2(out[0], out[1]);
         }
     }
     if (grows)
-        for (int i = tid; i < old * per; i += blockDim.x) {
+        for (int i = tid; i < old << per; i += blockDim.x) {
             uint2* at = reinterpret_cast<uint2*>(codes + (size_t)i * 8);
             const uint2 was = *at;
-            const bool both = ordinary && kv8_ordinary(s0);
-            *at = make_uint2(kv8_again<CODE>(was.x, s0, s, s0 * inv, both), kv8_again<CODE>(was.y, s0, s, s0 * inv, both));
+            *at = make_uint2(kv8_again<CODE>(was.x, s0, divisor), kv8_again<CODE>(was.y, s0, divisor));
         }
     if (which == 0)
         for (int slot = low + tid; slot < high; slot += blockDim.x) {
@@ -230,9 +210,10 @@ __device__ __forceinline__ unsigned evict_key(float w, int pos, int sink, long l
 template <bool CACHED>
 __global__ void __cluster_dims__(kSelectCtas, 1, 1) __launch_bounds__(kSelectThreads) kv8_select_kernel(const swlm_kv8_cache c, const swlm_kv8_evict a) {
     extern __shared__ unsigned keys[];
-    __shared__ unsigned hist[2][kDigits], all[kDigits];
+    __shared__ __align__(16) unsigned hist[2][kDigits];
+    static_assert(kDigits == 4 * kSelectThreads, "four digits of a thread");
     __shared__ int seg[3][kSelectWarps], counted[3];   // ties, free slots, moving tokens: of a warp, of the CTA
-    __shared__ unsigned found_digit, found_above;
+    __shared__ unsigned found_digit, found_above, found_all, sums[kSelectWarps];
     pdl_launch_dependents();
     pdl_wait();
     const cg::cluster_group cluster = cg::this_cluster();
@@ -264,38 +245,40 @@ __global__ void __cluster_dims__(kSelectCtas, 1, 1) __launch_bounds__(kSelectThr
             if ((k & mask) == prefix) atomicAdd(&mine[(k >> shift) & (kDigits - 1)], 1u);
         }
         cluster.sync();   // (what the pass before counted has been read by all)
-        for (int i = tid; i < kDigits; i += kSelectThreads) {
-            unsigned sum = 0;
+        // thread i has the four digits from kDigits - 4 - 4 i on: counts from the top down
+        const int low = kDigits - 4 - 4 * tid;
+        uint4 count = make_uint4(0, 0, 0, 0);
 #pragma unroll
-            for (int r = 0; r < kSelectCtas; ++r) sum += cluster.map_shared_rank(mine, r)[i];
-            all[i] = sum;
-            hist[(pass + 1) & 1][i] = 0;
+        for (int r = 0; r < kSelectCtas; ++r) {
+            const uint4 v = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(mine, r) + low);
+            count.x += v.x; count.y += v.y; count.z += v.z; count.w += v.w;
         }
+        *reinterpret_cast<uint4*>(hist[(pass + 1) & 1] + low) = make_uint4(0, 0, 0, 0);
+        const unsigned sum = count.x + count.y + count.z + count.w;
+        unsigned above = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned v = __shfl_up_sync(0xffffffffu, above, o);
+            if (lane >= o) above += v;
+        }
+        if (lane == 31) sums[warp] = above;
         __syncthreads();
-        if (warp == 0) {   // lane l has the 64 digits from the (31 - l)-th group on: counts from the top down
-            constexpr int PER = kDigits / 32;
-            const int group = (31 - lane) * PER;
-            unsigned sum = 0;
-#pragma unroll 8
-            for (int i = 0; i < PER; ++i) sum += all[group + (i + lane) % PER];   // (lanes meet different banks)
-            unsigned above = sum;
-            for (int o = 1; o < 32; o <<= 1) {
-                const unsigned v = __shfl_up_sync(0xffffffffu, above, o);
-                if (lane >= o) above += v;
-            }
-            above -= sum;   // keys of higher groups
-            if (above < (unsigned)want && above + sum >= (unsigned)want) {
-                int d = group + PER - 1;
-                while (above + all[d] < (unsigned)want) above += all[d--];
-                found_digit = (unsigned)d;
-                found_above = above;
-            }
+        for (int w = 0; w < warp; ++w) above += sums[w];
+        above -= sum;   // keys of higher digits
+        if (above < (unsigned)want && above + sum >= (unsigned)want) {
+            const unsigned n[4] = {count.w, count.z, count.y, count.x};
+            int d = 0;
+            while (above + n[d] < (unsigned)want) above += n[d++];
+            found_digit = (unsigned)(low + 3 - d);
+            found_above = above;
+            found_all = above + n[d] == (unsigned)want;
         }
         __syncthreads();
         const unsigned digits = (unsigned)(kDigits - 1) << shift;
         prefix = (prefix & ~digits) | found_digit << shift;   // (the last digit overlaps the one before it, with the same bits there)
         mask |= digits;
         want -= (int)found_above;
+        if (found_all) { want = len; break; }   // all keys with this prefix stay: none of those below it has to be told from another
         if (shift == 0) break;
     }
     const unsigned limit = prefix;   // keys above it stay, and the first `want` of those equal to it
@@ -313,11 +296,7 @@ __global__ void __cluster_dims__(kSelectCtas, 1, 1) __launch_bounds__(kSelectThr
         for (int w = 0; w < warp; ++w) prior += seg[what][w];
         return prior;
     };
-    auto of_ranks = [&](int what) {
-        int sum = 0;
-        for (int r = 0; r < rank; ++r) sum += cluster.map_shared_rank(counted, r)[what];
-        return sum;
-    };
+    auto of_ranks = [&](int what) { return (int)__reduce_add_sync(0xffffffffu, lane < rank ? (unsigned)cluster.map_shared_rank(counted, lane)[what] : 0u); };
     int ties = 0;
     for (int i = from; i < to; i += 32) ties += __popc(__ballot_sync(0xffffffffu, i + lane < to && key(min(i + lane, to - 1)) == limit));
     int tie0 = before(0, ties);
@@ -399,14 +378,14 @@ __global__ void __launch_bounds__(kMoveThreads) kv8_move_kernel(const swlm_kv8_c
     if (!changed && in_place) return;
     const unsigned char* from = static_cast<const unsigned char*>(which ? c.v : c.k) + head * c.capacity * c.head_dim;
     unsigned char* dst = static_cast<unsigned char*>(which ? to.v : to.k) + (head * to.capacity + base) * c.head_dim;
-    const int per = c.head_dim >> 4, units = n * per;
+    const int per = c.head_dim == 128 ? 3 : 2, units = n << per;   // log2 of the units of a token
     uint4 raw[kMoveUnits];
     unsigned top = 0;   // largest |value|, as the bits of a float that is not negative
 #pragma unroll
     for (int u = 0; u < kMoveUnits; ++u) {
         const int i = tid + u * (int)blockDim.x;
         if (i >= units) continue;
-        raw[u] = *reinterpret_cast<const uint4*>(from + (size_t)source[i / per] * c.head_dim + i % per * 16);
+        raw[u] = *reinterpret_cast<const uint4*>(from + (size_t)source[i >> per] * c.head_dim + (i & ((1 << per) - 1)) * 16);
         if (changed) {
             const unsigned w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
             __half2 m = __half2half2(__ushort_as_half(0));   // of each pair's |code|
@@ -416,7 +395,7 @@ __global__ void __launch_bounds__(kMoveThreads) kv8_move_kernel(const swlm_kv8_c
                 m = __hmax2_nan(m, __hmax2_nan(__habs2(*reinterpret_cast<const __half2*>(&lo)), __habs2(*reinterpret_cast<const __half2*>(&hi))));
             }
             const float2 both = __half22float2(m);
-            top = max(top, max(__float_as_uint(fabsf(both.x * scales[i / per])), __float_as_uint(fabsf(both.y * scales[i / per]))));
+            top = max(top, max(__float_as_uint(fabsf(both.x * scales[i >> per])), __float_as_uint(fabsf(both.y * scales[i >> per]))));
         }
     }
     if (!changed) {
@@ -429,8 +408,8 @@ __global__ void __launch_bounds__(kMoveThreads) kv8_move_kernel(const swlm_kv8_c
     } else {
         top = block_max(top, warps);
         const bool finite = top < 0x7F800000u;
-        const float s = finite ? __fdiv_rn(__uint_as_float(top), kv8_top<CODE>()) : kKv8NaN, inv = 1.f / s;
-        const bool ordinary = kv8_ordinary(s);
+        const float s = finite ? __fdiv_rn(__uint_as_float(top), kv8_top<CODE>()) : kKv8NaN;
+        const Divisor divisor(s);
         if (tid == 0) (which ? to.v_scale : to.k_scale)[head * (to.capacity / T) + blockIdx.x] = s;
 #pragma unroll
         for (int u = 0; u < kMoveUnits; ++u) {
@@ -438,11 +417,10 @@ __global__ void __launch_bounds__(kMoveThreads) kv8_move_kernel(const swlm_kv8_c
             if (i >= units) continue;
             const unsigned w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
             unsigned out[4] = {0, 0, 0, 0};
-            const float mine = scales[i / per], factor = mine * inv;
-            const bool both = ordinary && kv8_ordinary(mine);
+            const float mine = scales[i >> per];
             if (finite && s > 0.f)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) out[e] = kv8_again<CODE>(w[e], mine, s, factor, both);
+                for (int e = 0; e < 4; ++e) out[e] = kv8_again<CODE>(w[e], mine, divisor);
             *reinterpret_cast<uint4*>(dst + (size_t)i * 16) = make_uint4(out[0], out[1], out[2], out[3]);
         }
     }
@@ -466,8 +444,9 @@ int launch_kv8_append(const swlm_kv8_cache& c, const swlm_kv8_append& a, cudaStr
     // (a whole block in at most 8 units per thread; a single token's few values need no more than a warp, its block's older codes do)
     const int threads = std::min(kAppendThreads, std::max(32, c.block * c.head_dim / (8 * kAppendUnits)));
     const dim3 grid(blocks, 2u * (unsigned)c.kv_heads, (unsigned)c.batch);
-    return after_launch(c.code == SWLM_KV8_INT8 ? launch_k(kv8_append_kernel<SWLM_KV8_INT8>, grid, dim3(threads), 0, s, c, a)
-                                                : launch_k(kv8_append_kernel<SWLM_KV8_E4M3>, grid, dim3(threads), 0, s, c, a), "kv8 append launch");
+    auto launch = [&](auto kernel) { return after_launch(launch_k(kernel, grid, dim3(threads), 0, s, c, a), "kv8 append launch"); };
+    if (c.code == SWLM_KV8_INT8) return a.dtype == SWLM_KV8_FP16 ? launch(kv8_append_kernel<SWLM_KV8_INT8, true>) : launch(kv8_append_kernel<SWLM_KV8_INT8, false>);
+    return a.dtype == SWLM_KV8_FP16 ? launch(kv8_append_kernel<SWLM_KV8_E4M3, true>) : launch(kv8_append_kernel<SWLM_KV8_E4M3, false>);
 }
 
 int launch_kv8_lengths(int batch, const int32_t* in, const int32_t* counts, int n, int limit, const int32_t* refused, int32_t* out, cudaStream_t s) {

@@ -59,6 +59,33 @@ template <int CODE, int HIGH> __device__ __forceinline__ unsigned pair_of(unsign
     return v;
 }
 
+// Two fp32 operations as one instruction.
+__device__ __forceinline__ unsigned long long pair_bits(const float2& v) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+    return r;
+}
+__device__ __forceinline__ float2 bits_pair(unsigned long long v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(const float2& a, const float2& b, const float2& c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)), "l"(pair_bits(c)));
+    return bits_pair(r);
+}
+__device__ __forceinline__ float2 add2(const float2& a, const float2& b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)));
+    return bits_pair(r);
+}
+__device__ __forceinline__ float2 mul2(const float2& a, const float2& b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)));
+    return bits_pair(r);
+}
+
 // What is added to a score (log2) to make it log2 of a weight: minus the row's maximum and the logarithm of its sum. A row that attends
 // nothing has no weights.
 __device__ __forceinline__ float row_shift_of(float m, float l) { return l == 0.f ? -INFINITY : -((m == -INFINITY ? 0.f : m) + log2f(l)); }

@@ -34,32 +34,6 @@ struct PromptBars {
     int failed;
 };
 
-// Two fp32 operations as one instruction.
-__device__ __forceinline__ unsigned long long pair_bits(const float2& v) {
-    unsigned long long r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
-    return r;
-}
-__device__ __forceinline__ float2 bits_pair(unsigned long long v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ float2 fma2(const float2& a, const float2& b, const float2& c) {
-    unsigned long long r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)), "l"(pair_bits(c)));
-    return bits_pair(r);
-}
-__device__ __forceinline__ float2 add2(const float2& a, const float2& b) {
-    unsigned long long r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)));
-    return bits_pair(r);
-}
-__device__ __forceinline__ float2 mul2(const float2& a, const float2& b) {
-    unsigned long long r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)));
-    return bits_pair(r);
-}
 __device__ __forceinline__ float log2_of(float x) { float y; asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
 template <int HD> __host__ __device__ constexpr size_t prompt_smem() { return (size_t)kPaRows * HD * 2 + 4 * kPaKeys * HD * 2 + 1024; }
