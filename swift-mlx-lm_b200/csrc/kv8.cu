@@ -13,6 +13,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "kv8_device.cuh"
 #include "swlm_runtime.h"
@@ -48,8 +49,8 @@ struct Divisor {
     }
 };
 // The codes of four values, as a word.
-template <int CODE> __device__ __forceinline__ unsigned kv8_codes4(const float2& x, const float2& y, const Divisor& d) {
-    if (!d.ordinary)
+template <int CODE, bool ORDINARY> __device__ __forceinline__ unsigned kv8_codes4(const float2& x, const float2& y, const Divisor& d) {
+    if (!ORDINARY)
         return kv8_code<CODE>(__fdiv_rn(x.x, d.s)) | kv8_code<CODE>(__fdiv_rn(x.y, d.s)) << 8 | kv8_code<CODE>(__fdiv_rn(y.x, d.s)) << 16 | kv8_code<CODE>(__fdiv_rn(y.y, d.s)) << 24;
     float2 p = d.quotient(x), q = d.quotient(y);
     if (CODE == SWLM_KV8_INT8) {
@@ -65,7 +66,7 @@ template <int CODE> __device__ __forceinline__ unsigned kv8_codes4(const float2&
     return word;
 }
 // The word's codes, held at scale `from`, at another.
-template <int CODE> __device__ __forceinline__ unsigned kv8_again(unsigned word, float from, const Divisor& d) {
+template <int CODE, bool ORDINARY> __device__ __forceinline__ unsigned kv8_again(unsigned word, float from, const Divisor& d) {
     float2 x, y;
     const float2 from2 = make_float2(from, from);
     if (CODE == SWLM_KV8_INT8) {
@@ -78,7 +79,7 @@ template <int CODE> __device__ __forceinline__ unsigned kv8_again(unsigned word,
         x = __half22float2(*reinterpret_cast<const __half2*>(&lo));
         y = __half22float2(*reinterpret_cast<const __half2*>(&hi));
     }
-    return kv8_codes4<CODE>(mul2(x, from2), mul2(y, from2), d);
+    return kv8_codes4<CODE, ORDINARY>(mul2(x, from2), mul2(y, from2), d);
 }
 
 // Largest of a CTA's unsigned numbers, to all of its threads.
@@ -147,24 +148,28 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const swlm_k
     if (tid == 0) *scale = s;
     const bool grows = old && finite && s > s0;
     const Divisor divisor(s);
+    auto store = [&](auto ordinary) {
+        constexpr bool ORDINARY = decltype(ordinary)::value;
 #pragma unroll
-    for (int u = 0; u < kAppendUnits; ++u) {
-        const int i = tid + u * (int)blockDim.x;
-        if (i < units) {
+        for (int u = 0; u < kAppendUnits; ++u) {
+            const int i = tid + u * (int)blockDim.x;
+            if (i >= units) continue;
             const unsigned w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-            unsigned out[2] = {0, 0};
-            if (finite && s > 0.f)
+            unsigned out[2];
 #pragma unroll
-                for (int k = 0; k < 2; ++k) out[k] = kv8_codes4<CODE>(halves<F16>(w[2 * k]), halves<F16>(w[2 * k + 1]), divisor);
+            for (int k = 0; k < 2; ++k) out[k] = kv8_codes4<CODE, ORDINARY>(halves<F16>(w[2 * k]), halves<F16>(w[2 * k + 1]), divisor);
             *reinterpret_cast<uint2*>(codes + (old << (per + 3)) + i * 8) = make_uint2(out[0], out[1]);
         }
-    }
-    if (grows)
-        for (int i = tid; i < old << per; i += blockDim.x) {
-            uint2* at = reinterpret_cast<uint2*>(codes + (size_t)i * 8);
-            const uint2 was = *at;
-            *at = make_uint2(kv8_again<CODE>(was.x, s0, divisor), kv8_again<CODE>(was.y, s0, divisor));
-        }
+        if (grows)
+            for (int i = tid; i < old << per; i += blockDim.x) {
+                uint2* at = reinterpret_cast<uint2*>(codes + (size_t)i * 8);
+                const uint2 was = *at;
+                *at = make_uint2(kv8_again<CODE, ORDINARY>(was.x, s0, divisor), kv8_again<CODE, ORDINARY>(was.y, s0, divisor));
+            }
+    };
+    if (divisor.ordinary) store(std::true_type());
+    else if (finite && s > 0.f) store(std::false_type());
+    else for (int i = tid; i < units; i += blockDim.x) *reinterpret_cast<uint2*>(codes + (old << (per + 3)) + i * 8) = make_uint2(0, 0);   // zeros, or NaN by its scale
     if (which == 0)
         for (int slot = low + tid; slot < high; slot += blockDim.x) {
             const size_t at = (size_t)(b * (size_t)c.kv_heads + h) * c.capacity + slot;
@@ -411,18 +416,24 @@ __global__ void __launch_bounds__(kMoveThreads) kv8_move_kernel(const swlm_kv8_c
         const float s = finite ? __fdiv_rn(__uint_as_float(top), kv8_top<CODE>()) : kKv8NaN;
         const Divisor divisor(s);
         if (tid == 0) (which ? to.v_scale : to.k_scale)[head * (to.capacity / T) + blockIdx.x] = s;
+        auto store = [&](auto kind) {   // 0: zeros, or NaN by its scale
+            constexpr int KIND = decltype(kind)::value;
 #pragma unroll
-        for (int u = 0; u < kMoveUnits; ++u) {
-            const int i = tid + u * (int)blockDim.x;
-            if (i >= units) continue;
-            const unsigned w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-            unsigned out[4] = {0, 0, 0, 0};
-            const float mine = scales[i >> per];
-            if (finite && s > 0.f)
+            for (int u = 0; u < kMoveUnits; ++u) {
+                const int i = tid + u * (int)blockDim.x;
+                if (i >= units) continue;
+                const unsigned w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+                unsigned out[4] = {0, 0, 0, 0};
+                const float mine = scales[i >> per];
+                if (KIND)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) out[e] = kv8_again<CODE>(w[e], mine, divisor);
-            *reinterpret_cast<uint4*>(dst + (size_t)i * 16) = make_uint4(out[0], out[1], out[2], out[3]);
-        }
+                    for (int e = 0; e < 4; ++e) out[e] = kv8_again<CODE, KIND == 2>(w[e], mine, divisor);
+                *reinterpret_cast<uint4*>(dst + (size_t)i * 16) = make_uint4(out[0], out[1], out[2], out[3]);
+            }
+        };
+        if (divisor.ordinary) store(std::integral_constant<int, 2>());
+        else if (finite && s > 0.f) store(std::integral_constant<int, 1>());
+        else store(std::integral_constant<int, 0>());
     }
     if (which == 0)
         for (int i = tid; i < n; i += blockDim.x) {
