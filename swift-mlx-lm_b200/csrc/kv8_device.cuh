@@ -32,7 +32,7 @@ struct RowsPlan {
     // many rows whose weights are added: the shifted queries as fp16 in tiles of 64 rows, [batch][kv_heads][tiles][head_dim / 64][64][64], swizzled as the
     // products read them, and per row what turns a product into log2 of a weight: times the factor, times the key's scale, plus the shift
     __half* q16;
-    float* q_factor;  // [batch][kv_heads][row_tiles * 128]
+    float* q_factor;  // [batch][kv_heads][row_tiles * 256]
     float* q_shift;
     int* table;     // [batch + 1]: units before each sequence, and of all
 };
@@ -85,6 +85,8 @@ __device__ __forceinline__ float2 mul2(const float2& a, const float2& b) {
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)));
     return bits_pair(r);
 }
+
+__device__ __forceinline__ float log2_of(float x) { float y; asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
 // What is added to a score (log2) to make it log2 of a weight: minus the row's maximum and the logarithm of its sum. A row that attends
 // nothing has no weights.
@@ -157,7 +159,7 @@ __device__ __forceinline__ Parts parts_of(const RowsPlan& p, const Kv8Part& part
 }
 
 // The kernel of many rows (kv8_prompt.cu): rows of a CTA, keys of a tile.
-constexpr int kPromptRows = 128, kPromptKeys = 64;
+constexpr int kPromptRows = 256, kPromptKeys = 64;
 
 }  // namespace kv8
 

@@ -1,15 +1,17 @@
 // Attention of many query rows over a cache of 8-bit codes (prompt portions), on the 5th-generation tensor cores (tcgen05 / TMEM).
 //
-// A CTA has 128 rows, rows being the queries of a sequence times the heads of a group, and a run of its slots. Codes become fp16 numbers on their
-// way to shared memory, queries are shifted to fp16 (both exact, see kv8_attend.cu), so that scores are one product with fp32 sums; a tile's
-// scores take the factor of their block, probabilities that of the values' block over the largest so far (2^7 times, as fp16).
+// A CTA has 256 rows in two tiles of 128, rows being the queries of a sequence times the heads of a group, and a run of its slots. Codes become fp16
+// numbers on their way to shared memory, queries are shifted to fp16 (both exact, see kv8_attend.cu), so that scores are one product with fp32
+// sums; a tile's scores take the factor of their block, probabilities that of the values' block over the largest so far (2^7 times, as fp16).
 //
-// Roles: four warps bring keys and values from the cache, convert them and store them in the swizzled layout of the products' operands (two
-// slots each); the first of them also issues the MMAs (S = Q K^T of tile j + 1 while tile j is in its softmax: two score regions); four warps
-// do the softmax, a thread per row. Probabilities take the place of their scores in tensor memory and are read there as the A operand. The
-// reference maximum of a row moves only when it would grow by more than 2^8. Two CTAs share an SM.
+// Roles: three warps bring keys and values from the cache, convert them and store them in the swizzled layout of the products' operands (three
+// slots each, both row tiles read them); a warp issues the MMAs (S = Q K^T of key tile j + 1 while tile j is in its softmax: two score
+// regions per row tile); eight warps do the softmax, a thread per row. Probabilities take the place of their scores in tensor memory and are
+// read there as the A operand. The reference maximum of a row moves only when it would grow by more than 2^8.
 //
-// What bounds it, with heads of 128: 512 clocks of the tensor pipe per tile of 64 keys, 512 of the exponential unit (8192 of 16 per clock).
+// What bounds it, with heads of 128: 512 clocks of the tensor pipe per row tile and 64 keys, 512 of the exponential unit (8192 of 16 per clock). A
+// form with one row tile per CTA and two CTAs per SM, whose loaders also issued the products, took 391 us where this one takes XXX us (2048 tokens over
+// 8192, 32 / 8 heads of 128).
 #include <algorithm>
 
 #include "kv8_device.cuh"
@@ -19,60 +21,73 @@ namespace swlm {
 using namespace kv8;
 namespace {
 
-static_assert(kPromptRows == kPaRows && kPromptKeys == kPaKeys, "the shared helpers' tiles");
-constexpr int kSoftmaxThreads = 128, kMmaWarp = 4, kLoadThreads = 128, kPromptThreads = kSoftmaxThreads + kLoadThreads;
+constexpr int kTiles = kPromptRows / kPaRows;   // row tiles of a CTA
+static_assert(kTiles == 2 && kPromptKeys == kPaKeys, "the shared helpers' tiles");
+constexpr int kSoftmaxWarps = 4 * kTiles, kMmaWarp = kSoftmaxWarps, kLoadWarps = 3;
+constexpr int kPromptThreads = (kSoftmaxWarps + 1 + kLoadWarps) * 32;   // (with 13 warps a thread would have 128 registers and not 168: 456 us, spilled)
+constexpr int kSlots = 3;               // key and value tiles in shared memory
 constexpr float kFoldUnit = 0x1p-20f;   // value scales down to this part of the largest go into the exponent
 
-// Phases (a wait by parity cannot tell a phase from the one two before it): for tile j
-//   k_full[j & 1], v_full[j & 1], p_ready[j & 1]   waited for phase by phase by the warp that issues the MMAs
-//   s_full[j & 1]    phase by phase by the softmax warps; by the loaders before tile j + 2, whose scores cannot be there yet
-//   pv_done[j & 1]   by the loaders before tile j + 2, whose product cannot be there yet; by a softmax warp for tile j - 1 behind s_full(j): the scores of tile j are issued behind pv_done(j - 2), and tile j + 1's product waits for this warp
-//   q_ready, o_done  have one phase
+// Phases (a wait by parity cannot tell a phase from the one two before it), for key tile j and row tile t:
+//   k_full, v_full [j % 3]   phase by phase by the MMA warp
+//   k_free, v_free [j % 3]   phase by phase by the loaders, before tile j + 3
+//   s_full[t][j & 1]         phase by phase by the row tile's softmax warps
+//   p_ready[t][j & 1]        phase by phase by the MMA warp
+//   pv_done[t]               phase by phase by the MMA warp, for tile j - 1 before the scores of tile j + 1; by a softmax warp for tile j - 1 behind
+//                            s_full[t](j): those scores are issued behind pv_done(j - 2), and tile j's product waits for this warp
+//   q_ready, o_done          have one phase
 struct PromptBars {
-    unsigned long long q_ready, k_full[2], v_full[2], s_full[2], p_ready[2], pv_done[2], o_done;
+    unsigned long long q_ready, o_done, k_full[kSlots], v_full[kSlots], k_free[kSlots], v_free[kSlots], s_full[kTiles][2], p_ready[kTiles][2], pv_done[kTiles];
     unsigned tmem;
     int failed;
 };
 
-__device__ __forceinline__ float log2_of(float x) { float y; asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+template <int HD> __host__ __device__ constexpr size_t prompt_smem() { return (size_t)kPromptRows * HD * 2 + 2 * kSlots * kPaKeys * HD * 2 + 1024; }
 
-template <int HD> __host__ __device__ constexpr size_t prompt_smem() { return (size_t)kPaRows * HD * 2 + 4 * kPaKeys * HD * 2 + 1024; }
-
-template <int HD, int CODE>
-__global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const swlm_kv8_cache c, const swlm_kv8_attend a, const RowsPlan p, int* status) {
+// GROUPS: scales of a key tile (blocks of 16, 32 or at least 64 tokens)
+template <int HD, int CODE, int GROUPS>
+__global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swlm_kv8_cache c, const swlm_kv8_attend a, const RowsPlan p, int* status) {
     constexpr int HALVES = HD / 64;                        // 128-byte halves of a row
     constexpr unsigned Q_HALF = kPaRows * 128, Q_BYTES = HALVES * Q_HALF, KV_HALF = kPaKeys * 128, KV_BYTES = HALVES * KV_HALF;
-    constexpr unsigned kTmemCols = 256, O_COL = 128;       // scores / probabilities 0..63 and 64..127, output from 128 on
+    constexpr unsigned kTmemCols = 512, O_COL = 256;       // scores / probabilities of row tile t in 128 t + 0..63 and 64..127, output in 256 + 128 t
     extern __shared__ __align__(1024) unsigned char prompt_raw[];
     unsigned char* const sm = prompt_raw + ((1024 - (smem_u32(prompt_raw) & 1023)) & 1023);
-    unsigned char *const q_sm = sm, *const k_sm = sm + Q_BYTES, *const v_sm = k_sm + 2 * KV_BYTES;
+    unsigned char *const q_sm = sm, *const k_sm = sm + kTiles * Q_BYTES, *const v_sm = k_sm + kSlots * KV_BYTES;
     __shared__ __align__(8) PromptBars bars;
     pdl_launch_dependents();
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int b = blockIdx.z, h = blockIdx.y, G = a.heads / c.kv_heads, span = min(a.max_len, c.capacity);
-    const int tile = p.row_tiles - 1 - (int)blockIdx.x / p.splits, split = (int)blockIdx.x % p.splits;   // the longest rows first
+    const int block = p.row_tiles - 1 - (int)blockIdx.x / p.splits, split = (int)blockIdx.x % p.splits;   // the longest rows first
     const Kv8Part part = kv8_part(b, a.lengths, a.counts, a.starts, a.n, a.rows);
-    const int rows = part.count * G, row0 = tile * kPaRows;
-    if (row0 >= rows) return;
-    const int end = visible(part, min(row0 + kPaRows - 1, rows - 1) / G, span);   // of the tile's last query: it sees most
+    const int rows = part.count * G, block0 = block * kPromptRows;
+    if (block0 >= rows) return;
+    const int end = visible(part, min(block0 + kPromptRows - 1, rows - 1) / G, span);   // of the CTA's last query: it sees most
     const int key_lo = split * p.chunk;
     if (split > 0 && key_lo >= end) return;
-    const int n_tiles = (max(min(end - key_lo, p.chunk), 0) + kPaKeys - 1) / kPaKeys;
+    // key tiles of either row tile (its last query's); the second one has as many as the first or more, or none where it has no rows
+    auto tiles_of = [&](int t) {
+        const int first = block0 + t * kPaRows;
+        return first < rows ? (max(min(visible(part, min(first + kPaRows - 1, rows - 1) / G, span) - key_lo, p.chunk), 0) + kPaKeys - 1) / kPaKeys : 0;
+    };
+    const int tiles0 = tiles_of(0), tiles1 = tiles_of(1), n_tiles = max(tiles0, tiles1);
     const size_t head = (size_t)b * c.kv_heads + h;
     const int block_shift = 31 - __clz(c.block);
     volatile int* const failed = &bars.failed;
     auto fail = [&](int code) { atomicExch_system(status, code); *failed = 1; };
 
     if (tid == 0) {
-        mbar_init(&bars.q_ready, 4);
+        mbar_init(&bars.q_ready, kSoftmaxWarps);
         mbar_init(&bars.o_done, 1);
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&bars.k_full[i], kLoadThreads / 32);
-            mbar_init(&bars.v_full[i], kLoadThreads / 32);
-            mbar_init(&bars.s_full[i], 1);
-            mbar_init(&bars.p_ready[i], 4);
-            mbar_init(&bars.pv_done[i], 1);
+        for (int i = 0; i < kSlots; ++i) {
+            mbar_init(&bars.k_full[i], kLoadWarps);
+            mbar_init(&bars.v_full[i], kLoadWarps);
+            mbar_init(&bars.k_free[i], 1);
+            mbar_init(&bars.v_free[i], 1);
+        }
+        for (int t = 0; t < kTiles; ++t) {
+            for (int i = 0; i < 2; ++i) { mbar_init(&bars.s_full[t][i], 1); mbar_init(&bars.p_ready[t][i], 4); }
+            mbar_init(&bars.pv_done[t], 1);
         }
         bars.failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -87,10 +102,13 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const swl
     pa_after();
     const unsigned tm = bars.tmem;
 
-    if (warp >= kMmaWarp) {
-        // ---- keys and values: codes in, fp16 out; warp kMmaWarp issues the products ------------------------------------------------------------
-        constexpr int PIECES = HD / 16, PER = kPaKeys * PIECES / kLoadThreads, STEP = kPaKeys / PER;   // 16-byte pieces of a token, of this thread in a tile
-        const int lt = tid - kSoftmaxThreads, piece = lt % PIECES, key = lt / PIECES;                  // (keys key, key + STEP, ...)
+    if (warp > kMmaWarp) {
+        // ---- keys and values: codes in, fp16 out ------------------------------------------------------------------------------------------------
+        // A turn of a warp: 32 pieces of 16 bytes, that is ROWS tokens; its lanes are four pieces of a token's half, two tokens, (the halves,) ... The
+        // eight lanes of a phase of the stores below then meet different banks. Warp w has turns w, w + 3, ...
+        constexpr int ROWS = 512 / HD, TURNS = kPaKeys / ROWS, PER = (TURNS + kLoadWarps - 1) / kLoadWarps, STEP = kLoadWarps * ROWS;
+        const int w = warp - kMmaWarp - 1;
+        const int piece = (lane & 3) + (HD == 128 ? (lane >> 3 & 1) * 4 : 0), key = w * ROWS + (HD == 128 ? (lane >> 4) * 2 + (lane >> 2 & 1) : lane >> 2);   // key, key + STEP, ...
         const size_t at = (head * c.capacity + key_lo + key) * HD + piece * 16;
         const unsigned char* kg = static_cast<const unsigned char*>(c.k) + at;
         const unsigned char* vg = static_cast<const unsigned char*>(c.v) + at;
@@ -99,80 +117,105 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const swl
             const int slot = key_lo + j * kPaKeys + key;
 #pragma unroll
             for (int i = 0; i < PER; ++i)
-                r[i] = slot + i * STEP < end ? __ldg(reinterpret_cast<const uint4*>(src + i * STEP * HD)) : make_uint4(0, 0, 0, 0);   // (nothing that may be NaN)
+                r[i] = key + i * STEP < kPaKeys && slot + i * STEP < end ? __ldg(reinterpret_cast<const uint4*>(src + i * STEP * HD)) : make_uint4(0, 0, 0, 0);   // (nothing that may be NaN)
         };
-        // Two chunks of eight values per piece. The pieces of a row's second half go the other way round, so that the eight lanes of a phase meet
-        // different banks; STEP is a multiple of 8, so that all of this thread's rows have the same swizzle
-        static_assert(STEP % 8 == 0, "one swizzle");
-        const int chunk = piece * 2 & 7;
-        const bool other = piece >= 4;
-        const unsigned off = (piece >> 2) * KV_HALF + key * 128, off0 = off + (((chunk + other) ^ (key & 7)) << 4), off1 = off + (((chunk + !other) ^ (key & 7)) << 4);
+        const unsigned off = (piece >> 2) * KV_HALF + key * 128, off0 = off + (((piece * 2 & 7) ^ (key & 7)) << 4), off1 = off + (((piece * 2 & 7 | 1) ^ (key & 7)) << 4);
         auto store = [&](unsigned char* dst, const uint4 (&r)[PER]) {
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
-                const unsigned w[4] = {prepared<CODE>(other ? r[i].z : r[i].x), prepared<CODE>(other ? r[i].w : r[i].y), prepared<CODE>(other ? r[i].x : r[i].z),
-                                       prepared<CODE>(other ? r[i].y : r[i].w)};
-                *reinterpret_cast<uint4*>(dst + off0 + i * STEP * 128) = make_uint4(pair_of<CODE, 0>(w[0]), pair_of<CODE, 1>(w[0]), pair_of<CODE, 0>(w[1]), pair_of<CODE, 1>(w[1]));
-                *reinterpret_cast<uint4*>(dst + off1 + i * STEP * 128) = make_uint4(pair_of<CODE, 0>(w[2]), pair_of<CODE, 1>(w[2]), pair_of<CODE, 0>(w[3]), pair_of<CODE, 1>(w[3]));
+                if (key + i * STEP >= kPaKeys) continue;
+                const unsigned flip = (i * STEP & 4) << 4;   // (of the swizzle, where a step is an odd number of fours)
+                const unsigned w[4] = {prepared<CODE>(r[i].x), prepared<CODE>(r[i].y), prepared<CODE>(r[i].z), prepared<CODE>(r[i].w)};
+                *reinterpret_cast<uint4*>(dst + (off0 ^ flip) + i * STEP * 128) = make_uint4(pair_of<CODE, 0>(w[0]), pair_of<CODE, 1>(w[0]), pair_of<CODE, 0>(w[1]), pair_of<CODE, 1>(w[1]));
+                *reinterpret_cast<uint4*>(dst + (off1 ^ flip) + i * STEP * 128) = make_uint4(pair_of<CODE, 0>(w[2]), pair_of<CODE, 1>(w[2]), pair_of<CODE, 0>(w[3]), pair_of<CODE, 1>(w[3]));
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
         };
-        const bool issues = warp == kMmaWarp, el = elect_one();
-        const unsigned qd = umma_desc_lo(smem_u32(q_sm)), kd = umma_desc_lo(smem_u32(k_sm)), vd = pa_desc_mn_lo(smem_u32(v_sm), KV_HALF);
-        auto scores = [&](int j) {
-            pa_after();
-            if (el) {
-#pragma unroll
-                for (int kk = 0; kk < HD / 16; ++kk)
-                    pa_mma_ss(tm + (unsigned)(j & 1) * 64u, qd + (kk >> 2) * (Q_HALF / 16) + 2 * (kk & 3), kd + (j & 1) * (KV_BYTES / 16) + (kk >> 2) * (KV_HALF / 16) + 2 * (kk & 3),
-                              pa_idesc(kPaKeys, false, false), kk > 0 ? 1u : 0u);
-                umma_commit(&bars.s_full[j & 1]);
-            }
-            __syncwarp();
-        };
-        auto product = [&](int j) {   // false: a wait expired
-            if (!mbar_wait_warp(&bars.p_ready[j & 1], (unsigned)((j >> 1) & 1)) || !mbar_wait_warp(&bars.v_full[j & 1], (unsigned)((j >> 1) & 1))) return false;
-            pa_after();
-            if (el) {
-#pragma unroll
-                for (int kk = 0; kk < kPaKeys / 16; ++kk)
-                    pa_mma_ts(tm + O_COL, tm + (unsigned)(j & 1) * 64u + 8u * kk, vd + (j & 1) * (KV_BYTES / 16) + kk * (2048 / 16), pa_idesc(HD, true, false), kk > 0 || j > 0 ? 1u : 0u);
-                umma_commit(&bars.pv_done[j & 1]);
-            }
-            __syncwarp();
-            return true;
-        };
         bool ok = true;
         if (n_tiles) { load(kg, kr, 0); load(vg, vr, 0); }
-        for (int j = 0; j < n_tiles; ++j) {
+        for (int j = 0, slot = 0, round = 0; j < n_tiles; ++j) {
             kg += kPaKeys * HD;
             vg += kPaKeys * HD;
-            if (*failed || (j >= 2 && !mbar_wait_warp(&bars.s_full[j & 1], (unsigned)(((j - 2) >> 1) & 1)))) { ok = false; break; }
-            store(k_sm + (j & 1) * KV_BYTES, kr);
-            if (lane == 0) pa_arrive(&bars.k_full[j & 1]);
+            if (*failed || (round > 0 && !mbar_wait_warp(&bars.k_free[slot], (unsigned)((round - 1) & 1)))) { ok = false; break; }
+            store(k_sm + slot * KV_BYTES, kr);
+            if (lane == 0) pa_arrive(&bars.k_full[slot]);
             if (j + 1 < n_tiles) load(kg, kr, j + 1);
-            // (the product of tile j - 2 has read its values, and its probabilities in the region of tile j's scores)
-            if (j >= 2 && !mbar_wait_warp(&bars.pv_done[j & 1], (unsigned)(((j - 2) >> 1) & 1))) { ok = false; break; }
-            if (issues) {
-                if ((j == 0 && !mbar_wait_warp(&bars.q_ready, 0u)) || !mbar_wait_warp(&bars.k_full[j & 1], (unsigned)((j >> 1) & 1))) { ok = false; break; }
-                scores(j);
-            }
-            store(v_sm + (j & 1) * KV_BYTES, vr);
-            if (lane == 0) pa_arrive(&bars.v_full[j & 1]);
+            if (round > 0 && !mbar_wait_warp(&bars.v_free[slot], (unsigned)((round - 1) & 1))) { ok = false; break; }
+            store(v_sm + slot * KV_BYTES, vr);
+            if (lane == 0) pa_arrive(&bars.v_full[slot]);
             if (j + 1 < n_tiles) load(vg, vr, j + 1);
-            if (issues && j > 0 && !product(j - 1)) { ok = false; break; }
-        }
-        if (issues) {
-            if (ok && n_tiles) ok = product(n_tiles - 1);
-            if (el) umma_commit(&bars.o_done);   // also behind whatever was issued before a failure
-            __syncwarp();
-            ok = mbar_wait_warp(&bars.o_done, 0u) && ok;   // tensor memory is not freed under MMAs in flight
+            if (++slot == kSlots) { slot = 0; ++round; }
         }
         if (!ok && lane == 0) fail(31);
         __syncwarp();
+    } else if (warp == kMmaWarp) {
+        const bool el = elect_one();
+        const unsigned qd = umma_desc_lo(smem_u32(q_sm)), kd = umma_desc_lo(smem_u32(k_sm)), vd = pa_desc_mn_lo(smem_u32(v_sm), KV_HALF);
+        auto scores = [&](int j, int slot, int t) {
+            if (el) {
+#pragma unroll
+                for (int kk = 0; kk < HD / 16; ++kk)
+                    pa_mma_ss(tm + t * 128u + (unsigned)(j & 1) * 64u, qd + t * (Q_BYTES / 16) + (kk >> 2) * (Q_HALF / 16) + 2 * (kk & 3),
+                              kd + slot * (KV_BYTES / 16) + (kk >> 2) * (KV_HALF / 16) + 2 * (kk & 3), pa_idesc(kPaKeys, false, false), kk > 0 ? 1u : 0u);
+                umma_commit(&bars.s_full[t][j & 1]);
+            }
+            __syncwarp();
+        };
+        auto release = [&](unsigned long long* bar) {   // behind everything issued so far
+            if (el) umma_commit(bar);
+            __syncwarp();
+        };
+        bool ok = true;
+        if (n_tiles) {
+            ok = mbar_wait_warp(&bars.q_ready, 0u) && mbar_wait_warp(&bars.k_full[0], 0u);
+            if (ok) {
+                pa_after();
+                for (int t = 0; t < kTiles; ++t)
+                    if ((t ? tiles1 : tiles0) > 0) scores(0, 0, t);
+                release(&bars.k_free[0]);
+            }
+        }
+        for (int j = 0, slot = 0, phase = 0; j < n_tiles && ok; ++j) {
+            int next = slot + 1, next_phase = phase;
+            if (next == kSlots) { next = 0; next_phase ^= 1; }
+            if (j + 1 < n_tiles) {
+                if (!mbar_wait_warp(&bars.k_full[next], (unsigned)next_phase)) { ok = false; break; }
+                for (int t = 0; t < kTiles && ok; ++t) {
+                    if (j + 1 >= (t ? tiles1 : tiles0)) continue;
+                    // the region of tile j + 1 held the probabilities of tile j - 1
+                    if (j > 0 && !mbar_wait_warp(&bars.pv_done[t], (unsigned)((j - 1) & 1))) { ok = false; break; }
+                    pa_after();
+                    scores(j + 1, next, t);
+                }
+                if (!ok) break;
+                release(&bars.k_free[next]);
+            }
+            if (!mbar_wait_warp(&bars.v_full[slot], (unsigned)phase)) { ok = false; break; }
+            for (int t = 0; t < kTiles && ok; ++t) {
+                if (j >= (t ? tiles1 : tiles0)) continue;
+                if (!mbar_wait_warp(&bars.p_ready[t][j & 1], (unsigned)((j >> 1) & 1))) { ok = false; break; }
+                pa_after();
+                if (el) {
+#pragma unroll
+                    for (int kk = 0; kk < kPaKeys / 16; ++kk)
+                        pa_mma_ts(tm + O_COL + t * 128u, tm + t * 128u + (unsigned)(j & 1) * 64u + 8u * kk, vd + slot * (KV_BYTES / 16) + kk * (2048 / 16), pa_idesc(HD, true, false),
+                                  kk > 0 || j > 0 ? 1u : 0u);
+                    umma_commit(&bars.pv_done[t]);
+                }
+                __syncwarp();
+            }
+            if (ok) release(&bars.v_free[slot]);
+            slot = next;
+            phase = next_phase;
+        }
+        if (el) umma_commit(&bars.o_done);   // also behind whatever was issued before a failure
+        __syncwarp();
+        ok = mbar_wait_warp(&bars.o_done, 0u) && ok;   // tensor memory is not freed under MMAs in flight
+        if (!ok && lane == 0) fail(32);
+        __syncwarp();
     } else {
-        const int r = tid, row = row0 + r, i = min(row, rows - 1) / G;
+        const int t = warp >> 2, r = tid & (kPaRows - 1), row = block0 + tid, i = min(row, rows - 1) / G, tiles = t ? tiles1 : tiles0;   // r: of the row tile
         const bool row_ok = row < rows, f16 = a.dtype == SWLM_KV8_FP16;
         const int limit = visible(part, i, span);   // (rows past the last one attend what it does; they are not stored)
         float factor;
@@ -198,37 +241,38 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const swl
                 v.x = pack_half(x[0] * up, x[1] * up); v.y = pack_half(x[2] * up, x[3] * up);
                 v.z = pack_half(x[4] * up, x[5] * up); v.w = pack_half(x[6] * up, x[7] * up);
                 const int at = r * 128 + ((((d >> 3) & 7) ^ (r & 7)) << 4);
-                *reinterpret_cast<uint4*>(q_sm + (d >> 6) * Q_HALF + at) = v;
-                if (keeps) *reinterpret_cast<uint4*>(reinterpret_cast<unsigned char*>(p.q16) + (((head * p.row_tiles + tile) * 2 + (r >> 6)) * HALVES + (d >> 6)) * 8192 + (at & 8191)) = v;
+                *reinterpret_cast<uint4*>(q_sm + t * Q_BYTES + (d >> 6) * Q_HALF + at) = v;
+                if (keeps) *reinterpret_cast<uint4*>(reinterpret_cast<unsigned char*>(p.q16) + (((head * p.row_tiles + block) * (kPromptRows / 64) + (tid >> 6)) * HALVES + (d >> 6)) * 8192 + (at & 8191)) = v;
             }
-            if (keeps) p.q_factor[(head * p.row_tiles + tile) * kPaRows + r] = row_ok ? factor : 0.f;
+            if (keeps) p.q_factor[(head * p.row_tiles + block) * kPromptRows + tid] = row_ok ? factor : 0.f;
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) pa_arrive(&bars.q_ready);
         }
         // ---- softmax, a thread per row -------------------------------------------------------------------------------------------------------
-        const unsigned lanes = (unsigned)(warp * 32) << 16;
+        const unsigned lanes = (unsigned)((warp & 3) * 32) << 16, out_col = tm + lanes + O_COL + t * 128u;
         const float* ks = c.k_scale + head * (c.capacity >> block_shift);
         const float* vs = c.v_scale + head * (c.capacity >> block_shift);
         float m_ref = -INFINITY, l_run = 0.f, v_ref = 0x1p-100f, v_inv = 0x1p100f * kValueUnit;
-        float kn[4], vn[4];   // the next tile's scales, of 16 keys each; 0 behind the last token
+        constexpr int KEYS = kPaKeys / GROUPS;
+        float kn[GROUPS], vn[GROUPS];   // the next tile's scales; 0 behind the last token
         auto scales = [&](int j) {
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int slot = key_lo + j * kPaKeys + g * 16;
+            for (int g = 0; g < GROUPS; ++g) {
+                const int slot = key_lo + j * kPaKeys + g * KEYS;
                 kn[g] = slot < end ? __ldg(ks + (slot >> block_shift)) : 0.f;
                 vn[g] = slot < end ? __ldg(vs + (slot >> block_shift)) : 0.f;
             }
         };
-        if (n_tiles) scales(0);
+        if (tiles) scales(0);
         bool ok = true;
-        for (int j = 0; j < n_tiles; ++j) {
-            const unsigned region = tm + lanes + (unsigned)(j & 1) * 64u;
-            float fk[4], vt[4];
+        for (int j = 0; j < tiles; ++j) {
+            const unsigned region = tm + lanes + t * 128u + (unsigned)(j & 1) * 64u;
+            float fk[GROUPS], vt[GROUPS];
 #pragma unroll
-            for (int g = 0; g < 4; ++g) { fk[g] = factor * kn[g]; vt[g] = vn[g]; }
-            if (j + 1 < n_tiles) scales(j + 1);
-            if (!mbar_wait_warp(&bars.s_full[j & 1], (unsigned)((j >> 1) & 1))) { ok = false; break; }
+            for (int g = 0; g < GROUPS; ++g) { fk[g] = factor * kn[g]; vt[g] = vn[g]; }
+            if (j + 1 < tiles) scales(j + 1);
+            if (!mbar_wait_warp(&bars.s_full[t][j & 1], (unsigned)((j >> 1) & 1))) { ok = false; break; }
             pa_after();
             unsigned v[64];
             pa_ld32(region, v);
@@ -238,75 +282,80 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const swl
             const bool masked = !__all_sync(0xffffffffu, key0 + kPaKeys <= limit);
             float top = -INFINITY;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                float t = -INFINITY;
-                if (masked)
+            for (int g = 0; g < GROUPS; ++g) {
+                float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};   // (four chains)
+                if (masked) {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) t = fmaxf(t, key0 + g * 16 + e < limit ? __uint_as_float(v[g * 16 + e]) : -INFINITY);
-                else
+                    for (int e = 0; e < KEYS; ++e) most[e & 3] = fmaxf(most[e & 3], key0 + g * KEYS + e < limit ? __uint_as_float(v[g * KEYS + e]) : -INFINITY);
+                } else {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) t = fmaxf(t, __uint_as_float(v[g * 16 + e]));
-                if (t > -INFINITY) top = fmaxf(top, t * fk[g]);   // (factors are not negative: the largest score stays the largest)
+                    for (int e = 0; e < KEYS; ++e) most[e & 3] = fmaxf(most[e & 3], __uint_as_float(v[g * KEYS + e]));
+                }
+                const float x = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+                if (x > -INFINITY) top = fmaxf(top, x * fk[g]);   // (factors are not negative: the largest score stays the largest)
             }
             const bool moves = top > m_ref + kSlack;
-            const float v_top = fmaxf(fmaxf(vt[0], vt[1]), fmaxf(vt[2], vt[3]));
+            float v_top = vt[0];
+#pragma unroll
+            for (int g = 1; g < GROUPS; ++g) v_top = fmaxf(v_top, vt[g]);
             if (__any_sync(0xffffffffu, moves || v_top > v_ref)) {
                 float corr = moves ? pa_exp2(m_ref - top) : 1.f;   // 0 for a row's first keys
                 if (moves) { m_ref = top; l_run *= corr; }
                 if (v_top > v_ref) { corr *= v_ref / v_top; v_ref = v_top; v_inv = kValueUnit / v_top; }
                 if (j > 0) {   // the output so far: complete, and the next product waits for this warp
-                    if (!mbar_wait_warp(&bars.pv_done[(j - 1) & 1], (unsigned)(((j - 1) >> 1) & 1))) { ok = false; break; }
+                    if (!mbar_wait_warp(&bars.pv_done[t], (unsigned)((j - 1) & 1))) { ok = false; break; }
                     pa_after();
 #pragma unroll 1
                     for (int d = 0; d < HD; d += 16) {
                         unsigned o[16];
-                        pa_ld16(tm + lanes + O_COL + d, o);
+                        pa_ld16(out_col + d, o);
                         pa_wait_ld();
 #pragma unroll
                         for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-                        pa_st16(tm + lanes + O_COL + d, o);
+                        pa_st16(out_col + d, o);
                     }
                     pa_wait_st();
                 }
             }
             const float base = m_ref == -INFINITY ? 0.f : m_ref;   // nothing attended so far: all probabilities 0
-            float unit[4];
+            float unit[GROUPS];
             bool folds = !masked;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
+            for (int g = 0; g < GROUPS; ++g) {
                 unit[g] = vt[g] * v_inv;
                 folds = folds && unit[g] >= kFoldUnit * kValueUnit;
             }
             if (folds) {
                 // the unit goes into the exponent, and out of the sum again
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
+                for (int g = 0; g < GROUPS; ++g) {
                     const float shift = log2_of(unit[g]) - base;
                     const float2 fk2 = make_float2(fk[g], fk[g]), shift2 = make_float2(shift, shift);
-                    float2 sum = make_float2(0.f, 0.f);
+                    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        float2 x = fma2(make_float2(__uint_as_float(v[g * 16 + e]), __uint_as_float(v[g * 16 + e + 1])), fk2, shift2);
+                    for (int e = 0; e < KEYS; e += 2) {
+                        float2 x = fma2(make_float2(__uint_as_float(v[g * KEYS + e]), __uint_as_float(v[g * KEYS + e + 1])), fk2, shift2);
                         x = make_float2(pa_exp2(x.x), pa_exp2(x.y));
-                        sum = add2(sum, x);
-                        v[g * 8 + e / 2] = pack_half(x.x, x.y);
+                        sum[e >> 1 & 1] = add2(sum[e >> 1 & 1], x);
+                        v[(g * KEYS + e) / 2] = pack_half(x.x, x.y);
                     }
-                    l_run += __fdividef(sum.x + sum.y, unit[g]);
+                    const float2 all = add2(sum[0], sum[1]);
+                    l_run += __fdividef(all.x + all.y, unit[g]);
                 }
             } else {
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
+                for (int g = 0; g < GROUPS; ++g) {
 #pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
+                    for (int e = 0; e < KEYS; e += 2) {
                         float w[2];
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
-                            const bool sees = key0 + g * 16 + e + k < limit;   // (what a row does not attend may lie in a block that is NaN)
-                            const float x = sees ? pa_exp2(fmaf(__uint_as_float(v[g * 16 + e + k]), fk[g], -base)) : 0.f;
+                            const bool sees = key0 + g * KEYS + e + k < limit;   // (what a row does not attend may lie in a block that is NaN)
+                            const float x = sees ? pa_exp2(fmaf(__uint_as_float(v[g * KEYS + e + k]), fk[g], -base)) : 0.f;
                             l_run += x;
                             w[k] = sees ? x * unit[g] : 0.f;
                         }
-                        v[g * 8 + e / 2] = pack_half(w[0], w[1]);
+                        v[(g * KEYS + e) / 2] = pack_half(w[0], w[1]);
                     }
                 }
             }
@@ -314,7 +363,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const swl
             pa_wait_st();
             pa_before();
             __syncwarp();
-            if (lane == 0) pa_arrive(&bars.p_ready[j & 1]);
+            if (lane == 0) pa_arrive(&bars.p_ready[t][j & 1]);
         }
         if (ok && (!mbar_wait_warp(&bars.o_done, 0u) || *failed)) ok = false;
         if (!ok) fail(33);
@@ -322,16 +371,16 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const swl
         pa_after();
         if (ok) {
             const bool whole = end <= p.chunk;   // this CTA has all of the tile's slots
-            const size_t at = ((head * p.row_tiles + tile) * p.splits + split) * kPaRows + r;
+            const size_t at = ((head * p.row_tiles + block) * p.splits + split) * kPromptRows + tid;
             const float unit = v_ref * (1.f / kValueUnit);
             if (row_ok && (!whole || p.ml_always)) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m_ref, l_run);
-            if (p.q_shift && (whole || !row_ok)) p.q_shift[(head * p.row_tiles + tile) * kPaRows + r] = row_ok ? row_shift_of(m_ref, l_run) : -INFINITY;
+            if (p.q_shift && (whole || !row_ok)) p.q_shift[(head * p.row_tiles + block) * kPromptRows + tid] = row_ok ? row_shift_of(m_ref, l_run) : -INFINITY;
             unsigned short* dst = static_cast<unsigned short*>(a.out) + (int64_t)(part.start + i) * a.out_stride + (size_t)(h * G + min(row, rows - 1) - i * G) * HD;
 #pragma unroll 1
             for (int d = 0; d < HD; d += 16) {
                 unsigned o[16] = {};
-                if (n_tiles) {
-                    pa_ld16(tm + lanes + O_COL + d, o);
+                if (tiles) {
+                    pa_ld16(out_col + d, o);
                     pa_wait_ld();
                 }
                 if (row_ok)
@@ -403,9 +452,9 @@ __global__ void __launch_bounds__(kWeightThreads, 2) kv8_weights_kernel(const sw
         // Tile t of this CTA (slot t & 3): its copies are asked for behind s_free(t - 4), so its slot, rows and scores' region are free then
         const bool el = elect_one();
         const unsigned kd = umma_desc_lo(smem_u32(k_sm)), qd = umma_desc_lo(smem_u32(q_sm));
-        const unsigned char* q = reinterpret_cast<const unsigned char*>(p.q16) + (head * p.row_tiles * 2 + tile0) * Q_BYTES;
-        const float* factor = p.q_factor + head * p.row_tiles * kPaRows + (size_t)tile0 * kWeightRows;
-        const float* shift = p.q_shift + head * p.row_tiles * kPaRows + (size_t)tile0 * kWeightRows;
+        const unsigned char* q = reinterpret_cast<const unsigned char*>(p.q16) + (head * p.row_tiles * (kPromptRows / kWeightRows) + tile0) * Q_BYTES;
+        const float* factor = p.q_factor + head * p.row_tiles * kPromptRows + (size_t)tile0 * kWeightRows;
+        const float* shift = p.q_shift + head * p.row_tiles * kPromptRows + (size_t)tile0 * kWeightRows;
         int asked = 0;
         auto ask = [&]() {
             if (el) {
@@ -509,8 +558,9 @@ __global__ void __launch_bounds__(kWeightThreads, 2) kv8_weights_kernel(const sw
 
 template <int HD, int CODE>
 int launch_prompt(const swlm_kv8_cache& c, const swlm_kv8_attend& a, const RowsPlan& p, int* status, cudaStream_t s) {
-    const cudaError_t e = launch_k(kv8_prompt_kernel<HD, CODE>, dim3((unsigned)(p.row_tiles * p.splits), (unsigned)c.kv_heads, (unsigned)c.batch), dim3(kPromptThreads),
-                                   prompt_smem<HD>(), s, c, a, p, status);
+    const dim3 grid((unsigned)(p.row_tiles * p.splits), (unsigned)c.kv_heads, (unsigned)c.batch);
+    auto launch = [&](auto kernel) { return launch_k(kernel, grid, dim3(kPromptThreads), prompt_smem<HD>(), s, c, a, p, status); };
+    const cudaError_t e = c.block >= 64 ? launch(kv8_prompt_kernel<HD, CODE, 1>) : c.block == 32 ? launch(kv8_prompt_kernel<HD, CODE, 2>) : launch(kv8_prompt_kernel<HD, CODE, 4>);
     return e == cudaSuccess ? SWLM_OK : cuda_fail(e, "kv8 prompt attention launch");
 }
 template <int HD, int CODE>
@@ -523,7 +573,9 @@ int launch_weights(const swlm_kv8_cache& c, const swlm_kv8_attend& a, const Rows
 template <int HD, int CODE>
 int init_prompt() {
     SWLM_CUDA(cudaFuncSetAttribute(kv8_weights_kernel<HD, CODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)weights_smem<HD>()));
-    SWLM_CUDA(cudaFuncSetAttribute(kv8_prompt_kernel<HD, CODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prompt_smem<HD>()));
+    SWLM_CUDA(cudaFuncSetAttribute(kv8_prompt_kernel<HD, CODE, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prompt_smem<HD>()));
+    SWLM_CUDA(cudaFuncSetAttribute(kv8_prompt_kernel<HD, CODE, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prompt_smem<HD>()));
+    SWLM_CUDA(cudaFuncSetAttribute(kv8_prompt_kernel<HD, CODE, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prompt_smem<HD>()));
     return SWLM_OK;
 }
 
