@@ -591,8 +591,8 @@ RowsPlan rows_plan(const swlm_kv8_cache& c, const swlm_kv8_attend& a, size_t* by
     const long long groups = (long long)c.batch * c.kv_heads * p.row_tiles, units = groups * ((span + kUnit - 1) / kUnit);
     bool several;   // parts that have to be joined
     if (p.tiles > 2) {
-        // runs of at least eight key tiles, as many as make two CTAs per SM (one after the other)
-        const long long want = std::max<long long>(1, 2 * kSms / groups), most = (span + 8 * kPromptKeys - 1) / (8 * kPromptKeys);
+        // runs of at least four key tiles, as many as make two CTAs per SM (one after the other)
+        const long long want = std::max<long long>(1, 2 * kSms / groups), most = (span + 4 * kPromptKeys - 1) / (4 * kPromptKeys);
         const int runs = (int)std::min(want, most);
         p.chunk = ((span + runs - 1) / runs + kPromptKeys - 1) / kPromptKeys * kPromptKeys;
         p.splits = (span + p.chunk - 1) / p.chunk;

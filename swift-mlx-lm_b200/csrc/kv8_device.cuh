@@ -159,7 +159,7 @@ __device__ __forceinline__ Parts parts_of(const RowsPlan& p, const Kv8Part& part
 }
 
 // The kernel of many rows (kv8_prompt.cu): rows of a CTA, keys of a tile.
-constexpr int kPromptRows = 256, kPromptKeys = 64;
+constexpr int kPromptRows = 256, kPromptKeys = 128;
 
 }  // namespace kv8
 

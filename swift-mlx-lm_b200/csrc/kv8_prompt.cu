@@ -22,34 +22,32 @@ using namespace kv8;
 namespace {
 
 constexpr int kTiles = kPromptRows / kPaRows;   // row tiles of a CTA
-static_assert(kTiles == 2 && kPromptKeys == kPaKeys, "the shared helpers' tiles");
+static_assert(kTiles == 2, "tensor memory holds two row tiles");
 constexpr int kSoftmaxWarps = 4 * kTiles, kMmaWarp = kSoftmaxWarps, kLoadWarps = 3;
 constexpr int kPromptThreads = (kSoftmaxWarps + 1 + kLoadWarps) * 32;   // (with 13 warps a thread would have 128 registers and not 168: 456 us, spilled)
-constexpr int kSlots = 3;               // key and value tiles in shared memory
+constexpr int kSlots = 2;               // key and value tiles in shared memory
 constexpr float kFoldUnit = 0x1p-20f;   // value scales down to this part of the largest go into the exponent
 
-// Phases (a wait by parity cannot tell a phase from the one two before it), for key tile j and row tile t:
-//   k_full, v_full [j % 3]   phase by phase by the MMA warp
-//   k_free, v_free [j % 3]   phase by phase by the loaders, before tile j + 3
-//   s_full[t][j & 1]         phase by phase by the row tile's softmax warps
-//   p_ready[t][j & 1]        phase by phase by the MMA warp
-//   pv_done[t]               phase by phase by the MMA warp, for tile j - 1 before the scores of tile j + 1; by a softmax warp for tile j - 1 behind
-//                            s_full[t](j): those scores are issued behind pv_done(j - 2), and tile j's product waits for this warp
+// Phases (a wait by parity cannot tell a phase from the one two before it), for key tile j and row tile t; all are waited for phase by phase:
+//   k_full, v_full [j & 1]   by the MMA warp
+//   k_free, v_free [j & 1]   by the loaders, before tile j + 2
+//   s_full[t]                by the row tile's softmax warps. The scores of tile j are issued behind pv_done(j - 1), so that behind it the output may be scaled
+//   p_ready[t], pv_done[t]   by the MMA warp
 //   q_ready, o_done          have one phase
 struct PromptBars {
-    unsigned long long q_ready, o_done, k_full[kSlots], v_full[kSlots], k_free[kSlots], v_free[kSlots], s_full[kTiles][2], p_ready[kTiles][2], pv_done[kTiles];
+    unsigned long long q_ready, o_done, k_full[kSlots], v_full[kSlots], k_free[kSlots], v_free[kSlots], s_full[kTiles], p_ready[kTiles], pv_done[kTiles];
     unsigned tmem;
     int failed;
 };
 
-template <int HD> __host__ __device__ constexpr size_t prompt_smem() { return (size_t)kPromptRows * HD * 2 + 2 * kSlots * kPaKeys * HD * 2 + 1024; }
+template <int HD> __host__ __device__ constexpr size_t prompt_smem() { return (size_t)kPromptRows * HD * 2 + 2 * kSlots * kPromptKeys * HD * 2 + 1024; }
 
-// GROUPS: scales of a key tile (blocks of 16, 32 or at least 64 tokens)
+// GROUPS: scales of a key tile (blocks of 16, 32, 64 or 128 tokens: 8, 4, 2, 1)
 template <int HD, int CODE, int GROUPS>
 __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swlm_kv8_cache c, const swlm_kv8_attend a, const RowsPlan p, int* status) {
     constexpr int HALVES = HD / 64;                        // 128-byte halves of a row
-    constexpr unsigned Q_HALF = kPaRows * 128, Q_BYTES = HALVES * Q_HALF, KV_HALF = kPaKeys * 128, KV_BYTES = HALVES * KV_HALF;
-    constexpr unsigned kTmemCols = 512, O_COL = 256;       // scores / probabilities of row tile t in 128 t + 0..63 and 64..127, output in 256 + 128 t
+    constexpr unsigned Q_HALF = kPaRows * 128, Q_BYTES = HALVES * Q_HALF, KV_HALF = kPromptKeys * 128, KV_BYTES = HALVES * KV_HALF;
+    constexpr unsigned kTmemCols = 512, O_COL = 256;       // scores / probabilities of row tile t from 128 t on, output from 256 + 128 t on
     extern __shared__ __align__(1024) unsigned char prompt_raw[];
     unsigned char* const sm = prompt_raw + ((1024 - (smem_u32(prompt_raw) & 1023)) & 1023);
     unsigned char *const q_sm = sm, *const k_sm = sm + kTiles * Q_BYTES, *const v_sm = k_sm + kSlots * KV_BYTES;
@@ -68,7 +66,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
     // key tiles of either row tile (its last query's); the second one has as many as the first or more, or none where it has no rows
     auto tiles_of = [&](int t) {
         const int first = block0 + t * kPaRows;
-        return first < rows ? (max(min(visible(part, min(first + kPaRows - 1, rows - 1) / G, span) - key_lo, p.chunk), 0) + kPaKeys - 1) / kPaKeys : 0;
+        return first < rows ? (max(min(visible(part, min(first + kPaRows - 1, rows - 1) / G, span) - key_lo, p.chunk), 0) + kPromptKeys - 1) / kPromptKeys : 0;
     };
     const int tiles0 = tiles_of(0), tiles1 = tiles_of(1), n_tiles = max(tiles0, tiles1);
     const size_t head = (size_t)b * c.kv_heads + h;
@@ -86,7 +84,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
             mbar_init(&bars.v_free[i], 1);
         }
         for (int t = 0; t < kTiles; ++t) {
-            for (int i = 0; i < 2; ++i) { mbar_init(&bars.s_full[t][i], 1); mbar_init(&bars.p_ready[t][i], 4); }
+            mbar_init(&bars.s_full[t], 1);
+            mbar_init(&bars.p_ready[t], 4);
             mbar_init(&bars.pv_done[t], 1);
         }
         bars.failed = 0;
@@ -106,7 +105,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
         // ---- keys and values: codes in, fp16 out ------------------------------------------------------------------------------------------------
         // A turn of a warp: 32 pieces of 16 bytes, that is ROWS tokens; its lanes are four pieces of a token's half, two tokens, (the halves,) ... The
         // eight lanes of a phase of the stores below then meet different banks. Warp w has turns w, w + 3, ...
-        constexpr int ROWS = 512 / HD, TURNS = kPaKeys / ROWS, PER = (TURNS + kLoadWarps - 1) / kLoadWarps, STEP = kLoadWarps * ROWS;
+        constexpr int ROWS = 512 / HD, TURNS = kPromptKeys / ROWS, PER = (TURNS + kLoadWarps - 1) / kLoadWarps, STEP = kLoadWarps * ROWS;
         const int w = warp - kMmaWarp - 1;
         const int piece = (lane & 3) + (HD == 128 ? (lane >> 3 & 1) * 4 : 0), key = w * ROWS + (HD == 128 ? (lane >> 4) * 2 + (lane >> 2 & 1) : lane >> 2);   // key, key + STEP, ...
         const size_t at = (head * c.capacity + key_lo + key) * HD + piece * 16;
@@ -114,16 +113,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
         const unsigned char* vg = static_cast<const unsigned char*>(c.v) + at;
         uint4 kr[PER], vr[PER];
         auto load = [&](const unsigned char* src, uint4 (&r)[PER], int j) {
-            const int slot = key_lo + j * kPaKeys + key;
+            const int slot = key_lo + j * kPromptKeys + key;
 #pragma unroll
             for (int i = 0; i < PER; ++i)
-                r[i] = key + i * STEP < kPaKeys && slot + i * STEP < end ? __ldg(reinterpret_cast<const uint4*>(src + i * STEP * HD)) : make_uint4(0, 0, 0, 0);   // (nothing that may be NaN)
+                r[i] = key + i * STEP < kPromptKeys && slot + i * STEP < end ? __ldg(reinterpret_cast<const uint4*>(src + i * STEP * HD)) : make_uint4(0, 0, 0, 0);   // (nothing that may be NaN)
         };
         const unsigned off = (piece >> 2) * KV_HALF + key * 128, off0 = off + (((piece * 2 & 7) ^ (key & 7)) << 4), off1 = off + (((piece * 2 & 7 | 1) ^ (key & 7)) << 4);
         auto store = [&](unsigned char* dst, const uint4 (&r)[PER]) {
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
-                if (key + i * STEP >= kPaKeys) continue;
+                if (key + i * STEP >= kPromptKeys) continue;
                 const unsigned flip = (i * STEP & 4) << 4;   // (of the swizzle, where a step is an odd number of fours)
                 const unsigned w[4] = {prepared<CODE>(r[i].x), prepared<CODE>(r[i].y), prepared<CODE>(r[i].z), prepared<CODE>(r[i].w)};
                 *reinterpret_cast<uint4*>(dst + (off0 ^ flip) + i * STEP * 128) = make_uint4(pair_of<CODE, 0>(w[0]), pair_of<CODE, 1>(w[0]), pair_of<CODE, 0>(w[1]), pair_of<CODE, 1>(w[1]));
@@ -134,9 +133,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
         };
         bool ok = true;
         if (n_tiles) { load(kg, kr, 0); load(vg, vr, 0); }
-        for (int j = 0, slot = 0, round = 0; j < n_tiles; ++j) {
-            kg += kPaKeys * HD;
-            vg += kPaKeys * HD;
+        for (int j = 0; j < n_tiles; ++j) {
+            const int slot = j & 1, round = j >> 1;
+            kg += kPromptKeys * HD;
+            vg += kPromptKeys * HD;
             if (*failed || (round > 0 && !mbar_wait_warp(&bars.k_free[slot], (unsigned)((round - 1) & 1)))) { ok = false; break; }
             store(k_sm + slot * KV_BYTES, kr);
             if (lane == 0) pa_arrive(&bars.k_full[slot]);
@@ -145,20 +145,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
             store(v_sm + slot * KV_BYTES, vr);
             if (lane == 0) pa_arrive(&bars.v_full[slot]);
             if (j + 1 < n_tiles) load(vg, vr, j + 1);
-            if (++slot == kSlots) { slot = 0; ++round; }
         }
         if (!ok && lane == 0) fail(31);
         __syncwarp();
     } else if (warp == kMmaWarp) {
         const bool el = elect_one();
         const unsigned qd = umma_desc_lo(smem_u32(q_sm)), kd = umma_desc_lo(smem_u32(k_sm)), vd = pa_desc_mn_lo(smem_u32(v_sm), KV_HALF);
-        auto scores = [&](int j, int slot, int t) {
+        auto scores = [&](int slot, int t) {
             if (el) {
 #pragma unroll
                 for (int kk = 0; kk < HD / 16; ++kk)
-                    pa_mma_ss(tm + t * 128u + (unsigned)(j & 1) * 64u, qd + t * (Q_BYTES / 16) + (kk >> 2) * (Q_HALF / 16) + 2 * (kk & 3),
-                              kd + slot * (KV_BYTES / 16) + (kk >> 2) * (KV_HALF / 16) + 2 * (kk & 3), pa_idesc(kPaKeys, false, false), kk > 0 ? 1u : 0u);
-                umma_commit(&bars.s_full[t][j & 1]);
+                    pa_mma_ss(tm + t * 128u, qd + t * (Q_BYTES / 16) + (kk >> 2) * (Q_HALF / 16) + 2 * (kk & 3), kd + slot * (KV_BYTES / 16) + (kk >> 2) * (KV_HALF / 16) + 2 * (kk & 3),
+                              pa_idesc(kPromptKeys, false, false), kk > 0 ? 1u : 0u);
+                umma_commit(&bars.s_full[t]);
             }
             __syncwarp();
         };
@@ -172,42 +171,35 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
             if (ok) {
                 pa_after();
                 for (int t = 0; t < kTiles; ++t)
-                    if ((t ? tiles1 : tiles0) > 0) scores(0, 0, t);
+                    if ((t ? tiles1 : tiles0) > 0) scores(0, t);
                 release(&bars.k_free[0]);
             }
         }
-        for (int j = 0, slot = 0, phase = 0; j < n_tiles && ok; ++j) {
-            int next = slot + 1, next_phase = phase;
-            if (next == kSlots) { next = 0; next_phase ^= 1; }
-            if (j + 1 < n_tiles) {
-                if (!mbar_wait_warp(&bars.k_full[next], (unsigned)next_phase)) { ok = false; break; }
-                for (int t = 0; t < kTiles && ok; ++t) {
-                    if (j + 1 >= (t ? tiles1 : tiles0)) continue;
-                    // the region of tile j + 1 held the probabilities of tile j - 1
-                    if (j > 0 && !mbar_wait_warp(&bars.pv_done[t], (unsigned)((j - 1) & 1))) { ok = false; break; }
-                    pa_after();
-                    scores(j + 1, next, t);
-                }
-                if (!ok) break;
-                release(&bars.k_free[next]);
-            }
-            if (!mbar_wait_warp(&bars.v_full[slot], (unsigned)phase)) { ok = false; break; }
+        for (int j = 0; j < n_tiles && ok; ++j) {
+            const int slot = j & 1, next = slot ^ 1;
+            const unsigned phase = (unsigned)((j >> 1) & 1), next_phase = (unsigned)(((j + 1) >> 1) & 1);
+            if (!mbar_wait_warp(&bars.v_full[slot], phase) || (j + 1 < n_tiles && !mbar_wait_warp(&bars.k_full[next], next_phase))) { ok = false; break; }
             for (int t = 0; t < kTiles && ok; ++t) {
-                if (j >= (t ? tiles1 : tiles0)) continue;
-                if (!mbar_wait_warp(&bars.p_ready[t][j & 1], (unsigned)((j >> 1) & 1))) { ok = false; break; }
+                const int mine = t ? tiles1 : tiles0;
+                if (j >= mine) continue;
+                if (!mbar_wait_warp(&bars.p_ready[t], (unsigned)(j & 1))) { ok = false; break; }
                 pa_after();
                 if (el) {
 #pragma unroll
-                    for (int kk = 0; kk < kPaKeys / 16; ++kk)
-                        pa_mma_ts(tm + O_COL + t * 128u, tm + t * 128u + (unsigned)(j & 1) * 64u + 8u * kk, vd + slot * (KV_BYTES / 16) + kk * (2048 / 16), pa_idesc(HD, true, false),
-                                  kk > 0 || j > 0 ? 1u : 0u);
+                    for (int kk = 0; kk < kPromptKeys / 16; ++kk)
+                        pa_mma_ts(tm + O_COL + t * 128u, tm + t * 128u + 8u * kk, vd + slot * (KV_BYTES / 16) + kk * (2048 / 16), pa_idesc(HD, true, false), kk > 0 || j > 0 ? 1u : 0u);
                     umma_commit(&bars.pv_done[t]);
                 }
                 __syncwarp();
+                if (j + 1 < mine) {   // its scores take the place of the probabilities that the product reads
+                    if (!mbar_wait_warp(&bars.pv_done[t], (unsigned)(j & 1))) { ok = false; break; }
+                    pa_after();
+                    scores(next, t);
+                }
             }
-            if (ok) release(&bars.v_free[slot]);
-            slot = next;
-            phase = next_phase;
+            if (!ok) break;
+            release(&bars.v_free[slot]);
+            if (j + 1 < n_tiles) release(&bars.k_free[next]);
         }
         if (el) umma_commit(&bars.o_done);   // also behind whatever was issued before a failure
         __syncwarp();
@@ -254,45 +246,50 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
         const float* ks = c.k_scale + head * (c.capacity >> block_shift);
         const float* vs = c.v_scale + head * (c.capacity >> block_shift);
         float m_ref = -INFINITY, l_run = 0.f, v_ref = 0x1p-100f, v_inv = 0x1p100f * kValueUnit;
-        constexpr int KEYS = kPaKeys / GROUPS;
+        constexpr int KEYS = kPromptKeys / GROUPS;            // keys of a scale
+        constexpr int PARTS = KEYS < 64 ? 64 / KEYS : 1, N = 64 / PARTS;   // scales of half a tile, keys of it that share one
         float kn[GROUPS], vn[GROUPS];   // the next tile's scales; 0 behind the last token
         auto scales = [&](int j) {
 #pragma unroll
             for (int g = 0; g < GROUPS; ++g) {
-                const int slot = key_lo + j * kPaKeys + g * KEYS;
+                const int slot = key_lo + j * kPromptKeys + g * KEYS;
                 kn[g] = slot < end ? __ldg(ks + (slot >> block_shift)) : 0.f;
                 vn[g] = slot < end ? __ldg(vs + (slot >> block_shift)) : 0.f;
             }
         };
         if (tiles) scales(0);
         bool ok = true;
+        const unsigned region = tm + lanes + t * 128u;
         for (int j = 0; j < tiles; ++j) {
-            const unsigned region = tm + lanes + t * 128u + (unsigned)(j & 1) * 64u;
             float fk[GROUPS], vt[GROUPS];
 #pragma unroll
             for (int g = 0; g < GROUPS; ++g) { fk[g] = factor * kn[g]; vt[g] = vn[g]; }
             if (j + 1 < tiles) scales(j + 1);
-            if (!mbar_wait_warp(&bars.s_full[t][j & 1], (unsigned)((j >> 1) & 1))) { ok = false; break; }
+            if (!mbar_wait_warp(&bars.s_full[t], (unsigned)(j & 1))) { ok = false; break; }
             pa_after();
-            unsigned v[64];
-            pa_ld32(region, v);
-            pa_ld32(region + 32u, v + 32);
-            pa_wait_ld();
-            const int key0 = key_lo + j * kPaKeys;
-            const bool masked = !__all_sync(0xffffffffu, key0 + kPaKeys <= limit);
+            const int key0 = key_lo + j * kPromptKeys;
+            const bool masked = !__all_sync(0xffffffffu, key0 + kPromptKeys <= limit);
+            // A thread has no room for a tile's 128 scores: the halves are read for the largest one, and again for the probabilities
             float top = -INFINITY;
+            unsigned v[64];
 #pragma unroll
-            for (int g = 0; g < GROUPS; ++g) {
-                float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};   // (four chains)
-                if (masked) {
+            for (int half = 1; half >= 0; --half) {
+                pa_ld32(region + half * 64u, v);
+                pa_ld32(region + half * 64u + 32u, v + 32);
+                pa_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < KEYS; ++e) most[e & 3] = fmaxf(most[e & 3], key0 + g * KEYS + e < limit ? __uint_as_float(v[g * KEYS + e]) : -INFINITY);
-                } else {
+                for (int g = 0; g < PARTS; ++g) {
+                    float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};   // (four chains)
+                    if (masked) {
 #pragma unroll
-                    for (int e = 0; e < KEYS; ++e) most[e & 3] = fmaxf(most[e & 3], __uint_as_float(v[g * KEYS + e]));
+                        for (int e = 0; e < N; ++e) most[e & 3] = fmaxf(most[e & 3], key0 + half * 64 + g * N + e < limit ? __uint_as_float(v[g * N + e]) : -INFINITY);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < N; ++e) most[e & 3] = fmaxf(most[e & 3], __uint_as_float(v[g * N + e]));
+                    }
+                    const float x = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+                    if (x > -INFINITY) top = fmaxf(top, x * fk[(half * 64 + g * N) / KEYS]);   // (factors are not negative: the largest score stays the largest)
                 }
-                const float x = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
-                if (x > -INFINITY) top = fmaxf(top, x * fk[g]);   // (factors are not negative: the largest score stays the largest)
             }
             const bool moves = top > m_ref + kSlack;
             float v_top = vt[0];
@@ -302,9 +299,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
                 float corr = moves ? pa_exp2(m_ref - top) : 1.f;   // 0 for a row's first keys
                 if (moves) { m_ref = top; l_run *= corr; }
                 if (v_top > v_ref) { corr *= v_ref / v_top; v_ref = v_top; v_inv = kValueUnit / v_top; }
-                if (j > 0) {   // the output so far: complete, and the next product waits for this warp
-                    if (!mbar_wait_warp(&bars.pv_done[t], (unsigned)((j - 1) & 1))) { ok = false; break; }
-                    pa_after();
+                if (j > 0) {   // the output so far is complete, and the next product waits for this warp
 #pragma unroll 1
                     for (int d = 0; d < HD; d += 16) {
                         unsigned o[16];
@@ -314,7 +309,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
                         for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
                         pa_st16(out_col + d, o);
                     }
-                    pa_wait_st();
                 }
             }
             const float base = m_ref == -INFINITY ? 0.f : m_ref;   // nothing attended so far: all probabilities 0
@@ -325,45 +319,56 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
                 unit[g] = vt[g] * v_inv;
                 folds = folds && unit[g] >= kFoldUnit * kValueUnit;
             }
-            if (folds) {
-                // the unit goes into the exponent, and out of the sum again
+            // probabilities of the first half take the place of its first 32 columns, those of the second half that of the next 32
 #pragma unroll
-                for (int g = 0; g < GROUPS; ++g) {
-                    const float shift = log2_of(unit[g]) - base;
-                    const float2 fk2 = make_float2(fk[g], fk[g]), shift2 = make_float2(shift, shift);
-                    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-                    for (int e = 0; e < KEYS; e += 2) {
-                        float2 x = fma2(make_float2(__uint_as_float(v[g * KEYS + e]), __uint_as_float(v[g * KEYS + e + 1])), fk2, shift2);
-                        x = make_float2(pa_exp2(x.x), pa_exp2(x.y));
-                        sum[e >> 1 & 1] = add2(sum[e >> 1 & 1], x);
-                        v[(g * KEYS + e) / 2] = pack_half(x.x, x.y);
-                    }
-                    const float2 all = add2(sum[0], sum[1]);
-                    l_run += __fdividef(all.x + all.y, unit[g]);
+            for (int half = 0; half < 2; ++half) {
+                if (half) {   // (the first half is what was read last)
+                    pa_ld32(region + 64u, v);
+                    pa_ld32(region + 96u, v + 32);
+                    pa_wait_ld();
                 }
-            } else {
+                if (folds) {
+                    // the unit goes into the exponent, and out of the sum again
 #pragma unroll
-                for (int g = 0; g < GROUPS; ++g) {
+                    for (int g = 0; g < PARTS; ++g) {
+                        const int at = (half * 64 + g * N) / KEYS;
+                        const float shift = log2_of(unit[at]) - base;
+                        const float2 fk2 = make_float2(fk[at], fk[at]), shift2 = make_float2(shift, shift);
+                        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-                    for (int e = 0; e < KEYS; e += 2) {
-                        float w[2];
-#pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            const bool sees = key0 + g * KEYS + e + k < limit;   // (what a row does not attend may lie in a block that is NaN)
-                            const float x = sees ? pa_exp2(fmaf(__uint_as_float(v[g * KEYS + e + k]), fk[g], -base)) : 0.f;
-                            l_run += x;
-                            w[k] = sees ? x * unit[g] : 0.f;
+                        for (int e = 0; e < N; e += 2) {
+                            float2 x = fma2(make_float2(__uint_as_float(v[g * N + e]), __uint_as_float(v[g * N + e + 1])), fk2, shift2);
+                            x = make_float2(pa_exp2(x.x), pa_exp2(x.y));
+                            sum[e >> 1 & 1] = add2(sum[e >> 1 & 1], x);
+                            v[(g * N + e) / 2] = pack_half(x.x, x.y);
                         }
-                        v[(g * KEYS + e) / 2] = pack_half(w[0], w[1]);
+                        const float2 all = add2(sum[0], sum[1]);
+                        l_run += __fdividef(all.x + all.y, unit[at]);
+                    }
+                } else {
+#pragma unroll
+                    for (int g = 0; g < PARTS; ++g) {
+                        const int at = (half * 64 + g * N) / KEYS;
+#pragma unroll
+                        for (int e = 0; e < N; e += 2) {
+                            float w[2];
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                const bool sees = key0 + half * 64 + g * N + e + k < limit;   // (what a row does not attend may lie in a block that is NaN)
+                                const float x = sees ? pa_exp2(fmaf(__uint_as_float(v[g * N + e + k]), fk[at], -base)) : 0.f;
+                                l_run += x;
+                                w[k] = sees ? x * unit[at] : 0.f;
+                            }
+                            v[(g * N + e) / 2] = pack_half(w[0], w[1]);
+                        }
                     }
                 }
+                pa_st32(region + half * 32u, v);
             }
-            pa_st32(region, v);
             pa_wait_st();
             pa_before();
             __syncwarp();
-            if (lane == 0) pa_arrive(&bars.p_ready[t][j & 1]);
+            if (lane == 0) pa_arrive(&bars.p_ready[t]);
         }
         if (ok && (!mbar_wait_warp(&bars.o_done, 0u) || *failed)) ok = false;
         if (!ok) fail(33);
@@ -560,7 +565,8 @@ template <int HD, int CODE>
 int launch_prompt(const swlm_kv8_cache& c, const swlm_kv8_attend& a, const RowsPlan& p, int* status, cudaStream_t s) {
     const dim3 grid((unsigned)(p.row_tiles * p.splits), (unsigned)c.kv_heads, (unsigned)c.batch);
     auto launch = [&](auto kernel) { return launch_k(kernel, grid, dim3(kPromptThreads), prompt_smem<HD>(), s, c, a, p, status); };
-    const cudaError_t e = c.block >= 64 ? launch(kv8_prompt_kernel<HD, CODE, 1>) : c.block == 32 ? launch(kv8_prompt_kernel<HD, CODE, 2>) : launch(kv8_prompt_kernel<HD, CODE, 4>);
+    const cudaError_t e = c.block == 128 ? launch(kv8_prompt_kernel<HD, CODE, 1>) : c.block == 64 ? launch(kv8_prompt_kernel<HD, CODE, 2>) :
+                          c.block == 32 ? launch(kv8_prompt_kernel<HD, CODE, 4>) : launch(kv8_prompt_kernel<HD, CODE, 8>);
     return e == cudaSuccess ? SWLM_OK : cuda_fail(e, "kv8 prompt attention launch");
 }
 template <int HD, int CODE>
@@ -575,6 +581,7 @@ int init_prompt() {
     SWLM_CUDA(cudaFuncSetAttribute(kv8_weights_kernel<HD, CODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)weights_smem<HD>()));
     SWLM_CUDA(cudaFuncSetAttribute(kv8_prompt_kernel<HD, CODE, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prompt_smem<HD>()));
     SWLM_CUDA(cudaFuncSetAttribute(kv8_prompt_kernel<HD, CODE, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prompt_smem<HD>()));
+    SWLM_CUDA(cudaFuncSetAttribute(kv8_prompt_kernel<HD, CODE, 8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prompt_smem<HD>()));
     SWLM_CUDA(cudaFuncSetAttribute(kv8_prompt_kernel<HD, CODE, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prompt_smem<HD>()));
     return SWLM_OK;
 }
