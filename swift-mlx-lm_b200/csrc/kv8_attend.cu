@@ -20,6 +20,7 @@ namespace swlm {
 using namespace kv8;
 namespace {
 
+constexpr unsigned kMark = 0x9E3779B9u;   // of a word that counts arrivals
 constexpr int kStreamBatch = 512;               // sequences whose units a CTA adds up
 constexpr int kSaveRows = 64;                   // up to so many rows of a KV head the scores are kept for the weights, beyond they are worked out again
 
@@ -87,6 +88,37 @@ __device__ __forceinline__ void load_query(const unsigned short* src, bool valid
     for (int k = 0; k < HD / 16; ++k) {
         frag[k][0] = pack_half(x[4 * k] * up, x[4 * k + 1] * up);
         frag[k][1] = pack_half(x[4 * k + 2] * up, x[4 * k + 3] * up);
+    }
+}
+
+// Parts first, first + step, ... of a row's: their maxima and sums ml, pitch rows apart, and four values of each result. Sixteen are loaded at once.
+__device__ __forceinline__ void join_parts(const float* ml, const float* po, int pitch, int dim, int parts, int first, int step, float& m, float& l, float4& o) {
+    constexpr int AHEAD = 16;
+    m = -INFINITY;
+    l = 0.f;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s0 = first; s0 < parts; s0 += AHEAD * step) {
+        float2 x[AHEAD];
+        float4 v[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const size_t s = min(s0 + i * step, parts - 1);
+            x[i] = __ldcg(reinterpret_cast<const float2*>(ml + s * pitch * 2));
+            v[i] = __ldcg(reinterpret_cast<const float4*>(po + s * pitch * dim));
+        }
+        float top = m;
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) top = fmaxf(top, x[i].x);   // (the last part may come several times)
+        const float corr = m == -INFINITY ? 1.f : exp2_of(m - top);   // (no maximum so far: zeros, or NaN)
+        o.x *= corr; o.y *= corr; o.z *= corr; o.w *= corr; l *= corr;
+        m = top;
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const float f = s0 + i * step >= parts ? 0.f : x[i].x == -INFINITY ? 1.f : exp2_of(x[i].x - m);   // (a part without slots has zeros, or NaN)
+            if (f == 0.f) continue;
+            l += f * x[i].y;
+            o.x += f * v[i].x; o.y += f * v[i].y; o.z += f * v[i].z; o.w += f * v[i].w;
+        }
     }
 }
 
@@ -178,6 +210,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_r
         const int end = visible(part, min((row0 + TR - 1) / G, part.count - 1), span);   // of the tile's last query: it sees most
         const int from = unit0 * kUnit, to = min(unit1 * kUnit, end);
         const size_t head = (size_t)b * c.kv_heads + h;
+
+        if (!SAVE && p.arrived && !whole && tid == 0) {   // what the scratch held before is no count
+            unsigned long long* const word = p.arrived + head * p.row_tiles + tile;
+            const unsigned long long had = *static_cast<volatile unsigned long long*>(word);
+            if ((had >> 32) != kMark) atomicCAS(word, had, (unsigned long long)kMark << 32);
+        }
 
         // ring of this warp: its step number i covers the 32 slots from `first` + i * kUnit on. Whole tiles of 16 are read: they lie within the
         // capacity, a multiple of 16; what is beyond a row's last slot is masked.
@@ -427,12 +465,40 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_r
                 l += f * warp_l[w][r];
                 o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
             }
-            if (d == 0 && (SAVE || p.ml_always || !whole)) *reinterpret_cast<float2*>(p.part_ml + (slot * TR + r) * 2) = make_float2(m, l);
+            if (d == 0 && (SAVE || !whole)) *reinterpret_cast<float2*>(p.part_ml + (slot * TR + r) * 2) = make_float2(m, l);
             if (!whole) {
                 *reinterpret_cast<float4*>(p.part_o + (slot * TR + r) * HD + d) = o;
             } else {
                 const int i = row / G;
                 store_out(static_cast<unsigned short*>(a.out) + (int64_t)(part.start + i) * a.out_stride + (size_t)(h * G + row - i * G) * HD + d, o, l, f16);
+            }
+        }
+        if (!SAVE && p.arrived && !whole) {
+            // The last CTA of the tile to arrive joins its parts. The tile's word counts arrivals
+            // under the mark in its upper half; the last CTA sets it back to none.
+            const Shares shares(info[c.batch].x, (int)gridDim.x);
+            const int u0 = info[b].x + (h * sequence_tiles(part, G, TR) + tile) * sequence_units(part, span), c0 = shares.cta_of(u0);
+            const size_t place = head * p.row_tiles + tile + c0;   // of the first part
+            const int parts = shares.cta_of(u0 + sequence_units(part, span) - 1) - c0 + 1;
+            __syncthreads();
+            if (tid == 0) {
+                __threadfence();   // (the whole CTA's results, behind the barrier)
+                const bool last = (int)(unsigned)atomicAdd(p.arrived + head * p.row_tiles + tile, 1ull) + 1 == parts;
+                if (last) p.arrived[head * p.row_tiles + tile] = (unsigned long long)kMark << 32;
+                scan[0] = last;
+                __threadfence();
+            }
+            __syncthreads();
+            if (scan[0]) {
+                for (int item = tid; item < TR * (HD / 4); item += kThreads) {
+                    const int r = item / (HD / 4), d = item % (HD / 4) * 4, row = row0 + r;
+                    if (row >= rows) continue;
+                    float m, l;
+                    float4 o;
+                    join_parts(p.part_ml + (place * TR + r) * 2, p.part_o + (place * TR + r) * HD + d, TR, HD, parts, 0, 1, m, l, o);
+                    const int i = row / G;
+                    store_out(static_cast<unsigned short*>(a.out) + (int64_t)(part.start + i) * a.out_stride + (size_t)(h * G + row - i * G) * HD + d, o, l, f16);
+                }
             }
         }
         __syncthreads();   // the next one's copies take the results' place
@@ -461,7 +527,6 @@ constexpr int kJoinThreads = 256, kJoinTurns = 4, kJoinSlots = kJoinThreads * kJ
 template <int HD>
 __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const swlm_kv8_cache c, const swlm_kv8_attend a, const RowsPlan p, const int join) {
     constexpr int LANES = HD / 4, PER = kJoinThreads / LANES;   // lanes of a row, rows of a CTA
-    constexpr int AHEAD = 8;                                    // parts that are loaded before the first is used
     __shared__ float row_m[kSaveRows], row_inv[kSaveRows];
     __shared__ int row_limit[kSaveRows];
     __shared__ float group_m[PER], group_l[PER];
@@ -480,34 +545,9 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const swlm_kv8_c
         const int tile = min(row, rows - 1) / TR, r = min(row, rows - 1) - tile * TR;
         const Parts parts = parts_of(p, part, b, c.batch, head, h, tile, span, G);
         const bool on = row < rows && parts.count > 1;
-        const float* ml = p.part_ml + (parts.slot * TR + r) * 2;
-        const float* po = p.part_o + (parts.slot * TR + r) * HD + d;
         float m = -INFINITY, l = 0.f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (on)
-            for (int s0 = sub; s0 < parts.count; s0 += AHEAD * p.join_groups) {
-                float2 x[AHEAD];
-                float4 v[AHEAD];
-#pragma unroll
-                for (int i = 0; i < AHEAD; ++i) {
-                    const int s = min(s0 + i * p.join_groups, parts.count - 1);
-                    x[i] = *reinterpret_cast<const float2*>(ml + (size_t)s * TR * 2);
-                    v[i] = *reinterpret_cast<const float4*>(po + (size_t)s * TR * HD);
-                }
-                float top = m;
-#pragma unroll
-                for (int i = 0; i < AHEAD; ++i) top = fmaxf(top, x[i].x);   // (the last part may come several times)
-                const float corr = m == -INFINITY ? 1.f : exp2_of(m - top);   // (no maximum so far: zeros, or NaN)
-                o.x *= corr; o.y *= corr; o.z *= corr; o.w *= corr; l *= corr;
-                m = top;
-#pragma unroll
-                for (int i = 0; i < AHEAD; ++i) {
-                    const float f = s0 + i * p.join_groups >= parts.count ? 0.f : x[i].x == -INFINITY ? 1.f : exp2_of(x[i].x - m);   // (a part without slots has zeros, or NaN)
-                    if (f == 0.f) continue;
-                    l += f * x[i].y;
-                    o.x += f * v[i].x; o.y += f * v[i].y; o.z += f * v[i].z; o.w += f * v[i].w;
-                }
-            }
+        if (on) join_parts(p.part_ml + (parts.slot * TR + r) * 2, p.part_o + (parts.slot * TR + r) * HD + d, TR, HD, parts.count, sub, p.join_groups, m, l, o);
         if (p.join_groups > 1) {
             if (lane == 0) { group_m[group] = m; group_l[group] = l; }
             group_o[tid] = o;
@@ -590,7 +630,7 @@ RowsPlan rows_plan(const swlm_kv8_cache& c, const swlm_kv8_attend& a, size_t* by
     p.span = (span + kStep - 1) / kStep * kStep;
     const long long groups = (long long)c.batch * c.kv_heads * p.row_tiles, units = groups * ((span + kUnit - 1) / kUnit);
     bool several;   // parts that have to be joined
-    if (p.tiles > 2) {
+    if (p.rows > kSaveRows) {
         // runs of at least four key tiles, as many as make two CTAs per SM (one after the other)
         const long long want = std::max<long long>(1, 2 * kSms / groups), most = (span + 4 * kPromptKeys - 1) / (4 * kPromptKeys);
         const int runs = (int)std::min(want, most);
@@ -605,7 +645,6 @@ RowsPlan rows_plan(const swlm_kv8_cache& c, const swlm_kv8_attend& a, size_t* by
         several = p.stream && units > groups;
     }
     const size_t places = p.splits ? (size_t)groups * p.splits : (size_t)groups + p.ctas;
-    p.ml_always = a.accumulate && p.rows <= kSaveRows;
     // a group of lanes takes up to eight parts at once: as many groups as a row with the most parts has such turns
     const long long most = p.splits ? p.splits : std::min<long long>(units / groups, p.ctas / groups + 2);
     p.join_groups = most > 32 ? 8 : most > 16 ? 4 : most > 8 ? 2 : 1;
@@ -613,11 +652,16 @@ RowsPlan rows_plan(const swlm_kv8_cache& c, const swlm_kv8_attend& a, size_t* by
     char* base = static_cast<char*>(a.scratch);
     auto take = [&](size_t n) { char* q = base + at; at += align16(n); return q; };
     if (several) p.part_o = reinterpret_cast<float*>(take(places * 8 * p.tiles * c.head_dim * 4));
-    if (several || p.ml_always) {
+    const bool saves = a.accumulate && p.rows <= kSaveRows;
+    // Parts are joined by the last CTA of their tile to arrive where that is not much beside the CTAs' own work, by a second launch otherwise (and where
+    // that comes anyway, for the weights). us, 32 / 8 heads of 128: 8 x 8192 34.6 and 41.3, 1 x 131072 58 and 63; 1 x 16000 19.9 and 17.5, 6 x 5 over 16384 53 and 50
+    const bool arrives = several && p.stream && !saves && p.tiles == 1 && units >= 8LL * p.ctas;
+    if (several || saves) {
         p.part_ml = reinterpret_cast<float*>(take(places * 8 * p.tiles * 8));
-        if (p.stream) p.table = reinterpret_cast<int*>(take(((size_t)c.batch + 1) * 4));
+        if (p.stream && !arrives) p.table = reinterpret_cast<int*>(take(((size_t)c.batch + 1) * 4));
     }
-    if (a.accumulate && p.rows <= kSaveRows) {
+    if (arrives) p.arrived = reinterpret_cast<unsigned long long*>(take((size_t)groups * 8));
+    if (saves) {
         p.pitch = p.rows <= 2 ? 2 : (p.rows + 3) / 4 * 4;
         p.scores = reinterpret_cast<float*>(take((size_t)c.batch * c.kv_heads * p.span * p.pitch * 4));
     } else if (a.accumulate) {
@@ -648,7 +692,7 @@ int launch_rows(const swlm_kv8_cache& c, const swlm_kv8_attend& a, const RowsPla
         if (e != cudaSuccess) return cuda_fail(e, "kv8 attention launch");
     }
     const int span = std::min(a.max_len, c.capacity);
-    const int per = kJoinThreads / (HD / 4) / p.join_groups, join = p.part_o ? (p.rows + per - 1) / per : 0;
+    const int per = kJoinThreads / (HD / 4) / p.join_groups, join = p.part_o && !p.arrived ? (p.rows + per - 1) / per : 0;
     const int slots = p.pitch ? (span + kJoinSlots - 1) / kJoinSlots : 0;
     if (join + slots) {
         const cudaError_t j = launch_k(kv8_join_kernel<HD>, dim3((unsigned)(join + slots), (unsigned)c.kv_heads, (unsigned)c.batch), dim3(kJoinThreads), 0, s, c, a, p, join);

@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
             const bool whole = end <= p.chunk;   // this CTA has all of the tile's slots
             const size_t at = ((head * p.row_tiles + block) * p.splits + split) * kPromptRows + tid;
             const float unit = v_ref * (1.f / kValueUnit);
-            if (row_ok && (!whole || p.ml_always)) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m_ref, l_run);
+            if (row_ok && !whole) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m_ref, l_run);
             if (p.q_shift && (whole || !row_ok)) p.q_shift[(head * p.row_tiles + block) * kPromptRows + tid] = row_ok ? row_shift_of(m_ref, l_run) : -INFINITY;
             unsigned short* dst = static_cast<unsigned short*>(a.out) + (int64_t)(part.start + i) * a.out_stride + (size_t)(h * G + min(row, rows - 1) - i * G) * HD;
 #pragma unroll 1

@@ -195,6 +195,9 @@ ATTENDS = [
     (2, 8, 2, 64, 128, [0, 777], [190, 77]),                      # portions of prompts
     (1, 4, 4, 128, 64, [500], [129]),
     (1, 8, 1, 128, 64, [9000], [1]),
+    (1, 4, 1, 128, 16, [3000], [40]),                             # a portion whose slots are worked on in several runs
+    (1, 2, 1, 64, 32, [50], [700]),                               # several blocks of rows, causal from an almost empty cache
+    (2, 10, 2, 64, 64, [600, 30], [7, 13]),                       # 65 rows: one more than the scores are kept for
 ]
 
 
@@ -231,6 +234,31 @@ def test_attend(pkg, store, batch, heads, kv_heads, dim, block, lengths, counts,
     cap = (max(a + c for a, c in zip(lengths, counts)) + block) // block * block
     cache = Cache(pkg, batch, kv_heads, dim, cap, block, code).fill([max(0, a + c) for a, c in zip(lengths, counts)])
     check_attend(pkg, store, cache, batch, heads, dim, lengths, counts, dtype, accumulate)
+
+
+@pytest.mark.parametrize("batch,heads,kv_heads,dim,most", [(64, 16, 8, 64, 1400), (64, 4, 4, 128, 1900), (520, 1, 1, 64, 200)], ids=str)
+def test_attend_of_many_sequences(pkg, store, batch, heads, kv_heads, dim, most):
+    """Batches whose slots come in equal shares, several sequences to a CTA and sequences over several CTAs, which the last CTA to arrive joins; a batch
+    of one CTA per head. Empty, parked and full sequences between others. Twice with the same scratch: counters are back at none."""
+    g = torch.Generator().manual_seed(batch + dim)
+    lengths = [int(x) for x in torch.randint(0, most, (batch,), generator=g)]
+    lengths[0], lengths[3], lengths[4], lengths[-1] = most, -1, 0, most
+    counts = [0 if i % 17 == 5 else 1 for i in range(batch)]
+    cap = (most + 64) // 64 * 64
+    cache = Cache(pkg, batch, kv_heads, dim, cap, 64, 0).fill([max(0, a + c) for a, c in zip(lengths, counts)])
+    starts, rows = starts_of(counts)
+    q = torch.randn((rows, heads, dim), device="cuda").bfloat16()
+    out, at, n, first = torch.zeros_like(q), ints(*lengths), ints(*counts), ints(*starts)
+    step, scratch = attend_call(pkg, store, cache, q, out, at, dim ** -0.5, n, first, n=1)
+    for _ in range(2):
+        out.fill_(7.0)
+        store.lib.check(store.lib.swlm_op_kv8_attend_dev(store.handle, cache.described(), step, stream()))
+        torch.cuda.synchronize()
+        for b in range(0, batch, 1 if batch < 100 else 7):
+            if counts[b]:
+                want, tol, _, _ = attend(cache, q[starts[b]:starts[b] + 1], b, lengths[b], dim ** -0.5, cap)
+                assert ((out[starts[b]:starts[b] + 1].double() - want).abs() <= tol).all(), b
+    assert (scratch[step.scratch_bytes:] == 0xFF).all()
 
 
 @pytest.mark.parametrize("counts", [[1, 1], [40, 40]], ids=str)

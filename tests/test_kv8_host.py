@@ -108,16 +108,16 @@ def test_scratch_sizes(pkg, lib):
     assert lib.swlm_op_kv8_evict_scratch_bytes(cache, _evict(pkg)) == 2 * 2 * 40 * 16
     assert lib.swlm_op_kv8_attend_scratch_bytes(cache, _attend(pkg, heads=5)) == 0
     assert lib.swlm_op_kv8_evict_scratch_bytes(_cache(pkg, block=7), _evict(pkg)) == 0
-    # Partial results: a place of 8, 16 or 128 rows per tile and one per CTA (at most four on each of 148 SMs), or a tile's runs of slots
+    # Partial results: a place of 8, 16, 24 or 256 rows per tile and one per CTA (at most four on each of 148 SMs), or a tile's runs of slots
     # (no more than two CTAs per SM, plus one a tile); every row has its results, a maximum and a sum
     for heads, n, length in ((2, 1, 1), (8, 1, 4000), (16, 5, 8192), (8, 300, 2048)):
         wide = _cache(pkg, capacity=8192)
         rows = heads // 2 * n
-        tile = 8 if rows <= 8 else 16 if rows <= 64 else 128
-        tiles = 2 * 2 * -(-rows // tile)
+        tile = 8 if rows <= 8 else 24 if rows <= 64 else 256
+        tiles = 2 * 2 * -(-rows // min(tile, 16 if rows <= 64 else tile))
         plain, kept = (lib.swlm_op_kv8_attend_scratch_bytes(wide, _attend(pkg, heads=heads, n=n, max_len=length, accumulate=w, q_stride=heads * 64, out_stride=heads * 64))
                        for w in (0, 1))
-        assert plain <= (tiles + 592) * tile * (64 + 2) * 4 + 64
+        assert plain <= (tiles + 592) * (tile * (64 + 2) * 4 + 8) + 64
         assert plain == 0 or length > 128
         # weights: the scores of every slot, or the queries as fp16
-        assert kept - plain >= (2 * 2 * rows * length * 4 if rows <= 64 else 2 * 2 * rows * (64 * 2 + 8))
+        assert kept >= (2 * 2 * rows * length * 4 if rows <= 64 else 2 * 2 * rows * (64 * 2 + 8))
