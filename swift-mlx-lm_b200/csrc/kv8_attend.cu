@@ -7,11 +7,17 @@
 // a step of 16 tokens, which never crosses a block, takes its scale as one number behind it.
 //
 // Rows: the queries of a step times the heads of a group, 8 to a tile. A CTA has one tile (or two) and a run of slots of one (sequence,
-// KV head); its eight warps take steps of 16 tokens in turn, each over a ring of its own that cp.async fills. Scores come as S^T = K Q^T
-// (16 tokens x 8 rows, so that a decode step's four or eight rows fill the tile), probabilities are transposed in
-// registers (movmatrix) and meet the values as O^T = V^T P^T. The reference maximum of a row moves only when it would grow by more than 2^8.
-// Probabilities are rounded to fp16 (2^-11 of themselves) times 2^7 vs / vr, vr the largest value scale so far: values of blocks down to 2^-24 of
-// the largest scale keep that precision. Partial results of several runs are joined by a second launch, which also adds the weights.
+// KV head) after the other, the same number of slots for every CTA whatever the lengths are; its four warps take steps of 32 tokens in turn,
+// each over a ring of its own that cp.async fills. Scores come as S^T = K Q^T (16 tokens x 8 rows, so that a decode step's four or eight
+// rows fill the tile), probabilities are transposed in registers (movmatrix) and meet the values as O^T = V^T P^T. The reference
+// maximum of a row moves only when it would grow by more than 2^8. Probabilities are rounded to fp16 (2^-11 of themselves) times 2^7 vs / vr, vr
+// the largest value scale so far: values of blocks down to 2^-24 of the largest scale keep that precision. Partial results of a tile
+// are joined by a second launch, which also adds the weights.
+//
+// What bounds it: memory, and some ten us of start, join and dependent launch. 8 x 8192 tokens, 32 / 8 heads of 128, int8: 34.7 us for 134 MB (3.9 TB/s,
+// 0.59 of the measured copy; the steps alone 26 us, 0.79); 1 x 131072: 58 us (0.70). Without the products the steps take two us less. Runs
+// of slots per CTA of a grid over (run, KV head, sequence) took 41 and 70 us; two heads' tiles of 24 rows instead of 16 and 16 for five drafted
+// tokens were slower (55 us against 50).
 #include <algorithm>
 
 #include "kv8_device.cuh"
@@ -20,7 +26,6 @@ namespace swlm {
 using namespace kv8;
 namespace {
 
-constexpr unsigned kMark = 0x9E3779B9u;   // of a word that counts arrivals
 constexpr int kStreamBatch = 512;               // sequences whose units a CTA adds up
 constexpr int kSaveRows = 64;                   // up to so many rows of a KV head the scores are kept for the weights, beyond they are worked out again
 
@@ -91,9 +96,9 @@ __device__ __forceinline__ void load_query(const unsigned short* src, bool valid
     }
 }
 
-// Parts first, first + step, ... of a row's: their maxima and sums ml, pitch rows apart, and four values of each result. Sixteen are loaded at once.
+// Parts first, first + step, ... of a row's: their maxima and sums ml, pitch rows apart, and four values of each result. Eight are loaded at once.
 __device__ __forceinline__ void join_parts(const float* ml, const float* po, int pitch, int dim, int parts, int first, int step, float& m, float& l, float4& o) {
-    constexpr int AHEAD = 16;
+    constexpr int AHEAD = 8;
     m = -INFINITY;
     l = 0.f;
     o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -129,7 +134,6 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_r
     __shared__ float warp_m[kWarps][TR], warp_l[kWarps][TR];
     __shared__ int scan[kWarps + 1];
     int4* const info = reinterpret_cast<int4*>(sm + rows_smem<HD>());   // [batch + 1]: units before the sequence, its length, count, first row
-    pdl_launch_dependents();
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int G = a.heads / c.kv_heads, span = min(a.max_len, c.capacity);
@@ -210,12 +214,6 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_r
         const int end = visible(part, min((row0 + TR - 1) / G, part.count - 1), span);   // of the tile's last query: it sees most
         const int from = unit0 * kUnit, to = min(unit1 * kUnit, end);
         const size_t head = (size_t)b * c.kv_heads + h;
-
-        if (!SAVE && p.arrived && !whole && tid == 0) {   // what the scratch held before is no count
-            unsigned long long* const word = p.arrived + head * p.row_tiles + tile;
-            const unsigned long long had = *static_cast<volatile unsigned long long*>(word);
-            if ((had >> 32) != kMark) atomicCAS(word, had, (unsigned long long)kMark << 32);
-        }
 
         // ring of this warp: its step number i covers the 32 slots from `first` + i * kUnit on. Whole tiles of 16 are read: they lie within the
         // capacity, a multiple of 16; what is beyond a row's last slot is masked.
@@ -473,34 +471,6 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_r
                 store_out(static_cast<unsigned short*>(a.out) + (int64_t)(part.start + i) * a.out_stride + (size_t)(h * G + row - i * G) * HD + d, o, l, f16);
             }
         }
-        if (!SAVE && p.arrived && !whole) {
-            // The last CTA of the tile to arrive joins its parts. The tile's word counts arrivals
-            // under the mark in its upper half; the last CTA sets it back to none.
-            const Shares shares(info[c.batch].x, (int)gridDim.x);
-            const int u0 = info[b].x + (h * sequence_tiles(part, G, TR) + tile) * sequence_units(part, span), c0 = shares.cta_of(u0);
-            const size_t place = head * p.row_tiles + tile + c0;   // of the first part
-            const int parts = shares.cta_of(u0 + sequence_units(part, span) - 1) - c0 + 1;
-            __syncthreads();
-            if (tid == 0) {
-                __threadfence();   // (the whole CTA's results, behind the barrier)
-                const bool last = (int)(unsigned)atomicAdd(p.arrived + head * p.row_tiles + tile, 1ull) + 1 == parts;
-                if (last) p.arrived[head * p.row_tiles + tile] = (unsigned long long)kMark << 32;
-                scan[0] = last;
-                __threadfence();
-            }
-            __syncthreads();
-            if (scan[0]) {
-                for (int item = tid; item < TR * (HD / 4); item += kThreads) {
-                    const int r = item / (HD / 4), d = item % (HD / 4) * 4, row = row0 + r;
-                    if (row >= rows) continue;
-                    float m, l;
-                    float4 o;
-                    join_parts(p.part_ml + (place * TR + r) * 2, p.part_o + (place * TR + r) * HD + d, TR, HD, parts, 0, 1, m, l, o);
-                    const int i = row / G;
-                    store_out(static_cast<unsigned short*>(a.out) + (int64_t)(part.start + i) * a.out_stride + (size_t)(h * G + row - i * G) * HD + d, o, l, f16);
-                }
-            }
-        }
         __syncthreads();   // the next one's copies take the results' place
     }
 }
@@ -531,7 +501,6 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const swlm_kv8_c
     __shared__ int row_limit[kSaveRows];
     __shared__ float group_m[PER], group_l[PER];
     __shared__ float4 group_o[kJoinThreads];
-    pdl_launch_dependents();
     pdl_wait();
     const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x, G = a.heads / c.kv_heads, TR = 8 * p.tiles;
     const Kv8Part part = kv8_part(b, a.lengths, a.counts, a.starts, a.n, a.rows);
@@ -653,14 +622,10 @@ RowsPlan rows_plan(const swlm_kv8_cache& c, const swlm_kv8_attend& a, size_t* by
     auto take = [&](size_t n) { char* q = base + at; at += align16(n); return q; };
     if (several) p.part_o = reinterpret_cast<float*>(take(places * 8 * p.tiles * c.head_dim * 4));
     const bool saves = a.accumulate && p.rows <= kSaveRows;
-    // Parts are joined by the last CTA of their tile to arrive where that is not much beside the CTAs' own work, by a second launch otherwise (and where
-    // that comes anyway, for the weights). us, 32 / 8 heads of 128: 8 x 8192 34.6 and 41.3, 1 x 131072 58 and 63; 1 x 16000 19.9 and 17.5, 6 x 5 over 16384 53 and 50
-    const bool arrives = several && p.stream && !saves && p.tiles == 1 && units >= 8LL * p.ctas;
     if (several || saves) {
         p.part_ml = reinterpret_cast<float*>(take(places * 8 * p.tiles * 8));
-        if (p.stream && !arrives) p.table = reinterpret_cast<int*>(take(((size_t)c.batch + 1) * 4));
+        if (p.stream) p.table = reinterpret_cast<int*>(take(((size_t)c.batch + 1) * 4));
     }
-    if (arrives) p.arrived = reinterpret_cast<unsigned long long*>(take((size_t)groups * 8));
     if (saves) {
         p.pitch = p.rows <= 2 ? 2 : (p.rows + 3) / 4 * 4;
         p.scores = reinterpret_cast<float*>(take((size_t)c.batch * c.kv_heads * p.span * p.pitch * 4));
@@ -692,7 +657,7 @@ int launch_rows(const swlm_kv8_cache& c, const swlm_kv8_attend& a, const RowsPla
         if (e != cudaSuccess) return cuda_fail(e, "kv8 attention launch");
     }
     const int span = std::min(a.max_len, c.capacity);
-    const int per = kJoinThreads / (HD / 4) / p.join_groups, join = p.part_o && !p.arrived ? (p.rows + per - 1) / per : 0;
+    const int per = kJoinThreads / (HD / 4) / p.join_groups, join = p.part_o ? (p.rows + per - 1) / per : 0;
     const int slots = p.pitch ? (span + kJoinSlots - 1) / kJoinSlots : 0;
     if (join + slots) {
         const cudaError_t j = launch_k(kv8_join_kernel<HD>, dim3((unsigned)(join + slots), (unsigned)c.kv_heads, (unsigned)c.batch), dim3(kJoinThreads), 0, s, c, a, p, join);

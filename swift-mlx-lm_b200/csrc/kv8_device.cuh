@@ -1,4 +1,4 @@
-// Device code shared by the attention kernels over an 8-bit cache.
+// Device code shared by the kernels over an 8-bit cache.
 #pragma once
 
 #include "kv8.h"
@@ -25,7 +25,6 @@ struct RowsPlan {
     int span;       // slots that can be attended, rounded up to kStep
     int pitch;      // rows of a slot's kept scores (0: not kept)
     int join_groups;   // groups of lanes that share a row's parts
-    unsigned long long* arrived;   // [(sequence, KV head, tile)]: CTAs that have left their part (few rows, no weights)
     float* part_o;  // [places][8 * tiles][head_dim], not normalised; places: (sequence, KV head, tile) + CTA, or of many rows * splits + run
     float* part_ml; // [places][8 * tiles][2]: reference maximum (log2), sum
     float* scores;  // [batch][kv_heads][span][pitch], log2

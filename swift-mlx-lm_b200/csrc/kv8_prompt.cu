@@ -4,14 +4,16 @@
 // numbers on their way to shared memory, queries are shifted to fp16 (both exact, see kv8_attend.cu), so that scores are one product with fp32
 // sums; a tile's scores take the factor of their block, probabilities that of the values' block over the largest so far (2^7 times, as fp16).
 //
-// Roles: three warps bring keys and values from the cache, convert them and store them in the swizzled layout of the products' operands (three
-// slots each, both row tiles read them); a warp issues the MMAs (S = Q K^T of key tile j + 1 while tile j is in its softmax: two score
-// regions per row tile); eight warps do the softmax, a thread per row. Probabilities take the place of their scores in tensor memory and are
-// read there as the A operand. The reference maximum of a row moves only when it would grow by more than 2^8.
+// Roles: three warps bring keys and values from the cache, convert them and store them in the swizzled layout of the products' operands (two
+// slots of 128 tokens each, which both row tiles read); a warp issues the MMAs (O += P V, then S = Q K^T of the next key tile, for one row tile
+// and the other in turn); eight warps do the softmax, a thread per row. Probabilities take the place of their scores in tensor memory
+// and are read there as the A operand. The reference maximum of a row moves only when it would grow by more than 2^8.
 //
-// What bounds it, with heads of 128: 512 clocks of the tensor pipe per row tile and 64 keys, 512 of the exponential unit (8192 of 16 per clock). A
-// form with one row tile per CTA and two CTAs per SM, whose loaders also issued the products, took 391 us where this one takes XXX us (2048 tokens over
-// 8192, 32 / 8 heads of 128).
+// What bounds it (2048 tokens over 8192, 32 / 8 heads of 128: 297 us, 810 TFLOP/s, 0.49 of the measured rate): the chain of a row tile, softmax (two
+// warps of a scheduler share the exponential unit, 2048 clocks a tile), product, next scores, of which the other row tile fills the gaps only
+// in part; and 256 CTAs on 148 SMs. Steps to here: one row tile per CTA, two CTAs per SM 732 us; the loaders' first warp
+// issuing the MMAs, paired fp32 operations 391; two row tiles that share the conversions, a warp for the MMAs 306; key tiles of 128 instead of 64
+// with two score regions 297.
 #include <algorithm>
 
 #include "kv8_device.cuh"
@@ -52,7 +54,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
     unsigned char* const sm = prompt_raw + ((1024 - (smem_u32(prompt_raw) & 1023)) & 1023);
     unsigned char *const q_sm = sm, *const k_sm = sm + kTiles * Q_BYTES, *const v_sm = k_sm + kSlots * KV_BYTES;
     __shared__ __align__(8) PromptBars bars;
-    pdl_launch_dependents();
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int b = blockIdx.z, h = blockIdx.y, G = a.heads / c.kv_heads, span = min(a.max_len, c.capacity);
@@ -424,7 +425,6 @@ __global__ void __launch_bounds__(kWeightThreads, 2) kv8_weights_kernel(const sw
     unsigned char* const q_sm = k_sm + HALVES * K_HALF;
     __shared__ __align__(16) float rows_sm[kWeightSlots][2][kWeightRows];   // factors, shifts
     __shared__ __align__(8) WeightBars bars;
-    pdl_launch_dependents();
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int b = blockIdx.z, h = blockIdx.y, G = a.heads / c.kv_heads, span = min(a.max_len, c.capacity);

@@ -236,8 +236,9 @@ def test_attend(pkg, store, batch, heads, kv_heads, dim, block, lengths, counts,
     check_attend(pkg, store, cache, batch, heads, dim, lengths, counts, dtype, accumulate)
 
 
+@pytest.mark.parametrize("accumulate", [False, True])
 @pytest.mark.parametrize("batch,heads,kv_heads,dim,most", [(64, 16, 8, 64, 1400), (64, 4, 4, 128, 1900), (520, 1, 1, 64, 200)], ids=str)
-def test_attend_of_many_sequences(pkg, store, batch, heads, kv_heads, dim, most):
+def test_attend_of_many_sequences(pkg, store, batch, heads, kv_heads, dim, most, accumulate):
     """Batches whose slots come in equal shares, several sequences to a CTA and sequences over several CTAs, which the last CTA to arrive joins; a batch
     of one CTA per head. Empty, parked and full sequences between others. Twice with the same scratch: counters are back at none."""
     g = torch.Generator().manual_seed(batch + dim)
@@ -249,15 +250,22 @@ def test_attend_of_many_sequences(pkg, store, batch, heads, kv_heads, dim, most)
     starts, rows = starts_of(counts)
     q = torch.randn((rows, heads, dim), device="cuda").bfloat16()
     out, at, n, first = torch.zeros_like(q), ints(*lengths), ints(*counts), ints(*starts)
-    step, scratch = attend_call(pkg, store, cache, q, out, at, dim ** -0.5, n, first, n=1)
+    step, scratch = attend_call(pkg, store, cache, q, out, at, dim ** -0.5, n, first, n=1, accumulate=accumulate)
+    before = cache.weight.clone()
     for _ in range(2):
         out.fill_(7.0)
+        cache.weight.copy_(before)
         store.lib.check(store.lib.swlm_op_kv8_attend_dev(store.handle, cache.described(), step, stream()))
         torch.cuda.synchronize()
         for b in range(0, batch, 1 if batch < 100 else 7):
             if counts[b]:
-                want, tol, _, _ = attend(cache, q[starts[b]:starts[b] + 1], b, lengths[b], dim ** -0.5, cap)
+                want, tol, weight, weight_tol = attend(cache, q[starts[b]:starts[b] + 1], b, lengths[b], dim ** -0.5, cap)
                 assert ((out[starts[b]:starts[b] + 1].double() - want).abs() <= tol).all(), b
+                if accumulate:
+                    weight += before[b].double()
+                    assert ((cache.weight[b].double() - weight).abs() <= weight_tol + 2.0 ** -24 * weight.abs()).all(), b
+            else:
+                assert torch.equal(cache.weight[b], before[b])
     assert (scratch[step.scratch_bytes:] == 0xFF).all()
 
 
@@ -534,6 +542,31 @@ def test_a_captured_step_replays_at_other_lengths(pkg, store):
         results.append([x.clone() for x in cache.arrays() + to.arrays() + [out, lengths, seen]])
     assert all(same_bits(x, y) for x, y in zip(*results))
     assert lengths.tolist() == [503, 80] and refused.tolist() == [0, 0]
+
+
+def test_a_cache_whose_offsets_pass_32_bits(pkg, store):
+    """The last head's codes lie behind 4 GB: append, both kinds of attention and an eviction in place give what they give in a small cache."""
+    heads, cap, small = 9, 1 << 23, 512
+    big, little = ({"k": torch.empty((1, heads, n, 64), dtype=torch.uint8, device="cuda"), "v": torch.empty((1, heads, n, 64), dtype=torch.uint8, device="cuda"),
+                    "k_scale": torch.empty((1, heads, n // 64), device="cuda"), "v_scale": torch.empty((1, heads, n // 64), device="cuda"),
+                    "weight": torch.empty((1, heads, n), device="cuda"), "slot_pos": torch.empty((1, heads, n), dtype=torch.int32, device="cuda")} for n in (cap, small))
+    results = []
+    for arrays in (big, little):
+        cache = Cache(pkg, 1, 1, 64, 64, 64, 0)
+        for name, x in arrays.items():
+            setattr(cache, name, x)
+        g = torch.Generator(device="cuda").manual_seed(7)
+        k, v = (torch.randn((300, heads * 64), generator=g, device="cuda").bfloat16() for _ in range(2))
+        append(pkg, store, cache, k, v, ints(0), n=300)
+        outs = []
+        for n in (1, 80):
+            q = torch.randn((n, heads, 64), generator=g, device="cuda").bfloat16()
+            out = torch.zeros_like(q)
+            do_attend(pkg, store, cache, q, out, ints(300 - n), 0.125, n=n, max_len=small, accumulate=True)
+            outs.append(out)
+        evict(pkg, store, cache, cache, 200, 4, 20, ints(300), ints(300), max_len=small)
+        results.append(outs + [cache.k[0, :, :200].clone(), cache.v[0, :, :200].clone(), cache.k_scale[0, :, :4].clone(), cache.weight[0, :, :200].clone(), cache.slot_pos[0, :, :200].clone()])
+    assert all(same_bits(x, y) for x, y in zip(*results))
 
 
 def test_two_calls_at_once(pkg, store):
