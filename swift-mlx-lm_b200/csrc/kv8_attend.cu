@@ -600,9 +600,15 @@ RowsPlan rows_plan(const swlm_kv8_cache& c, const swlm_kv8_attend& a, size_t* by
     const long long groups = (long long)c.batch * c.kv_heads * p.row_tiles, units = groups * ((span + kUnit - 1) / kUnit);
     bool several;   // parts that have to be joined
     if (p.rows > kSaveRows) {
-        // runs of at least four key tiles, as many as make two CTAs per SM (one after the other)
-        const long long want = std::max<long long>(1, 2 * kSms / groups), most = (span + 4 * kPromptKeys - 1) / (4 * kPromptKeys);
-        const int runs = (int)std::min(want, most);
+        // Runs of slots per block of rows: as many as cost least, in key tiles: rounds of one CTA per SM, each its tiles and a start and end of about two;
+        // with several runs a join, and each run's results to memory and back (portions of 300 tokens over 2000: 41 us in three runs, 58 with twice as many)
+        const int tiles = (span + kPromptKeys - 1) / kPromptKeys;
+        int runs = 1;
+        double least = 1e30;
+        for (int r = 1; r <= std::min(tiles, kSms); ++r) {
+            const double rounds = (double)((groups * r + kSms - 1) / kSms), cost = rounds * ((tiles + r - 1) / r + 2) + (r > 1 ? 3 + 0.016 * groups * r : 0.0);
+            if (cost < least) { least = cost; runs = r; }
+        }
         p.chunk = ((span + runs - 1) / runs + kPromptKeys - 1) / kPromptKeys * kPromptKeys;
         p.splits = (span + p.chunk - 1) / p.chunk;
         several = p.splits > 1;
