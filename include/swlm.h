@@ -356,7 +356,8 @@ int swlm_op_kv8_append_dev(swlm_ctx* ctx, const swlm_kv8_cache* cache, const swl
  * accumulate: weight[b][h][slot] += the softmax weights that the step's queries of all heads of the group have for the slot.
  * Scores, softmax and sums are fp32; probabilities meet the values as fp16. An infinity or NaN in a query makes that query's results (and,
  * accumulated, the weights that it adds) NaN.
- * scratch: swlm_op_kv8_attend_scratch_bytes() (0: none needed), 16-byte aligned, not shared by calls that may overlap. */
+ * scratch: swlm_op_kv8_attend_scratch_bytes() (0: none needed), 16-byte aligned, not shared by calls that may overlap. A bounded wait that
+ * expires on the device makes the context's next swlm_op_kv8_attend_dev return SWLM_ERR_TIMEOUT without doing anything; results since then are not valid. */
 typedef struct swlm_kv8_attend {
     const void* q;
     void* out;

@@ -14,10 +14,9 @@
 // the largest value scale so far: values of blocks down to 2^-24 of the largest scale keep that precision. Partial results of a tile
 // are joined by a second launch, which also adds the weights.
 //
-// What bounds it: memory, and some ten us of start, join and dependent launch. 8 x 8192 tokens, 32 / 8 heads of 128, int8: 34.7 us for 134 MB (3.9 TB/s,
-// 0.59 of the measured copy; the steps alone 26 us, 0.79); 1 x 131072: 58 us (0.70). Without the products the steps take two us less. Runs
-// of slots per CTA of a grid over (run, KV head, sequence) took 41 and 70 us; two heads' tiles of 24 rows instead of 16 and 16 for five drafted
-// tokens were slower (55 us against 50).
+// What bounds it: memory, and some ten us of start, merge and the second launch. 8 x 8192 tokens, 32 / 8 heads of 128, int8: 33.5 us for 134 MB (0.61
+// of the measured copy; 26 us without merge and second launch); 1 x 131072: 53.6 us (0.77). Without the products of either kind a pass takes 2 to 5 us
+// less. The next launch waits for this one's end instead of being let in early: its CTAs on the SMs cost 8 of 49 us (8 x 8192 with weights).
 #include <algorithm>
 
 #include "kv8_device.cuh"
