@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
             const int slot = key_lo + j * kPromptKeys + key;
 #pragma unroll
             for (int i = 0; i < PER; ++i)
-                r[i] = key + i * STEP < kPromptKeys && slot + i * STEP < end ? __ldg(reinterpret_cast<const uint4*>(src + i * STEP * HD)) : make_uint4(0, 0, 0, 0);   // (nothing that may be NaN)
+                r[i] = key + i * STEP < kPromptKeys && slot + i * STEP < end ? *reinterpret_cast<const uint4*>(src + i * STEP * HD) : make_uint4(0, 0, 0, 0);   // (nothing that may be NaN)
         };
         const unsigned off = (piece >> 2) * KV_HALF + key * 128, off0 = off + (((piece * 2 & 7) ^ (key & 7)) << 4), off1 = off + (((piece * 2 & 7 | 1) ^ (key & 7)) << 4);
         auto store = [&](unsigned char* dst, const uint4 (&r)[PER]) {
@@ -254,8 +254,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
 #pragma unroll
             for (int g = 0; g < GROUPS; ++g) {
                 const int slot = key_lo + j * kPromptKeys + g * KEYS;
-                kn[g] = slot < end ? __ldg(ks + (slot >> block_shift)) : 0.f;
-                vn[g] = slot < end ? __ldg(vs + (slot >> block_shift)) : 0.f;
+                kn[g] = slot < end ? ks[slot >> block_shift] : 0.f;
+                vn[g] = slot < end ? vs[slot >> block_shift] : 0.f;
             }
         };
         if (tiles) scales(0);
@@ -507,7 +507,7 @@ __global__ void __launch_bounds__(kWeightThreads, 2) kv8_weights_kernel(const sw
         const unsigned off = (piece >> 2) * K_HALF;
 #pragma unroll 4
         for (int r = row; r < kWeightKeys; r += STEP) {
-            const uint4 v = key0 + r < end ? __ldg(reinterpret_cast<const uint4*>(src + (size_t)r * HD)) : make_uint4(0, 0, 0, 0);
+            const uint4 v = key0 + r < end ? *reinterpret_cast<const uint4*>(src + (size_t)r * HD) : make_uint4(0, 0, 0, 0);
             const unsigned w[4] = {prepared<CODE>(v.x), prepared<CODE>(v.y), prepared<CODE>(v.z), prepared<CODE>(v.w)};
             *reinterpret_cast<uint4*>(k_sm + off + r * 128 + ((chunk ^ (r & 7)) << 4)) = make_uint4(pair_of<CODE, 0>(w[0]), pair_of<CODE, 1>(w[0]), pair_of<CODE, 0>(w[1]), pair_of<CODE, 1>(w[1]));
             *reinterpret_cast<uint4*>(k_sm + off + r * 128 + (((chunk + 1) ^ (r & 7)) << 4)) = make_uint4(pair_of<CODE, 0>(w[2]), pair_of<CODE, 1>(w[2]), pair_of<CODE, 0>(w[3]), pair_of<CODE, 1>(w[3]));
