@@ -191,7 +191,7 @@ __global__ void kv8_lengths_kernel(int batch, const int32_t* in, const int32_t* 
 
 // ---- evict -----------------------------------------------------------------------------------------------------------------
 
-constexpr int kSelectCtas = 8, kSelectThreads = 512, kSelectWarps = kSelectThreads / 32;   // CTAs of a cluster
+constexpr int kSelectThreads = 512, kSelectWarps = kSelectThreads / 32, kSelectSlots = 4096;   // slots of a CTA, up to eight CTAs
 constexpr int kDigitBits = 11, kDigits = 1 << kDigitBits;
 constexpr int kCachedKeys = 24 * 1024;   // keys of a CTA that stay in shared memory between the passes
 
@@ -214,8 +214,8 @@ __device__ __forceinline__ unsigned evict_key(float w, int pos, int sink, long l
 }
 
 // One cluster per (sequence, KV head); its CTAs have equal runs of slots. The digits' counts of all of them are added up by each.
-template <bool CACHED>
-__global__ void __cluster_dims__(kSelectCtas, 1, 1) __launch_bounds__(kSelectThreads) kv8_select_kernel(const swlm_kv8_cache c, const swlm_kv8_evict a) {
+template <int CTAS, bool CACHED>
+__global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(kSelectThreads) kv8_select_kernel(const swlm_kv8_cache c, const swlm_kv8_evict a) {
     extern __shared__ unsigned keys[];
     __shared__ __align__(16) unsigned hist[2][kDigits];
     static_assert(kDigits == 4 * kSelectThreads, "four digits of a thread");
@@ -223,7 +223,11 @@ __global__ void __cluster_dims__(kSelectCtas, 1, 1) __launch_bounds__(kSelectThr
     __shared__ unsigned found_digit, found_above, found_all, sums[kSelectWarps];
     pdl_wait();
     const cg::cluster_group cluster = cg::this_cluster();
-    const int b = blockIdx.y, h = blockIdx.x / kSelectCtas, rank = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    auto sync = [&]() {
+        if constexpr (CTAS == 1) __syncthreads();
+        else cluster.sync();
+    };
+    const int b = blockIdx.y, h = blockIdx.x / CTAS, rank = CTAS == 1 ? 0 : (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int len = min(min(a.lengths[b], a.max_len), c.capacity), keep = a.keep;
     if (len <= keep) return;   // (the whole cluster) nothing leaves: the second kernel does not look at the plan
     const size_t head = (size_t)b * c.kv_heads + h;
@@ -231,7 +235,7 @@ __global__ void __cluster_dims__(kSelectCtas, 1, 1) __launch_bounds__(kSelectThr
     const int32_t* pos = c.slot_pos + head * c.capacity;
     const long long recent_from = (long long)a.seen[b] - a.recent;
     // this CTA's slots: first .. last - 1
-    const int share = (len + kSelectCtas * 32 - 1) / (kSelectCtas * 32) * 32, first = min(rank * share, len), last = min(first + share, len);
+    const int share = (len + CTAS * 32 - 1) / (CTAS * 32) * 32, first = min(rank * share, len), last = min(first + share, len);
     auto key_of = [&](int i) { return evict_key(weight[i], pos[i], a.sink, recent_from); };
     for (int i = tid; i < 2 * kDigits; i += kSelectThreads) hist[0][i] = 0;
     if (CACHED) {
@@ -250,13 +254,13 @@ __global__ void __cluster_dims__(kSelectCtas, 1, 1) __launch_bounds__(kSelectThr
             const unsigned k = key(i);
             if ((k & mask) == prefix) atomicAdd(&mine[(k >> shift) & (kDigits - 1)], 1u);
         }
-        cluster.sync();   // (what the pass before counted has been read by all)
+        sync();   // (what the pass before counted has been read by all)
         // thread i has the four digits from kDigits - 4 - 4 i on: counts from the top down
         const int low = kDigits - 4 - 4 * tid;
         uint4 count = make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int r = 0; r < kSelectCtas; ++r) {
-            const uint4 v = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(mine, r) + low);
+        for (int r = 0; r < CTAS; ++r) {
+            const uint4 v = *reinterpret_cast<const uint4*>((CTAS == 1 ? mine : cluster.map_shared_rank(mine, r)) + low);
             count.x += v.x; count.y += v.y; count.z += v.z; count.w += v.w;
         }
         *reinterpret_cast<uint4*>(hist[(pass + 1) & 1] + low) = make_uint4(0, 0, 0, 0);
@@ -302,11 +306,11 @@ __global__ void __cluster_dims__(kSelectCtas, 1, 1) __launch_bounds__(kSelectThr
         for (int w = 0; w < warp; ++w) prior += seg[what][w];
         return prior;
     };
-    auto of_ranks = [&](int what) { return (int)__reduce_add_sync(0xffffffffu, lane < rank ? (unsigned)cluster.map_shared_rank(counted, lane)[what] : 0u); };
+    auto of_ranks = [&](int what) { return CTAS == 1 ? 0 : (int)__reduce_add_sync(0xffffffffu, lane < rank ? (unsigned)cluster.map_shared_rank(counted, lane)[what] : 0u); };
     int ties = 0;
     for (int i = from; i < to; i += 32) ties += __popc(__ballot_sync(0xffffffffu, i + lane < to && key(min(i + lane, to - 1)) == limit));
     int tie0 = before(0, ties);
-    cluster.sync();
+    sync();
     tie0 += of_ranks(0);
     auto walk = [&](auto&& each) {   // each(slot, within, stays)
         int t = tie0;
@@ -326,7 +330,7 @@ __global__ void __cluster_dims__(kSelectCtas, 1, 1) __launch_bounds__(kSelectThr
         moving += __popc(__ballot_sync(0xffffffffu, stays && slot >= keep));
     });
     int free0 = before(1, free_slots), move0 = before(2, moving);
-    cluster.sync();
+    sync();
     free0 += of_ranks(1);
     move0 += of_ranks(2);
     const EvictPlan plan(a.scratch, head, keep);
@@ -344,7 +348,7 @@ __global__ void __cluster_dims__(kSelectCtas, 1, 1) __launch_bounds__(kSelectThr
         free0 += __popc(f);
         move0 += __popc(m);
     });
-    cluster.sync();   // no CTA leaves while another may read its counts
+    if constexpr (CTAS > 1) cluster.sync();   // no CTA leaves while another may read its counts
 }
 
 constexpr int kMoveThreads = 256, kMoveUnits = 4;   // a unit: 16 codes
@@ -465,7 +469,7 @@ int launch_kv8_lengths(int batch, const int32_t* in, const int32_t* counts, int 
 }
 
 int kv8_init() {
-    SWLM_CUDA(cudaFuncSetAttribute(kv8_select_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kCachedKeys * 4));
+    SWLM_CUDA((cudaFuncSetAttribute(kv8_select_kernel<8, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kCachedKeys * 4)));
     return kv8_attend_init();
 }
 
@@ -475,13 +479,14 @@ int launch_kv8_evict(const swlm_kv8_cache& c, const swlm_kv8_cache& to, const sw
     const int span = std::min(a.max_len, c.capacity);
     cudaError_t e = cudaSuccess;
     if (span > a.keep) {
-        const dim3 grid((unsigned)c.kv_heads * kSelectCtas, (unsigned)c.batch);
-        const int share = (span + kSelectCtas * 32 - 1) / (kSelectCtas * 32) * 32;
-        if (share <= kCachedKeys) {
-            e = launch_k(kv8_select_kernel<true>, grid, dim3(kSelectThreads), (size_t)share * 4, s, c, a);
-        } else {
-            e = launch_k(kv8_select_kernel<false>, grid, dim3(kSelectThreads), 0, s, c, a);
-        }
+        // A barrier of a cluster costs what a thousand slots do, and CTAs beside it are other heads' (us, eviction of a quarter, 1 / 2 / 4 / 8 CTAs):
+        // 128 heads x 1000 slots 30.9 / 32.7 / 45.5 / 92.7, 32 x 4352 40.0 / 38.6 / 38.6 / 47.4, 8 x 12000 51 / 41 / 35 / 36, 2 x 32768 151 / 49 / 35 / 32
+        const int ctas = span <= kSelectSlots ? 1 : span <= 2 * kSelectSlots ? 2 : span <= 4 * kSelectSlots ? 4 : 8;
+        const dim3 grid((unsigned)c.kv_heads * ctas, (unsigned)c.batch);
+        const int share = (span + ctas * 32 - 1) / (ctas * 32) * 32;   // their keys stay in shared memory, up to kCachedKeys (only eight CTAs can have more)
+        auto launch = [&](auto kernel) { return launch_k(kernel, grid, dim3(kSelectThreads), share <= kCachedKeys ? (size_t)share * 4 : 0, s, c, a); };
+        e = ctas == 1 ? launch(kv8_select_kernel<1, true>) : ctas == 2 ? launch(kv8_select_kernel<2, true>) : ctas == 4 ? launch(kv8_select_kernel<4, true>) :
+            share <= kCachedKeys ? launch(kv8_select_kernel<8, true>) : launch(kv8_select_kernel<8, false>);
         if (e != cudaSuccess) return cuda_fail(e, "kv8 selection launch");
     } else if (c.k == to.k) {
         return SWLM_OK;   // in place, and no sequence can have more than `keep` tokens
