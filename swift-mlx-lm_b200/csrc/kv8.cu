@@ -192,7 +192,7 @@ __global__ void kv8_lengths_kernel(int batch, const int32_t* in, const int32_t* 
 // ---- evict -----------------------------------------------------------------------------------------------------------------
 
 constexpr int kSelectThreads = 512, kSelectWarps = kSelectThreads / 32, kSelectSlots = 4096;   // slots of a CTA, up to eight CTAs
-constexpr int kDigitBits = 11, kDigits = 1 << kDigitBits;
+constexpr int kDigitBits = 11, kDigits = 1 << kDigitBits, kGroups = kDigits / 32;
 constexpr int kCachedKeys = 24 * 1024;   // keys of a CTA that stay in shared memory between the passes
 
 // Scratch of one (sequence, KV head): where slot j < keep comes from (j itself, or ~i: the i-th of the tokens that move), the slots of the
@@ -217,10 +217,11 @@ __device__ __forceinline__ unsigned evict_key(float w, int pos, int sink, long l
 template <int CTAS, bool CACHED>
 __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(kSelectThreads) kv8_select_kernel(const swlm_kv8_cache c, const swlm_kv8_evict a) {
     extern __shared__ unsigned keys[];
-    __shared__ __align__(16) unsigned hist[2][kDigits];
-    static_assert(kDigits == 4 * kSelectThreads, "four digits of a thread");
+    __shared__ __align__(16) unsigned hist[2][kDigits];   // counts of a pass, of this CTA
+    __shared__ unsigned groups[2][kGroups];               // and of the 32 digits of a group
+    __shared__ unsigned coarse[CTAS][kGroups], fine[CTAS][32];   // all CTAs' counts of the groups, and of the digits of the one that was found
+    static_assert(kDigits == 4 * kSelectThreads && kGroups * 8 == kSelectThreads, "four digits of a thread, eight threads of a group");
     __shared__ int seg[3][kSelectWarps], counted[3];   // ties, free slots, moving tokens: of a warp, of the CTA
-    __shared__ unsigned found_digit, found_above, found_all, sums[kSelectWarps];
     pdl_wait();
     const cg::cluster_group cluster = cg::this_cluster();
     auto sync = [&]() {
@@ -239,11 +240,25 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(kSelectThreads) k
     auto key_of = [&](int i) { return evict_key(weight[i], pos[i], a.sink, recent_from); };
     for (int i = tid; i < 2 * kDigits; i += kSelectThreads) hist[0][i] = 0;
     if (CACHED) {
-#pragma unroll 4
+#pragma unroll 8
         for (int i = first + tid; i < last; i += kSelectThreads) keys[i - first] = key_of(i);
     }
     auto key = [&](int i) { return CACHED ? keys[i - first] : key_of(i); };
     __syncthreads();
+
+    auto own_counts = [&](const unsigned* counts) {
+        const uint4 v = *reinterpret_cast<const uint4*>(counts + 4 * tid);
+        return v.x + v.y + v.z + v.w;
+    };
+    auto of_rank = [&](auto* mine, int r) { return CTAS == 1 ? mine : cluster.map_shared_rank(mine, r); };
+    auto prefix_sum = [&](unsigned v) {   // of the lanes up to this one
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned u = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += u;
+        }
+        return v;
+    };
 
     // radix selection of the keep-th largest key, from the top digit down
     unsigned prefix = 0, mask = 0;
@@ -254,40 +269,46 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(kSelectThreads) k
             const unsigned k = key(i);
             if ((k & mask) == prefix) atomicAdd(&mine[(k >> shift) & (kDigits - 1)], 1u);
         }
+        __syncthreads();
+        unsigned sum = own_counts(mine);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        if ((lane & 7) == 0) groups[pass & 1][tid >> 3] = sum;
         sync();   // (what the pass before counted has been read by all)
-        // thread i has the four digits from kDigits - 4 - 4 i on: counts from the top down
-        const int low = kDigits - 4 - 4 * tid;
-        uint4 count = make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int r = 0; r < CTAS; ++r) {
-            const uint4 v = *reinterpret_cast<const uint4*>((CTAS == 1 ? mine : cluster.map_shared_rank(mine, r)) + low);
-            count.x += v.x; count.y += v.y; count.z += v.z; count.w += v.w;
-        }
-        *reinterpret_cast<uint4*>(hist[(pass + 1) & 1] + low) = make_uint4(0, 0, 0, 0);
-        const unsigned sum = count.x + count.y + count.z + count.w;
-        unsigned above = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const unsigned v = __shfl_up_sync(0xffffffffu, above, o);
-            if (lane >= o) above += v;
-        }
-        if (lane == 31) sums[warp] = above;
+        *reinterpret_cast<uint4*>(hist[(pass + 1) & 1] + 4 * tid) = make_uint4(0, 0, 0, 0);
+        // the group of digits that the wanted key is in, then the digit: 3 KB of other CTAs' counts instead of all 64 KB; every warp finds the same
+        if (tid < CTAS * kGroups) coarse[tid / kGroups][tid % kGroups] = of_rank(groups[pass & 1], tid / kGroups)[tid % kGroups];
         __syncthreads();
-        for (int w = 0; w < warp; ++w) above += sums[w];
-        above -= sum;   // keys of higher digits
-        if (above < (unsigned)want && above + sum >= (unsigned)want) {
-            const unsigned n[4] = {count.w, count.z, count.y, count.x};
-            int d = 0;
-            while (above + n[d] < (unsigned)want) above += n[d++];
-            found_digit = (unsigned)(low + 3 - d);
-            found_above = above;
-            found_all = above + n[d] == (unsigned)want;
+        unsigned above;
+        int group = 0, digit = 0;
+        {
+            unsigned hi = 0, lo = 0;   // lane l has groups 63 - 2 l and 62 - 2 l: from the top down
+#pragma unroll
+            for (int r = 0; r < CTAS; ++r) { hi += coarse[r][kGroups - 1 - 2 * lane]; lo += coarse[r][kGroups - 2 - 2 * lane]; }
+            const unsigned upto = prefix_sum(hi + lo), before = upto - hi - lo;
+            const int l = __ffs(__ballot_sync(0xffffffffu, upto >= (unsigned)want)) - 1;
+            const bool first_of = before + hi >= (unsigned)want;
+            group = __shfl_sync(0xffffffffu, first_of ? kGroups - 1 - 2 * lane : kGroups - 2 - 2 * lane, l);
+            above = __shfl_sync(0xffffffffu, first_of ? before : before + hi, l);
         }
+        if (tid < CTAS * 32) fine[tid >> 5][lane] = of_rank(mine, tid >> 5)[group * 32 + lane];
         __syncthreads();
+        bool found_all;
+        {
+            unsigned n = 0;   // lane l has digit 31 - l of the group
+#pragma unroll
+            for (int r = 0; r < CTAS; ++r) n += fine[r][31 - lane];
+            const unsigned upto = above + prefix_sum(n);
+            const int l = __ffs(__ballot_sync(0xffffffffu, upto >= (unsigned)want)) - 1;
+            digit = group * 32 + 31 - l;
+            above = __shfl_sync(0xffffffffu, upto - n, l);   // keys of higher digits
+            found_all = __shfl_sync(0xffffffffu, upto, l) == (unsigned)want;
+        }
         const unsigned digits = (unsigned)(kDigits - 1) << shift;
-        prefix = (prefix & ~digits) | found_digit << shift;   // (the last digit overlaps the one before it, with the same bits there)
+        prefix = (prefix & ~digits) | (unsigned)digit << shift;   // (the last digit overlaps the one before it, with the same bits there)
         mask |= digits;
-        want -= (int)found_above;
+        want -= (int)above;
         if (found_all) { want = len; break; }   // all keys with this prefix stay: none of those below it has to be told from another
         if (shift == 0) break;
     }
@@ -296,50 +317,61 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(kSelectThreads) k
     // a run of slots per warp: ties first, then free slots below `keep` and staying ones from it on, each numbered in slot order
     const int run = (last - first + kSelectThreads - 1) / kSelectThreads * 32, from = min(first + warp * run, last), to = min(from + run, last);
     const unsigned below = (1u << lane) - 1u;
-    auto before = [&](int what, int own) {   // how many there are in the runs before this warp's, of all CTAs
-        if (lane == 0) seg[what][warp] = own;
-        __syncthreads();
-        int sum = 0;
-        for (int w = 0; w < kSelectWarps; ++w) sum += seg[what][w];
-        if (tid == 0) counted[what] = sum;
-        int prior = 0;
-        for (int w = 0; w < warp; ++w) prior += seg[what][w];
-        return prior;
+    auto before = [&](int what) {   // of seg[what]: how many there are in the runs before this warp's, of this CTA
+        const unsigned v = lane < kSelectWarps ? (unsigned)seg[what][lane] : 0u, all = __reduce_add_sync(0xffffffffu, v);
+        if (tid == 0) counted[what] = (int)all;
+        return (int)__reduce_add_sync(0xffffffffu, lane < warp ? v : 0u);
     };
     auto of_ranks = [&](int what) { return CTAS == 1 ? 0 : (int)__reduce_add_sync(0xffffffffu, lane < rank ? (unsigned)cluster.map_shared_rank(counted, lane)[what] : 0u); };
-    int ties = 0;
-    for (int i = from; i < to; i += 32) ties += __popc(__ballot_sync(0xffffffffu, i + lane < to && key(min(i + lane, to - 1)) == limit));
-    int tie0 = before(0, ties);
-    sync();
-    tie0 += of_ranks(0);
-    auto walk = [&](auto&& each) {   // each(slot, within, stays)
+    int tie0 = 0;
+    if (want < len) {   // (the same in all CTAs)
+        int ties = 0;
+        for (int i = from; i < to; i += 32) ties += __popc(__ballot_sync(0xffffffffu, i + lane < to && key(min(i + lane, to - 1)) == limit));
+        if (lane == 0) seg[0][warp] = ties;
+        __syncthreads();
+        tie0 = before(0);
+        sync();
+        tie0 += of_ranks(0);
+    }
+    auto walk = [&](auto&& each) {   // each(slot, free, moving): the lanes whose slots below `keep` are free, and whose tokens behind it stay
         int t = tie0;
+#pragma unroll 4
         for (int i = from; i < to; i += 32) {
             const int slot = i + lane;
             const bool in = slot < to;
             const unsigned k = key(min(slot, to - 1));
-            const unsigned tied = __ballot_sync(0xffffffffu, in && k == limit);
-            const bool stays = in && (k > limit || (k == limit && t + __popc(tied & below) < want));
-            t += __popc(tied);
-            each(slot, in, stays);
+            bool stays = k >= limit;
+            if (want < len) {
+                const unsigned tied = __ballot_sync(0xffffffffu, in && k == limit);
+                stays = k > limit || (k == limit && t + __popc(tied & below) < want);
+                t += __popc(tied);
+            }
+            const unsigned changes = __ballot_sync(0xffffffffu, in && stays == (slot >= keep)), kept = __ballot_sync(0xffffffffu, slot < keep);
+            each(slot, changes & kept, changes & ~kept);
         }
     };
-    int free_slots = 0, moving = 0;
-    walk([&](int slot, bool in, bool stays) {
-        free_slots += __popc(__ballot_sync(0xffffffffu, in && slot < keep && !stays));
-        moving += __popc(__ballot_sync(0xffffffffu, stays && slot >= keep));
+    int free0 = 0, move0 = 0;
+    walk([&](int, unsigned f, unsigned m) {
+        free0 += __popc(f);
+        move0 += __popc(m);
     });
-    int free0 = before(1, free_slots), move0 = before(2, moving);
+    if (lane == 0) {
+        seg[1][warp] = free0;
+        seg[2][warp] = move0;
+    }
+    __syncthreads();
+    free0 = before(1);
+    move0 = before(2);
     sync();
     free0 += of_ranks(1);
     move0 += of_ranks(2);
+    if constexpr (CTAS > 1) cluster.barrier_arrive();   // (of the CTAs that may leave when all have read its counts)
     const EvictPlan plan(a.scratch, head, keep);
     const float* ks = c.k_scale + head * (c.capacity / c.block);
     const float* vs = c.v_scale + head * (c.capacity / c.block);
-    walk([&](int slot, bool in, bool stays) {
-        const unsigned f = __ballot_sync(0xffffffffu, in && slot < keep && !stays), m = __ballot_sync(0xffffffffu, stays && slot >= keep);
-        if (in && slot < keep) plan.source[slot] = stays ? slot : ~(free0 + __popc(f & below));
-        if (stays && slot >= keep) {
+    walk([&](int slot, unsigned f, unsigned m) {
+        if (slot < min(to, keep)) plan.source[slot] = f >> lane & 1u ? ~(free0 + __popc(f & below)) : slot;
+        if (m >> lane & 1u) {
             const int i = move0 + __popc(m & below);
             plan.moved[i] = slot;
             plan.k_scale[i] = ks[slot / c.block];
@@ -348,7 +380,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(kSelectThreads) k
         free0 += __popc(f);
         move0 += __popc(m);
     });
-    if constexpr (CTAS > 1) cluster.sync();   // no CTA leaves while another may read its counts
+    if constexpr (CTAS > 1) cluster.barrier_wait();
 }
 
 constexpr int kMoveThreads = 256, kMoveUnits = 4;   // a unit: 16 codes
@@ -426,9 +458,9 @@ __global__ void __launch_bounds__(kMoveThreads) kv8_move_kernel(const swlm_kv8_c
             for (int u = 0; u < kMoveUnits; ++u) {
                 const int i = tid + u * (int)blockDim.x;
                 if (i >= units) continue;
+                const float mine = scales[i >> per];
                 const unsigned w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
                 unsigned out[4] = {0, 0, 0, 0};
-                const float mine = scales[i >> per];
                 if (KIND)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) out[e] = kv8_again<CODE, KIND == 2>(w[e], mine, divisor);
