@@ -12,19 +12,23 @@
 // rows fill the tile), probabilities are transposed in registers (movmatrix) and meet the values as O^T = V^T P^T. The reference
 // maximum of a row moves only when it would grow by more than 2^8. Probabilities are rounded to fp16 (2^-11 of themselves) times 2^7 vs / vr, vr
 // the largest value scale so far: values of blocks down to 2^-24 of the largest scale keep that precision. Partial results of a tile
-// are joined by a second launch, which also adds the weights.
+// are joined by a second launch, which also adds the weights, or by the cluster of CTAs that has all of a tile's slots.
 //
 // What bounds it: memory, and some ten us of start, merge and the second launch. 8 x 8192 tokens, 32 / 8 heads of 128, int8: 33.5 us for 134 MB (0.61
 // of the measured copy; 26 us without merge and second launch); 1 x 131072: 53.6 us (0.77). Without the products of either kind a pass takes 2 to 5 us
 // less. The next launch waits for this one's end instead of being let in early: its CTAs on the SMs cost 8 of 49 us (8 x 8192 with weights).
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #include "kv8_device.cuh"
 
 namespace swlm {
 using namespace kv8;
+namespace cg = cooperative_groups;
 namespace {
 
+constexpr int kClusterCtas = 8;                 // of a cluster, at most
 constexpr int kStreamBatch = 512;               // sequences whose units a CTA adds up
 constexpr int kSaveRows = 64;                   // up to so many rows of a KV head the scores are kept for the weights, beyond they are worked out again
 
@@ -126,11 +130,39 @@ __device__ __forceinline__ void join_parts(const float* ml, const float* po, int
     }
 }
 
+// Four values of a row's result over the CTAs of a cluster, and the row's sum.
+__device__ __forceinline__ float4 join_cluster(const cg::cluster_group& cluster, int ctas, float2* ml, float* out, float& l) {
+    float2 x[kClusterCtas];
+    float4 v[kClusterCtas];
+    float m = -INFINITY;
+#pragma unroll
+    for (int s = 0; s < kClusterCtas; ++s)
+        if (s < ctas) {
+            x[s] = *cluster.map_shared_rank(ml, s);
+            v[s] = *cluster.map_shared_rank(reinterpret_cast<float4*>(out), s);
+        }
+#pragma unroll
+    for (int s = 0; s < kClusterCtas; ++s)
+        if (s < ctas) m = fmaxf(m, x[s].x);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    l = 0.f;
+#pragma unroll
+    for (int s = 0; s < kClusterCtas; ++s)
+        if (s < ctas) {
+            const float f = x[s].x == -INFINITY ? 1.f : exp2_of(x[s].x - m);   // (a part without slots has zeros, or NaN)
+            l += f * x[s].y;
+            o.x += f * v[s].x; o.y += f * v[s].y; o.z += f * v[s].z; o.w += f * v[s].w;
+        }
+    return o;
+}
+
 template <int HD, int CODE, int NT, bool SAVE>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_rows_kernel(const swlm_kv8_cache c, const swlm_kv8_attend a, const RowsPlan p) {
     constexpr int KS = HD / 16, MT = HD / 16, NS = stages<HD>(), SB = stage_bytes<HD>(), TR = 8 * NT;
     extern __shared__ __align__(16) unsigned char sm[];
     __shared__ float warp_m[kWarps][TR], warp_l[kWarps][TR];
+    __shared__ float2 part_ml[TR];   // of this CTA, for the others of its cluster
+    __shared__ float row_m[TR], row_inv[TR];
     __shared__ int scan[kWarps + 1];
     int4* const info = reinterpret_cast<int4*>(sm + rows_smem<HD>());   // [batch + 1]: units before the sequence, its length, count, first row
     pdl_wait();
@@ -204,7 +236,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_r
             u += unit1 - unit0;
         } else {
             part = kv8_part(b, a.lengths, a.counts, a.starts, a.n, a.rows);
-            h = blockIdx.y; tile = blockIdx.x; unit0 = 0; unit1 = sequence_units(part, span);
+            // a cluster of CTAs, or one, has all slots of a tile: equal shares of its units
+            const int units = sequence_units(part, span), rank = (int)blockIdx.x % p.cluster;
+            h = blockIdx.y; tile = (int)blockIdx.x / p.cluster;
+            unit0 = units * rank / p.cluster;
+            unit1 = units * (rank + 1) / p.cluster;
             u = u_end;
             if (tile * TR >= part.count * G) break;
         }
@@ -462,6 +498,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_r
                 l += f * warp_l[w][r];
                 o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
             }
+            if (p.cluster > 1) {
+                if (d == 0) part_ml[r] = make_float2(m, l);
+                *reinterpret_cast<float4*>(outs + (size_t)r * HD + d) = o;   // (the first warp's, which nobody else reads)
+                continue;
+            }
             if (d == 0 && (SAVE || !whole)) *reinterpret_cast<float2*>(p.part_ml + (slot * TR + r) * 2) = make_float2(m, l);
             if (!whole) {
                 *reinterpret_cast<float4*>(p.part_o + (slot * TR + r) * HD + d) = o;
@@ -469,6 +510,47 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_r
                 const int i = row / G;
                 store_out(static_cast<unsigned short*>(a.out) + (int64_t)(part.start + i) * a.out_stride + (size_t)(h * G + row - i * G) * HD + d, o, l, f16);
             }
+        }
+        if (p.cluster > 1) {
+            // ---- the cluster's results together ----
+            const cg::cluster_group cluster = cg::this_cluster();
+            const int rank = (int)cluster.block_rank();
+            cluster.sync();
+            for (int item = rank * kThreads + tid; item < TR * (HD / 4); item += p.cluster * kThreads) {
+                const int r = item / (HD / 4), d = item % (HD / 4) * 4, row = row0 + r;
+                if (row >= rows) continue;
+                float l;
+                const float4 o = join_cluster(cluster, p.cluster, part_ml + r, outs + (size_t)r * HD + d, l);
+                const int i = row / G;
+                store_out(static_cast<unsigned short*>(a.out) + (int64_t)(part.start + i) * a.out_stride + (size_t)(h * G + row - i * G) * HD + d, o, l, f16);
+            }
+            if (SAVE && tid < TR) {
+                float m = -INFINITY, l = 0.f;
+                for (int s = 0; s < p.cluster; ++s) m = fmaxf(m, cluster.map_shared_rank(part_ml, s)[tid].x);
+                for (int s = 0; s < p.cluster; ++s) {
+                    const float2 v = cluster.map_shared_rank(part_ml, s)[tid];
+                    l += v.x == -INFINITY ? v.y : exp2_of(v.x - m) * v.y;
+                }
+                row_m[tid] = m == -INFINITY ? 0.f : m;
+                row_inv[tid] = l == 0.f ? 0.f : 1.f / l;
+            }
+            cluster.barrier_arrive();
+            if (SAVE) {   // this CTA's slots of all rows: there is one tile
+                __syncthreads();
+                float* const w = c.weight + head * c.capacity;
+                for (int slot = from + tid; slot < to; slot += kThreads) {
+                    const float* const sc = p.scores + (head * p.span + slot) * p.pitch;
+                    float sum = 0.f;
+                    for (int r = 0; r < rows; r += 2) {
+                        const float2 v = *reinterpret_cast<const float2*>(sc + r);
+                        if (slot < visible(part, r / G, span)) sum += exp2_of(v.x - row_m[r]) * row_inv[r];
+                        if (r + 1 < rows && slot < visible(part, (r + 1) / G, span)) sum += exp2_of(v.y - row_m[r + 1]) * row_inv[r + 1];
+                    }
+                    w[slot] += sum;
+                }
+            }
+            cluster.barrier_wait();   // no CTA leaves while others read its results
+            break;
         }
         __syncthreads();   // the next one's copies take the results' place
     }
@@ -591,6 +673,7 @@ constexpr size_t align16(size_t v) { return (v + 15) & ~(size_t)15; }
 
 RowsPlan rows_plan(const swlm_kv8_cache& c, const swlm_kv8_attend& a, size_t* bytes) {
     RowsPlan p{};
+    p.cluster = 1;
     const int span = std::min(a.max_len, c.capacity), G = a.heads / c.kv_heads;
     p.rows = a.n * G;
     p.tiles = p.rows <= 8 ? 1 : p.rows <= kSaveRows ? 2 : kPromptRows / 8;
@@ -614,7 +697,13 @@ RowsPlan rows_plan(const swlm_kv8_cache& c, const swlm_kv8_attend& a, size_t* by
     } else {
         // CTAs that fill the GPU once, or one per unit where there are fewer
         const int fill = kSms * (p.tiles > 1 ? 2 : c.head_dim == 128 ? rows_ctas<128>() : rows_ctas<64>());
-        p.stream = c.batch <= kStreamBatch && units < (1LL << 30) && groups < 16 * fill;
+        // A cluster joins its own results, and adds its own slots' weights, in one launch, where its CTAs have few units each and all clusters run at once. us,
+        // against two launches (32 / 8 heads of 128, int8): 1 x 1000 slots 7.0 / 8.8, 4 x 1000 7.4 / 9.6, 4 x 4000 12.9 / 16.6, 16 x 1000 13.0 / 17.6,
+        // 1 x 8000 (eight units a CTA) 12.6 / 12.7; with weights (and a copy of them, some 5) 1 x 2000 12.4 / 14.0, but 1 x 4000 (four) 16.5 / 13.8
+        const int per = (int)std::min<long long>(units / groups, 1 << 24), deep = a.accumulate ? 2 : 4;
+        while (p.cluster < kClusterCtas && p.cluster < per && 2 * p.cluster * groups <= fill) p.cluster *= 2;
+        if (per > deep * p.cluster || (a.accumulate && p.row_tiles > 1)) p.cluster = 1;
+        p.stream = p.cluster == 1 && c.batch <= kStreamBatch && units < (1LL << 30) && groups < 16 * fill;
         p.ctas = p.stream ? (int)std::min<long long>(fill, units) : 0;
         several = p.stream && units > groups;
     }
@@ -627,7 +716,7 @@ RowsPlan rows_plan(const swlm_kv8_cache& c, const swlm_kv8_attend& a, size_t* by
     auto take = [&](size_t n) { char* q = base + at; at += align16(n); return q; };
     if (several) p.part_o = reinterpret_cast<float*>(take(places * 8 * p.tiles * c.head_dim * 4));
     const bool saves = a.accumulate && p.rows <= kSaveRows;
-    if (several || saves) {
+    if (several || (saves && p.cluster == 1)) {
         p.part_ml = reinterpret_cast<float*>(take(places * 8 * p.tiles * 8));
         if (p.stream) p.table = reinterpret_cast<int*>(take(((size_t)c.batch + 1) * 4));
     }
@@ -646,8 +735,8 @@ RowsPlan rows_plan(const swlm_kv8_cache& c, const swlm_kv8_attend& a, size_t* by
 
 template <int HD, int CODE, int NT>
 cudaError_t launch_tiles(const dim3& grid, size_t smem, const swlm_kv8_cache& c, const swlm_kv8_attend& a, const RowsPlan& p, cudaStream_t s) {
-    return p.pitch ? launch_k(kv8_rows_kernel<HD, CODE, NT, true>, grid, dim3(kThreads), smem, s, c, a, p)
-                   : launch_k(kv8_rows_kernel<HD, CODE, NT, false>, grid, dim3(kThreads), smem, s, c, a, p);
+    auto launch = [&](auto kernel) { return p.cluster > 1 ? launch_clusters(kernel, p.cluster, grid, dim3(kThreads), smem, s, c, a, p) : launch_k(kernel, grid, dim3(kThreads), smem, s, c, a, p); };
+    return p.pitch ? launch(kv8_rows_kernel<HD, CODE, NT, true>) : launch(kv8_rows_kernel<HD, CODE, NT, false>);
 }
 
 template <int HD, int CODE>
@@ -656,14 +745,14 @@ int launch_rows(const swlm_kv8_cache& c, const swlm_kv8_attend& a, const RowsPla
         const int rc = launch_kv8_prompt(c, a, p, status, s);
         if (rc) return rc;
     } else {
-        const dim3 grid = p.stream ? dim3((unsigned)p.ctas) : dim3((unsigned)p.row_tiles, (unsigned)c.kv_heads, (unsigned)c.batch);
+        const dim3 grid = p.stream ? dim3((unsigned)p.ctas) : dim3((unsigned)(p.row_tiles * p.cluster), (unsigned)c.kv_heads, (unsigned)c.batch);
         const size_t smem = rows_smem<HD>() + (p.stream ? ((size_t)c.batch + 1) * sizeof(int4) : 0);
         const cudaError_t e = p.tiles == 1 ? launch_tiles<HD, CODE, 1>(grid, smem, c, a, p, s) : launch_tiles<HD, CODE, 2>(grid, smem, c, a, p, s);
         if (e != cudaSuccess) return cuda_fail(e, "kv8 attention launch");
     }
     const int span = std::min(a.max_len, c.capacity);
     const int per = kJoinThreads / (HD / 4) / p.join_groups, join = p.part_o ? (p.rows + per - 1) / per : 0;
-    const int slots = p.pitch ? (span + kJoinSlots - 1) / kJoinSlots : 0;
+    const int slots = p.pitch && p.cluster == 1 ? (span + kJoinSlots - 1) / kJoinSlots : 0;
     if (join + slots) {
         const cudaError_t j = launch_k(kv8_join_kernel<HD>, dim3((unsigned)(join + slots), (unsigned)c.kv_heads, (unsigned)c.batch), dim3(kJoinThreads), 0, s, c, a, p, join);
         if (j != cudaSuccess) return cuda_fail(j, "kv8 join launch");

@@ -21,6 +21,7 @@ struct RowsPlan {
     int row_tiles;  // of a KV head at most, of 8 * tiles rows each
     int rows;       // n * group
     int stream, ctas;   // CTAs over equal shares of all units (stream), or one per (sequence, KV head, tile)
+    int cluster;    // CTAs of a cluster that shares the slots of one (sequence, KV head, tile) and joins its results itself (1: none)
     int splits, chunk;  // the kernel of many rows: slots of a tile in runs of `chunk` (splits 0: the kernel of few rows)
     int span;       // slots that can be attended, rounded up to kStep
     int pitch;      // rows of a slot's kept scores (0: not kept)

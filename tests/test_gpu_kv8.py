@@ -239,8 +239,8 @@ def test_attend(pkg, store, batch, heads, kv_heads, dim, block, lengths, counts,
 @pytest.mark.parametrize("accumulate", [False, True])
 @pytest.mark.parametrize("batch,heads,kv_heads,dim,most", [(64, 16, 8, 64, 1400), (64, 4, 4, 128, 1900), (520, 1, 1, 64, 200)], ids=str)
 def test_attend_of_many_sequences(pkg, store, batch, heads, kv_heads, dim, most, accumulate):
-    """Batches whose slots come in equal shares, several sequences to a CTA and sequences over several CTAs, which the last CTA to arrive joins; a batch
-    of one CTA per head. Empty, parked and full sequences between others. Twice with the same scratch: counters are back at none."""
+    """Batches whose slots come in equal shares, several sequences to a CTA and sequences over several CTAs, and a batch of one CTA per head. Empty, parked
+    and full sequences between others. Twice with the same scratch."""
     g = torch.Generator().manual_seed(batch + dim)
     lengths = [int(x) for x in torch.randint(0, most, (batch,), generator=g)]
     lengths[0], lengths[3], lengths[4], lengths[-1] = most, -1, 0, most
@@ -267,6 +267,20 @@ def test_attend_of_many_sequences(pkg, store, batch, heads, kv_heads, dim, most,
             else:
                 assert torch.equal(cache.weight[b], before[b])
     assert (scratch[step.scratch_bytes:] == 0xFF).all()
+
+
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("max_len", [130, 300, 900, 2048, 4096, None])
+@pytest.mark.parametrize("batch,heads,kv_heads,dim,lengths,counts", [
+    (1, 8, 8, 128, [4000], [1]),
+    (4, 14, 2, 64, [1030, -1, 0, 128], [2, 1, 1, 0]),              # fourteen rows; parked, empty and without a token
+    (2, 10, 2, 128, [255, 1999], [5, 3]),                          # 25 rows: two tiles
+    (20, 8, 4, 64, [97 * i for i in range(20)], [1] * 20),         # two or four CTAs a cluster
+], ids=str)
+def test_attend_whoever_joins(pkg, store, batch, heads, kv_heads, dim, lengths, counts, max_len, accumulate):
+    """The same sequences where clusters of two, four or eight CTAs have a head's slots, some of them none, and where shares of the GPU have them: which, goes by max_len."""
+    cache = Cache(pkg, batch, kv_heads, dim, 16384, 64, 1).fill([max(0, a + c) for a, c in zip(lengths, counts)])
+    check_attend(pkg, store, cache, batch, heads, dim, lengths, counts, torch.bfloat16, accumulate, max_len=max_len)
 
 
 @pytest.mark.parametrize("counts", [[1, 1], [40, 40]], ids=str)
