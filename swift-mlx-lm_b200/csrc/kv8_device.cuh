@@ -26,6 +26,7 @@ struct RowsPlan {
     int span;       // slots that can be attended, rounded up to kStep
     int pitch;      // rows of a slot's kept scores (0: not kept)
     int join_groups;   // groups of lanes that share a row's parts
+    int join_lanes;    // lanes that share a slot's rows, as a power of two
     float* part_o;  // [places][8 * tiles][head_dim], not normalised; places: (sequence, KV head, tile) + CTA, or of many rows * splits + run
     float* part_ml; // [places][8 * tiles][2]: reference maximum (log2), sum
     float* scores;  // [batch][kv_heads][span][pitch], log2
