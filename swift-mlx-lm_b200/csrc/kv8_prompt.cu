@@ -56,8 +56,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
     __shared__ __align__(8) PromptBars bars;
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int b = blockIdx.z, h = blockIdx.y, G = a.heads / c.kv_heads, span = min(a.max_len, c.capacity);
-    const int block = p.row_tiles - 1 - (int)blockIdx.x / p.splits, split = (int)blockIdx.x % p.splits;   // the longest rows first
+    const int G = a.heads / c.kv_heads, span = min(a.max_len, c.capacity);
+    // The longest rows first, of all heads, so that the last round of CTAs is of the shortest (2048 tokens into an empty cache, 32 / 8 heads of 128: 72 us, head
+    // by head 94); sequence by sequence, as only the device knows which one is long
+    const int turn = (int)blockIdx.x / c.kv_heads, h = (int)blockIdx.x - turn * c.kv_heads, split = turn % p.splits;
+    const int b = turn / p.splits / p.row_tiles, block = p.row_tiles - 1 - (turn / p.splits - b * p.row_tiles);
     const Kv8Part part = kv8_part(b, a.lengths, a.counts, a.starts, a.n, a.rows);
     const int rows = part.count * G, block0 = block * kPromptRows;
     if (block0 >= rows) return;
@@ -563,7 +566,7 @@ __global__ void __launch_bounds__(kWeightThreads, 2) kv8_weights_kernel(const sw
 
 template <int HD, int CODE>
 int launch_prompt(const swlm_kv8_cache& c, const swlm_kv8_attend& a, const RowsPlan& p, int* status, cudaStream_t s) {
-    const dim3 grid((unsigned)(p.row_tiles * p.splits), (unsigned)c.kv_heads, (unsigned)c.batch);
+    const dim3 grid((unsigned)c.batch * c.kv_heads * p.row_tiles * p.splits);
     auto launch = [&](auto kernel) { return launch_k(kernel, grid, dim3(kPromptThreads), prompt_smem<HD>(), s, c, a, p, status); };
     const cudaError_t e = c.block == 128 ? launch(kv8_prompt_kernel<HD, CODE, 1>) : c.block == 64 ? launch(kv8_prompt_kernel<HD, CODE, 2>) :
                           c.block == 32 ? launch(kv8_prompt_kernel<HD, CODE, 4>) : launch(kv8_prompt_kernel<HD, CODE, 8>);
