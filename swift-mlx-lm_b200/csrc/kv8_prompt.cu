@@ -9,11 +9,11 @@
 // and the other in turn); eight warps do the softmax, a thread per row. Probabilities take the place of their scores in tensor memory
 // and are read there as the A operand. The reference maximum of a row moves only when it would grow by more than 2^8.
 //
-// What bounds it (2048 tokens over 8192, 32 / 8 heads of 128: 297 us, 810 TFLOP/s, 0.49 of the measured rate): the chain of a row tile, softmax (two
+// What bounds it (2048 tokens over 6144, 32 / 8 heads of 128: 278 us, 865 TFLOP/s, 0.53 of the measured rate): the chain of a row tile, softmax (two
 // warps of a scheduler share the exponential unit, 2048 clocks a tile), product, next scores, of which the other row tile fills the gaps only
 // in part; and 256 CTAs on 148 SMs. Steps to here: one row tile per CTA, two CTAs per SM 732 us; the loaders' first warp
 // issuing the MMAs, paired fp32 operations 391; two row tiles that share the conversions, a warp for the MMAs 306; key tiles of 128 instead of 64
-// with two score regions 297.
+// with two score regions 297; the longest rows of all heads first 278.
 #include <algorithm>
 
 #include "kv8_device.cuh"
