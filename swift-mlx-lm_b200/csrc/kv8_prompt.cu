@@ -408,25 +408,28 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
 }
 
 // The weights of many rows: weight_j += sum over rows i of exp2(s_ij + shift_i), with the rows' totals known. A CTA has 128 keys, the rows of the products
-// (S^T = K Q^T: a thread per key, so that nothing is added across threads), and walks the row tiles that attend them. Four slots: the
-// queries of a tile, their factors and shifts come as bulk copies while the tiles before are multiplied and summed.
+// (S^T = K Q^T: a thread per key, so that nothing is added across threads), and walks the row tiles that attend them. The
+// queries of a tile, their factors and shifts come as bulk copies, SLOTS - 1 tiles ahead, while the tiles before are multiplied and summed; scores have two
+// regions. Three CTAs of an SM fill each other's waits (3 x 777 rows, heads of 64, both kernels: 137 us, with two 160; 2048 over 6144, heads of 128: 507 and 524).
+// With heads of 128 they have room for two slots only, and where there are no three CTAs per SM four are faster (2048 into an empty cache 177 us, with two slots 185).
 constexpr int kWeightKeys = 128, kWeightRows = 64, kWeightSlots = 4, kWeightThreads = kWeightKeys + 32;
 struct WeightBars {
-    unsigned long long k_ready, o_done, q_full[kWeightSlots], s_full[kWeightSlots], s_free[kWeightSlots];
+    unsigned long long k_ready, o_done, q_full[kWeightSlots], s_full[2], s_free[2];
     unsigned tmem;
     int failed;
 };
-template <int HD> __host__ __device__ constexpr size_t weights_smem() { return (size_t)kWeightKeys * HD * 2 + (size_t)kWeightSlots * kWeightRows * HD * 2 + 1024; }
+template <int HD, int SLOTS> __host__ __device__ constexpr size_t weights_smem() { return (size_t)kWeightKeys * HD * 2 + (size_t)SLOTS * kWeightRows * HD * 2 + 1024; }
 
-template <int HD, int CODE>
-__global__ void __launch_bounds__(kWeightThreads, 2) kv8_weights_kernel(const swlm_kv8_cache c, const swlm_kv8_attend a, const RowsPlan p, int* status) {
+template <int HD, int CODE, int SLOTS>
+__global__ void __launch_bounds__(kWeightThreads, 3) kv8_weights_kernel(const swlm_kv8_cache c, const swlm_kv8_attend a, const RowsPlan p, int* status) {
     constexpr int HALVES = HD / 64;
     constexpr unsigned K_HALF = kWeightKeys * 128, Q_HALF = kWeightRows * 128, Q_BYTES = HALVES * Q_HALF;
-    constexpr unsigned kTmemCols = kWeightSlots * 64;
+    constexpr unsigned kTmemCols = 128;   // two regions of scores
+    static_assert((SLOTS & (SLOTS - 1)) == 0 && SLOTS >= 2 && SLOTS <= kWeightSlots, "slots");
     extern __shared__ __align__(1024) unsigned char weights_raw[];
     unsigned char* const k_sm = weights_raw + ((1024 - (smem_u32(weights_raw) & 1023)) & 1023);
     unsigned char* const q_sm = k_sm + HALVES * K_HALF;
-    __shared__ __align__(16) float rows_sm[kWeightSlots][2][kWeightRows];   // factors, shifts
+    __shared__ __align__(16) float rows_sm[SLOTS][2][kWeightRows];   // factors, shifts
     __shared__ __align__(8) WeightBars bars;
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -442,7 +445,8 @@ __global__ void __launch_bounds__(kWeightThreads, 2) kv8_weights_kernel(const sw
     if (tid == 0) {
         mbar_init(&bars.k_ready, 4);
         mbar_init(&bars.o_done, 1);
-        for (int i = 0; i < kWeightSlots; ++i) { mbar_init(&bars.q_full[i], 1); mbar_init(&bars.s_full[i], 1); mbar_init(&bars.s_free[i], 4); }
+        for (int i = 0; i < SLOTS; ++i) mbar_init(&bars.q_full[i], 1);
+        for (int i = 0; i < 2; ++i) { mbar_init(&bars.s_full[i], 1); mbar_init(&bars.s_free[i], 4); }
         bars.failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -457,7 +461,7 @@ __global__ void __launch_bounds__(kWeightThreads, 2) kv8_weights_kernel(const sw
     const unsigned tm = bars.tmem;
 
     if (warp == 4) {
-        // Tile t of this CTA (slot t & 3): its copies are asked for behind s_free(t - 4), so its slot, rows and scores' region are free then
+        // Tile t of this CTA: its copies are asked for behind s_free(t - SLOTS), its products behind s_free(t - 2), so its slot, rows and scores' region are free then
         const bool el = elect_one();
         const unsigned kd = umma_desc_lo(smem_u32(k_sm)), qd = umma_desc_lo(smem_u32(q_sm));
         const unsigned char* q = reinterpret_cast<const unsigned char*>(p.q16) + (head * p.row_tiles * (kPromptRows / kWeightRows) + tile0) * Q_BYTES;
@@ -466,7 +470,7 @@ __global__ void __launch_bounds__(kWeightThreads, 2) kv8_weights_kernel(const sw
         int asked = 0;
         auto ask = [&]() {
             if (el) {
-                const int slot = asked & (kWeightSlots - 1);
+                const int slot = asked & (SLOTS - 1);
                 const unsigned bar = smem_u32(&bars.q_full[slot]);
                 mbar_expect(bar, Q_BYTES + 2 * kWeightRows * 4);
                 bulk_load(smem_u32(q_sm) + slot * Q_BYTES, q + (size_t)asked * Q_BYTES, Q_BYTES, bar);
@@ -476,30 +480,28 @@ __global__ void __launch_bounds__(kWeightThreads, 2) kv8_weights_kernel(const sw
             __syncwarp();
             ++asked;
         };
-        while (asked < tiles && asked < kWeightSlots - 1) ask();
+        while (asked < tiles && asked < SLOTS - 1) ask();
         bool ok = mbar_wait_warp(&bars.k_ready, 0u);
         for (int t = 0; t < tiles && ok; ++t) {
-            const int slot = t & (kWeightSlots - 1);
-            if (*failed || !mbar_wait_warp(&bars.q_full[slot], (unsigned)((t / kWeightSlots) & 1))) { ok = false; break; }
+            const int slot = t & (SLOTS - 1);
+            if (*failed || !mbar_wait_warp(&bars.q_full[slot], (unsigned)((t / SLOTS) & 1))) { ok = false; break; }
             pa_after();
             if (el) {
 #pragma unroll
                 for (int kk = 0; kk < HD / 16; ++kk)
-                    pa_mma_ss(tm + slot * 64u, kd + (kk >> 2) * (K_HALF / 16) + 2 * (kk & 3), qd + slot * (Q_BYTES / 16) + (kk >> 2) * (Q_HALF / 16) + 2 * (kk & 3),
+                    pa_mma_ss(tm + (t & 1) * 64u, kd + (kk >> 2) * (K_HALF / 16) + 2 * (kk & 3), qd + slot * (Q_BYTES / 16) + (kk >> 2) * (Q_HALF / 16) + 2 * (kk & 3),
                               pa_idesc(kWeightRows, false, false), kk > 0 ? 1u : 0u);
-                umma_commit(&bars.s_full[slot]);
+                umma_commit(&bars.s_full[t & 1]);
             }
             __syncwarp();
-            if (asked < tiles) {
-                // the slot of tile t + 3, which tile t - 1 had
-                if (t > 0 && !mbar_wait_warp(&bars.s_free[(t - 1) & (kWeightSlots - 1)], (unsigned)(((t - 1) / kWeightSlots) & 1))) { ok = false; break; }
-                ask();
-            }
+            // what tile t - 1 had: the region of tile t + 1, the slot of tile t + SLOTS - 1
+            if (t > 0 && t + 1 < tiles && !mbar_wait_warp(&bars.s_free[(t - 1) & 1], (unsigned)(((t - 1) >> 1) & 1))) { ok = false; break; }
+            if (asked < tiles) ask();
         }
         if (el) umma_commit(&bars.o_done);
         __syncwarp();
         ok = mbar_wait_warp(&bars.o_done, 0u) && ok;   // tensor memory is not freed under MMAs in flight, nor shared memory left under copies
-        for (int t = max(0, asked - kWeightSlots); t < asked; ++t) ok = mbar_wait_warp(&bars.q_full[t & (kWeightSlots - 1)], (unsigned)((t / kWeightSlots) & 1)) && ok;
+        for (int t = max(0, asked - SLOTS); t < asked; ++t) ok = mbar_wait_warp(&bars.q_full[t & (SLOTS - 1)], (unsigned)((t / SLOTS) & 1)) && ok;
         if (!ok && lane == 0) fail(34);
         __syncwarp();
     } else {
@@ -527,13 +529,12 @@ __global__ void __launch_bounds__(kWeightThreads, 2) kv8_weights_kernel(const sw
         float2 sum = make_float2(0.f, 0.f);
         bool ok = true;
         for (int t = 0; t < tiles; ++t) {
-            const int slot = t & (kWeightSlots - 1);
-            const unsigned phase = (unsigned)((t / kWeightSlots) & 1);
-            if (!mbar_wait_warp(&bars.q_full[slot], phase) || !mbar_wait_warp(&bars.s_full[slot], phase)) { ok = false; break; }
+            const int slot = t & (SLOTS - 1);
+            if (!mbar_wait_warp(&bars.q_full[slot], (unsigned)((t / SLOTS) & 1)) || !mbar_wait_warp(&bars.s_full[t & 1], (unsigned)((t >> 1) & 1))) { ok = false; break; }
             pa_after();
             unsigned v[64];
-            pa_ld32(tm + lanes + slot * 64u, v);
-            pa_ld32(tm + lanes + slot * 64u + 32u, v + 32);
+            pa_ld32(tm + lanes + (t & 1) * 64u, v);
+            pa_ld32(tm + lanes + (t & 1) * 64u + 32u, v + 32);
             pa_wait_ld();
             const bool masked = !__all_sync(0xffffffffu, first <= (long long)t * kWeightRows);
 #pragma unroll
@@ -554,7 +555,7 @@ __global__ void __launch_bounds__(kWeightThreads, 2) kv8_weights_kernel(const sw
             }
             pa_before();
             __syncwarp();
-            if (lane == 0) pa_arrive(&bars.s_free[slot]);
+            if (lane == 0) pa_arrive(&bars.s_free[t & 1]);
         }
         if (!ok) fail(35);
         else if (key < end) c.weight[head * c.capacity + key] += sum.x + sum.y;
@@ -574,14 +575,19 @@ int launch_prompt(const swlm_kv8_cache& c, const swlm_kv8_attend& a, const RowsP
 }
 template <int HD, int CODE>
 int launch_weights(const swlm_kv8_cache& c, const swlm_kv8_attend& a, const RowsPlan& p, int* status, cudaStream_t s) {
-    const int span = std::min(a.max_len, c.capacity);
-    const cudaError_t e = launch_k(kv8_weights_kernel<HD, CODE>, dim3((unsigned)((span + kWeightKeys - 1) / kWeightKeys), (unsigned)c.kv_heads, (unsigned)c.batch), dim3(kWeightThreads),
-                                   weights_smem<HD>(), s, c, a, p, status);
+    const int span = std::min(a.max_len, c.capacity), tiles = (span + kWeightKeys - 1) / kWeightKeys;
+    const dim3 grid((unsigned)tiles, (unsigned)c.kv_heads, (unsigned)c.batch);
+    auto launch = [&](auto kernel, size_t smem) { return launch_k(kernel, grid, dim3(kWeightThreads), smem, s, c, a, p, status); };
+    cudaError_t e;
+    if constexpr (HD == 64) e = launch(kv8_weights_kernel<HD, CODE, 4>, weights_smem<HD, 4>());
+    else if ((long long)tiles * c.kv_heads * c.batch > 2 * kSms) e = launch(kv8_weights_kernel<HD, CODE, 2>, weights_smem<HD, 2>());
+    else e = launch(kv8_weights_kernel<HD, CODE, 4>, weights_smem<HD, 4>());
     return e == cudaSuccess ? SWLM_OK : cuda_fail(e, "kv8 prompt weights launch");
 }
 template <int HD, int CODE>
 int init_prompt() {
-    SWLM_CUDA(cudaFuncSetAttribute(kv8_weights_kernel<HD, CODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)weights_smem<HD>()));
+    SWLM_CUDA((cudaFuncSetAttribute(kv8_weights_kernel<HD, CODE, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)weights_smem<HD, 4>())));
+    if constexpr (HD == 128) SWLM_CUDA((cudaFuncSetAttribute(kv8_weights_kernel<HD, CODE, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)weights_smem<HD, 2>())));
     SWLM_CUDA(cudaFuncSetAttribute(kv8_prompt_kernel<HD, CODE, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prompt_smem<HD>()));
     SWLM_CUDA(cudaFuncSetAttribute(kv8_prompt_kernel<HD, CODE, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prompt_smem<HD>()));
     SWLM_CUDA(cudaFuncSetAttribute(kv8_prompt_kernel<HD, CODE, 8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prompt_smem<HD>()));

@@ -283,6 +283,15 @@ def test_attend_whoever_joins(pkg, store, batch, heads, kv_heads, dim, lengths, 
     check_attend(pkg, store, cache, batch, heads, dim, lengths, counts, torch.bfloat16, accumulate, max_len=max_len)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("code", [0, 1])
+def test_weights_of_portions_by_many_ctas(pkg, store, dim, code):
+    """Portions of a batch whose key tiles are more than the CTAs that run at once: one that fills the cache, from an empty cache, without tokens, of a few rows."""
+    lengths, counts = [1700, 0, 900, 1300, -3], [340, 333, 0, 17, 70]
+    cache = Cache(pkg, 5, 4, dim, 2048, 64, code).fill([max(0, a + c) for a, c in zip(lengths, counts)])
+    check_attend(pkg, store, cache, 5, 16, dim, lengths, counts, torch.float16, True)
+
+
 @pytest.mark.parametrize("counts", [[1, 1], [40, 40]], ids=str)
 def test_attend_cuts_at_max_len(pkg, store, counts):
     """Slots behind max_len are not attended, whatever the lengths say (a length far beyond the capacity among them)."""
