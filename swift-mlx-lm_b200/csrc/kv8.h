@@ -19,6 +19,7 @@ size_t kv8_evict_scratch(const swlm_kv8_cache& c, const swlm_kv8_evict& a);
 int launch_kv8_lengths(int batch, const int32_t* in, const int32_t* counts, int n, int limit, const int32_t* refused, int32_t* out, cudaStream_t s);
 // status: a word that the device sets when a bounded wait expires
 int launch_kv8_attend(const swlm_kv8_cache& c, const swlm_kv8_attend& a, int* status, cudaStream_t s);
+bool kv8_attend_grid_fits(const swlm_kv8_cache& c, const swlm_kv8_attend& a);
 size_t kv8_attend_scratch(const swlm_kv8_cache& c, const swlm_kv8_attend& a);
 
 #ifdef __CUDACC__

@@ -20,6 +20,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <climits>
 
 #include "kv8_device.cuh"
 
@@ -681,7 +682,7 @@ RowsPlan rows_plan(const swlm_kv8_cache& c, const swlm_kv8_attend& a, size_t* by
     p.tiles = p.rows <= 8 ? 1 : p.rows <= kSaveRows ? 2 : kPromptRows / 8;
     p.row_tiles = (p.rows + 8 * p.tiles - 1) / (8 * p.tiles);
     p.span = (span + kStep - 1) / kStep * kStep;
-    const long long groups = (long long)c.batch * c.kv_heads * p.row_tiles, units = groups * ((span + kUnit - 1) / kUnit);
+    const long long groups = (long long)c.batch * c.kv_heads * p.row_tiles, units = p.rows > kSaveRows ? 0 : groups * ((span + kUnit - 1) / kUnit);
     bool several;   // parts that have to be joined
     if (p.rows > kSaveRows) {
         // Runs of slots per block of rows: as many as cost least, in key tiles: rounds of one CTA per SM, each its tiles and a start and end of about two;
@@ -792,6 +793,13 @@ int kv8_attend_init() {
     if (!rc) rc = init_rows<64, SWLM_KV8_E4M3>();
     if (!rc) rc = kv8_prompt_init();
     return rc;
+}
+
+// The grid of many rows is one number: CTAs of all (sequence, KV head, block of rows, run).
+bool kv8_attend_grid_fits(const swlm_kv8_cache& c, const swlm_kv8_attend& a) {
+    size_t bytes;
+    const RowsPlan p = rows_plan(c, a, &bytes);
+    return !p.splits || (long long)c.batch * c.kv_heads * p.row_tiles * p.splits <= INT_MAX;
 }
 
 size_t kv8_attend_scratch(const swlm_kv8_cache& c, const swlm_kv8_attend& a) {

@@ -121,3 +121,19 @@ def test_scratch_sizes(pkg, lib):
         assert plain == 0 or length > 128
         # weights: the scores of every slot, or the queries as fp16
         assert kept >= (2 * 2 * rows * length * 4 if rows <= 64 else 2 * 2 * rows * (64 * 2 + 8))
+
+
+@pytest.mark.parametrize("batch,n,max_len", [(8192, 65537 * 256, 128), (65535, 1 << 22, 128), (8192, 1 << 29, 1 << 20)], ids=str)
+def test_steps_of_more_ctas_than_a_grid_has(pkg, lib, batch, n, max_len):
+    """An upper bound n whose blocks of rows, of all sequences and heads, are 2^31 or more. (Without scratch, so that nothing could be launched.)"""
+    cache = _cache(pkg, batch=batch, kv_heads=8, capacity=1 << 20)
+    step = _attend(pkg, heads=8, n=n, rows=batch, max_len=max_len, q_stride=512, out_stride=512, accumulate=1, scratch=0, scratch_bytes=0)
+    assert lib.swlm_op_kv8_attend_scratch_bytes(cache, step) == 0
+    assert lib.swlm_op_kv8_attend_dev(CTX, cache, step, None) == INVALID
+    assert b"rows" in lib.swlm_last_error()
+
+
+def test_steps_of_nearly_as_many_ctas_as_a_grid_has(pkg, lib):
+    cache = _cache(pkg, batch=8192, kv_heads=8, capacity=1 << 20)
+    step = _attend(pkg, heads=8, n=32767 * 256, rows=8192, max_len=128, q_stride=512, out_stride=512, accumulate=1)
+    assert lib.swlm_op_kv8_attend_scratch_bytes(cache, step) > 0
