@@ -352,7 +352,9 @@ int swlm_op_kv8_append_dev(swlm_ctx* ctx, const swlm_kv8_cache* cache, const swl
 /* Queries of the same step, after its append: query i of sequence b attends the slots below lengths[b] + i + 1, cut to max_len and the
  * capacity; one that attends nothing (lengths[b] < 0 parks a sequence) gets zeros. Row r of query head h lies at q + r * q_stride +
  * h * head_dim; query heads h * heads / kv_heads ... share KV head h. Rows of `out` that no sequence has stay as they are, as do the rows of
- * a sequence whose rows are not within 0..rows-1 or whose counts[b] > n or < 0 (nothing of such a sequence is worked on).
+ * a sequence whose rows are not within 0..rows-1, whose counts[b] > n or < 0, or with refused[b] != 0 (nothing of such a sequence is worked on).
+ * refused: what the step's append wrote there. The tokens of a sequence that it refused (a parked one's too) are not in the cache, so its queries
+ * would attend slots without tokens, and accumulate would add their weights (NULL: no sequence was refused).
  * accumulate: weight[b][h][slot] += the softmax weights that the step's queries of all heads of the group have for the slot.
  * Scores, softmax and sums are fp32; probabilities meet the values as fp16. An infinity or NaN in a query makes that query's results (and,
  * accumulated, the weights that it adds) NaN.
@@ -374,6 +376,7 @@ typedef struct swlm_kv8_attend {
     int32_t rows;          /* rows of q and out */
     int32_t max_len;       /* no sequence has more tokens than this, its new ones included; what lies behind is not attended */
     int32_t accumulate;
+    const int32_t* refused;   /* [batch], or NULL */
 } swlm_kv8_attend;
 size_t swlm_op_kv8_attend_scratch_bytes(const swlm_kv8_cache* cache, const swlm_kv8_attend* step);   /* the pointers are not looked at; 0 for what the call refuses */
 int swlm_op_kv8_attend_dev(swlm_ctx* ctx, const swlm_kv8_cache* cache, const swlm_kv8_attend* step, void* cuda_stream);

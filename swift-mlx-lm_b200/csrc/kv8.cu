@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const swlm_k
     __shared__ unsigned warps[kAppendThreads / 32];
     pdl_wait();
     const int b = blockIdx.z, h = blockIdx.y >> 1, which = blockIdx.y & 1, tid = threadIdx.x, T = c.block;
-    const Kv8Part part = kv8_part(b, a.lengths, a.counts, a.starts, a.n, a.rows);
+    const Kv8Part part = kv8_part(b, a.lengths, a.counts, a.starts, nullptr, a.n, a.rows);
     const bool ok = part.fits && part.len >= 0 && (long long)part.len + part.count <= c.capacity;
     if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0 && a.refused) a.refused[b] = ok ? 0 : 1;
     if (!ok) return;
@@ -636,6 +636,7 @@ int swlm_op_kv8_attend_dev(swlm_ctx* ctx, const swlm_kv8_cache* cache, const swl
     if (!rows_ok(a.q, a.q_stride, width) || !rows_ok(a.out, a.out_stride, width)) return refuse("q and out must be 16-byte aligned, their strides multiples of 8 and at least heads * head_dim");
     if (!(a.scale > 0.f) || a.scale > 1e30f) return refuse("the scale must be positive and finite");
     if (a.accumulate && !c.weight) return refuse("accumulate needs the cache's weight array");
+    if (!aligned(a.refused, 4)) return refuse("counters must be 4-byte aligned");
     const size_t need = kv8_attend_scratch(c, a);
     if (need && (!a.scratch || !aligned(a.scratch, 16) || a.scratch_bytes < need)) { set_error("kv8: %zu bytes of 16-byte aligned scratch are needed", need); return SWLM_ERR_INVALID; }
     SWLM_CUDA(cudaSetDevice(ctx->device));

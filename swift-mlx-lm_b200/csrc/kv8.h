@@ -25,17 +25,18 @@ size_t kv8_attend_scratch(const swlm_kv8_cache& c, const swlm_kv8_attend& a);
 #ifdef __CUDACC__
 constexpr float kKv8NaN = __builtin_nanf("");
 
-// A sequence's part in a step: where it stands and the rows of its tokens; count 0 where it has none, or where what it says does not fit.
+// A sequence's part in a step: where it stands and the rows of its tokens; count 0 where it has none, where what it says does not fit, or where
+// `refused` (may be null) says that its tokens were not appended.
 struct Kv8Part {
     int len, count, start;
     bool fits;
 };
-__device__ __forceinline__ Kv8Part kv8_part(int b, const int32_t* lengths, const int32_t* counts, const int32_t* starts, int n, int rows) {
+__device__ __forceinline__ Kv8Part kv8_part(int b, const int32_t* lengths, const int32_t* counts, const int32_t* starts, const int32_t* refused, int n, int rows) {
     Kv8Part p;
     p.len = lengths[b];
     p.count = counts ? counts[b] : n;
     const long long start = starts ? (long long)starts[b] : (long long)b * n;
-    p.fits = p.count >= 0 && p.count <= n && (p.count == 0 || (start >= 0 && start + p.count <= rows));
+    p.fits = p.count >= 0 && p.count <= n && (p.count == 0 || (start >= 0 && start + p.count <= rows)) && !(refused && refused[b]);
     if (!p.fits) p.count = 0;
     p.start = p.count ? (int)start : 0;
     return p;

@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_r
             int mine = 0;
             Kv8Part q{};
             if (b0 + tid < c.batch) {
-                q = kv8_part(b0 + tid, a.lengths, a.counts, a.starts, a.n, a.rows);
+                q = kv8_part(b0 + tid, a.lengths, a.counts, a.starts, a.refused, a.n, a.rows);
                 if (q.count) mine = sequence_units(q, span) * sequence_tiles(q, G, TR) * c.kv_heads;
             }
             int sum = mine;
@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_r
             unit1 = min(per, unit0 + u_end - u);
             u += unit1 - unit0;
         } else {
-            part = kv8_part(b, a.lengths, a.counts, a.starts, a.n, a.rows);
+            part = kv8_part(b, a.lengths, a.counts, a.starts, a.refused, a.n, a.rows);
             // a cluster of CTAs, or one, has all slots of a tile: equal shares of its units
             const int units = sequence_units(part, span), rank = (int)blockIdx.x % p.cluster;
             h = blockIdx.y; tile = (int)blockIdx.x / p.cluster;
@@ -585,7 +585,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const swlm_kv8_c
     __shared__ float4 group_o[kJoinThreads];
     pdl_wait();
     const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x, G = a.heads / c.kv_heads, TR = 8 * p.tiles;
-    const Kv8Part part = kv8_part(b, a.lengths, a.counts, a.starts, a.n, a.rows);
+    const Kv8Part part = kv8_part(b, a.lengths, a.counts, a.starts, a.refused, a.n, a.rows);
     const int rows = part.count * G, span = min(a.max_len, c.capacity);
     if (rows == 0) return;
     const size_t head = (size_t)b * c.kv_heads + h;

@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
     // by head 94); sequence by sequence, as only the device knows which one is long
     const int turn = (int)blockIdx.x / c.kv_heads, h = (int)blockIdx.x - turn * c.kv_heads, split = turn % p.splits;
     const int b = turn / p.splits / p.row_tiles, block = p.row_tiles - 1 - (turn / p.splits - b * p.row_tiles);
-    const Kv8Part part = kv8_part(b, a.lengths, a.counts, a.starts, a.n, a.rows);
+    const Kv8Part part = kv8_part(b, a.lengths, a.counts, a.starts, a.refused, a.n, a.rows);
     const int rows = part.count * G, block0 = block * kPromptRows;
     if (block0 >= rows) return;
     const int end = visible(part, min(block0 + kPromptRows - 1, rows - 1) / G, span);   // of the CTA's last query: it sees most
@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(kWeightThreads, 3) kv8_weights_kernel(const sw
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int b = blockIdx.z, h = blockIdx.y, G = a.heads / c.kv_heads, span = min(a.max_len, c.capacity);
-    const Kv8Part part = kv8_part(b, a.lengths, a.counts, a.starts, a.n, a.rows);
+    const Kv8Part part = kv8_part(b, a.lengths, a.counts, a.starts, a.refused, a.n, a.rows);
     const int rows = part.count * G, end = rows ? visible(part, part.count - 1, span) : 0, key0 = (int)blockIdx.x * kWeightKeys;
     if (key0 >= end) return;
     const size_t head = (size_t)b * c.kv_heads + h;

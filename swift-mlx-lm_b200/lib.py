@@ -143,7 +143,7 @@ class Kv8Attend(C.Structure):
 
     _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_int64), ("out_stride", C.c_int64)] + [
         (f, C.c_void_p) for f in ("lengths", "counts", "starts", "scratch")] + [("scratch_bytes", C.c_uint64), ("scale", C.c_float)] + [
-        (f, C.c_int32) for f in ("dtype", "heads", "n", "rows", "max_len", "accumulate")]
+        (f, C.c_int32) for f in ("dtype", "heads", "n", "rows", "max_len", "accumulate")] + [("refused", C.c_void_p)]
 
 
 class Kv8Evict(C.Structure):

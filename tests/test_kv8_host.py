@@ -137,3 +137,8 @@ def test_steps_of_nearly_as_many_ctas_as_a_grid_has(pkg, lib):
     cache = _cache(pkg, batch=8192, kv_heads=8, capacity=1 << 20)
     step = _attend(pkg, heads=8, n=32767 * 256, rows=8192, max_len=128, q_stride=512, out_stride=512, accumulate=1)
     assert lib.swlm_op_kv8_attend_scratch_bytes(cache, step) > 0
+
+
+def test_refused_must_be_aligned(pkg, lib):
+    assert lib.swlm_op_kv8_attend_dev(CTX, _cache(pkg), _attend(pkg, refused=66), None) == INVALID
+    assert b"4-byte" in lib.swlm_last_error()
