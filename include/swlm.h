@@ -358,8 +358,9 @@ int swlm_op_kv8_append_dev(swlm_ctx* ctx, const swlm_kv8_cache* cache, const swl
  * accumulate: weight[b][h][slot] += the softmax weights that the step's queries of all heads of the group have for the slot.
  * Scores, softmax and sums are fp32; probabilities meet the values as fp16. An infinity or NaN in a query makes that query's results (and,
  * accumulated, the weights that it adds) NaN.
- * scratch: swlm_op_kv8_attend_scratch_bytes() (0: none needed), 16-byte aligned, not shared by calls that may overlap. A bounded wait that
- * expires on the device makes the context's next swlm_op_kv8_attend_dev return SWLM_ERR_TIMEOUT without doing anything; results since then are not valid. */
+ * scratch: swlm_op_kv8_attend_scratch_bytes() (0: none needed), 16-byte aligned, not shared by calls that may overlap.
+ * Waits on the device are bounded. Once one has expired, results and weights since then are not valid, and the context's swlm_op_kv8_attend_dev and
+ * swlm_op_kv8_evict_dev, on every stream, return SWLM_ERR_TIMEOUT without doing anything until swlm_op_kv8_status has reported it. */
 typedef struct swlm_kv8_attend {
     const void* q;
     void* out;
@@ -380,6 +381,11 @@ typedef struct swlm_kv8_attend {
 } swlm_kv8_attend;
 size_t swlm_op_kv8_attend_scratch_bytes(const swlm_kv8_cache* cache, const swlm_kv8_attend* step);   /* the pointers are not looked at; 0 for what the call refuses */
 int swlm_op_kv8_attend_dev(swlm_ctx* ctx, const swlm_kv8_cache* cache, const swlm_kv8_attend* step, void* cuda_stream);
+/* SWLM_ERR_TIMEOUT where a wait of the context's attention calls has expired since the last call, which it forgets then. It does not wait: call it
+ * behind a synchronisation of the streams in question. The replays of a captured step report nothing themselves, so whoever replays one asks here. */
+int swlm_op_kv8_status(swlm_ctx* ctx);
+/* Probe: what an expired wait would leave behind (0: none), for tests of a host's handling of it. */
+int swlm_write_kv8_status(swlm_ctx* ctx, int code);
 
 /* Of every (sequence, KV head) with more than `keep` tokens: the tokens of positions below `sink` and the last `recent` ones (positions from
  * seen[b] - recent on; seen[b] counts all tokens so far here) are protected, then those of the largest weights stay (a NaN counts as the

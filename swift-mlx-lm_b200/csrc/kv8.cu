@@ -601,6 +601,13 @@ int evict_shape_ok(const swlm_kv8_cache& c, const swlm_kv8_evict& a) {
     return SWLM_OK;
 }
 
+// (`code`: what the kernels left in the context's word)
+int expired(int code) {
+    if (!code) return SWLM_OK;
+    set_error("kv8: a bounded device-side wait of an earlier attention call expired (code %d): results since then are not valid", code);
+    return SWLM_ERR_TIMEOUT;
+}
+
 cudaStream_t stream_of(swlm_ctx* ctx, void* s) { return s ? static_cast<cudaStream_t>(s) : ctx->stream; }
 
 }  // namespace
@@ -640,12 +647,19 @@ int swlm_op_kv8_attend_dev(swlm_ctx* ctx, const swlm_kv8_cache* cache, const swl
     const size_t need = kv8_attend_scratch(c, a);
     if (need && (!a.scratch || !aligned(a.scratch, 16) || a.scratch_bytes < need)) { set_error("kv8: %zu bytes of 16-byte aligned scratch are needed", need); return SWLM_ERR_INVALID; }
     SWLM_CUDA(cudaSetDevice(ctx->device));
-    if (*static_cast<volatile int*>(ctx->kv8_status)) {
-        set_error("kv8: a bounded device-side wait of an earlier call expired (code %d): its results are not valid", *ctx->kv8_status);
-        *ctx->kv8_status = 0;
-        return SWLM_ERR_TIMEOUT;
-    }
+    if ((rc = expired(__atomic_load_n(ctx->kv8_status, __ATOMIC_RELAXED)))) return rc;
     return launch_kv8_attend(c, a, ctx->kv8_status, stream_of(ctx, cuda_stream));
+}
+
+int swlm_op_kv8_status(swlm_ctx* ctx) {
+    if (!ctx) return refuse("null argument");
+    return expired(__atomic_exchange_n(ctx->kv8_status, 0, __ATOMIC_RELAXED));
+}
+
+int swlm_write_kv8_status(swlm_ctx* ctx, int code) {
+    if (!ctx) return refuse("null argument");
+    __atomic_store_n(ctx->kv8_status, code, __ATOMIC_RELAXED);
+    return SWLM_OK;
 }
 
 size_t swlm_op_kv8_evict_scratch_bytes(const swlm_kv8_cache* cache, const swlm_kv8_evict* how) {
@@ -675,6 +689,7 @@ int swlm_op_kv8_evict_dev(swlm_ctx* ctx, const swlm_kv8_cache* cache, const swlm
     const size_t need = kv8_evict_scratch(c, a);
     if (!a.scratch || !aligned(a.scratch, 16) || a.scratch_bytes < need) { set_error("kv8: %zu bytes of 16-byte aligned scratch are needed", need); return SWLM_ERR_INVALID; }
     SWLM_CUDA(cudaSetDevice(ctx->device));
+    if ((rc = expired(__atomic_load_n(ctx->kv8_status, __ATOMIC_RELAXED)))) return rc;   // the weights that it would go by may not be valid
     return launch_kv8_evict(c, d, a, stream_of(ctx, cuda_stream));
 }
 

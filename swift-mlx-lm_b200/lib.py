@@ -234,6 +234,8 @@ SIGNATURES = {
     "swlm_op_kv8_append_dev": (_I, [_P, C.POINTER(Kv8Cache), C.POINTER(Kv8Append), _P]),
     "swlm_op_kv8_attend_scratch_bytes": (C.c_size_t, [C.POINTER(Kv8Cache), C.POINTER(Kv8Attend)]),
     "swlm_op_kv8_attend_dev": (_I, [_P, C.POINTER(Kv8Cache), C.POINTER(Kv8Attend), _P]),
+    "swlm_op_kv8_status": (_I, [_P]),
+    "swlm_write_kv8_status": (_I, [_P, _I]),
     "swlm_op_kv8_evict_scratch_bytes": (C.c_size_t, [C.POINTER(Kv8Cache), C.POINTER(Kv8Evict)]),
     "swlm_op_kv8_evict_dev": (_I, [_P, C.POINTER(Kv8Cache), C.POINTER(Kv8Cache), C.POINTER(Kv8Evict), _P]),
     "swlm_op_kv8_lengths_dev": (_I, [_P, _I, _P, _P, _I, _I, _P, _P, _P]),

@@ -142,3 +142,8 @@ def test_steps_of_nearly_as_many_ctas_as_a_grid_has(pkg, lib):
 def test_refused_must_be_aligned(pkg, lib):
     assert lib.swlm_op_kv8_attend_dev(CTX, _cache(pkg), _attend(pkg, refused=66), None) == INVALID
     assert b"4-byte" in lib.swlm_last_error()
+
+
+def test_status_of_no_context(pkg, lib):
+    assert lib.swlm_op_kv8_status(None) == INVALID
+    assert lib.swlm_write_kv8_status(None, 1) == INVALID
