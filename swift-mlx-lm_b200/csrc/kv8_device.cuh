@@ -31,7 +31,7 @@ struct RowsPlan {
     float* part_ml; // [places][8 * tiles][2]: reference maximum (log2), sum
     float* scores;  // [batch][kv_heads][span][pitch], log2
     // many rows whose weights are added: the shifted queries as fp16 in tiles of 64 rows, [batch][kv_heads][tiles][head_dim / 64][64][64], swizzled as the
-    // products read them, and per row what turns a product into log2 of a weight: times the factor, times the key's scale, plus the shift
+    // products read them, and per row what turns a product into log2 of a weight: times (factor times the key's scale), plus the shift
     __half* q16;
     float* q_factor;  // [batch][kv_heads][row_tiles * 256]
     float* q_shift;

@@ -540,8 +540,9 @@ __global__ void __launch_bounds__(kWeightThreads, 3) kv8_weights_kernel(const sw
 #pragma unroll
             for (int e = 0; e < kWeightRows; e += 4) {
                 const float4 f = *reinterpret_cast<const float4*>(&rows_sm[slot][0][e]), m = *reinterpret_cast<const float4*>(&rows_sm[slot][1][e]);
-                float2 x = fma2(mul2(make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), scale2), make_float2(f.x, f.y), make_float2(m.x, m.y));
-                float2 y = fma2(mul2(make_float2(__uint_as_float(v[e + 2]), __uint_as_float(v[e + 3])), scale2), make_float2(f.z, f.w), make_float2(m.z, m.w));
+                // (the row's factor meets the key's scale first, as in the attention: either alone may take the product out of range)
+                float2 x = fma2(make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), mul2(make_float2(f.x, f.y), scale2), make_float2(m.x, m.y));
+                float2 y = fma2(make_float2(__uint_as_float(v[e + 2]), __uint_as_float(v[e + 3])), mul2(make_float2(f.z, f.w), scale2), make_float2(m.z, m.w));
                 x = make_float2(pa_exp2(x.x), pa_exp2(x.y));
                 y = make_float2(pa_exp2(y.x), pa_exp2(y.y));
                 if (masked) {
