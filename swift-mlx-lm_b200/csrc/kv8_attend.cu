@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_r
         }
         all_see = min(all_see, __shfl_xor_sync(0xffffffffu, all_see, 1));
         all_see = min(all_see, __shfl_xor_sync(0xffffffffu, all_see, 2));
-        float acc[NT][MT][4], m_ref[NT][2], top_ok[NT][2], l_run[NT][2], v_ref = 0x1p-100f, v_inv = 0x1p100f * kValueUnit;
+        float acc[NT][MT][4], m_ref[NT][2], top_ok[NT][2], l_run[NT][2], v_ref = kValueRef, v_inv = kValueUnit / kValueRef;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll

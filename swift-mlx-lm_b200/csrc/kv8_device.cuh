@@ -10,6 +10,7 @@ constexpr int kSms = 148;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.f;                   // log2 of what a probability may exceed 1 by
 constexpr float kValueUnit = 128.f;             // 2^7: probabilities up to 2^8 stay within fp16
+constexpr float kValueRef = 0x1p-120f;          // values' scales are taken relative to the largest so far, or to this, whose inverse times 2^7 is still finite
 
 // The kernel of few rows:
 constexpr int kWarps = 4, kThreads = kWarps * 32;

@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
         const unsigned lanes = (unsigned)((warp & 3) * 32) << 16, out_col = tm + lanes + O_COL + t * 128u;
         const float* ks = c.k_scale + head * (c.capacity >> block_shift);
         const float* vs = c.v_scale + head * (c.capacity >> block_shift);
-        float m_ref = -INFINITY, l_run = 0.f, v_ref = 0x1p-100f, v_inv = 0x1p100f * kValueUnit;
+        float m_ref = -INFINITY, l_run = 0.f, v_ref = kValueRef, v_inv = kValueUnit / kValueRef;
         constexpr int KEYS = kPromptKeys / GROUPS;            // keys of a scale
         constexpr int PARTS = KEYS < 64 ? 64 / KEYS : 1, N = 64 / PARTS;   // scales of half a tile, keys of it that share one
         float kn[GROUPS], vn[GROUPS];   // the next tile's scales; 0 behind the last token
