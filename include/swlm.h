@@ -356,8 +356,9 @@ int swlm_op_kv8_append_dev(swlm_ctx* ctx, const swlm_kv8_cache* cache, const swl
  * refused: what the step's append wrote there. The tokens of a sequence that it refused (a parked one's too) are not in the cache, so its queries
  * would attend slots without tokens, and accumulate would add their weights (NULL: no sequence was refused).
  * accumulate: weight[b][h][slot] += the softmax weights that the step's queries of all heads of the group have for the slot.
- * Scores, softmax and sums are fp32; probabilities meet the values as fp16. An infinity or NaN in a query makes that query's results (and,
- * accumulated, the weights that it adds) NaN.
+ * Scores, softmax and sums are fp32. Probabilities meet the values as fp16 numbers: off by 2^-11 of themselves, or, where a block's value scale is
+ * less than 2^-21 / probability of the largest that the query attends, by 2^-32 of that scale. For results in fp16 they are the sum of two such
+ * numbers (2^-22). An infinity or NaN in a query makes that query's results (and, accumulated, the weights that it adds) NaN.
  * scratch: swlm_op_kv8_attend_scratch_bytes() (0: none needed), 16-byte aligned, not shared by calls that may overlap.
  * Waits on the device are bounded. Once one has expired, results and weights since then are not valid, and the context's swlm_op_kv8_attend_dev and
  * swlm_op_kv8_evict_dev, on every stream, return SWLM_ERR_TIMEOUT without doing anything until swlm_op_kv8_status has reported it. */

@@ -10,8 +10,10 @@
 // KV head) after the other, the same number of slots for every CTA whatever the lengths are; its four warps take steps of 32 tokens in turn,
 // each over a ring of its own that cp.async fills. Scores come as S^T = K Q^T (16 tokens x 8 rows, so that a decode step's four or eight
 // rows fill the tile), probabilities are transposed in registers (movmatrix) and meet the values as O^T = V^T P^T. The reference
-// maximum of a row moves only when it would grow by more than 2^8. Probabilities are rounded to fp16 (2^-11 of themselves) times 2^7 vs / vr, vr
-// the largest value scale so far: values of blocks down to 2^-24 of the largest scale keep that precision. Partial results of a tile
+// maximum of a row moves only when it would grow by more than 2^8. Probabilities are rounded to fp16 as p 2^7 vs / vr, vr the largest value
+// scale so far: off by 2^-11 of themselves where p vs / vr >= 2^-21, below that by 2^-32 of vr. bf16 results do not show it. For fp16 results, which
+// have as many bits, what the rounding has left follows as a second product (2^-22 of themselves where p vs / vr >= 2^-10): 41 ragged sequences of 4091
+// tokens 29.3 us, with one product 28.5; error against 64 bits 2.1e-4 (of which rounding the result is 2.1e-4) and 2.7e-4. Partial results of a tile
 // are joined by a second launch, which also adds the weights, or by the cluster of CTAs that has all of a tile's slots.
 //
 // What bounds it: memory, and some ten us of start, merge and the second launch. 8 x 8192 tokens, 32 / 8 heads of 128, int8: 33.5 us for 134 MB (0.61
@@ -157,7 +159,7 @@ __device__ __forceinline__ float4 join_cluster(const cg::cluster_group& cluster,
     return o;
 }
 
-template <int HD, int CODE, int NT, bool SAVE>
+template <int HD, int CODE, int NT, bool SAVE, bool F16>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_rows_kernel(const swlm_kv8_cache c, const swlm_kv8_attend a, const RowsPlan p) {
     constexpr int KS = HD / 16, MT = HD / 16, NS = stages<HD>(), SB = stage_bytes<HD>(), TR = 8 * NT;
     extern __shared__ __align__(16) unsigned char sm[];
@@ -169,7 +171,6 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_r
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int G = a.heads / c.kv_heads, span = min(a.max_len, c.capacity);
-    const bool f16 = a.dtype == SWLM_KV8_FP16;
     const int block_shift = 31 - __clz(c.block);
 
     // ---- this CTA's units ----
@@ -288,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_r
         for (int nt = 0; nt < NT; ++nt) {
             const int r = row0 + nt * 8 + g, i = min(r, rows - 1) / G;
             float down;
-            load_query<HD>(static_cast<const unsigned short*>(a.q) + (int64_t)(part.start + i) * a.q_stride + (size_t)(h * G + min(r, rows - 1) - i * G) * HD, r < rows, f16, t,
+            load_query<HD>(static_cast<const unsigned short*>(a.q) + (int64_t)(part.start + i) * a.q_stride + (size_t)(h * G + min(r, rows - 1) - i * G) * HD, r < rows, F16, t,
                            qf[nt], down);
             down *= a.scale * kLog2e;
 #pragma unroll
@@ -412,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_r
 #pragma unroll
                         for (int e = 0; e < 4; ++e) acc[nt][j][e] *= corr;
             }
-            unsigned pf[kSub][NT][2];
+            unsigned pf[kSub][NT][2], pr[kSub][NT][2];   // (pr: what rounding has left of them, for results in fp16)
 #pragma unroll
             for (int sub = 0; sub < kSub; ++sub) {
                 const float unit = v_scale[sub] * v_inv;
@@ -426,8 +427,13 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_r
                         w[e] = pr * unit;
                         if (masked && s[sub][nt][e] == -INFINITY) w[e] = 0.f;   // (a slot that the row does not attend may lie in a block that is NaN)
                     }
-                    pf[sub][nt][0] = transpose8x8(pack_half(w[0], w[1]));
-                    pf[sub][nt][1] = transpose8x8(pack_half(w[2], w[3]));
+                    const unsigned p0 = pack_half(w[0], w[1]), p1 = pack_half(w[2], w[3]);
+                    pf[sub][nt][0] = transpose8x8(p0);
+                    pf[sub][nt][1] = transpose8x8(p1);
+                    if (F16) {
+                        pr[sub][nt][0] = transpose8x8(pack_rest(w[0], w[1], p0));
+                        pr[sub][nt][1] = transpose8x8(pack_rest(w[2], w[3], p1));
+                    }
                 }
             }
             // ---- values ----
@@ -449,7 +455,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_r
                         const unsigned lo = __byte_perm(v0, v1, half ? 0x7362 : 0x5140), hi = __byte_perm(v2, v3, half ? 0x7362 : 0x5140);
                         const unsigned a0 = pair_of<CODE, 0>(lo), a1 = pair_of<CODE, 1>(lo), a2 = pair_of<CODE, 0>(hi), a3 = pair_of<CODE, 1>(hi);
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) mma(acc[nt][2 * w + half], a0, a1, a2, a3, pf[sub][nt][0], pf[sub][nt][1]);
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma(acc[nt][2 * w + half], a0, a1, a2, a3, pf[sub][nt][0], pf[sub][nt][1]);
+                            if (F16) mma(acc[nt][2 * w + half], a0, a1, a2, a3, pr[sub][nt][0], pr[sub][nt][1]);
+                        }
                     }
                 }
             }
@@ -509,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_r
                 *reinterpret_cast<float4*>(p.part_o + (slot * TR + r) * HD + d) = o;
             } else {
                 const int i = row / G;
-                store_out(static_cast<unsigned short*>(a.out) + (int64_t)(part.start + i) * a.out_stride + (size_t)(h * G + row - i * G) * HD + d, o, l, f16);
+                store_out(static_cast<unsigned short*>(a.out) + (int64_t)(part.start + i) * a.out_stride + (size_t)(h * G + row - i * G) * HD + d, o, l, F16);
             }
         }
         if (p.cluster > 1) {
@@ -523,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_r
                 float l;
                 const float4 o = join_cluster(cluster, p.cluster, part_ml + r, outs + (size_t)r * HD + d, l);
                 const int i = row / G;
-                store_out(static_cast<unsigned short*>(a.out) + (int64_t)(part.start + i) * a.out_stride + (size_t)(h * G + row - i * G) * HD + d, o, l, f16);
+                store_out(static_cast<unsigned short*>(a.out) + (int64_t)(part.start + i) * a.out_stride + (size_t)(h * G + row - i * G) * HD + d, o, l, F16);
             }
             if (SAVE && tid < TR) {
                 float m = -INFINITY, l = 0.f;
@@ -743,7 +752,8 @@ RowsPlan rows_plan(const swlm_kv8_cache& c, const swlm_kv8_attend& a, size_t* by
 template <int HD, int CODE, int NT>
 cudaError_t launch_tiles(const dim3& grid, size_t smem, const swlm_kv8_cache& c, const swlm_kv8_attend& a, const RowsPlan& p, cudaStream_t s) {
     auto launch = [&](auto kernel) { return p.cluster > 1 ? launch_clusters(kernel, p.cluster, grid, dim3(kThreads), smem, s, c, a, p) : launch_k(kernel, grid, dim3(kThreads), smem, s, c, a, p); };
-    return p.pitch ? launch(kv8_rows_kernel<HD, CODE, NT, true>) : launch(kv8_rows_kernel<HD, CODE, NT, false>);
+    if (a.dtype == SWLM_KV8_FP16) return p.pitch ? launch(kv8_rows_kernel<HD, CODE, NT, true, true>) : launch(kv8_rows_kernel<HD, CODE, NT, false, true>);
+    return p.pitch ? launch(kv8_rows_kernel<HD, CODE, NT, true, false>) : launch(kv8_rows_kernel<HD, CODE, NT, false, false>);
 }
 
 template <int HD, int CODE>
@@ -770,7 +780,9 @@ int launch_rows(const swlm_kv8_cache& c, const swlm_kv8_attend& a, const RowsPla
 
 template <int HD, int CODE, int NT, bool SAVE>
 int init_one() {
-    SWLM_CUDA(cudaFuncSetAttribute(kv8_rows_kernel<HD, CODE, NT, SAVE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(rows_smem<HD>() + (kStreamBatch + 1) * sizeof(int4))));
+    constexpr int smem = (int)(rows_smem<HD>() + (kStreamBatch + 1) * sizeof(int4));
+    SWLM_CUDA((cudaFuncSetAttribute(kv8_rows_kernel<HD, CODE, NT, SAVE, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)));
+    SWLM_CUDA((cudaFuncSetAttribute(kv8_rows_kernel<HD, CODE, NT, SAVE, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)));
     return SWLM_OK;
 }
 template <int HD, int CODE>

@@ -45,6 +45,11 @@ __device__ __forceinline__ unsigned pack_half(float a, float b) {
     return *reinterpret_cast<const unsigned*>(&v);
 }
 
+// What rounding (a, b) to the fp16 pair v has left, as another pair: both together are the numbers to 2^-22 of themselves.
+__device__ __forceinline__ unsigned pack_rest(float a, float b, unsigned v) {
+    const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&v));
+    return pack_half(a - r.x, b - r.y);
+}
 
 // Codes to fp16, exactly. int8: with the sign bit turned a byte u = c + 128 is the low byte of 1024 + u.
 template <int CODE> __device__ __forceinline__ unsigned prepared(unsigned word) { return CODE == SWLM_KV8_INT8 ? word ^ 0x80808080u : word; }

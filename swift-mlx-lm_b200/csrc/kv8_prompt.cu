@@ -2,7 +2,8 @@
 //
 // A CTA has 256 rows in two tiles of 128, rows being the queries of a sequence times the heads of a group, and a run of its slots. Codes become fp16
 // numbers on their way to shared memory, queries are shifted to fp16 (both exact, see kv8_attend.cu), so that scores are one product with fp32
-// sums; a tile's scores take the factor of their block, probabilities that of the values' block over the largest so far (2^7 times, as fp16).
+// sums; a tile's scores take the factor of their block, probabilities that of the values' block over the largest so far (2^7 times, as fp16; for
+// fp16 results as two fp16 numbers, whose products the values meet one after the other: 3 x 777 rows with weights, heads of 64, 148 us, with one 138).
 //
 // Roles: three warps bring keys and values from the cache, convert them and store them in the swizzled layout of the products' operands (two
 // slots of 128 tokens each, which both row tiles read); a warp issues the MMAs (O += P V, then S = Q K^T of the next key tile, for one row tile
@@ -15,6 +16,7 @@
 // issuing the MMAs, paired fp32 operations 391; two row tiles that share the conversions, a warp for the MMAs 306; key tiles of 128 instead of 64
 // with two score regions 297; the longest rows of all heads first 278.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv8_device.cuh"
 #include "tc_attention.cuh"
@@ -45,7 +47,9 @@ struct PromptBars {
 template <int HD> __host__ __device__ constexpr size_t prompt_smem() { return (size_t)kPromptRows * HD * 2 + 2 * kSlots * kPromptKeys * HD * 2 + 1024; }
 
 // GROUPS: scales of a key tile (blocks of 16, 32, 64 or 128 tokens: 8, 4, 2, 1)
-template <int HD, int CODE, int GROUPS>
+// F16: queries and results are fp16. Of 16 probabilities the columns of their scores hold the fp16 numbers (8 columns) and what rounding has left (8); else
+// the numbers alone, those of a tile in the first 64 of its 128 columns.
+template <int HD, int CODE, int GROUPS, bool F16>
 __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swlm_kv8_cache c, const swlm_kv8_attend a, const RowsPlan p, int* status) {
     constexpr int HALVES = HD / 64;                        // 128-byte halves of a row
     constexpr unsigned Q_HALF = kPaRows * 128, Q_BYTES = HALVES * Q_HALF, KV_HALF = kPromptKeys * 128, KV_BYTES = HALVES * KV_HALF;
@@ -191,7 +195,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
                 if (el) {
 #pragma unroll
                     for (int kk = 0; kk < kPromptKeys / 16; ++kk)
-                        pa_mma_ts(tm + O_COL + t * 128u, tm + t * 128u + 8u * kk, vd + slot * (KV_BYTES / 16) + kk * (2048 / 16), pa_idesc(HD, true, false), kk > 0 || j > 0 ? 1u : 0u);
+#pragma unroll
+                        for (int rest = 0; rest < (F16 ? 2 : 1); ++rest)
+                            pa_mma_ts(tm + O_COL + t * 128u, tm + t * 128u + (F16 ? 16u : 8u) * kk + 8u * rest, vd + slot * (KV_BYTES / 16) + kk * (2048 / 16), pa_idesc(HD, true, false),
+                                      kk > 0 || rest > 0 || j > 0 ? 1u : 0u);
                     umma_commit(&bars.pv_done[t]);
                 }
                 __syncwarp();
@@ -212,7 +219,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
         __syncwarp();
     } else {
         const int t = warp >> 2, r = tid & (kPaRows - 1), row = block0 + tid, i = min(row, rows - 1) / G, tiles = t ? tiles1 : tiles0;   // r: of the row tile
-        const bool row_ok = row < rows, f16 = a.dtype == SWLM_KV8_FP16;
+        const bool row_ok = row < rows;
         const int limit = visible(part, i, span);   // (rows past the last one attend what it does; they are not stored)
         float factor;
         // ---- q: this thread's row, shifted to fp16 ----------------------------------------------------------------------------------------
@@ -227,12 +234,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
             }
             const bool keeps = p.q16 && split == 0;   // for the launch that adds the weights
             float up;
-            row_shift(f16 ? __half2float(__ushort_as_half((unsigned short)top)) : __uint_as_float(top << 16), up, factor);
+            row_shift(F16 ? __half2float(__ushort_as_half((unsigned short)top)) : __uint_as_float(top << 16), up, factor);
             factor *= a.scale * kLog2e;
 #pragma unroll 4
             for (int d = 0; d < HD; d += 8) {
                 float x[8];
-                widen(*reinterpret_cast<const uint4*>(src + d), f16, x);
+                widen(*reinterpret_cast<const uint4*>(src + d), F16, x);
                 uint4 v;
                 v.x = pack_half(x[0] * up, x[1] * up); v.y = pack_half(x[2] * up, x[3] * up);
                 v.z = pack_half(x[4] * up, x[5] * up); v.w = pack_half(x[6] * up, x[7] * up);
@@ -323,7 +330,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
                 unit[g] = vt[g] * v_inv;
                 folds = folds && unit[g] >= kFoldUnit * kValueUnit;
             }
-            // probabilities of the first half take the place of its first 32 columns, those of the second half that of the next 32
+            // Probabilities of a half take the place of its own scores (F16), or those of the first half that of its first 32 columns and those of the second that of
+            // the next 32. `put`: the e-th pair of 16 scores, which all have been read when the first is written
+            auto put = [&](unsigned (&out)[16], int e, float x, float y) {
+                out[e] = pack_half(x, y);
+                if (F16) out[8 + e] = pack_rest(x, y, out[e]);
+            };
+            auto keep = [&](const unsigned (&out)[16], int at) {
+#pragma unroll
+                for (int e = 0; e < (F16 ? 16 : 8); ++e) v[F16 ? at + e : at / 2 + e] = out[e];
+            };
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 if (half) {   // (the first half is what was read last)
@@ -340,11 +356,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
                         const float2 fk2 = make_float2(fk[at], fk[at]), shift2 = make_float2(shift, shift);
                         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-                        for (int e = 0; e < N; e += 2) {
-                            float2 x = fma2(make_float2(__uint_as_float(v[g * N + e]), __uint_as_float(v[g * N + e + 1])), fk2, shift2);
-                            x = make_float2(pa_exp2(x.x), pa_exp2(x.y));
-                            sum[e >> 1 & 1] = add2(sum[e >> 1 & 1], x);
-                            v[(g * N + e) / 2] = pack_half(x.x, x.y);
+                        for (int e0 = 0; e0 < N; e0 += 16) {
+                            unsigned out[16];
+#pragma unroll
+                            for (int e = 0; e < 16; e += 2) {
+                                const int i = g * N + e0 + e;
+                                float2 x = fma2(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), fk2, shift2);
+                                x = make_float2(pa_exp2(x.x), pa_exp2(x.y));
+                                sum[e >> 1 & 1] = add2(sum[e >> 1 & 1], x);
+                                put(out, e / 2, x.x, x.y);
+                            }
+                            keep(out, g * N + e0);
                         }
                         const float2 all = add2(sum[0], sum[1]);
                         l_run += __fdividef(all.x + all.y, unit[at]);
@@ -354,20 +376,27 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
                     for (int g = 0; g < PARTS; ++g) {
                         const int at = (half * 64 + g * N) / KEYS;
 #pragma unroll
-                        for (int e = 0; e < N; e += 2) {
-                            float w[2];
+                        for (int e0 = 0; e0 < N; e0 += 16) {
+                            unsigned out[16];
 #pragma unroll
-                            for (int k = 0; k < 2; ++k) {
-                                const bool sees = key0 + half * 64 + g * N + e + k < limit;   // (what a row does not attend may lie in a block that is NaN)
-                                const float x = sees ? pa_exp2(fmaf(__uint_as_float(v[g * N + e + k]), fk[at], -base)) : 0.f;
-                                l_run += x;
-                                w[k] = sees ? x * unit[at] : 0.f;
+                            for (int e = 0; e < 16; e += 2) {
+                                float w[2];
+#pragma unroll
+                                for (int k = 0; k < 2; ++k) {
+                                    const int i = g * N + e0 + e + k;
+                                    const bool sees = key0 + half * 64 + i < limit;   // (what a row does not attend may lie in a block that is NaN)
+                                    const float x = sees ? pa_exp2(fmaf(__uint_as_float(v[i]), fk[at], -base)) : 0.f;
+                                    l_run += x;
+                                    w[k] = sees ? x * unit[at] : 0.f;
+                                }
+                                put(out, e / 2, w[0], w[1]);
                             }
-                            v[(g * N + e) / 2] = pack_half(w[0], w[1]);
+                            keep(out, g * N + e0);
                         }
                     }
                 }
-                pa_st32(region + half * 32u, v);
+                pa_st32(region + half * (F16 ? 64u : 32u), v);
+                if (F16) pa_st32(region + half * 64u + 32u, v + 32);
             }
             pa_wait_st();
             pa_before();
@@ -396,7 +425,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
 #pragma unroll
                     for (int e = 0; e < 16; e += 4) {
                         const float4 x = make_float4(__uint_as_float(o[e]) * unit, __uint_as_float(o[e + 1]) * unit, __uint_as_float(o[e + 2]) * unit, __uint_as_float(o[e + 3]) * unit);
-                        if (whole) store_out(dst + d + e, x, l_run, f16);
+                        if (whole) store_out(dst + d + e, x, l_run, F16);
                         else *reinterpret_cast<float4*>(p.part_o + at * HD + d + e) = x;
                     }
             }
@@ -570,8 +599,12 @@ template <int HD, int CODE>
 int launch_prompt(const swlm_kv8_cache& c, const swlm_kv8_attend& a, const RowsPlan& p, int* status, cudaStream_t s) {
     const dim3 grid((unsigned)c.batch * c.kv_heads * p.row_tiles * p.splits);
     auto launch = [&](auto kernel) { return launch_k(kernel, grid, dim3(kPromptThreads), prompt_smem<HD>(), s, c, a, p, status); };
-    const cudaError_t e = c.block == 128 ? launch(kv8_prompt_kernel<HD, CODE, 1>) : c.block == 64 ? launch(kv8_prompt_kernel<HD, CODE, 2>) :
-                          c.block == 32 ? launch(kv8_prompt_kernel<HD, CODE, 4>) : launch(kv8_prompt_kernel<HD, CODE, 8>);
+    auto of_type = [&](auto f16) {
+        constexpr bool F16 = decltype(f16)::value;
+        return c.block == 128 ? launch(kv8_prompt_kernel<HD, CODE, 1, F16>) : c.block == 64 ? launch(kv8_prompt_kernel<HD, CODE, 2, F16>) :
+               c.block == 32 ? launch(kv8_prompt_kernel<HD, CODE, 4, F16>) : launch(kv8_prompt_kernel<HD, CODE, 8, F16>);
+    };
+    const cudaError_t e = a.dtype == SWLM_KV8_FP16 ? of_type(std::true_type()) : of_type(std::false_type());
     return e == cudaSuccess ? SWLM_OK : cuda_fail(e, "kv8 prompt attention launch");
 }
 template <int HD, int CODE>
@@ -589,10 +622,11 @@ template <int HD, int CODE>
 int init_prompt() {
     SWLM_CUDA((cudaFuncSetAttribute(kv8_weights_kernel<HD, CODE, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)weights_smem<HD, 4>())));
     if constexpr (HD == 128) SWLM_CUDA((cudaFuncSetAttribute(kv8_weights_kernel<HD, CODE, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)weights_smem<HD, 2>())));
-    SWLM_CUDA(cudaFuncSetAttribute(kv8_prompt_kernel<HD, CODE, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prompt_smem<HD>()));
-    SWLM_CUDA(cudaFuncSetAttribute(kv8_prompt_kernel<HD, CODE, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prompt_smem<HD>()));
-    SWLM_CUDA(cudaFuncSetAttribute(kv8_prompt_kernel<HD, CODE, 8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prompt_smem<HD>()));
-    SWLM_CUDA(cudaFuncSetAttribute(kv8_prompt_kernel<HD, CODE, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prompt_smem<HD>()));
+    auto each = [](auto kernel) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prompt_smem<HD>()); };
+    for (const cudaError_t e : {each(kv8_prompt_kernel<HD, CODE, 1, false>), each(kv8_prompt_kernel<HD, CODE, 2, false>), each(kv8_prompt_kernel<HD, CODE, 4, false>),
+                                each(kv8_prompt_kernel<HD, CODE, 8, false>), each(kv8_prompt_kernel<HD, CODE, 1, true>), each(kv8_prompt_kernel<HD, CODE, 2, true>),
+                                each(kv8_prompt_kernel<HD, CODE, 4, true>), each(kv8_prompt_kernel<HD, CODE, 8, true>)})
+        SWLM_CUDA(e);
     return SWLM_OK;
 }
 
