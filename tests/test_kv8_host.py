@@ -147,3 +147,34 @@ def test_refused_must_be_aligned(pkg, lib):
 def test_status_of_no_context(pkg, lib):
     assert lib.swlm_op_kv8_status(None) == INVALID
     assert lib.swlm_write_kv8_status(None, 1) == INVALID
+
+
+SCRATCH = [
+    # kv_heads, heads, head_dim, batch, n, max_len, CTAs of a launch with equal shares (0: none), rows of a tile, runs of slots of many rows
+    (8, 32, 128, 8, 1, 8192, 3 * 148, 8, 0),     # a tile per (sequence, head), three CTAs on an SM
+    (8, 32, 64, 41, 1, 8192, 4 * 148, 8, 0),     # four with heads of 64
+    (8, 32, 128, 6, 5, 8192, 2 * 148, 16, 0),    # 20 rows: two tiles of 16, two CTAs on an SM
+    (1, 4, 128, 3, 1, 8192, 3 * 64, 8, 0),       # as many CTAs as there are runs of 128 slots
+    (8, 32, 128, 1, 1, 1000, 0, 8, 0),           # clusters, which join their results themselves
+    (2, 2, 64, 600, 1, 256, 0, 8, 0),            # more sequences than shares are dealt of: a CTA has all slots
+    (8, 32, 128, 1, 2048, 8192, 0, 256, 1),      # portions: as many CTAs as fill the GPU without runs
+    (1, 4, 128, 1, 40, 8192, 0, 256, 64),        # one block of rows: a key tile per CTA
+]
+
+
+@pytest.mark.parametrize("accumulate", [0, 1])
+@pytest.mark.parametrize("kv_heads,heads,dim,batch,n,max_len,ctas,tile,runs", SCRATCH, ids=str)
+def test_scratch_is_what_the_kernels_write(pkg, lib, kv_heads, heads, dim, batch, n, max_len, ctas, tile, runs, accumulate):
+    """Partial results have a place for every tile and one more per CTA of the shares, or one for every run of a tile's slots; a place has the tile's rows, each
+    its results, a maximum and a sum. Weights need the kept scores of every slot and row, or the queries as fp16 with a factor and a shift each."""
+    cache = _cache(pkg, kv_heads=kv_heads, head_dim=dim, batch=batch, capacity=8192)
+    step = _attend(pkg, heads=heads, n=n, rows=batch * n, max_len=max_len, q_stride=heads * dim, out_stride=heads * dim, accumulate=accumulate)
+    rows, groups = heads // kv_heads * n, batch * kv_heads
+    tiles = groups * -(-rows // tile)
+    need = (tiles + ctas) * tile * (dim + 2) * 4 + (batch + 1) * 4 if ctas else tiles * runs * tile * (dim + 2) * 4 if runs > 1 else 0
+    if accumulate:
+        pitch = 2 if rows <= 2 else -(-rows // 4) * 4
+        need += groups * -(-max_len // 32) * 32 * pitch * 4 if rows <= 64 else tiles * tile * (dim * 2 + 8)
+        need += tiles * tile * 8 if batch > 512 else 0   # (the rows' maxima and sums alone, for the launch that adds the weights)
+    got = lib.swlm_op_kv8_attend_scratch_bytes(cache, step)
+    assert need <= got <= need + 8 * 16
