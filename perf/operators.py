@@ -159,6 +159,38 @@ def prepare(case, seed):
 
 # ---- the framework's calls ----------------------------------------------------------------------------------------------
 
+def _context():
+    """The package and the context of the device: a program makes them once."""
+    if not hasattr(_context, "made"):
+        import __graft_entry__
+        pkg = __graft_entry__.load_package()
+        _context.made = pkg, pkg.WeightStore(0)
+    return _context.made
+
+
+def _prepare_own(state):
+    _context()
+    if state["case"]["kind"] == "append":
+        _hold_last_blocks(state)
+
+
+def _hold_last_blocks(state):
+    """Codes and scales of the blocks that sequences end in, which an append may scale anew: every pass finds them as they were before the step. The cache
+    lies in one allocation of words, so that one copy brings them back."""
+    case, cache = state["case"], state["cache"]
+    b, h, cap, d = cache["k"].shape
+    t, codes, scales = case["block"], cache["k"].numel() // 4, cache["k_scale"].numel()
+    state["words"] = words = torch.cat([cache[x].reshape(-1).view(torch.int32) for x in ("k", "v", "k_scale", "v_scale")])
+    for x, part in zip(("k", "v", "k_scale", "v_scale"), words.split([codes, codes, scales, scales])):
+        cache[x] = part.view(cache[x].dtype).view(cache[x].shape)
+    head = torch.arange(b * h, device="cuda")
+    block = (state["lengths"].long() // t).repeat_interleave(h)
+    of_codes = ((head * cap + block * t)[:, None] * (d // 4) + torch.arange(t * d // 4, device="cuda")).reshape(-1)
+    of_scales = 2 * codes + head * (cap // t) + block
+    state["last"] = torch.cat([of_codes, of_codes + codes, of_scales, of_scales + scales])
+    state["held"] = words[state["last"]]
+
+
 def _described(pkg, case, cache):
     return pkg.Kv8Cache(k=cache["k"].data_ptr(), v=cache["v"].data_ptr(), k_scale=cache["k_scale"].data_ptr(), v_scale=cache["v_scale"].data_ptr(),
                         weight=cache["weight"].data_ptr(), slot_pos=cache["slot_pos"].data_ptr(), batch=case["batch"], kv_heads=case["kv_heads"],
@@ -166,35 +198,37 @@ def _described(pkg, case, cache):
                         code=pkg.KV8_INT8 if case["code"] == INT8 else pkg.KV8_E4M3)
 
 
-def _prepare_own(state):
-    """The descriptions and the scratch that a program makes once and keeps beside its buffers."""
-    import __graft_entry__
-    pkg = __graft_entry__.load_package()
+def _run_own(state):
+    pkg, store = _context()
+    # (a null stream stands for the context's own; 1 is CUDA's handle of the default stream that torch works on)
+    lib, handle, stream = store.lib, store.handle, torch.cuda.current_stream().cuda_stream or 1
     case, cache = state["case"], state["cache"]
-    store = state["store"] = pkg.WeightStore(0)
-    lib = state["lib"] = store.lib
-    state["described"] = _described(pkg, case, cache)
-    dtype = pkg.KV8_BF16 if case["dtype"] == "bf16" else pkg.KV8_FP16
-    lengths, counts, starts = (state[f].data_ptr() for f in ("lengths", "counts", "starts"))
+    if case["kind"] == "append":
+        state["words"].index_copy_(0, state["last"], state["held"])
+    described, lengths = _described(pkg, case, cache), state["lengths"].data_ptr()
     if case["kind"] == "append":
         stride = case["kv_heads"] * case["head_dim"]
-        state["call"] = pkg.Kv8Append(k=state["k"].data_ptr(), v=state["v"].data_ptr(), k_stride=stride, v_stride=stride, lengths=lengths, counts=counts,
-                                      starts=starts, seen=state["seen"].data_ptr(), dtype=dtype, n=case["tokens"], rows=state["k"].shape[0])
+        call = pkg.Kv8Append(k=state["k"].data_ptr(), v=state["v"].data_ptr(), k_stride=stride, v_stride=stride, lengths=lengths, counts=state["counts"].data_ptr(),
+                             starts=state["starts"].data_ptr(), seen=state["seen"].data_ptr(), dtype=pkg.KV8_BF16 if case["dtype"] == "bf16" else pkg.KV8_FP16,
+                             n=case["tokens"], rows=state["k"].shape[0])
+        lib.check(lib.swlm_op_kv8_append_dev(handle, described, call, stream))
     elif case["kind"] == "attend":
         stride = case["heads"] * case["head_dim"]
-        call = state["call"] = pkg.Kv8Attend(q=state["q"].data_ptr(), out=state["out"].data_ptr(), q_stride=stride, out_stride=stride, lengths=lengths,
-                                             counts=counts, starts=starts, scale=case["head_dim"] ** -0.5, dtype=dtype, heads=case["heads"], n=case["tokens"],
-                                             rows=state["q"].shape[0], max_len=case["context"] + case["tokens"], accumulate=int(case["weights"]))
-        call.scratch_bytes = lib.swlm_op_kv8_attend_scratch_bytes(state["described"], call)
-        state["scratch"] = torch.empty(max(16, call.scratch_bytes), dtype=torch.uint8, device="cuda")
-        call.scratch = state["scratch"].data_ptr()
+        call = pkg.Kv8Attend(q=state["q"].data_ptr(), out=state["out"].data_ptr(), q_stride=stride, out_stride=stride, lengths=lengths,
+                             counts=state["counts"].data_ptr(), starts=state["starts"].data_ptr(), scale=case["head_dim"] ** -0.5,
+                             dtype=pkg.KV8_BF16 if case["dtype"] == "bf16" else pkg.KV8_FP16, heads=case["heads"], n=case["tokens"],
+                             rows=state["q"].shape[0], max_len=case["context"] + case["tokens"], accumulate=int(case["weights"]))
+        call.scratch_bytes = lib.swlm_op_kv8_attend_scratch_bytes(described, call)
+        scratch = torch.empty(max(16, call.scratch_bytes), dtype=torch.uint8, device="cuda")
+        call.scratch = scratch.data_ptr()
+        lib.check(lib.swlm_op_kv8_attend_dev(handle, described, call, stream))
     else:
-        state["described_kept"] = _described(pkg, case, state["kept"])
-        call = state["call"] = pkg.Kv8Evict(lengths=lengths, seen=state["seen"].data_ptr(), keep=case["keep"], sink=min(4, case["keep"] // 4),
-                                            recent=min(32, case["keep"] // 4), max_len=case["context"])
-        call.scratch_bytes = lib.swlm_op_kv8_evict_scratch_bytes(state["described"], call)
-        state["scratch"] = torch.empty(max(16, call.scratch_bytes), dtype=torch.uint8, device="cuda")
-        call.scratch = state["scratch"].data_ptr()
+        call = pkg.Kv8Evict(lengths=lengths, seen=state["seen"].data_ptr(), keep=case["keep"], sink=min(4, case["keep"] // 4),
+                            recent=min(32, case["keep"] // 4), max_len=case["context"])
+        call.scratch_bytes = lib.swlm_op_kv8_evict_scratch_bytes(described, call)
+        scratch = torch.empty(max(16, call.scratch_bytes), dtype=torch.uint8, device="cuda")
+        call.scratch = scratch.data_ptr()
+        lib.check(lib.swlm_op_kv8_evict_dev(handle, described, _described(pkg, case, state["kept"]), call, stream))
 
 
 def run(state):
@@ -202,14 +236,7 @@ def run(state):
     if case["kind"] == "attend" and case["weights"]:
         cache["weight"].copy_(state["before"])   # every pass adds to the sums as they were before the step
     if own:
-        # (a null stream stands for the context's own; 1 is CUDA's handle of the default stream that torch works on)
-        lib, handle, stream = state["lib"], state["store"].handle, torch.cuda.current_stream().cuda_stream or 1
-        if case["kind"] == "append":
-            lib.check(lib.swlm_op_kv8_append_dev(handle, state["described"], state["call"], stream))
-        elif case["kind"] == "attend":
-            lib.check(lib.swlm_op_kv8_attend_dev(handle, state["described"], state["call"], stream))
-        else:
-            lib.check(lib.swlm_op_kv8_evict_dev(handle, state["described"], state["described_kept"], state["call"], stream))
+        _run_own(state)
     else:
         {"append": _plain_append, "attend": _plain_attend, "evict": _plain_evict}[case["kind"]](state)
     if case["kind"] == "attend":
