@@ -313,6 +313,7 @@ int swlm_op_flash_decode_noalloc_dev(swlm_ctx* ctx, int b, int heads, int kv_hea
  * are advanced behind the last layer with swlm_op_kv8_lengths_dev. */
 enum { SWLM_KV8_INT8 = 0, SWLM_KV8_E4M3 = 1 };   /* swlm_kv8_cache.code */
 enum { SWLM_KV8_BF16 = 0, SWLM_KV8_FP16 = 1 };   /* type of keys, values, queries and results */
+enum { SWLM_KV8_P_BY_TYPE = 0, SWLM_KV8_P_ONE = 1, SWLM_KV8_P_TWO = 2 };   /* fp16 numbers that a probability meets the values as */
 
 typedef struct swlm_kv8_cache {
     void* k;            /* codes [batch][kv_heads][capacity][head_dim], 16-byte aligned as v is */
@@ -356,9 +357,10 @@ int swlm_op_kv8_append_dev(swlm_ctx* ctx, const swlm_kv8_cache* cache, const swl
  * refused: what the step's append wrote there. The tokens of a sequence that it refused (a parked one's too) are not in the cache, so its queries
  * would attend slots without tokens, and accumulate would add their weights (NULL: no sequence was refused).
  * accumulate: weight[b][h][slot] += the softmax weights that the step's queries of all heads of the group have for the slot.
- * Scores, softmax and sums are fp32. Probabilities meet the values as fp16 numbers: off by 2^-11 of themselves, or, where a block's value scale is
- * less than 2^-21 / probability of the largest that the query attends, by 2^-32 of that scale. For results in fp16 they are the sum of two such
- * numbers (2^-22). An infinity or NaN in a query makes that query's results (and, accumulated, the weights that it adds) NaN.
+ * Scores, softmax and sums are fp32. probabilities: they meet the values as one fp16 number each, off by 2^-11 of themselves, or, where a block's
+ * value scale is less than 2^-21 / probability of the largest that the query attends, by 2^-32 of that scale; or as the sum of two (2^-22), which
+ * takes up to a third longer. BY_TYPE: two for results in fp16, where the error of one is as large as that of rounding the result, one for bf16.
+ * An infinity or NaN in a query makes that query's results (and, accumulated, the weights that it adds) NaN.
  * scratch: swlm_op_kv8_attend_scratch_bytes() (0: none needed), 16-byte aligned, not shared by calls that may overlap.
  * Waits on the device are bounded. Once one has expired, results and weights since then are not valid, and the context's swlm_op_kv8_attend_dev and
  * swlm_op_kv8_evict_dev, on every stream, return SWLM_ERR_TIMEOUT without doing anything until swlm_op_kv8_status has reported it. */
@@ -378,6 +380,7 @@ typedef struct swlm_kv8_attend {
     int32_t rows;          /* rows of q and out */
     int32_t max_len;       /* no sequence has more tokens than this, its new ones included; what lies behind is not attended */
     int32_t accumulate;
+    int32_t probabilities; /* SWLM_KV8_P_BY_TYPE, _ONE or _TWO */
     const int32_t* refused;   /* [batch], or NULL */
 } swlm_kv8_attend;
 size_t swlm_op_kv8_attend_scratch_bytes(const swlm_kv8_cache* cache, const swlm_kv8_attend* step);   /* the pointers are not looked at; 0 for what the call refuses */

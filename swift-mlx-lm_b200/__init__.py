@@ -8,7 +8,7 @@ Nothing here computes: every numeric path goes through the C ABI declared in inc
 and loading fails loudly when the CUDA library has not been built.
 """
 from .lib import Library, SwlmError, build_library, load_library  # noqa: F401
-from .lib import KV8_BF16, KV8_E4M3, KV8_FP16, KV8_INT8, Kv8Append, Kv8Attend, Kv8Cache, Kv8Evict  # noqa: F401
+from .lib import KV8_BF16, KV8_E4M3, KV8_FP16, KV8_INT8, KV8_P_BY_TYPE, KV8_P_ONE, KV8_P_TWO, Kv8Append, Kv8Attend, Kv8Cache, Kv8Evict  # noqa: F401
 from .formats import (  # noqa: F401
     AffineQ4Group64Format,
     AffineQ4Group128Format,

@@ -581,6 +581,7 @@ int attend_shape_ok(const swlm_kv8_cache& c, const swlm_kv8_attend& a) {
     if (a.heads < 1 || a.heads % c.kv_heads) { set_error("kv8: %d query heads do not divide by %d KV heads", a.heads, c.kv_heads); return SWLM_ERR_INVALID; }
     if ((int64_t)a.n * (a.heads / c.kv_heads) > kKv8MaxLen) return refuse("too many query rows");
     if (a.max_len < 1 || a.max_len > kKv8MaxLen) return refuse("max_len out of range");
+    if (a.probabilities != SWLM_KV8_P_BY_TYPE && a.probabilities != SWLM_KV8_P_ONE && a.probabilities != SWLM_KV8_P_TWO) return refuse("unknown form of the probabilities");
     if (!kv8_attend_grid_fits(c, a)) return refuse("too many query rows");
     return SWLM_OK;
 }

@@ -11,9 +11,10 @@
 // each over a ring of its own that cp.async fills. Scores come as S^T = K Q^T (16 tokens x 8 rows, so that a decode step's four or eight
 // rows fill the tile), probabilities are transposed in registers (movmatrix) and meet the values as O^T = V^T P^T. The reference
 // maximum of a row moves only when it would grow by more than 2^8. Probabilities are rounded to fp16 as p 2^7 vs / vr, vr the largest value
-// scale so far: off by 2^-11 of themselves where p vs / vr >= 2^-21, below that by 2^-32 of vr. bf16 results do not show it. For fp16 results, which
-// have as many bits, what the rounding has left follows as a second product (2^-22 of themselves where p vs / vr >= 2^-10): 41 ragged sequences of 4091
-// tokens 29.3 us, with one product 28.5; error against 64 bits 2.1e-4 (of which rounding the result is 2.1e-4) and 2.7e-4. Partial results of a tile
+// scale so far: off by 2^-11 of themselves where p vs / vr >= 2^-21, below that by 2^-32 of vr. bf16 results do not show it. fp16 results, which
+// have as many bits, do: unless the caller chooses, what the rounding has left follows there as a second product (2^-22 of themselves where
+// p vs / vr >= 2^-10). Error against 64 bits, 41 ragged sequences of 4091 tokens in fp16: 2.7e-4 with one product, 2.1e-4 with two, of which rounding the
+// result is 2.1e-4; 27.5 and 28.8 us, five tokens of six sequences over 16384 48.0 and 54.0. Partial results of a tile
 // are joined by a second launch, which also adds the weights, or by the cluster of CTAs that has all of a tile's slots.
 //
 // What bounds it: memory, and some ten us of start, merge and the second launch. 8 x 8192 tokens, 32 / 8 heads of 128, int8: 33.5 us for 134 MB (0.61
@@ -159,7 +160,8 @@ __device__ __forceinline__ float4 join_cluster(const cg::cluster_group& cluster,
     return o;
 }
 
-template <int HD, int CODE, int NT, bool SAVE, bool F16>
+// TWO: probabilities meet the values as two fp16 numbers.
+template <int HD, int CODE, int NT, bool SAVE, bool TWO>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_rows_kernel(const swlm_kv8_cache c, const swlm_kv8_attend a, const RowsPlan p) {
     constexpr int KS = HD / 16, MT = HD / 16, NS = stages<HD>(), SB = stage_bytes<HD>(), TR = 8 * NT;
     extern __shared__ __align__(16) unsigned char sm[];
@@ -171,6 +173,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_r
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int G = a.heads / c.kv_heads, span = min(a.max_len, c.capacity);
+    const bool f16 = a.dtype == SWLM_KV8_FP16;
     const int block_shift = 31 - __clz(c.block);
 
     // ---- this CTA's units ----
@@ -289,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_r
         for (int nt = 0; nt < NT; ++nt) {
             const int r = row0 + nt * 8 + g, i = min(r, rows - 1) / G;
             float down;
-            load_query<HD>(static_cast<const unsigned short*>(a.q) + (int64_t)(part.start + i) * a.q_stride + (size_t)(h * G + min(r, rows - 1) - i * G) * HD, r < rows, F16, t,
+            load_query<HD>(static_cast<const unsigned short*>(a.q) + (int64_t)(part.start + i) * a.q_stride + (size_t)(h * G + min(r, rows - 1) - i * G) * HD, r < rows, f16, t,
                            qf[nt], down);
             down *= a.scale * kLog2e;
 #pragma unroll
@@ -413,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_r
 #pragma unroll
                         for (int e = 0; e < 4; ++e) acc[nt][j][e] *= corr;
             }
-            unsigned pf[kSub][NT][2], pr[kSub][NT][2];   // (pr: what rounding has left of them, for results in fp16)
+            unsigned pf[kSub][NT][2], pr[kSub][NT][2];   // (pr: what rounding has left of them)
 #pragma unroll
             for (int sub = 0; sub < kSub; ++sub) {
                 const float unit = v_scale[sub] * v_inv;
@@ -430,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_r
                     const unsigned p0 = pack_half(w[0], w[1]), p1 = pack_half(w[2], w[3]);
                     pf[sub][nt][0] = transpose8x8(p0);
                     pf[sub][nt][1] = transpose8x8(p1);
-                    if (F16) {
+                    if (TWO) {
                         pr[sub][nt][0] = transpose8x8(pack_rest(w[0], w[1], p0));
                         pr[sub][nt][1] = transpose8x8(pack_rest(w[2], w[3], p1));
                     }
@@ -457,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_r
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
                             mma(acc[nt][2 * w + half], a0, a1, a2, a3, pf[sub][nt][0], pf[sub][nt][1]);
-                            if (F16) mma(acc[nt][2 * w + half], a0, a1, a2, a3, pr[sub][nt][0], pr[sub][nt][1]);
+                            if (TWO) mma(acc[nt][2 * w + half], a0, a1, a2, a3, pr[sub][nt][0], pr[sub][nt][1]);
                         }
                     }
                 }
@@ -518,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_r
                 *reinterpret_cast<float4*>(p.part_o + (slot * TR + r) * HD + d) = o;
             } else {
                 const int i = row / G;
-                store_out(static_cast<unsigned short*>(a.out) + (int64_t)(part.start + i) * a.out_stride + (size_t)(h * G + row - i * G) * HD + d, o, l, F16);
+                store_out(static_cast<unsigned short*>(a.out) + (int64_t)(part.start + i) * a.out_stride + (size_t)(h * G + row - i * G) * HD + d, o, l, f16);
             }
         }
         if (p.cluster > 1) {
@@ -532,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? rows_ctas<HD>() : 2) kv8_r
                 float l;
                 const float4 o = join_cluster(cluster, p.cluster, part_ml + r, outs + (size_t)r * HD + d, l);
                 const int i = row / G;
-                store_out(static_cast<unsigned short*>(a.out) + (int64_t)(part.start + i) * a.out_stride + (size_t)(h * G + row - i * G) * HD + d, o, l, F16);
+                store_out(static_cast<unsigned short*>(a.out) + (int64_t)(part.start + i) * a.out_stride + (size_t)(h * G + row - i * G) * HD + d, o, l, f16);
             }
             if (SAVE && tid < TR) {
                 float m = -INFINITY, l = 0.f;
@@ -752,7 +755,7 @@ RowsPlan rows_plan(const swlm_kv8_cache& c, const swlm_kv8_attend& a, size_t* by
 template <int HD, int CODE, int NT>
 cudaError_t launch_tiles(const dim3& grid, size_t smem, const swlm_kv8_cache& c, const swlm_kv8_attend& a, const RowsPlan& p, cudaStream_t s) {
     auto launch = [&](auto kernel) { return p.cluster > 1 ? launch_clusters(kernel, p.cluster, grid, dim3(kThreads), smem, s, c, a, p) : launch_k(kernel, grid, dim3(kThreads), smem, s, c, a, p); };
-    if (a.dtype == SWLM_KV8_FP16) return p.pitch ? launch(kv8_rows_kernel<HD, CODE, NT, true, true>) : launch(kv8_rows_kernel<HD, CODE, NT, false, true>);
+    if (kv8_two_products(a)) return p.pitch ? launch(kv8_rows_kernel<HD, CODE, NT, true, true>) : launch(kv8_rows_kernel<HD, CODE, NT, false, true>);
     return p.pitch ? launch(kv8_rows_kernel<HD, CODE, NT, true, false>) : launch(kv8_rows_kernel<HD, CODE, NT, false, false>);
 }
 

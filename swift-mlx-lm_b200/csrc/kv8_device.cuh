@@ -170,6 +170,10 @@ constexpr int kPromptRows = 256, kPromptKeys = 128;
 
 }  // namespace kv8
 
+// Whether probabilities meet the values as two fp16 numbers.
+inline bool kv8_two_products(const swlm_kv8_attend& a) {
+    return a.probabilities == SWLM_KV8_P_TWO || (a.probabilities == SWLM_KV8_P_BY_TYPE && a.dtype == SWLM_KV8_FP16);
+}
 int kv8_prompt_init();
 int launch_kv8_prompt_weights(const swlm_kv8_cache& c, const swlm_kv8_attend& a, const kv8::RowsPlan& p, int* status, cudaStream_t s);
 int launch_kv8_prompt(const swlm_kv8_cache& c, const swlm_kv8_attend& a, const kv8::RowsPlan& p, int* status, cudaStream_t s);

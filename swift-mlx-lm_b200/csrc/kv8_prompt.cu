@@ -2,8 +2,8 @@
 //
 // A CTA has 256 rows in two tiles of 128, rows being the queries of a sequence times the heads of a group, and a run of its slots. Codes become fp16
 // numbers on their way to shared memory, queries are shifted to fp16 (both exact, see kv8_attend.cu), so that scores are one product with fp32
-// sums; a tile's scores take the factor of their block, probabilities that of the values' block over the largest so far (2^7 times, as fp16; for
-// fp16 results as two fp16 numbers, whose products the values meet one after the other: 3 x 777 rows with weights, heads of 64, 148 us, with one 138).
+// sums; a tile's scores take the factor of their block, probabilities that of the values' block over the largest so far (2^7 times, as fp16
+// or as two fp16 numbers, whose products follow one another: 3 x 777 rows with weights, heads of 64, 147 us, with one 136; 2048 over 6144 361 and 276).
 //
 // Roles: three warps bring keys and values from the cache, convert them and store them in the swizzled layout of the products' operands (two
 // slots of 128 tokens each, which both row tiles read); a warp issues the MMAs (O += P V, then S = Q K^T of the next key tile, for one row tile
@@ -47,9 +47,9 @@ struct PromptBars {
 template <int HD> __host__ __device__ constexpr size_t prompt_smem() { return (size_t)kPromptRows * HD * 2 + 2 * kSlots * kPromptKeys * HD * 2 + 1024; }
 
 // GROUPS: scales of a key tile (blocks of 16, 32, 64 or 128 tokens: 8, 4, 2, 1)
-// F16: queries and results are fp16. Of 16 probabilities the columns of their scores hold the fp16 numbers (8 columns) and what rounding has left (8); else
-// the numbers alone, those of a tile in the first 64 of its 128 columns.
-template <int HD, int CODE, int GROUPS, bool F16>
+// TWO: probabilities meet the values as two fp16 numbers. Of 16 probabilities the columns of their scores hold the fp16 numbers (8 columns) and what rounding has
+// left (8); else the numbers alone, those of a tile in the first 64 of its 128 columns.
+template <int HD, int CODE, int GROUPS, bool TWO>
 __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swlm_kv8_cache c, const swlm_kv8_attend a, const RowsPlan p, int* status) {
     constexpr int HALVES = HD / 64;                        // 128-byte halves of a row
     constexpr unsigned Q_HALF = kPaRows * 128, Q_BYTES = HALVES * Q_HALF, KV_HALF = kPromptKeys * 128, KV_BYTES = HALVES * KV_HALF;
@@ -196,8 +196,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
 #pragma unroll
                     for (int kk = 0; kk < kPromptKeys / 16; ++kk)
 #pragma unroll
-                        for (int rest = 0; rest < (F16 ? 2 : 1); ++rest)
-                            pa_mma_ts(tm + O_COL + t * 128u, tm + t * 128u + (F16 ? 16u : 8u) * kk + 8u * rest, vd + slot * (KV_BYTES / 16) + kk * (2048 / 16), pa_idesc(HD, true, false),
+                        for (int rest = 0; rest < (TWO ? 2 : 1); ++rest)
+                            pa_mma_ts(tm + O_COL + t * 128u, tm + t * 128u + (TWO ? 16u : 8u) * kk + 8u * rest, vd + slot * (KV_BYTES / 16) + kk * (2048 / 16), pa_idesc(HD, true, false),
                                       kk > 0 || rest > 0 || j > 0 ? 1u : 0u);
                     umma_commit(&bars.pv_done[t]);
                 }
@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
         __syncwarp();
     } else {
         const int t = warp >> 2, r = tid & (kPaRows - 1), row = block0 + tid, i = min(row, rows - 1) / G, tiles = t ? tiles1 : tiles0;   // r: of the row tile
-        const bool row_ok = row < rows;
+        const bool row_ok = row < rows, f16 = a.dtype == SWLM_KV8_FP16;
         const int limit = visible(part, i, span);   // (rows past the last one attend what it does; they are not stored)
         float factor;
         // ---- q: this thread's row, shifted to fp16 ----------------------------------------------------------------------------------------
@@ -234,12 +234,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
             }
             const bool keeps = p.q16 && split == 0;   // for the launch that adds the weights
             float up;
-            row_shift(F16 ? __half2float(__ushort_as_half((unsigned short)top)) : __uint_as_float(top << 16), up, factor);
+            row_shift(f16 ? __half2float(__ushort_as_half((unsigned short)top)) : __uint_as_float(top << 16), up, factor);
             factor *= a.scale * kLog2e;
 #pragma unroll 4
             for (int d = 0; d < HD; d += 8) {
                 float x[8];
-                widen(*reinterpret_cast<const uint4*>(src + d), F16, x);
+                widen(*reinterpret_cast<const uint4*>(src + d), f16, x);
                 uint4 v;
                 v.x = pack_half(x[0] * up, x[1] * up); v.y = pack_half(x[2] * up, x[3] * up);
                 v.z = pack_half(x[4] * up, x[5] * up); v.w = pack_half(x[6] * up, x[7] * up);
@@ -330,15 +330,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
                 unit[g] = vt[g] * v_inv;
                 folds = folds && unit[g] >= kFoldUnit * kValueUnit;
             }
-            // Probabilities of a half take the place of its own scores (F16), or those of the first half that of its first 32 columns and those of the second that of
+            // Probabilities of a half take the place of its own scores (TWO), or those of the first half that of its first 32 columns and those of the second that of
             // the next 32. `put`: the e-th pair of 16 scores, which all have been read when the first is written
             auto put = [&](unsigned (&out)[16], int e, float x, float y) {
                 out[e] = pack_half(x, y);
-                if (F16) out[8 + e] = pack_rest(x, y, out[e]);
+                if (TWO) out[8 + e] = pack_rest(x, y, out[e]);
             };
             auto keep = [&](const unsigned (&out)[16], int at) {
 #pragma unroll
-                for (int e = 0; e < (F16 ? 16 : 8); ++e) v[F16 ? at + e : at / 2 + e] = out[e];
+                for (int e = 0; e < (TWO ? 16 : 8); ++e) v[TWO ? at + e : at / 2 + e] = out[e];
             };
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
@@ -395,8 +395,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
                         }
                     }
                 }
-                pa_st32(region + half * (F16 ? 64u : 32u), v);
-                if (F16) pa_st32(region + half * 64u + 32u, v + 32);
+                pa_st32(region + half * (TWO ? 64u : 32u), v);
+                if (TWO) pa_st32(region + half * 64u + 32u, v + 32);
             }
             pa_wait_st();
             pa_before();
@@ -425,7 +425,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
 #pragma unroll
                     for (int e = 0; e < 16; e += 4) {
                         const float4 x = make_float4(__uint_as_float(o[e]) * unit, __uint_as_float(o[e + 1]) * unit, __uint_as_float(o[e + 2]) * unit, __uint_as_float(o[e + 3]) * unit);
-                        if (whole) store_out(dst + d + e, x, l_run, F16);
+                        if (whole) store_out(dst + d + e, x, l_run, f16);
                         else *reinterpret_cast<float4*>(p.part_o + at * HD + d + e) = x;
                     }
             }
@@ -599,12 +599,12 @@ template <int HD, int CODE>
 int launch_prompt(const swlm_kv8_cache& c, const swlm_kv8_attend& a, const RowsPlan& p, int* status, cudaStream_t s) {
     const dim3 grid((unsigned)c.batch * c.kv_heads * p.row_tiles * p.splits);
     auto launch = [&](auto kernel) { return launch_k(kernel, grid, dim3(kPromptThreads), prompt_smem<HD>(), s, c, a, p, status); };
-    auto of_type = [&](auto f16) {
-        constexpr bool F16 = decltype(f16)::value;
-        return c.block == 128 ? launch(kv8_prompt_kernel<HD, CODE, 1, F16>) : c.block == 64 ? launch(kv8_prompt_kernel<HD, CODE, 2, F16>) :
-               c.block == 32 ? launch(kv8_prompt_kernel<HD, CODE, 4, F16>) : launch(kv8_prompt_kernel<HD, CODE, 8, F16>);
+    auto with = [&](auto two) {
+        constexpr bool TWO = decltype(two)::value;
+        return c.block == 128 ? launch(kv8_prompt_kernel<HD, CODE, 1, TWO>) : c.block == 64 ? launch(kv8_prompt_kernel<HD, CODE, 2, TWO>) :
+               c.block == 32 ? launch(kv8_prompt_kernel<HD, CODE, 4, TWO>) : launch(kv8_prompt_kernel<HD, CODE, 8, TWO>);
     };
-    const cudaError_t e = a.dtype == SWLM_KV8_FP16 ? of_type(std::true_type()) : of_type(std::false_type());
+    const cudaError_t e = kv8_two_products(a) ? with(std::true_type()) : with(std::false_type());
     return e == cudaSuccess ? SWLM_OK : cuda_fail(e, "kv8 prompt attention launch");
 }
 template <int HD, int CODE>

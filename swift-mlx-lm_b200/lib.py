@@ -122,6 +122,7 @@ class BuffersDesc(C.Structure):
 # What the operators over an 8-bit cache take (include/swlm.h); device pointers as integers, 0 for none.
 KV8_INT8, KV8_E4M3 = 0, 1   # codes
 KV8_BF16, KV8_FP16 = 0, 1   # keys, values, queries and results
+KV8_P_BY_TYPE, KV8_P_ONE, KV8_P_TWO = 0, 1, 2   # fp16 numbers that a probability meets the values as
 
 
 class Kv8Cache(C.Structure):
@@ -143,7 +144,7 @@ class Kv8Attend(C.Structure):
 
     _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_int64), ("out_stride", C.c_int64)] + [
         (f, C.c_void_p) for f in ("lengths", "counts", "starts", "scratch")] + [("scratch_bytes", C.c_uint64), ("scale", C.c_float)] + [
-        (f, C.c_int32) for f in ("dtype", "heads", "n", "rows", "max_len", "accumulate")] + [("refused", C.c_void_p)]
+        (f, C.c_int32) for f in ("dtype", "heads", "n", "rows", "max_len", "accumulate", "probabilities")] + [("refused", C.c_void_p)]
 
 
 class Kv8Evict(C.Structure):

@@ -2,8 +2,8 @@
 import pytest
 import torch
 
-from plain_kv8 import HALF, TOP, Cache, numbers
-from test_gpu_kv8 import do_attend, ints, store  # noqa: F401
+from plain_kv8 import HALF, TOP, Cache, attend, numbers
+from test_gpu_kv8 import attend_call, do_attend, ints, same_bits, store, stream  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -38,3 +38,25 @@ def test_fp16_results_are_rounded_once(pkg, store, heads, dim, n, before, code, 
     tol = (prob + 2.0 ** -22 + (total / 16 + 32) * 2.0 ** -22) * size + total * 2.0 ** -25 * each.max() * TOP[code] / 128
     tol = tol + (want.abs() + tol) * HALF[torch.float16] + 2.0 ** -25
     assert ((out.double() - want).abs() <= tol).all(), ((out.double() - want).abs() / tol).max()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("n,length", [(1, 900), (5, 300), (40, 700)])
+def test_a_caller_chooses_how_probabilities_meet_values(pkg, store, n, length, dtype):  # noqa: F811
+    """By type is two for fp16 and one for bf16, bit for bit; either is within the bounds of one number, and the other differs from it in fp16."""
+    cache = Cache(pkg, 1, 2, 128, 1024, 32, 0).fill([length])
+    q = torch.randn((n, 8, 128), generator=torch.Generator(device="cuda").manual_seed(9), device="cuda").to(dtype)
+    outs, lengths = [], ints(length - n)
+    want, tol, _, _ = attend(cache, q, 0, length - n, 0.09, 1024)
+    for how in (pkg.KV8_P_BY_TYPE, pkg.KV8_P_ONE, pkg.KV8_P_TWO):
+        out = torch.zeros_like(q)
+        step, scratch = attend_call(pkg, store, cache, q, out, lengths, 0.09, n=n)
+        step.probabilities = how
+        store.lib.check(store.lib.swlm_op_kv8_attend_dev(store.handle, cache.described(), step, stream()))
+        torch.cuda.synchronize()
+        assert ((out.double() - want).abs() <= tol).all(), how
+        outs.append(out)
+    assert same_bits(outs[0], outs[2 if dtype == torch.float16 else 1])
+    if dtype == torch.float16:
+        assert not same_bits(outs[1], outs[2])
+        assert (outs[2].double() - want).norm() < (outs[1].double() - want).norm()

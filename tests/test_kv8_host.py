@@ -178,3 +178,10 @@ def test_scratch_is_what_the_kernels_write(pkg, lib, kv_heads, heads, dim, batch
         need += tiles * tile * 8 if batch > 512 else 0   # (the rows' maxima and sums alone, for the launch that adds the weights)
     got = lib.swlm_op_kv8_attend_scratch_bytes(cache, step)
     assert need <= got <= need + 8 * 16
+
+
+@pytest.mark.parametrize("how", [-1, 3])
+def test_unknown_forms_of_the_probabilities(pkg, lib, how):
+    step = _attend(pkg, probabilities=how, accumulate=1, scratch=0, scratch_bytes=0)
+    assert lib.swlm_op_kv8_attend_dev(CTX, _cache(pkg), step, None) == INVALID
+    assert b"probabilities" in lib.swlm_last_error() and lib.swlm_op_kv8_attend_scratch_bytes(_cache(pkg), step) == 0
