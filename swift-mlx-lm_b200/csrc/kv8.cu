@@ -9,8 +9,9 @@
 //          `keep` are written, so that the blocks need no order among them, also in place; the scales of the sources, which the last block
 //          may share with slots that are written, are taken along by the first kernel.
 //
-// What bounds them: append of 6272 tokens (8 heads of 128) 12 us for 39 MB, half of it instructions (18 a value and warp lane, most of the quotient); of one
-// token the launch. Eviction of 4 x 32768 tokens to 4096 (73 MB): 48 us, of which the selection, a chain of passes over shared memory and
+// What bounds them: append of 6272 tokens (8 heads of 128) 11.8 us for 39 MB, 10.1 where no scale of a block with older tokens grows: a CTA's load, search,
+// barrier, quotients and stores one after the other, with 41 % of the warps and 57 to 65 % of the issue slots busy (18 instructions a value and warp
+// lane, most of the quotient); of one token the launch. Eviction of 4 x 32768 tokens to 4096 (73 MB): 48 us, of which the selection, a chain of passes over shared memory and
 // barriers of the cluster, takes half (with the counts of all digits read from every CTA, and a pass over ties that nobody has to tell apart, 56) and
 // the move, mostly instructions, half; 1 x 4352 to 4096: 17.6 us, nearly all of it latency.
 #include <cooperative_groups.h>

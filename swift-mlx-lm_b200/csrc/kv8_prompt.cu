@@ -439,7 +439,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const swl
 // The weights of many rows: weight_j += sum over rows i of exp2(s_ij + shift_i), with the rows' totals known. A CTA has 128 keys, the rows of the products
 // (S^T = K Q^T: a thread per key, so that nothing is added across threads), and walks the row tiles that attend them. The
 // queries of a tile, their factors and shifts come as bulk copies, SLOTS - 1 tiles ahead, while the tiles before are multiplied and summed; scores have two
-// regions. Three CTAs of an SM fill each other's waits (3 x 777 rows, heads of 64, both kernels: 137 us, with two 160; 2048 over 6144, heads of 128: 507 and 524).
+// regions. Three CTAs of an SM fill each other's waits (3 x 777 rows, heads of 64, both kernels, one product of the probabilities: 136 us, with two CTAs 160; 2048
+// over 6144, heads of 128: 507 and 524).
 // With heads of 128 they have room for two slots only, and where there are no three CTAs per SM four are faster (2048 into an empty cache 177 us, with two slots 185).
 constexpr int kWeightKeys = 128, kWeightRows = 64, kWeightSlots = 4, kWeightThreads = kWeightKeys + 32;
 struct WeightBars {

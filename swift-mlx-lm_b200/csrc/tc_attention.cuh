@@ -9,7 +9,7 @@ namespace swlm {
 
 constexpr int kPaRows = 128, kPaKeys = 64;   // rows of a query tile, keys of a key tile
 
-// (descriptors by their low words; `b_hi`: the high word of B's)
+// (descriptors by their low words)
 __device__ __forceinline__ void pa_mma_ss(unsigned d, unsigned a_lo, unsigned b_lo, unsigned idesc, unsigned acc) {
     asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}"
                  ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(kUmmaDescHi), "r"(idesc), "r"(acc) : "memory");
