@@ -302,7 +302,7 @@ def _plain_quantize(x):
     rows, width = x.shape
     wide = torch.nn.functional.pad(x, (0, _blocks(width) * BLOCK - width)).view(rows, -1, BLOCK)
     fraction, exponent = torch.frexp(wide.abs().amax(dim=2))   # 448 = 0.875 * 2^9
-    exponent = (exponent - torch.where(fraction > 0.875, 8, 9)).clamp(min=-126)
+    exponent = torch.where(fraction > 0, exponent - torch.where(fraction > 0.875, 8, 9), -126).clamp(min=-126)
     scale = torch.where(fraction.isfinite(), ((exponent + 127) << 23).int().view(torch.float32), math.nan)
     codes = (wide / scale[:, :, None]).clamp(-TOP, TOP).to(torch.float8_e4m3fn)
     return codes.view(rows, -1)[:, :width], scale.t().contiguous()
@@ -401,7 +401,7 @@ def _double_quantize(x):
     for at in range(0, x.shape[1], BLOCK):
         part = x[:, at:at + BLOCK]
         fraction, exponent = torch.frexp(part.abs().amax(dim=1, keepdim=True) / TOP)
-        s = torch.exp2((exponent - (fraction == 0.5).int()).clamp(min=-126).double())
+        s = torch.exp2(torch.where(fraction > 0, exponent - (fraction == 0.5).int(), -126).clamp(min=-126).double())
         y = part / s
         step = torch.exp2((torch.frexp(y).exponent - 1).clamp(min=-6).double() - 3)
         codes[:, at:at + BLOCK] = (y / step).round() * step
