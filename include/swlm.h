@@ -416,6 +416,105 @@ int swlm_op_kv8_evict_dev(swlm_ctx* ctx, const swlm_kv8_cache* cache, const swlm
 int swlm_op_kv8_lengths_dev(swlm_ctx* ctx, int batch, const int32_t* in, const int32_t* counts, int n, int limit, const int32_t* refused,
                             int32_t* out, void* cuda_stream);
 
+/* ---- a caller's weights held in 8-bit floating point, one scale per block of 128 x 128; rows sorted by expert -----------
+ * No counterpart in the reference. Four operators, which together are a routed feed-forward over such weights:
+ *
+ *   expert sort   the (token, choice) pairs in the order of their experts,
+ *   quantize      rows become e4m3 codes, those of the sorted pairs gathered on the way,
+ *   product       such rows times a matrix of e4m3 codes, or the gated pair of two; with experts every row meets its own expert's,
+ *   expert sum    the experts' rows back at their tokens, weighted and added up.
+ *
+ * A held value is code * scale: rows have a scale per row and 128 columns, matrices one per 128 rows and 128 columns. All calls are enqueued on
+ * `cuda_stream` (NULL = the context's own stream) without synchronising and without allocating, read choices and offsets on the device, and can be
+ * captured into a graph. Pointers are device memory of the context's device. Calls at once may share what they only read; none has scratch. */
+enum { SWLM_F8_BF16 = 0, SWLM_F8_FP16 = 1, SWLM_F8_FP32 = 2, SWLM_F8_E4M3 = 3 };   /* type of rows */
+enum { SWLM_F8_PLAIN = 0, SWLM_F8_SILU = 1, SWLM_F8_GELU = 2, SWLM_F8_CLAMPED = 3 };   /* swlm_f8_product.act */
+
+typedef struct swlm_f8_rows {
+    void* codes;            /* row r at codes + r * stride, 16-byte aligned */
+    float* scale;           /* of row r and columns 128 b ..: scale[b * scale_stride + r] */
+    int64_t stride;         /* bytes, a multiple of 16 */
+    int64_t scale_stride;   /* at least the rows */
+} swlm_f8_rows;
+
+typedef struct swlm_f8_weight {
+    const void* codes;      /* [experts][n] rows of `stride` bytes, 16-byte aligned; entries behind the k-th of a row are not looked at */
+    const float* scale;     /* [experts][ceil(n / 128)][ceil(k / 128)] */
+    int64_t stride;         /* a multiple of 16 */
+} swlm_f8_weight;
+
+/* Row r of the result are the codes of row source[r] of x (NULL: row r; where source[r] is not within 0..x_rows-1 the row stays as it is). The
+ * scale of 128 columns is the smallest power of two that is at least their largest |value| / 448, and not below 2^-126: a code is the e4m3 number nearest to
+ * value / scale, ties to even, and nothing else is rounded. Columns among which is an infinity or a NaN get NaN as scale and codes. */
+typedef struct swlm_f8_quantize {
+    const void* x;          /* row r at x + r * x_stride elements; 16-byte aligned, rows too */
+    int64_t x_stride;
+    const int32_t* source;
+    swlm_f8_rows out;
+    int32_t dtype;          /* of x: SWLM_F8_BF16, _FP16 or _FP32 */
+    int32_t rows, width;    /* of the result; width > 0 */
+    int32_t x_rows;
+} swlm_f8_quantize;
+int swlm_op_f8_quantize_dev(swlm_ctx* ctx, const swlm_f8_quantize* how, void* cuda_stream);
+
+/* y[r][c] = sum over blocks b of 128 columns: x.scale[b][r] * w.scale[c / 128][b] * (codes of row r . codes of w's row c within the block), the sums in
+ * fp32. act other than SWLM_F8_PLAIN: y = act(w x) * (up x), `up` a second matrix of w's shape: SiLU, GELU (tanh) or, as the clamped experts of
+ * SWLM_STEP_ROUTED_MLP have it, g = min(w x, limit), u = clamp(up x, -limit, limit), g * sigmoid(alpha * g) * (u + 1).
+ * dtype SWLM_F8_E4M3: the result is quantized as swlm_op_f8_quantize_dev does, into codes y and scales y_scale.
+ * experts > 0: rows offsets[e] .. offsets[e + 1] - 1 meet matrix e; offsets [experts + 1] ascend, what exceeds `rows` is cut off, and rows of y that no expert
+ * has stay as they are. experts 0: all rows meet the one matrix.
+ * A product of two scales is one fp32 number (2^-126 .. 2^127), as is every partial sum.
+ * Waits on the device are bounded. Once one has expired, results since then are not valid, and the context's swlm_op_f8_product_dev returns
+ * SWLM_ERR_TIMEOUT without doing anything until swlm_op_f8_status has reported it. */
+typedef struct swlm_f8_product {
+    swlm_f8_rows x;
+    swlm_f8_weight w, up;
+    const int32_t* offsets;
+    void* y;                /* row r at y + r * y_stride elements; 16-byte aligned, rows too; not memory that the call reads */
+    int64_t y_stride;
+    float* y_scale;
+    int64_t y_scale_stride;
+    int32_t rows, n, k;     /* n columns of the result */
+    int32_t experts;
+    int32_t dtype;          /* of y */
+    int32_t act;            /* SWLM_F8_PLAIN, _SILU, _GELU or _CLAMPED */
+    float alpha, limit;
+} swlm_f8_product;
+int swlm_op_f8_product_dev(swlm_ctx* ctx, const swlm_f8_product* how, void* cuda_stream);
+/* SWLM_ERR_TIMEOUT where a wait of the context's products has expired since the last call, which it forgets then. It does not wait: call it behind a
+ * synchronisation of the streams in question. The replays of a captured product report nothing themselves, so whoever replays one asks here. */
+int swlm_op_f8_status(swlm_ctx* ctx);
+/* Probe: what an expired wait would leave behind (0: none), for tests of a host's handling of it. */
+int swlm_write_f8_status(swlm_ctx* ctx, int code);
+
+/* Rows for the pairs (t, j) whose choice[t][j] is within 0..experts-1: ascending by expert, and of one expert by t, then j. offsets[e] = first row
+ * of expert e, offsets[experts] = all rows; source[r] = the token t of row r, -1 behind the last row; place[t][j] = its row, -1 for the other
+ * pairs (identity experts, parked sequences). */
+typedef struct swlm_expert_sort {
+    const int32_t* choice;  /* [tokens][top] */
+    int32_t* offsets;       /* [experts + 1] */
+    int32_t* source;        /* [tokens * top] */
+    int32_t* place;         /* [tokens][top] */
+    int32_t tokens, top, experts;   /* experts <= 1024 */
+} swlm_expert_sort;
+int swlm_op_expert_sort_dev(swlm_ctx* ctx, const swlm_expert_sort* how, void* cuda_stream);
+
+/* out[t] = sum over j of weight[t][j] * y[place[t][j]], in fp32 and in the order of j, + add[t] (NULL: nothing). A place that is not within 0..y_rows-1 adds
+ * nothing, whatever its weight. add may be out; out is otherwise not memory that the call reads. */
+typedef struct swlm_expert_sum {
+    const void* y;          /* rows of y_dtype; pointers and rows of y, add and out are 16-byte aligned, strides count elements */
+    int64_t y_stride;
+    const int32_t* place;   /* [tokens][top] */
+    const float* weight;    /* [tokens][top] */
+    const void* add;        /* rows of dtype */
+    int64_t add_stride;
+    void* out;              /* rows of dtype */
+    int64_t out_stride;
+    int32_t tokens, top, width, y_rows;
+    int32_t y_dtype, dtype; /* SWLM_F8_BF16, _FP16 or _FP32 */
+} swlm_expert_sum;
+int swlm_op_expert_sum_dev(swlm_ctx* ctx, const swlm_expert_sum* how, void* cuda_stream);
+
 #ifdef __cplusplus
 }
 #endif

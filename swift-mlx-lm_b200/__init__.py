@@ -9,6 +9,8 @@ and loading fails loudly when the CUDA library has not been built.
 """
 from .lib import Library, SwlmError, build_library, load_library  # noqa: F401
 from .lib import KV8_BF16, KV8_E4M3, KV8_FP16, KV8_INT8, KV8_P_BY_TYPE, KV8_P_ONE, KV8_P_TWO, Kv8Append, Kv8Attend, Kv8Cache, Kv8Evict  # noqa: F401
+from .lib import F8_BF16, F8_CLAMPED, F8_E4M3, F8_FP16, F8_FP32, F8_GELU, F8_PLAIN, F8_SILU, F8Product, F8Quantize, F8Rows, F8Weight  # noqa: F401
+from .lib import ExpertSort, ExpertSum  # noqa: F401
 from .formats import (  # noqa: F401
     AffineQ4Group64Format,
     AffineQ4Group128Format,

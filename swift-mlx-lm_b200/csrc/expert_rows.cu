@@ -1,0 +1,222 @@
+// Rows sorted by expert, and back at their tokens, weighted and added up.
+#include <algorithm>
+
+#include <cooperative_groups.h>
+
+#include "f8.h"
+
+namespace cg = cooperative_groups;
+
+namespace swlm {
+namespace {
+
+// ---- sort --------------------------------------------------------------------------------------------------------------------
+// A stable counting sort by one cluster: every warp has a run of neighbouring pairs and counts its experts; sums over warps and, through distributed
+// shared memory, over the cluster's CTAs give every warp its first row of every expert; then it numbers its pairs, 32 at a time, by those before
+// them of the same expert. No number depends on the order in which warps get there.
+constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortUnroll = 4;
+
+__global__ void __launch_bounds__(kSortThreads) expert_sort_kernel(const swlm_expert_sort a) {
+    extern __shared__ int counts[];        // [kSortWarps][experts]: pairs of each warp, then each warp's next row
+    __shared__ int total[kExpertMax], before[kSortWarps];
+    pdl_wait();
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, E = a.experts;
+    const int pairs = a.tokens * a.top, runs = ctas * kSortWarps, each = (pairs + 32 * runs - 1) / (32 * runs) * 32;   // (at most 2^30 + 2^14)
+    const int first = (int)min((long long)(rank * kSortWarps + warp) * each, (long long)pairs), last = min(first + each, pairs);
+    int* const mine = counts + warp * E;
+    for (int i = tid; i < kSortWarps * E; i += kSortThreads) counts[i] = 0;
+    __syncthreads();
+    for (int i = first + lane; i < last; i += 32 * kSortUnroll) {
+        int e[kSortUnroll];
+#pragma unroll
+        for (int u = 0; u < kSortUnroll; ++u) e[u] = i + 32 * u < last ? a.choice[i + 32 * u] : -1;
+#pragma unroll
+        for (int u = 0; u < kSortUnroll; ++u)
+            if (e[u] >= 0 && e[u] < E) atomicAdd(mine + e[u], 1);
+    }
+    __syncthreads();
+    int sum = 0;   // of expert `tid`
+    if (tid < E) {
+        for (int w = 0; w < kSortWarps; ++w) {   // pairs of the warps before w
+            const int c = counts[w * E + tid];
+            counts[w * E + tid] = sum;
+            sum += c;
+        }
+        total[tid] = sum;
+    }
+    cluster.sync();
+    int all = 0, others = 0;
+    if (tid < E)
+        for (int c = 0; c < ctas; ++c) {
+            const int v = *cluster.map_shared_rank(total + tid, c);
+            others += c < rank ? v : 0;
+            all += v;
+        }
+    int scan = all;   // rows of the experts up to this one
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, scan, o);
+        if (lane >= o) scan += v;
+    }
+    if (lane == 31) before[warp] = scan;
+    __syncthreads();
+    int base = 0, rows = 0;
+    for (int w = 0; w < kSortWarps; ++w) {
+        base += w < warp ? before[w] : 0;
+        rows += before[w];
+    }
+    base += scan - all;
+    if (tid < E) {
+        if (rank == 0) {
+            a.offsets[tid] = base;
+            if (tid == E - 1) a.offsets[E] = rows;
+        }
+        for (int w = 0; w < kSortWarps; ++w) counts[w * E + tid] += base + others;
+    }
+    __syncthreads();
+    for (int i = rows + rank * kSortThreads + tid; i < pairs; i += ctas * kSortThreads) a.source[i] = -1;
+    for (int i0 = first; i0 < last; i0 += 32 * kSortUnroll) {
+        int e[kSortUnroll];
+#pragma unroll
+        for (int u = 0; u < kSortUnroll; ++u) {
+            const int i = i0 + 32 * u + lane;
+            e[u] = i < last ? a.choice[i] : -1;
+            if (e[u] >= E) e[u] = -1;
+        }
+#pragma unroll
+        for (int u = 0; u < kSortUnroll; ++u) {
+            const int i = i0 + 32 * u + lane;
+            const unsigned same = __match_any_sync(0xffffffffu, e[u]);
+            const int next = e[u] >= 0 ? mine[e[u]] : 0;
+            __syncwarp();
+            if (e[u] >= 0 && (same >> lane) == 1u) mine[e[u]] = next + __popc(same);   // (the last of them)
+            __syncwarp();
+            if (i < last) {
+                const int row = e[u] >= 0 ? next + __popc(same & ((1u << lane) - 1u)) : -1;
+                a.place[i] = row;
+                if (row >= 0) a.source[row] = i / a.top;
+            }
+        }
+    }
+    cluster.sync();   // the others have read `total`
+}
+
+// ---- sum ---------------------------------------------------------------------------------------------------------------------
+// A thread has eight columns of a token and runs through the token's rows in their order, up to eight loads on their way at once.
+constexpr int kSumThreads = 256, kSumUnroll = 8;
+
+template <int DTYPE> __device__ __forceinline__ void load8(const void* p, float (&x)[8]) {
+    if (DTYPE == SWLM_F8_FP32) {
+        const float4 a = static_cast<const float4*>(p)[0], b = static_cast<const float4*>(p)[1];
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else {
+        const uint4 v = *static_cast<const uint4*>(p);
+        const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = DTYPE == SWLM_F8_FP16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[i])) : make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+            x[2 * i] = f.x; x[2 * i + 1] = f.y;
+        }
+    }
+}
+template <int DTYPE> __device__ __forceinline__ float load1(const void* p, int i) {
+    if (DTYPE == SWLM_F8_FP32) return static_cast<const float*>(p)[i];
+    return DTYPE == SWLM_F8_FP16 ? __half2float(static_cast<const __half*>(p)[i]) : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+template <int DTYPE> __device__ __forceinline__ void store1(void* p, int i, float v) {
+    if (DTYPE == SWLM_F8_FP32) static_cast<float*>(p)[i] = v;
+    else if (DTYPE == SWLM_F8_FP16) static_cast<__half*>(p)[i] = __float2half_rn(v);
+    else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+template <int DTYPE> __device__ __forceinline__ void store8(void* p, const float (&x)[8]) {
+    if (DTYPE == SWLM_F8_FP32) {
+        static_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+        static_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+        unsigned w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (DTYPE == SWLM_F8_FP16) { const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]); w[i] = *reinterpret_cast<const unsigned*>(&h); }
+            else { const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]); w[i] = *reinterpret_cast<const unsigned*>(&h); }
+        }
+        *static_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+template <int Y, int OUT>
+__global__ void __launch_bounds__(kSumThreads) expert_sum_kernel(const swlm_expert_sum a) {
+    constexpr int YSIZE = Y == SWLM_F8_FP32 ? 4 : 2, SIZE = OUT == SWLM_F8_FP32 ? 4 : 2;
+    pdl_wait();
+    const unsigned chunks = (a.width + 7) / 8;
+    const long long at = (long long)blockIdx.x * kSumThreads + threadIdx.x;
+    const long long t = at / chunks;
+    if (t >= a.tokens) return;
+    const int col = (int)(at - t * chunks) * 8, rest = a.width - col;
+    const int* place = a.place + t * a.top;
+    const float* weight = a.weight + t * a.top;
+    const unsigned char* y = static_cast<const unsigned char*>(a.y) + (long long)col * YSIZE;
+    float sum[8] = {};
+    for (int j0 = 0; j0 < a.top; j0 += kSumUnroll) {
+        float x[kSumUnroll][8], w[kSumUnroll];
+#pragma unroll
+        for (int j = 0; j < kSumUnroll; ++j) {
+            const int row = j0 + j < a.top ? place[j0 + j] : -1;
+            const bool has = row >= 0 && row < a.y_rows;
+            w[j] = has ? weight[j0 + j] : 0.f;
+            const unsigned char* p = y + (long long)row * a.y_stride * YSIZE;
+            if (has && rest >= 8) load8<Y>(p, x[j]);
+            else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[j][e] = has && e < rest ? load1<Y>(p, e) : 0.f;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kSumUnroll; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum[e] = fmaf(w[j], x[j][e], sum[e]);
+    }
+    unsigned char* out = static_cast<unsigned char*>(a.out) + (t * a.out_stride + col) * SIZE;
+    const unsigned char* add = a.add ? static_cast<const unsigned char*>(a.add) + (t * a.add_stride + col) * SIZE : nullptr;
+    if (rest >= 8) {
+        if (add) {
+            float x[8];
+            load8<OUT>(add, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum[e] += x[e];
+        }
+        store8<OUT>(out, sum);
+    } else {
+        for (int e = 0; e < rest; ++e) store1<OUT>(out, e, add ? sum[e] + load1<OUT>(add, e) : sum[e]);
+    }
+}
+
+template <int Y> void (*sum_kernel(int dtype))(swlm_expert_sum) {
+    return dtype == SWLM_F8_FP32 ? expert_sum_kernel<Y, SWLM_F8_FP32> : dtype == SWLM_F8_FP16 ? expert_sum_kernel<Y, SWLM_F8_FP16> : expert_sum_kernel<Y, SWLM_F8_BF16>;
+}
+
+}  // namespace
+
+int expert_rows_init() {
+    SWLM_CUDA(cudaFuncSetAttribute(expert_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortWarps * kExpertMax * 4));
+    return SWLM_OK;
+}
+
+int launch_expert_sort(const swlm_expert_sort& a, cudaStream_t s) {
+    const long long pairs = (long long)a.tokens * a.top;
+    int ctas = 1;
+    while (ctas < 8 && pairs > (long long)ctas * 2 * kSortThreads) ctas *= 2;
+    const cudaError_t e = launch_clusters(expert_sort_kernel, ctas, dim3(ctas), dim3(kSortThreads), (size_t)kSortWarps * a.experts * 4, s, a);
+    return e == cudaSuccess ? SWLM_OK : cuda_fail(e, "expert sort launch");
+}
+
+int launch_expert_sum(const swlm_expert_sum& a, cudaStream_t s) {
+    if (a.tokens == 0) return SWLM_OK;
+    const long long threads = (long long)a.tokens * ((a.width + 7) / 8), ctas = (threads + kSumThreads - 1) / kSumThreads;
+    if (ctas > 0x7FFFFFFFll) { set_error("f8: too many tokens for a width of %d", a.width); return SWLM_ERR_INVALID; }
+    void (*kernel)(swlm_expert_sum) = a.y_dtype == SWLM_F8_FP32 ? sum_kernel<SWLM_F8_FP32>(a.dtype) : a.y_dtype == SWLM_F8_FP16 ? sum_kernel<SWLM_F8_FP16>(a.dtype) : sum_kernel<SWLM_F8_BF16>(a.dtype);
+    const cudaError_t e = launch_k(kernel, dim3((unsigned)ctas), dim3(kSumThreads), 0, s, a);
+    return e == cudaSuccess ? SWLM_OK : cuda_fail(e, "expert sum launch");
+}
+
+}  // namespace swlm

@@ -19,6 +19,7 @@
 
 #include <sys/mman.h>
 
+#include "f8.h"
 #include "kv8.h"
 #include "swlm_runtime.h"
 
@@ -1397,9 +1398,12 @@ int swlm_ctx_create(int device_id, int tp_rank, int tp_size, swlm_ctx** out) {
     if (!rc) rc = grouped_init();
     if (!rc) rc = retention_init();
     if (!rc) rc = kv8_init();
-    if (!rc && (e = cudaHostAlloc((void**)&ctx->kv8_status, sizeof(int), cudaHostAllocMapped)) != cudaSuccess) rc = cuda_fail(e, "status word");
+    if (!rc) rc = f8_product_init();
+    if (!rc) rc = expert_rows_init();
+    if (!rc && (e = cudaHostAlloc((void**)&ctx->kv8_status, 2 * sizeof(int), cudaHostAllocMapped)) != cudaSuccess) rc = cuda_fail(e, "status word");
     if (rc) { cudaStreamDestroy(ctx->stream); delete ctx; return rc; }
-    *ctx->kv8_status = 0;
+    ctx->f8_status = ctx->kv8_status + 1;
+    *ctx->kv8_status = *ctx->f8_status = 0;
     *out = ctx;
     return SWLM_OK;
 }

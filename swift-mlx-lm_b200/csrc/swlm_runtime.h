@@ -155,6 +155,7 @@ struct swlm_ctx {
     unsigned* op_counters = nullptr; size_t op_counter_count = 0;
     int* tc_status = nullptr;  // device word the tcgen05 GEMM sets when one of its bounded waits expired
     int* kv8_status = nullptr; // the same of attention over an 8-bit cache, in host memory: its calls and evictions read it, swlm_op_kv8_status clears it
+    int* f8_status = nullptr;  // the word behind it, of products in 8-bit floating point: they read it, swlm_op_f8_status clears it
     // Lifetime: plans keep their context alive, states their plan. A destroy call on an object that still has
     // users only marks it; the memory goes when the last user is destroyed (hosts with garbage-collected
     // wrappers release objects in no particular order).

@@ -154,6 +154,50 @@ class Kv8Evict(C.Structure):
         (f, C.c_int32) for f in ("keep", "sink", "recent", "max_len")]
 
 
+# What the operators over 8-bit float weights and over rows sorted by expert take (include/swlm.h).
+F8_BF16, F8_FP16, F8_FP32, F8_E4M3 = 0, 1, 2, 3        # type of rows
+F8_PLAIN, F8_SILU, F8_GELU, F8_CLAMPED = 0, 1, 2, 3   # F8Product.act
+
+
+class F8Rows(C.Structure):
+    """Mirror of `swlm_f8_rows`."""
+
+    _fields_ = [("codes", C.c_void_p), ("scale", C.c_void_p), ("stride", C.c_int64), ("scale_stride", C.c_int64)]
+
+
+class F8Weight(C.Structure):
+    """Mirror of `swlm_f8_weight`."""
+
+    _fields_ = [("codes", C.c_void_p), ("scale", C.c_void_p), ("stride", C.c_int64)]
+
+
+class F8Quantize(C.Structure):
+    """Mirror of `swlm_f8_quantize`."""
+
+    _fields_ = [("x", C.c_void_p), ("x_stride", C.c_int64), ("source", C.c_void_p), ("out", F8Rows)] + [
+        (f, C.c_int32) for f in ("dtype", "rows", "width", "x_rows")]
+
+
+class F8Product(C.Structure):
+    """Mirror of `swlm_f8_product`."""
+
+    _fields_ = [("x", F8Rows), ("w", F8Weight), ("up", F8Weight), ("offsets", C.c_void_p), ("y", C.c_void_p), ("y_stride", C.c_int64), ("y_scale", C.c_void_p),
+                ("y_scale_stride", C.c_int64)] + [(f, C.c_int32) for f in ("rows", "n", "k", "experts", "dtype", "act")] + [("alpha", C.c_float), ("limit", C.c_float)]
+
+
+class ExpertSort(C.Structure):
+    """Mirror of `swlm_expert_sort`."""
+
+    _fields_ = [(f, C.c_void_p) for f in ("choice", "offsets", "source", "place")] + [(f, C.c_int32) for f in ("tokens", "top", "experts")]
+
+
+class ExpertSum(C.Structure):
+    """Mirror of `swlm_expert_sum`."""
+
+    _fields_ = [("y", C.c_void_p), ("y_stride", C.c_int64), ("place", C.c_void_p), ("weight", C.c_void_p), ("add", C.c_void_p), ("add_stride", C.c_int64),
+                ("out", C.c_void_p), ("out_stride", C.c_int64)] + [(f, C.c_int32) for f in ("tokens", "top", "width", "y_rows", "y_dtype", "dtype")]
+
+
 # name -> (restype, argtypes); every symbol include/swlm.h declares
 _P = C.c_void_p
 _I = C.c_int
@@ -240,6 +284,12 @@ SIGNATURES = {
     "swlm_op_kv8_evict_scratch_bytes": (C.c_size_t, [C.POINTER(Kv8Cache), C.POINTER(Kv8Evict)]),
     "swlm_op_kv8_evict_dev": (_I, [_P, C.POINTER(Kv8Cache), C.POINTER(Kv8Cache), C.POINTER(Kv8Evict), _P]),
     "swlm_op_kv8_lengths_dev": (_I, [_P, _I, _P, _P, _I, _I, _P, _P, _P]),
+    "swlm_op_f8_quantize_dev": (_I, [_P, C.POINTER(F8Quantize), _P]),
+    "swlm_op_f8_product_dev": (_I, [_P, C.POINTER(F8Product), _P]),
+    "swlm_op_f8_status": (_I, [_P]),
+    "swlm_write_f8_status": (_I, [_P, _I]),
+    "swlm_op_expert_sort_dev": (_I, [_P, C.POINTER(ExpertSort), _P]),
+    "swlm_op_expert_sum_dev": (_I, [_P, C.POINTER(ExpertSum), _P]),
 }
 
 
