@@ -20,8 +20,8 @@ int launch_f8_product(const swlm_f8_product& a, int* status, cudaStream_t s);
 int launch_expert_sort(const swlm_expert_sort& a, cudaStream_t s);
 int launch_expert_sum(const swlm_expert_sum& a, cudaStream_t s);
 
-inline int f8_blocks(int width) { return (width + kF8Block - 1) / kF8Block; }
-inline int f8_size(int dtype) { return dtype == SWLM_F8_FP32 ? 4 : dtype == SWLM_F8_E4M3 ? 1 : 2; }
+__host__ __device__ inline int f8_blocks(int width) { return (width + kF8Block - 1) / kF8Block; }
+__host__ __device__ inline int f8_size(int dtype) { return dtype == SWLM_F8_FP32 ? 4 : dtype == SWLM_F8_E4M3 ? 1 : 2; }
 
 #ifdef __CUDACC__
 // A block's scale from the bits of its largest |value|, m 2^e: the smallest power of two that is at least m 2^e / (1.75 * 2^8), so 2^(e - 8) while

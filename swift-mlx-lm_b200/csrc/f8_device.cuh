@@ -1,0 +1,88 @@
+// Device code shared by the products in 8-bit floating point.
+#pragma once
+
+#include "f8.h"
+#include "tc_device.cuh"
+
+namespace swlm {
+namespace f8 {
+
+constexpr int kSms = 148;
+
+// kind::f8f6f4: D fp32, A = B = e4m3, both K-major; 32 columns of K each
+__host__ __device__ constexpr unsigned idesc(int m, int n) { return (1u << 4) | ((unsigned)(n >> 3) << 17) | ((unsigned)(m >> 4) << 24); }
+// (descriptors by their low words)
+template <int CG>
+__device__ __forceinline__ void umma(unsigned d_tmem, unsigned a_lo, unsigned b_lo, unsigned desc, unsigned accumulate) {
+    if (CG == 1)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+            "setp.ne.b32 p, %5, 0;\n\t"
+            "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %4, p;\n\t}"
+            ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(kUmmaDescHi), "r"(desc), "r"(accumulate) : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+            "setp.ne.b32 p, %5, 0;\n\t"
+            "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+            "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a, b, %4, p;\n\t}"
+            ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(kUmmaDescHi), "r"(desc), "r"(accumulate) : "memory");
+}
+// arrival at a barrier (of both CTAs of the pair) when the MMAs issued so far are done
+template <int CG>
+__device__ __forceinline__ void commit(unsigned long long* bar) {
+    if (CG == 1) umma_commit(bar);
+    else asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((unsigned short)3) : "memory");
+}
+__device__ __forceinline__ unsigned cluster_place(unsigned addr, int rank) {   // the same shared-memory place in another CTA of the cluster
+    unsigned r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void arrive(unsigned bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void arrive_cluster(unsigned bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+
+// 32 columns of a warp's 32 lanes of tensor memory; they are there behind landed(). Both are volatile, as is the use in add_scaled: they stay in their order.
+__device__ __forceinline__ void tmem_load(unsigned (&v)[32], unsigned at) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(at) : "memory");
+}
+__device__ __forceinline__ void landed() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Two fp32 numbers as one register pair, and acc += (a, b) * s.
+__device__ __forceinline__ unsigned long long pair_of(float a, float b) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 of_pair(unsigned long long v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ void add_scaled(unsigned long long& acc, unsigned a, unsigned b, unsigned long long s) {
+    asm volatile("{\n\t.reg .b64 x;\n\tmov.b64 x, {%1, %2};\n\tfma.rn.f32x2 %0, x, %3, %0;\n\t}" : "+l"(acc) : "r"(a), "r"(b), "l"(s));
+}
+__device__ __forceinline__ unsigned pack2(float a, float b, bool f16) {
+    if (f16) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const unsigned*>(&h); }
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const unsigned*>(&h);
+}
+// f8_gated without a branch between values: their exponentials overlap
+__device__ __forceinline__ float gated(float g, float u, int act, float alpha, float limit) {
+    const bool clamped = act == SWLM_F8_CLAMPED;
+    if (clamped) {
+        g = g > limit ? limit : g;
+        u = (u > limit ? limit : u < -limit ? -limit : u) + 1.0f;
+    }
+    const float z = act == SWLM_F8_GELU ? 1.5957691216f * (g + 0.044715f * g * g * g) : clamped ? alpha * g : g;
+    return 0.25f * g * four_over(1.0f + expf(-z)) * u;
+}
+
+}  // namespace f8
+}  // namespace swlm

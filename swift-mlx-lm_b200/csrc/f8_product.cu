@@ -1,99 +1,441 @@
-// Products of rows and matrices in 8-bit floating point.
+// Products of rows and matrices in 8-bit floating point: y = sum over blocks of 128 columns of sx sw (x . w), on tcgen05.
+//
+// The products of a block's codes are exact and summed in fp32 in tensor memory; two scales belong to every block, so its sums leave tensor memory before the
+// next block's are added: registers hold acc += (sx sw) sums, in fp32. A block is 128 bytes of a row, one swizzle row and four MMAs of K = 32.
 #include <algorithm>
 
-#include <cuda_fp8.h>
+#include <cooperative_groups.h>
 
-#include "f8.h"
+#include "f8_device.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace swlm {
+using namespace f8;
 namespace {
 
-constexpr int kTileRows = 32, kTileCols = 128, kThreads = 256, kStep = 32;
+// ---- many rows ---------------------------------------------------------------------------------------------------------------
+// Persistent CTAs, alone (CG = 1) or in pairs (2) that share a tile of 128 CG rows x 256 columns of accumulators: lanes of tensor memory are rows of
+// x, a thread has one row and 128 of the columns. A warp for the copies, one for the MMAs, eight that take a block's sums out of one of two buffers of
+// tensor memory while the next block's are multiplied into the other. GATED: the accumulators of 64 columns of w lie before those of the same 64
+// of `up`, so that a thread has both, and a tile gives 128 columns of the result.
+// Registers are dealt out anew after the start: 128 threads x 56 for the first four warps, two of which have nothing to do, 256 x 224 for the takers' 128 sums
+// and the 64 that are on their way, together the 384 x 168 of the launch.
+constexpr int kWideWarps = 12, kWideThreads = kWideWarps * 32, kWideTakers = 8;
+constexpr int kAccCols = 256, kCodesBytes = kF8Block * kF8Block;   // 128 rows of a block
+constexpr int kScaleDepth = 4;      // blocks whose scales are on their way, and that have room for theirs in shared memory
+constexpr int kStageRow = 80, kPassBytes = 64;   // results on their way out: 64 bytes of each of a warp's 32 rows (the odd pitch keeps 16-byte accesses off each other's banks)
 
-__device__ __forceinline__ float code_value(unsigned char c) {
-    __nv_fp8_e4m3 v;
-    v.__x = c;
-    return (float)v;
+struct WideParams {
+    const float *x_scale, *w_scale, *up_scale;
+    long long x_scale_stride, y_stride, y_scale_stride;
+    unsigned char* y;
+    float* y_scale;
+    const int* offsets;
+    int* status;
+    int rows, n, blocks, experts;       // blocks of K
+    int col_blocks, col_tiles;          // of n: scales of a matrix, tiles
+    int dtype, act;
+    float alpha, limit;
+};
+
+template <int CG> __host__ __device__ constexpr int wide_stages() { return CG == 1 ? 4 : 6; }
+template <int CG> __host__ __device__ constexpr int wide_stage_bytes() { return kCodesBytes + kAccCols / CG * kF8Block; }
+template <int CG> __host__ __device__ constexpr size_t wide_smem() {
+    return 1024 + (size_t)wide_stages<CG>() * wide_stage_bytes<CG>() + kWideTakers * 32 * kStageRow + kScaleDepth * 128 * 8 + 2 * 128 * 4 + (kExpertMax + 1) * 4;
+}
+static_assert(wide_smem<1>() <= 232448 && wide_smem<2>() <= 232448, "shared memory");
+
+struct WideTile { int expert, row0, end, col; };   // rows row0 .. end - 1 (of which a tile has 128 CG at most), tile of columns
+
+// Tiles of the experts before each (experts 0: all rows are one expert's), then tile `t`.
+template <int CG>
+__device__ __forceinline__ WideTile wide_tile(const WideParams& p, const int* first_tile, int t) {
+    constexpr int ROWS = 128 * CG;
+    WideTile w{0, 0, p.rows, 0};
+    if (p.experts) {
+        int lo = 0, hi = p.experts - 1;   // the last expert whose tiles start at or before t
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (first_tile[mid] <= t) lo = mid; else hi = mid - 1;
+        }
+        w.expert = lo;
+        w.row0 = min(max(p.offsets[lo], 0), p.rows);
+        w.end = min(max(p.offsets[lo + 1], w.row0), p.rows);
+        t -= first_tile[lo];
+    }
+    // the shorter side first: what it sweeps stays in L2
+    const int row_tiles = (w.end - w.row0 + ROWS - 1) / ROWS;
+    int r;
+    if (row_tiles <= p.col_tiles) { r = t % row_tiles; w.col = t / row_tiles; }
+    else { w.col = t % p.col_tiles; r = t / p.col_tiles; }
+    w.row0 += r * ROWS;
+    return w;
 }
 
-// A CTA has 128 columns of the result (a block of its scales) of 32 rows at a time, of one expert; a thread 4 rows x 4 columns.
-template <bool GATED>
-__global__ void __launch_bounds__(kThreads) f8_product_kernel(const swlm_f8_product a) {
-    __shared__ float xs[kTileRows][kStep + 1], ws[GATED ? 2 : 1][kTileCols][kStep + 1];
-    pdl_wait();
-    const int expert = blockIdx.z, tid = threadIdx.x, tx = tid & 31, ty = tid >> 5, col0 = blockIdx.x * kTileCols, kb = (a.k + 127) / 128, nb = (a.n + 127) / 128;
-    int from = 0, to = a.rows;
-    if (a.experts) { from = min(max(a.offsets[expert], 0), a.rows); to = min(max(a.offsets[expert + 1], from), a.rows); }
-    for (int row0 = from + (int)blockIdx.y * kTileRows; row0 < to; row0 += gridDim.y * kTileRows) {
-        float acc[GATED ? 2 : 1][4][4] = {};
-        for (int b = 0; b < kb; ++b) {
-            float part[GATED ? 2 : 1][4][4] = {};
-            for (int k0 = b * 128; k0 < min(b * 128 + 128, a.k); k0 += kStep) {
-                for (int i = tid; i < kTileRows * kStep; i += kThreads) {
-                    const int r = row0 + i / kStep, k = k0 + i % kStep;
-                    xs[i / kStep][i % kStep] = r < to && k < a.k ? code_value(static_cast<const unsigned char*>(a.x.codes)[(long long)r * a.x.stride + k]) : 0.f;
-                }
-                for (int g = 0; g < (GATED ? 2 : 1); ++g) {
-                    const swlm_f8_weight& w = g ? a.up : a.w;
-                    for (int i = tid; i < kTileCols * kStep; i += kThreads) {
-                        const int c = col0 + i / kStep, k = k0 + i % kStep;
-                        ws[g][i / kStep][i % kStep] = c < a.n && k < a.k ? code_value(static_cast<const unsigned char*>(w.codes)[((long long)expert * a.n + c) * w.stride + k]) : 0.f;
-                    }
-                }
-                __syncthreads();
-                for (int k = 0; k < kStep; ++k)
-                    for (int g = 0; g < (GATED ? 2 : 1); ++g)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) part[g][i][j] = fmaf(xs[ty * 4 + i][k], ws[g][tx + 32 * j][k], part[g][i][j]);
-                __syncthreads();
-            }
-            for (int g = 0; g < (GATED ? 2 : 1); ++g) {
-                const float sw = (g ? a.up : a.w).scale[((long long)expert * nb + blockIdx.x) * kb + b];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int r = row0 + ty * 4 + i;
-                    const float s = r < to ? a.x.scale[(long long)b * a.x.scale_stride + r] * sw : 0.f;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[g][i][j] = fmaf(part[g][i][j], s, acc[g][i][j]);
-                }
-            }
-        }
-        for (int i = 0; i < 4; ++i) {
-            const int r = row0 + ty * 4 + i;
-            float v[4];
-            unsigned top = 0;
-            for (int j = 0; j < 4; ++j) {
-                v[j] = GATED ? f8_gated(acc[0][i][j], acc[GATED ? 1 : 0][i][j], a.act, a.alpha, a.limit) : acc[0][i][j];
-                if (col0 + tx + 32 * j < a.n) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
-            }
-            const F8Scale s(__reduce_max_sync(0xffffffffu, top));
-            if (r >= to) continue;
-            for (int j = 0; j < 4; ++j) {
-                const int c = col0 + tx + 32 * j;
-                if (c >= a.n) continue;
-                const long long at = (long long)r * a.y_stride + c;
-                if (a.dtype == SWLM_F8_FP32) static_cast<float*>(a.y)[at] = v[j];
-                else if (a.dtype == SWLM_F8_FP16) static_cast<__half*>(a.y)[at] = __float2half_rn(v[j]);
-                else if (a.dtype == SWLM_F8_BF16) static_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16_rn(v[j]);
-                else static_cast<unsigned char*>(a.y)[at] = (unsigned char)f8_codes4(v[j] * s.inverse, 0.f, 0.f, 0.f);
-            }
-            if (a.dtype == SWLM_F8_E4M3 && tx == 0) a.y_scale[blockIdx.x * a.y_scale_stride + r] = s.scale;
+template <int CG, bool GATED>
+__global__ void __launch_bounds__(kWideThreads, 1) f8_wide_kernel(const WideParams p, const __grid_constant__ CUtensorMap xmap,
+                                                                  const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap upmap) {
+    constexpr int STAGES = wide_stages<CG>(), STAGE = wide_stage_bytes<CG>(), ROWS = 128 * CG, COLS = GATED ? 128 : 256;
+    extern __shared__ __align__(1024) unsigned char wide_raw[];
+    unsigned char* const ring = wide_raw + ((1024 - (smem_u32(wide_raw) & 1023)) & 1023);   // swizzle atoms
+    unsigned char* const staging = ring + STAGES * STAGE;
+    float2* const scales = reinterpret_cast<float2*>(staging + kWideTakers * 32 * kStageRow);   // [kScaleDepth][128]
+    unsigned* const tops = reinterpret_cast<unsigned*>(scales + kScaleDepth * 128);             // [2][128]
+    int* const first_tile = reinterpret_cast<int*>(tops + 256);                                // [experts + 1]
+    __shared__ __align__(8) unsigned long long full[STAGES], empty[STAGES], sums_full[2], sums_empty[2];
+    __shared__ unsigned tmem_base;
+    __shared__ int warp_tiles[kWideWarps];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = CG == 2 ? (int)(blockIdx.x & 1) : 0;
+    if (tid == 0) {
+        for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&sums_full[i], 1 + 2); mbar_init(&sums_empty[i], CG * kWideTakers); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        if (CG == 1) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(2 * kAccCols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(2 * kAccCols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
         }
     }
+    pdl_wait();
+    int tiles = (p.rows + ROWS - 1) / ROWS * p.col_tiles;
+    if (p.experts) {
+        constexpr int PER = (kExpertMax + kWideThreads - 1) / kWideThreads;
+        int c[PER], sum = 0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int e = tid * PER + j;
+            c[j] = 0;
+            if (e < p.experts) {
+                const int from = min(max(p.offsets[e], 0), p.rows), to = min(max(p.offsets[e + 1], from), p.rows);
+                c[j] = (to - from + ROWS - 1) / ROWS * p.col_tiles;
+            }
+            sum += c[j];
+        }
+        int scan = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, scan, o);
+            if (lane >= o) scan += v;
+        }
+        if (lane == 31) warp_tiles[warp] = scan;
+        __syncthreads();
+        tiles = 0;
+        for (int w = 0; w < kWideWarps; ++w) { scan += w < warp ? warp_tiles[w] : 0; tiles += warp_tiles[w]; }
+        scan -= sum;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int e = tid * PER + j;
+            if (e < p.experts) first_tile[e] = scan;
+            scan += c[j];
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (CG == 2) cg::this_cluster().sync();   // both CTAs' barriers are ready
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const unsigned tmem = tmem_base;
+    const int first = (int)blockIdx.x / CG, step = (int)gridDim.x / CG;
+    if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0) {
+        // The warp runs its loop as a whole, one lane issues. Of a pair both CTAs' copies count on the barrier of the one that issues the MMAs.
+        const bool el = elect_one();
+        const unsigned full0 = CG == 1 ? smem_u32(&full[0]) : cluster_place(smem_u32(&full[0]), 0), at = smem_u32(ring);
+        auto load = [&](unsigned dst, const CUtensorMap* map, int col, int row, int s) {
+            if (CG == 1) tma_load_2d(dst, map, col, row, full0 + 8u * s);
+            else tma_load_2d_pair(dst, map, col, row, full0 + 8u * s);
+        };
+        int s = 0, issued = 0;
+        unsigned par = 1;
+        bool ok = true;
+        for (int t = first; t < tiles && ok; t += step) {
+            const WideTile tile = wide_tile<CG>(p, first_tile, t);
+            const int x_row = tile.row0 + rank * 128, w_row = tile.expert * p.n + tile.col * COLS + rank * (COLS / 2);
+            for (int b = 0; b < p.blocks; ++b) {
+                if (!mbar_wait_warp(&empty[s], par)) { ok = false; break; }
+                if (el) {
+                    const unsigned dst = at + s * STAGE;
+                    if (rank == 0) mbar_expect(full0 + 8u * s, (unsigned)(CG * STAGE));
+                    load(dst, &xmap, b * kF8Block, x_row, s);
+                    if (GATED) {
+#pragma unroll
+                        for (int i = 0; i < 2 / CG; ++i) {
+                            load(dst + kCodesBytes * (1 + i), &wmap, b * kF8Block, w_row + 64 * i, s);
+                            load(dst + kCodesBytes * (1 + i) + kCodesBytes / 2, &upmap, b * kF8Block, w_row + 64 * i, s);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 2 / CG; ++i) load(dst + kCodesBytes * (1 + i), &wmap, b * kF8Block, w_row + 128 * i, s);
+                    }
+                }
+                __syncwarp();
+                ++issued;
+                if (++s == STAGES) { s = 0; par ^= 1u; }
+            }
+        }
+        if (!ok) {   // copies already requested still write shared memory (in a pair's second CTA, whose barrier this is not, the limit of the wait is the time they get)
+            if (el) atomicExch_system(p.status, 11);
+            for (int i = max(issued - STAGES, 0); i < issued; ++i) mbar_wait_warp(&full[i % STAGES], (unsigned)((i / STAGES) & 1));
+        }
+    } else if (warp == 1) {
+        if (rank == 0) {
+            constexpr unsigned desc = idesc(128 * CG, kAccCols);
+            const bool el = elect_one();
+            int s = 0, it = 0;
+            unsigned par = 0;
+            bool ok = true;
+            for (int t = first; t < tiles && ok; t += step)
+                for (int b = 0; b < p.blocks; ++b, ++it) {
+                    const unsigned empty_par = (unsigned)(~(it >> 1) & 1);
+                    // (what the barriers guard is read by the tensor cores: no ordinary load has to see another CTA's stores)
+                    ok = mbar_wait_warp(&sums_empty[it & 1], empty_par) && mbar_wait_warp(&full[s], par);
+                    if (!ok) { if (el) atomicExch_system(p.status, 12); break; }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (el) {
+                        const unsigned a = umma_desc_lo(smem_u32(ring + s * STAGE)), w = a + kCodesBytes / 16;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) umma<CG>(tmem + (it & 1) * kAccCols, a + 2 * j, w + 2 * j, desc, j > 0);
+                        commit<CG>(&empty[s]);
+                        commit<CG>(&sums_full[it & 1]);
+                    }
+                    __syncwarp();
+                    if (++s == STAGES) { s = 0; par ^= 1u; }
+                }
+        }
+    } else {
+        // Two warps for the scales, 64 rows each: what the accumulators of a row are worth, as two factors (of the two halves of the columns, or of w's
+        // and up's), is in shared memory before the sums are said to be there. A slot is free again by then: the takers have left block
+        // it - 4 before block it - 2 was multiplied.
+        const int r0 = (warp - 2) * 64 + 2 * lane;
+        struct Ahead { float x[2], w[2]; } ahead[kScaleDepth];
+        WideTile tile{};
+        int t = first, b = 0;      // the block that is asked for next
+        bool any = t < tiles;
+        if (any) tile = wide_tile<CG>(p, first_tile, t);
+        auto ask = [&](Ahead& a) {
+            if (!any) return;
+            const int row = tile.row0 + rank * 128 + r0, block = GATED ? tile.col : 2 * tile.col;
+            const float* x = p.x_scale + b * p.x_scale_stride + row;
+            const long long at = ((long long)tile.expert * p.col_blocks + block) * p.blocks + b;
+            a.x[0] = row < tile.end ? __ldg(x) : 0.f;
+            a.x[1] = row + 1 < tile.end ? __ldg(x + 1) : 0.f;
+            a.w[0] = __ldg(p.w_scale + at);
+            a.w[1] = GATED ? __ldg(p.up_scale + at) : block + 1 < p.col_blocks ? __ldg(p.w_scale + at + p.blocks) : 0.f;
+            if (++b == p.blocks) {
+                b = 0; t += step;
+                any = t < tiles;
+                if (any) tile = wide_tile<CG>(p, first_tile, t);
+            }
+        };
+        const int total = first < tiles ? (tiles - 1 - first) / step + 1 : 0;
+        const long long all = (long long)total * p.blocks;
+#pragma unroll
+        for (int u = 0; u < kScaleDepth; ++u) ask(ahead[u]);
+        bool ok = true;
+        for (long long it0 = 0; it0 < all && ok; it0 += kScaleDepth) {
+#pragma unroll
+            for (int u = 0; u < kScaleDepth; ++u) {
+                const long long it = it0 + u;
+                if (it >= all || !ok) break;
+                if (it >= 2) ok = mbar_wait_warp(&sums_full[u & 1], (unsigned)(((it >> 1) - 1) & 1));
+                if (!ok) { if (lane == 0) atomicExch_system(p.status, 14); break; }
+                const Ahead now = ahead[u];
+                *reinterpret_cast<float4*>(scales + u * 128 + r0) = make_float4(now.x[0] * now.w[0], now.x[0] * now.w[1], now.x[1] * now.w[0], now.x[1] * now.w[1]);
+                __syncwarp();
+                if (lane == 0) arrive(smem_u32(&sums_full[u & 1]));
+                ask(ahead[u]);
+            }
+        }
+    }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        // A warp has the 32 lanes of its quarter (warp & 3) and one half of the columns.
+        const int taker = warp - 4, quarter = warp & 3, half = taker >> 2;
+        const unsigned at = tmem + ((unsigned)(quarter * 32) << 16) + 128u * half;
+        const unsigned given[2] = {CG == 1 ? smem_u32(&sums_empty[0]) : cluster_place(smem_u32(&sums_empty[0]), 0), CG == 1 ? smem_u32(&sums_empty[1]) : cluster_place(smem_u32(&sums_empty[1]), 0)};
+        unsigned char* const out = staging + taker * 32 * kStageRow;
+        int it = 0;
+        bool ok = true;
+        for (int t = first; t < tiles && ok; t += step) {
+            unsigned long long acc[64];
+#pragma unroll
+            for (int i = 0; i < 64; ++i) acc[i] = 0;
+            for (int b = 0; b < p.blocks; ++b, ++it) {
+                ok = mbar_wait_warp(&sums_full[it & 1], (unsigned)((it >> 1) & 1));
+                if (!ok) { if (lane == 0) atomicExch_system(p.status, 13); break; }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                unsigned v[2][32];
+                const unsigned from = at + (it & 1) * kAccCols;
+                tmem_load(v[0], from);
+                const float2 factor = scales[(it & (kScaleDepth - 1)) * 128 + quarter * 32 + lane];
+                const float sl = GATED || !half ? factor.x : factor.y, sh = GATED || half ? factor.y : factor.x;
+                const unsigned long long low = pair_of(sl, sl), high = pair_of(sh, sh);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    landed();
+                    if (c < 3) tmem_load(v[(c + 1) & 1], from + 32 * (c + 1));
+                    else {   // all of them are in registers: the buffer is free
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) { if (CG == 1) arrive(given[it & 1]); else arrive_cluster(given[it & 1]); }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) add_scaled(acc[16 * c + i], v[c & 1][2 * i], v[c & 1][2 * i + 1], c < 2 ? low : high);
+                }
+            }
+            if (!ok) break;
+            const WideTile done = wide_tile<CG>(p, first_tile, t);
+            // ---- results: value i of the thread is column col0 + i of its row ----
+            constexpr int VALUES = GATED ? 64 : 128;
+            float value[VALUES];
+#pragma unroll
+            for (int i = 0; i < VALUES; i += 2) {
+                const float2 g = of_pair(acc[i / 2]);
+                value[i] = g.x; value[i + 1] = g.y;
+                if (GATED) {
+                    const float2 u = of_pair(acc[32 + i / 2]);
+                    value[i] = gated(g.x, u.x, p.act, p.alpha, p.limit);
+                    value[i + 1] = gated(g.y, u.y, p.act, p.alpha, p.limit);
+                }
+            }
+            const int row0 = done.row0 + rank * 128 + quarter * 32, col0 = done.col * COLS + half * VALUES, size = f8_size(p.dtype);
+            if (p.dtype == SWLM_F8_E4M3) {
+                unsigned top = 0;
+#pragma unroll
+                for (int i = 0; i < VALUES; ++i) top = max(top, col0 + i < p.n ? __float_as_uint(value[i]) & 0x7FFFFFFFu : 0u);
+                if (GATED) {   // the other half of the block's columns is another warp's
+                    tops[half * 128 + quarter * 32 + lane] = top;
+                    asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
+                    top = max(top, tops[(half ^ 1) * 128 + quarter * 32 + lane]);
+                    asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
+                }
+                const F8Scale s(top);
+                if (row0 + lane < done.end && col0 < p.n && !(GATED && half)) p.y_scale[(long long)(col0 / kF8Block) * p.y_scale_stride + row0 + lane] = s.scale;
+#pragma unroll
+                for (int i = 0; i < VALUES; ++i) value[i] *= s.inverse;
+            }
+            auto send = [&](int col) {   // 64 bytes of each row, from column `col` on, are in the staging rows
+                __syncwarp();
+                const int per = 16 / size, c = col + (lane & 3) * per, rest = p.n - c;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = (lane >> 2) + 8 * i;
+                    const unsigned char* src = out + r * kStageRow + (lane & 3) * 16;
+                    if (row0 + r < done.end && rest > 0) {
+                        unsigned char* dst = p.y + ((long long)(row0 + r) * p.y_stride + c) * size;
+                        if (rest >= per) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
+                        else if (size == 1) { for (int e = 0; e < rest; ++e) dst[e] = src[e]; }
+                        else if (size == 2) { for (int e = 0; e < rest; ++e) reinterpret_cast<unsigned short*>(dst)[e] = reinterpret_cast<const unsigned short*>(src)[e]; }
+                        else { for (int e = 0; e < rest; ++e) reinterpret_cast<unsigned*>(dst)[e] = reinterpret_cast<const unsigned*>(src)[e]; }
+                    }
+                }
+                __syncwarp();
+            };
+            uint4* const put = reinterpret_cast<uint4*>(out + lane * kStageRow);
+            if (p.dtype == SWLM_F8_FP32) {
+#pragma unroll
+                for (int c = 0; c < VALUES; c += 16) {
+                    if (col0 + c >= p.n) break;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) put[i] = make_uint4(__float_as_uint(value[c + 4 * i]), __float_as_uint(value[c + 4 * i + 1]), __float_as_uint(value[c + 4 * i + 2]), __float_as_uint(value[c + 4 * i + 3]));
+                    send(col0 + c);
+                }
+            } else if (p.dtype == SWLM_F8_E4M3) {
+#pragma unroll
+                for (int c = 0; c < VALUES; c += 64) {
+                    if (col0 + c >= p.n) break;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float* f = value + c + 16 * i;
+                        put[i] = make_uint4(f8_codes4(f[0], f[1], f[2], f[3]), f8_codes4(f[4], f[5], f[6], f[7]), f8_codes4(f[8], f[9], f[10], f[11]), f8_codes4(f[12], f[13], f[14], f[15]));
+                    }
+                    send(col0 + c);
+                }
+            } else {
+                const bool f16 = p.dtype == SWLM_F8_FP16;
+#pragma unroll
+                for (int c = 0; c < VALUES; c += 32) {
+                    if (col0 + c >= p.n) break;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float* f = value + c + 8 * i;
+                        put[i] = make_uint4(pack2(f[0], f[1], f16), pack2(f[2], f[3], f16), pack2(f[4], f[5], f16), pack2(f[6], f[7], f16));
+                    }
+                    send(col0 + c);
+                }
+            }
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (CG == 2) cg::this_cluster().sync();   // no MMA of the pair reads tensor memory or arrives at a barrier of a CTA that has left
+    if (warp == 1) {
+        if (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * kAccCols) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * kAccCols) : "memory");
+    }
+}
+
+// ---- launches ----------------------------------------------------------------------------------------------------------------
+// Rows of bytes as a 2-D tensor, k columns valid (beyond: zeros); box = 128 columns x box_rows, 128-byte swizzle
+int code_map(const void* p, int64_t stride, int64_t rows, int k, int box_rows, CUtensorMap* map) {
+    TensorMapEncodeFn fn = tensor_map_encode_fn();
+    if (!fn) { set_error("f8: cuTensorMapEncodeTiled is not available"); return SWLM_ERR_CUDA; }
+    const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)stride};
+    const cuuint32_t box[2] = {(cuuint32_t)kF8Block, (cuuint32_t)box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) { set_error("f8: cuTensorMapEncodeTiled failed (%d)", (int)r); return SWLM_ERR_CUDA; }
+    return SWLM_OK;
+}
+
+template <int CG, bool GATED>
+int wide_attr() {
+    SWLM_CUDA(cudaFuncSetAttribute(f8_wide_kernel<CG, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)wide_smem<CG>()));
+    return SWLM_OK;
+}
+
+template <int CG, bool GATED>
+int wide_launch(const swlm_f8_product& a, int* status, cudaStream_t s) {
+    constexpr int COLS = GATED ? 128 : 256;
+    WideParams p{};
+    p.x_scale = a.x.scale; p.x_scale_stride = a.x.scale_stride; p.w_scale = a.w.scale; p.up_scale = a.up.scale;
+    p.y = static_cast<unsigned char*>(a.y); p.y_stride = a.y_stride; p.y_scale = a.y_scale; p.y_scale_stride = a.y_scale_stride;
+    p.offsets = a.offsets; p.status = status; p.rows = a.rows; p.n = a.n; p.blocks = f8_blocks(a.k); p.experts = a.experts;
+    p.col_blocks = f8_blocks(a.n); p.col_tiles = (a.n + COLS - 1) / COLS; p.dtype = a.dtype; p.act = a.act; p.alpha = a.alpha; p.limit = a.limit;
+    const int64_t matrix_rows = (int64_t)std::max(a.experts, 1) * a.n;
+    CUtensorMap xmap, wmap, upmap;
+    int rc = code_map(a.x.codes, a.x.stride, a.rows, a.k, 128, &xmap);
+    if (!rc) rc = code_map(a.w.codes, a.w.stride, matrix_rows, a.k, GATED ? 64 : 128, &wmap);
+    upmap = wmap;
+    if (!rc && GATED) rc = code_map(a.up.codes, a.up.stride, matrix_rows, a.k, 64, &upmap);
+    if (rc) return rc;
+    // (at most this many tiles: an expert's last one may have a single row)
+    const int64_t tiles = std::min<int64_t>(((int64_t)a.rows / (128 * CG) + std::max(a.experts, 1)) * p.col_tiles, kSms / CG);
+    const cudaError_t e = launch_clusters(f8_wide_kernel<CG, GATED>, CG, dim3((unsigned)(CG * tiles)), dim3(kWideThreads), wide_smem<CG>(), s, p, xmap, wmap, upmap);
+    return e == cudaSuccess ? SWLM_OK : cuda_fail(e, "product launch");
 }
 
 }  // namespace
 
-int f8_product_init() { return SWLM_OK; }
+int f8_product_init() {
+    int rc;
+    if ((rc = wide_attr<1, false>()) || (rc = wide_attr<1, true>()) || (rc = wide_attr<2, false>()) || (rc = wide_attr<2, true>())) return rc;
+    return SWLM_OK;
+}
 
 int launch_f8_product(const swlm_f8_product& a, int* status, cudaStream_t s) {
-    (void)status;
     if (a.rows == 0) return SWLM_OK;
-    const dim3 grid(f8_blocks(a.n), std::min((a.rows + kTileRows - 1) / kTileRows, 64), std::max(a.experts, 1));
-    const cudaError_t e = launch_k(a.act == SWLM_F8_PLAIN ? f8_product_kernel<false> : f8_product_kernel<true>, grid, dim3(kThreads), 0, s, a);
-    return e == cudaSuccess ? SWLM_OK : cuda_fail(e, "product launch");
+    const bool gated = a.act != SWLM_F8_PLAIN, pairs = a.rows > 128 * std::max(a.experts, 1);
+    if (pairs) return gated ? wide_launch<2, true>(a, status, s) : wide_launch<2, false>(a, status, s);
+    return gated ? wide_launch<1, true>(a, status, s) : wide_launch<1, false>(a, status, s);
 }
 
 }  // namespace swlm
