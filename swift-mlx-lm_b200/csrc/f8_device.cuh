@@ -8,6 +8,7 @@ namespace swlm {
 namespace f8 {
 
 constexpr int kSms = 148;
+constexpr int kCodesBytes = kF8Block * kF8Block;   // 128 rows of a block
 
 // kind::f8f6f4: D fp32, A = B = e4m3, both K-major; 32 columns of K each
 __host__ __device__ constexpr unsigned idesc(int m, int n) { return (1u << 4) | ((unsigned)(n >> 3) << 17) | ((unsigned)(m >> 4) << 24); }
@@ -40,10 +41,17 @@ __device__ __forceinline__ unsigned cluster_place(unsigned addr, int rank) {   /
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
+// A shared-memory address that the compiler keeps in a register: in kernels of clusters it otherwise puts it together again wherever it is used, from a special
+// register that takes tens of cycles to read.
+__device__ __forceinline__ unsigned held_address(const void* p) {
+    unsigned r;
+    asm volatile("mov.u32 %0, %1;" : "=r"(r) : "r"(smem_u32(p)));
+    return r;
+}
 __device__ __forceinline__ void arrive(unsigned bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void arrive_cluster(unsigned bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 
-// 32 columns of a warp's 32 lanes of tensor memory; they are there behind landed(). Both are volatile, as is the use in add_scaled: they stay in their order.
+// 32 (or 16) columns of a warp's 32 lanes of tensor memory; they are there behind landed(). Both are volatile, as is the use in add_scaled: they stay in their order.
 __device__ __forceinline__ void tmem_load(unsigned (&v)[32], unsigned at) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -51,6 +59,13 @@ __device__ __forceinline__ void tmem_load(unsigned (&v)[32], unsigned at) {
           "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
           "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
           "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(at) : "memory");
+}
+__device__ __forceinline__ void tmem_load(unsigned (&v)[16], unsigned at) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
         : "r"(at) : "memory");
 }
 __device__ __forceinline__ void landed() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -84,5 +99,22 @@ __device__ __forceinline__ float gated(float g, float u, int act, float alpha, f
     return 0.25f * g * four_over(1.0f + expf(-z)) * u;
 }
 
+// Rows of bytes as a 2-D tensor, k columns valid (beyond: zeros); box = 128 columns x box_rows, 128-byte swizzle
+inline int code_map(const void* p, int64_t stride, int64_t rows, int k, int box_rows, CUtensorMap* map) {
+    TensorMapEncodeFn fn = tensor_map_encode_fn();
+    if (!fn) { set_error("f8: cuTensorMapEncodeTiled is not available"); return SWLM_ERR_CUDA; }
+    const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)stride};
+    const cuuint32_t box[2] = {(cuuint32_t)kF8Block, (cuuint32_t)box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) { set_error("f8: cuTensorMapEncodeTiled failed (%d)", (int)r); return SWLM_ERR_CUDA; }
+    return SWLM_OK;
+}
+
 }  // namespace f8
+
+int f8_few_init();
+int launch_f8_few(const swlm_f8_product& a, int* status, cudaStream_t s);
 }  // namespace swlm

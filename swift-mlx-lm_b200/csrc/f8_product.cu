@@ -22,9 +22,9 @@ namespace {
 // Registers are dealt out anew after the start: 128 threads x 56 for the first four warps, two of which have nothing to do, 256 x 224 for the takers' 128 sums
 // and the 64 that are on their way, together the 384 x 168 of the launch.
 constexpr int kWideWarps = 12, kWideThreads = kWideWarps * 32, kWideTakers = 8;
-constexpr int kAccCols = 256, kCodesBytes = kF8Block * kF8Block;   // 128 rows of a block
+constexpr int kAccCols = 256;
 constexpr int kScaleDepth = 4;      // blocks whose scales are on their way, and that have room for theirs in shared memory
-constexpr int kStageRow = 80, kPassBytes = 64;   // results on their way out: 64 bytes of each of a warp's 32 rows (the odd pitch keeps 16-byte accesses off each other's banks)
+constexpr int kStageRow = 80;   // results on their way out: 64 bytes of each of a warp's 32 rows (the odd pitch keeps 16-byte accesses off each other's banks)
 
 struct WideParams {
     const float *x_scale, *w_scale, *up_scale;
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) f8_wide_kernel(const WidePara
                 for (int b = 0; b < p.blocks; ++b, ++it) {
                     const unsigned empty_par = (unsigned)(~(it >> 1) & 1);
                     // (what the barriers guard is read by the tensor cores: no ordinary load has to see another CTA's stores)
-                    ok = mbar_wait_warp(&sums_empty[it & 1], empty_par) && mbar_wait_warp(&full[s], par);
+                    ok = mbar_wait_warp(&full[s], par) && mbar_wait_warp(&sums_empty[it & 1], empty_par);
                     if (!ok) { if (el) atomicExch_system(p.status, 12); break; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     if (el) {
@@ -223,10 +223,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) f8_wide_kernel(const WidePara
             const int row = tile.row0 + rank * 128 + r0, block = GATED ? tile.col : 2 * tile.col;
             const float* x = p.x_scale + b * p.x_scale_stride + row;
             const long long at = ((long long)tile.expert * p.col_blocks + block) * p.blocks + b;
-            a.x[0] = row < tile.end ? __ldg(x) : 0.f;
-            a.x[1] = row + 1 < tile.end ? __ldg(x + 1) : 0.f;
-            a.w[0] = __ldg(p.w_scale + at);
-            a.w[1] = GATED ? __ldg(p.up_scale + at) : block + 1 < p.col_blocks ? __ldg(p.w_scale + at + p.blocks) : 0.f;
+            a.x[0] = row < tile.end ? *x : 0.f;
+            a.x[1] = row + 1 < tile.end ? x[1] : 0.f;
+            a.w[0] = p.w_scale[at];
+            a.w[1] = GATED ? p.up_scale[at] : block + 1 < p.col_blocks ? p.w_scale[at + p.blocks] : 0.f;
             if (++b == p.blocks) {
                 b = 0; t += step;
                 any = t < tiles;
@@ -382,20 +382,6 @@ __global__ void __launch_bounds__(kWideThreads, 1) f8_wide_kernel(const WidePara
 }
 
 // ---- launches ----------------------------------------------------------------------------------------------------------------
-// Rows of bytes as a 2-D tensor, k columns valid (beyond: zeros); box = 128 columns x box_rows, 128-byte swizzle
-int code_map(const void* p, int64_t stride, int64_t rows, int k, int box_rows, CUtensorMap* map) {
-    TensorMapEncodeFn fn = tensor_map_encode_fn();
-    if (!fn) { set_error("f8: cuTensorMapEncodeTiled is not available"); return SWLM_ERR_CUDA; }
-    const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)stride};
-    const cuuint32_t box[2] = {(cuuint32_t)kF8Block, (cuuint32_t)box_rows};
-    const cuuint32_t estr[2] = {1, 1};
-    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, box, estr,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) { set_error("f8: cuTensorMapEncodeTiled failed (%d)", (int)r); return SWLM_ERR_CUDA; }
-    return SWLM_OK;
-}
-
 template <int CG, bool GATED>
 int wide_attr() {
     SWLM_CUDA(cudaFuncSetAttribute(f8_wide_kernel<CG, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)wide_smem<CG>()));
@@ -427,15 +413,15 @@ int wide_launch(const swlm_f8_product& a, int* status, cudaStream_t s) {
 
 int f8_product_init() {
     int rc;
-    if ((rc = wide_attr<1, false>()) || (rc = wide_attr<1, true>()) || (rc = wide_attr<2, false>()) || (rc = wide_attr<2, true>())) return rc;
+    if ((rc = f8_few_init()) || (rc = wide_attr<1, false>()) || (rc = wide_attr<1, true>()) || (rc = wide_attr<2, false>()) || (rc = wide_attr<2, true>())) return rc;
     return SWLM_OK;
 }
 
 int launch_f8_product(const swlm_f8_product& a, int* status, cudaStream_t s) {
     if (a.rows == 0) return SWLM_OK;
-    const bool gated = a.act != SWLM_F8_PLAIN, pairs = a.rows > 128 * std::max(a.experts, 1);
-    if (pairs) return gated ? wide_launch<2, true>(a, status, s) : wide_launch<2, false>(a, status, s);
-    return gated ? wide_launch<1, true>(a, status, s) : wide_launch<1, false>(a, status, s);
+    const int each = (a.rows + std::max(a.experts, 1) - 1) / std::max(a.experts, 1);
+    if (each <= 128) return launch_f8_few(a, status, s);
+    return a.act != SWLM_F8_PLAIN ? wide_launch<2, true>(a, status, s) : wide_launch<2, false>(a, status, s);
 }
 
 }  // namespace swlm
