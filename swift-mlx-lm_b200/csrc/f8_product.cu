@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) f8_wide_kernel(const WidePara
     if (warp == 0) {
         // The warp runs its loop as a whole, one lane issues. Of a pair both CTAs' copies count on the barrier of the one that issues the MMAs.
         const bool el = elect_one();
-        const unsigned full0 = CG == 1 ? smem_u32(&full[0]) : cluster_place(smem_u32(&full[0]), 0), at = smem_u32(ring);
+        const unsigned full0 = CG == 1 ? held_address(&full[0]) : cluster_place(smem_u32(&full[0]), 0), empty0 = held_address(&empty[0]), at = held_address(ring);
         auto load = [&](unsigned dst, const CUtensorMap* map, int col, int row, int s) {
             if (CG == 1) tma_load_2d(dst, map, col, row, full0 + 8u * s);
             else tma_load_2d_pair(dst, map, col, row, full0 + 8u * s);
@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) f8_wide_kernel(const WidePara
             const WideTile tile = wide_tile<CG>(p, first_tile, t);
             const int x_row = tile.row0 + rank * 128, w_row = tile.expert * p.n + tile.col * COLS + rank * (COLS / 2);
             for (int b = 0; b < p.blocks; ++b) {
-                if (!mbar_wait_warp(&empty[s], par)) { ok = false; break; }
+                if (!mbar_wait_warp(empty0 + 8u * s, par)) { ok = false; break; }
                 if (el) {
                     const unsigned dst = at + s * STAGE;
                     if (rank == 0) mbar_expect(full0 + 8u * s, (unsigned)(CG * STAGE));
@@ -187,25 +187,27 @@ __global__ void __launch_bounds__(kWideThreads, 1) f8_wide_kernel(const WidePara
         if (rank == 0) {
             constexpr unsigned desc = idesc(128 * CG, kAccCols);
             const bool el = elect_one();
-            int s = 0, it = 0;
-            unsigned par = 0;
+            const unsigned full0 = held_address(&full[0]), sums0 = held_address(&sums_empty[0]), at = umma_desc_lo(held_address(ring));
+            int s = 0;
+            unsigned par = 0, buffer = 0, sums_par = 1;
             bool ok = true;
             for (int t = first; t < tiles && ok; t += step)
-                for (int b = 0; b < p.blocks; ++b, ++it) {
-                    const unsigned empty_par = (unsigned)(~(it >> 1) & 1);
+                for (int b = 0; b < p.blocks; ++b) {
                     // (what the barriers guard is read by the tensor cores: no ordinary load has to see another CTA's stores)
-                    ok = mbar_wait_warp(&full[s], par) && mbar_wait_warp(&sums_empty[it & 1], empty_par);
+                    ok = mbar_wait_warp(full0 + 8u * s, par) && mbar_wait_warp(sums0 + 8u * buffer, sums_par);
                     if (!ok) { if (el) atomicExch_system(p.status, 12); break; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     if (el) {
-                        const unsigned a = umma_desc_lo(smem_u32(ring + s * STAGE)), w = a + kCodesBytes / 16;
+                        const unsigned a = at + s * (STAGE / 16), w = a + kCodesBytes / 16, sums = tmem + buffer * kAccCols;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) umma<CG>(tmem + (it & 1) * kAccCols, a + 2 * j, w + 2 * j, desc, j > 0);
+                        for (int j = 0; j < 4; ++j) umma<CG>(sums, a + 2 * j, w + 2 * j, desc, j > 0);
                         commit<CG>(&empty[s]);
-                        commit<CG>(&sums_full[it & 1]);
+                        commit<CG>(&sums_full[buffer]);
                     }
                     __syncwarp();
                     if (++s == STAGES) { s = 0; par ^= 1u; }
+                    buffer ^= 1u;
+                    sums_par ^= buffer ^ 1u;
                 }
         }
     } else {
@@ -213,6 +215,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) f8_wide_kernel(const WidePara
         // and up's), is in shared memory before the sums are said to be there. A slot is free again by then: the takers have left block
         // it - 4 before block it - 2 was multiplied.
         const int r0 = (warp - 2) * 64 + 2 * lane;
+        const unsigned full0 = held_address(&sums_full[0]);
+        float2* const mine = scales + r0;
         struct Ahead { float x[2], w[2]; } ahead[kScaleDepth];
         WideTile tile{};
         int t = first, b = 0;      // the block that is asked for next
@@ -234,21 +238,21 @@ __global__ void __launch_bounds__(kWideThreads, 1) f8_wide_kernel(const WidePara
             }
         };
         const int total = first < tiles ? (tiles - 1 - first) / step + 1 : 0;
-        const long long all = (long long)total * p.blocks;
+        const int all = total * p.blocks;
 #pragma unroll
         for (int u = 0; u < kScaleDepth; ++u) ask(ahead[u]);
         bool ok = true;
-        for (long long it0 = 0; it0 < all && ok; it0 += kScaleDepth) {
+        for (int it0 = 0; it0 < all && ok; it0 += kScaleDepth) {
 #pragma unroll
             for (int u = 0; u < kScaleDepth; ++u) {
-                const long long it = it0 + u;
+                const int it = it0 + u;
                 if (it >= all || !ok) break;
-                if (it >= 2) ok = mbar_wait_warp(&sums_full[u & 1], (unsigned)(((it >> 1) - 1) & 1));
+                if (it >= 2) ok = mbar_wait_warp(full0 + 8u * (u & 1), (unsigned)(((it >> 1) - 1) & 1));
                 if (!ok) { if (lane == 0) atomicExch_system(p.status, 14); break; }
                 const Ahead now = ahead[u];
-                *reinterpret_cast<float4*>(scales + u * 128 + r0) = make_float4(now.x[0] * now.w[0], now.x[0] * now.w[1], now.x[1] * now.w[0], now.x[1] * now.w[1]);
+                *reinterpret_cast<float4*>(mine + u * 128) = make_float4(now.x[0] * now.w[0], now.x[0] * now.w[1], now.x[1] * now.w[0], now.x[1] * now.w[1]);
                 __syncwarp();
-                if (lane == 0) arrive(smem_u32(&sums_full[u & 1]));
+                if (lane == 0) arrive(full0 + 8u * (u & 1));
                 ask(ahead[u]);
             }
         }
@@ -258,36 +262,40 @@ __global__ void __launch_bounds__(kWideThreads, 1) f8_wide_kernel(const WidePara
         // A warp has the 32 lanes of its quarter (warp & 3) and one half of the columns.
         const int taker = warp - 4, quarter = warp & 3, half = taker >> 2;
         const unsigned at = tmem + ((unsigned)(quarter * 32) << 16) + 128u * half;
-        const unsigned given[2] = {CG == 1 ? smem_u32(&sums_empty[0]) : cluster_place(smem_u32(&sums_empty[0]), 0), CG == 1 ? smem_u32(&sums_empty[1]) : cluster_place(smem_u32(&sums_empty[1]), 0)};
+        const unsigned full0 = held_address(&sums_full[0]), given0 = CG == 1 ? held_address(&sums_empty[0]) : cluster_place(smem_u32(&sums_empty[0]), 0);
+        const unsigned factors = held_address(scales) + 8u * (quarter * 32 + lane) + (GATED ? 0u : 4u * half);
         unsigned char* const out = staging + taker * 32 * kStageRow;
-        int it = 0;
+        unsigned buffer = 0, par = 0, slot = 0;
         bool ok = true;
         for (int t = first; t < tiles && ok; t += step) {
             unsigned long long acc[64];
 #pragma unroll
             for (int i = 0; i < 64; ++i) acc[i] = 0;
-            for (int b = 0; b < p.blocks; ++b, ++it) {
-                ok = mbar_wait_warp(&sums_full[it & 1], (unsigned)((it >> 1) & 1));
+            for (int b = 0; b < p.blocks; ++b) {
+                ok = mbar_wait_warp(full0 + 8u * buffer, par);
                 if (!ok) { if (lane == 0) atomicExch_system(p.status, 13); break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                unsigned v[2][32];
-                const unsigned from = at + (it & 1) * kAccCols;
-                tmem_load(v[0], from);
-                const float2 factor = scales[(it & (kScaleDepth - 1)) * 128 + quarter * 32 + lane];
-                const float sl = GATED || !half ? factor.x : factor.y, sh = GATED || half ? factor.y : factor.x;
-                const unsigned long long low = pair_of(sl, sl), high = pair_of(sh, sh);
+                const unsigned from = at + buffer * kAccCols;
+                float s_low, s_high;
+                if (GATED) asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(s_low), "=f"(s_high) : "r"(factors + slot) : "memory");
+                else { asm volatile("ld.shared.f32 %0, [%1];" : "=f"(s_low) : "r"(factors + slot) : "memory"); s_high = s_low; }
+                const unsigned long long low = pair_of(s_low, s_low), high = pair_of(s_high, s_high);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
+                for (int c = 0; c < 8; ++c) {
+                    unsigned v[16];
+                    tmem_load(v, from + 16 * c);
                     landed();
-                    if (c < 3) tmem_load(v[(c + 1) & 1], from + 32 * (c + 1));
-                    else {   // all of them are in registers: the buffer is free
+                    if (c == 7) {   // all of them are in registers: the buffer is free
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                         __syncwarp();
-                        if (lane == 0) { if (CG == 1) arrive(given[it & 1]); else arrive_cluster(given[it & 1]); }
+                        if (lane == 0) { if (CG == 1) arrive(given0 + 8u * buffer); else arrive_cluster(given0 + 8u * buffer); }
                     }
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) add_scaled(acc[16 * c + i], v[c & 1][2 * i], v[c & 1][2 * i + 1], c < 2 ? low : high);
+                    for (int i = 0; i < 8; ++i) add_scaled(acc[8 * c + i], v[2 * i], v[2 * i + 1], c < 4 ? low : high);
                 }
+                buffer ^= 1u;
+                par ^= buffer ^ 1u;
+                slot = (slot + 1024u) & (1024u * kScaleDepth - 1u);
             }
             if (!ok) break;
             const WideTile done = wide_tile<CG>(p, first_tile, t);
