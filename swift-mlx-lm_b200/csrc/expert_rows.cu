@@ -14,7 +14,7 @@ namespace {
 // A stable counting sort by one cluster: every warp has a run of neighbouring pairs and counts its experts; sums over warps and, through distributed
 // shared memory, over the cluster's CTAs give every warp its first row of every expert; then it numbers its pairs, 32 at a time, by those before
 // them of the same expert. No number depends on the order in which warps get there.
-constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortUnroll = 4;
+constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortUnroll = 4, kSortCtas = 16;
 
 __global__ void __launch_bounds__(kSortThreads) expert_sort_kernel(const swlm_expert_sort a) {
     extern __shared__ int counts[];        // [kSortWarps][experts]: pairs of each warp, then each warp's next row
@@ -38,21 +38,26 @@ __global__ void __launch_bounds__(kSortThreads) expert_sort_kernel(const swlm_ex
     __syncthreads();
     int sum = 0;   // of expert `tid`
     if (tid < E) {
-        for (int w = 0; w < kSortWarps; ++w) {   // pairs of the warps before w
-            const int c = counts[w * E + tid];
-            counts[w * E + tid] = sum;
-            sum += c;
+#pragma unroll
+        for (int w0 = 0; w0 < kSortWarps; w0 += 16) {   // pairs of the warps before each
+            int c[16];
+#pragma unroll
+            for (int w = 0; w < 16; ++w) c[w] = counts[(w0 + w) * E + tid];
+#pragma unroll
+            for (int w = 0; w < 16; ++w) { counts[(w0 + w) * E + tid] = sum; sum += c[w]; }
         }
         total[tid] = sum;
     }
     cluster.sync();
     int all = 0, others = 0;
-    if (tid < E)
-        for (int c = 0; c < ctas; ++c) {
-            const int v = *cluster.map_shared_rank(total + tid, c);
+    if (tid < E) {
+#pragma unroll
+        for (int c = 0; c < kSortCtas; ++c) {
+            const int v = c < ctas ? *cluster.map_shared_rank(total + tid, c) : 0;
             others += c < rank ? v : 0;
             all += v;
         }
+    }
     int scan = all;   // rows of the experts up to this one
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -72,7 +77,8 @@ __global__ void __launch_bounds__(kSortThreads) expert_sort_kernel(const swlm_ex
             a.offsets[tid] = base;
             if (tid == E - 1) a.offsets[E] = rows;
         }
-        for (int w = 0; w < kSortWarps; ++w) counts[w * E + tid] += base + others;
+#pragma unroll 16
+        for (int w = 0; w < kSortWarps; ++w) atomicAdd(counts + w * E + tid, base + others);   // (no thread waits for what it reads)
     }
     __syncthreads();
     for (int i = rows + rank * kSortThreads + tid; i < pairs; i += ctas * kSortThreads) a.source[i] = -1;
@@ -103,23 +109,36 @@ __global__ void __launch_bounds__(kSortThreads) expert_sort_kernel(const swlm_ex
 }
 
 // ---- sum ---------------------------------------------------------------------------------------------------------------------
-// A thread has eight columns of a token and runs through the token's rows in their order, up to eight loads on their way at once.
-constexpr int kSumThreads = 256, kSumUnroll = 8;
+// A thread has eight columns of a token and runs through the token's rows in their order; the rows' values are held as they came until they are added, so that
+// 128 bytes a thread are on their way at once and four CTAs fit an SM.
+constexpr int kSumThreads = 256;
 
-template <int DTYPE> __device__ __forceinline__ void load8(const void* p, float (&x)[8]) {
-    if (DTYPE == SWLM_F8_FP32) {
-        const float4 a = static_cast<const float4*>(p)[0], b = static_cast<const float4*>(p)[1];
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    } else {
-        const uint4 v = *static_cast<const uint4*>(p);
-        const unsigned w[4] = {v.x, v.y, v.z, v.w};
+template <int DTYPE> struct Values8 {   // eight values as they are held
+    static constexpr int WORDS = DTYPE == SWLM_F8_FP32 ? 2 : 1, SIZE = DTYPE == SWLM_F8_FP32 ? 4 : 2;
+    uint4 v[WORDS];
+    __device__ __forceinline__ void load(const void* p) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = DTYPE == SWLM_F8_FP16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[i])) : make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
-            x[2 * i] = f.x; x[2 * i + 1] = f.y;
+        for (int i = 0; i < WORDS; ++i) v[i] = static_cast<const uint4*>(p)[i];
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) v[i] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void widen(float (&x)[8]) const {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) {
+            const unsigned w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (DTYPE == SWLM_F8_FP32) x[4 * i + j] = __uint_as_float(w[j]);
+                else {
+                    const float2 f = DTYPE == SWLM_F8_FP16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[j])) : make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u));
+                    x[2 * j] = f.x; x[2 * j + 1] = f.y;
+                }
+            }
         }
     }
-}
+};
 template <int DTYPE> __device__ __forceinline__ float load1(const void* p, int i) {
     if (DTYPE == SWLM_F8_FP32) return static_cast<const float*>(p)[i];
     return DTYPE == SWLM_F8_FP16 ? __half2float(static_cast<const __half*>(p)[i]) : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
@@ -145,8 +164,8 @@ template <int DTYPE> __device__ __forceinline__ void store8(void* p, const float
 }
 
 template <int Y, int OUT>
-__global__ void __launch_bounds__(kSumThreads) expert_sum_kernel(const swlm_expert_sum a) {
-    constexpr int YSIZE = Y == SWLM_F8_FP32 ? 4 : 2, SIZE = OUT == SWLM_F8_FP32 ? 4 : 2;
+__global__ void __launch_bounds__(kSumThreads, 4) expert_sum_kernel(const swlm_expert_sum a) {
+    constexpr int YSIZE = Values8<Y>::SIZE, SIZE = Values8<OUT>::SIZE, UNROLL = 8 / Values8<Y>::WORDS;
     pdl_wait();
     const unsigned chunks = (a.width + 7) / 8;
     const long long at = (long long)blockIdx.x * kSumThreads + threadIdx.x;
@@ -156,39 +175,46 @@ __global__ void __launch_bounds__(kSumThreads) expert_sum_kernel(const swlm_expe
     const int* place = a.place + t * a.top;
     const float* weight = a.weight + t * a.top;
     const unsigned char* y = static_cast<const unsigned char*>(a.y) + (long long)col * YSIZE;
+    unsigned char* out = static_cast<unsigned char*>(a.out) + (t * a.out_stride + col) * SIZE;
+    const unsigned char* add = a.add ? static_cast<const unsigned char*>(a.add) + (t * a.add_stride + col) * SIZE : nullptr;
+    if (rest < 8) {   // a token's last columns, whose number is no multiple of eight
+        for (int e = 0; e < rest; ++e) {
+            float sum = 0.f;
+            for (int j = 0; j < a.top; ++j)
+                if (place[j] >= 0 && place[j] < a.y_rows) sum = fmaf(weight[j], load1<Y>(y + (long long)place[j] * a.y_stride * YSIZE, e), sum);
+            store1<OUT>(out, e, add ? sum + load1<OUT>(add, e) : sum);
+        }
+        return;
+    }
+    Values8<OUT> base;
+    if (add) base.load(add);
     float sum[8] = {};
-    for (int j0 = 0; j0 < a.top; j0 += kSumUnroll) {
-        float x[kSumUnroll][8], w[kSumUnroll];
+    for (int j0 = 0; j0 < a.top; j0 += UNROLL) {
+        Values8<Y> held[UNROLL];
+        float w[UNROLL];
 #pragma unroll
-        for (int j = 0; j < kSumUnroll; ++j) {
+        for (int j = 0; j < UNROLL; ++j) {
             const int row = j0 + j < a.top ? place[j0 + j] : -1;
             const bool has = row >= 0 && row < a.y_rows;
             w[j] = has ? weight[j0 + j] : 0.f;
-            const unsigned char* p = y + (long long)row * a.y_stride * YSIZE;
-            if (has && rest >= 8) load8<Y>(p, x[j]);
-            else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[j][e] = has && e < rest ? load1<Y>(p, e) : 0.f;
-            }
+            if (has) held[j].load(y + (long long)row * a.y_stride * YSIZE);
+            else held[j].zero();
         }
 #pragma unroll
-        for (int j = 0; j < kSumUnroll; ++j)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) sum[e] = fmaf(w[j], x[j][e], sum[e]);
-    }
-    unsigned char* out = static_cast<unsigned char*>(a.out) + (t * a.out_stride + col) * SIZE;
-    const unsigned char* add = a.add ? static_cast<const unsigned char*>(a.add) + (t * a.add_stride + col) * SIZE : nullptr;
-    if (rest >= 8) {
-        if (add) {
+        for (int j = 0; j < UNROLL; ++j) {
             float x[8];
-            load8<OUT>(add, x);
+            held[j].widen(x);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) sum[e] += x[e];
+            for (int e = 0; e < 8; ++e) sum[e] = fmaf(w[j], x[e], sum[e]);
         }
-        store8<OUT>(out, sum);
-    } else {
-        for (int e = 0; e < rest; ++e) store1<OUT>(out, e, add ? sum[e] + load1<OUT>(add, e) : sum[e]);
     }
+    if (add) {
+        float x[8];
+        base.widen(x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += x[e];
+    }
+    store8<OUT>(out, sum);
 }
 
 template <int Y> void (*sum_kernel(int dtype))(swlm_expert_sum) {
@@ -199,13 +225,14 @@ template <int Y> void (*sum_kernel(int dtype))(swlm_expert_sum) {
 
 int expert_rows_init() {
     SWLM_CUDA(cudaFuncSetAttribute(expert_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortWarps * kExpertMax * 4));
+    SWLM_CUDA(cudaFuncSetAttribute(expert_sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     return SWLM_OK;
 }
 
 int launch_expert_sort(const swlm_expert_sort& a, cudaStream_t s) {
     const long long pairs = (long long)a.tokens * a.top;
     int ctas = 1;
-    while (ctas < 8 && pairs > (long long)ctas * 2 * kSortThreads) ctas *= 2;
+    while (ctas < kSortCtas && pairs > (long long)ctas * 2 * kSortThreads) ctas *= 2;
     const cudaError_t e = launch_clusters(expert_sort_kernel, ctas, dim3(ctas), dim3(kSortThreads), (size_t)kSortWarps * a.experts * 4, s, a);
     return e == cudaSuccess ? SWLM_OK : cuda_fail(e, "expert sort launch");
 }

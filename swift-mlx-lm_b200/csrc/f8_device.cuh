@@ -90,6 +90,73 @@ __device__ __forceinline__ float gated(float g, float u, int act, float alpha, f
     return 0.25f * g * four_over(1.0f + expf(-z)) * u;
 }
 
+// Work as tiles of `rows` rows x a tile of columns, those of one expert after those of the other (experts 0: one has all rows). CTAs take them in turn.
+struct TileShape { const int* offsets; int rows, experts, tile_rows, col_tiles; };
+struct Tile { int expert, row0, end, col; };   // rows row0 .. end - 1 (of which a tile has tile_rows at most), tile of columns
+
+// An expert's rows, cut to those there are.
+__device__ __forceinline__ int2 expert_rows(const TileShape& p, int e) {
+    const int from = min(max(p.offsets[e], 0), p.rows);
+    return make_int2(from, min(max(p.offsets[e + 1], from), p.rows));
+}
+// Fills first_tile [experts] with the tiles of the experts before each, by all threads of a CTA, and returns the number of tiles; `warps`: a number per warp. A
+// barrier has to follow.
+template <int THREADS>
+__device__ __forceinline__ int count_tiles(const TileShape& p, int* first_tile, int* warps) {
+    if (!p.experts) return (p.rows + p.tile_rows - 1) / p.tile_rows * p.col_tiles;
+    constexpr int PER = (kExpertMax + THREADS - 1) / THREADS;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int c[PER], sum = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int e = tid * PER + j;
+        c[j] = 0;
+        if (e < p.experts) {
+            const int2 r = expert_rows(p, e);
+            c[j] = (r.y - r.x + p.tile_rows - 1) / p.tile_rows * p.col_tiles;
+        }
+        sum += c[j];
+    }
+    int scan = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, scan, o);
+        if (lane >= o) scan += v;
+    }
+    if (lane == 31) warps[warp] = scan;
+    __syncthreads();
+    int tiles = 0;
+    for (int w = 0; w < THREADS / 32; ++w) { scan += w < warp ? warps[w] : 0; tiles += warps[w]; }
+    scan -= sum;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int e = tid * PER + j;
+        if (e < p.experts) first_tile[e] = scan;
+        scan += c[j];
+    }
+    return tiles;
+}
+__device__ __forceinline__ Tile tile_at(const TileShape& p, const int* first_tile, int t) {
+    Tile w{0, 0, p.rows, 0};
+    if (p.experts) {
+        int lo = 0, hi = p.experts - 1;   // the last expert whose tiles start at or before t
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (first_tile[mid] <= t) lo = mid; else hi = mid - 1;
+        }
+        const int2 r = expert_rows(p, lo);
+        w.expert = lo; w.row0 = r.x; w.end = r.y;
+        t -= first_tile[lo];
+    }
+    // the shorter side first: what it sweeps stays in L2
+    const int row_tiles = (w.end - w.row0 + p.tile_rows - 1) / p.tile_rows;
+    int r;
+    if (row_tiles <= p.col_tiles) { r = t % row_tiles; w.col = t / row_tiles; }
+    else { w.col = t % p.col_tiles; r = t / p.col_tiles; }
+    w.row0 += r * p.tile_rows;
+    return w;
+}
+
 // Rows of bytes as a 2-D tensor, k columns valid (beyond: zeros); box = 128 columns x box_rows, 128-byte swizzle
 inline int code_map(const void* p, int64_t stride, int64_t rows, int k, int box_rows, CUtensorMap* map) {
     TensorMapEncodeFn fn = tensor_map_encode_fn();
@@ -106,6 +173,9 @@ inline int code_map(const void* p, int64_t stride, int64_t rows, int k, int box_
 
 }  // namespace f8
 
+// A product of few rows: rows of x per tile, CTAs of a cluster that share K, and what it takes, about (us).
+struct F8FewForm { int nt, ranges; double cost; };
+F8FewForm f8_few_form(int rows, int n, int k, int experts, bool gated);
 int f8_few_init();
-int launch_f8_few(const swlm_f8_product& a, int* status, cudaStream_t s);
+int launch_f8_few(const swlm_f8_product& a, const F8FewForm& form, int* status, cudaStream_t s);
 }  // namespace swlm

@@ -15,7 +15,7 @@ using namespace f8;
 namespace {
 
 // ---- many rows ---------------------------------------------------------------------------------------------------------------
-// Persistent CTAs, alone (CG = 1) or in pairs (2) that share a tile of 128 CG rows x 256 columns of accumulators: lanes of tensor memory are rows of
+// Persistent pairs of CTAs that share a tile of 256 rows x 256 columns of accumulators: lanes of tensor memory are rows of
 // x, a thread has one row and 128 of the columns. A warp for the copies, one for the MMAs, eight that take a block's sums out of one of two buffers of
 // tensor memory while the next block's are multiplied into the other. GATED: the accumulators of 64 columns of w lie before those of the same 64
 // of `up`, so that a thread has both, and a tile gives 128 columns of the result.
@@ -31,161 +31,83 @@ struct WideParams {
     long long x_scale_stride, y_stride, y_scale_stride;
     unsigned char* y;
     float* y_scale;
-    const int* offsets;
+    TileShape tiles;
     int* status;
-    int rows, n, blocks, experts;       // blocks of K
-    int col_blocks, col_tiles;          // of n: scales of a matrix, tiles
+    int n, blocks, col_blocks;          // blocks of K; of n: scales of a matrix
     int dtype, act;
     float alpha, limit;
 };
 
-template <int CG> __host__ __device__ constexpr int wide_stages() { return CG == 1 ? 4 : 6; }
-template <int CG> __host__ __device__ constexpr int wide_stage_bytes() { return kCodesBytes + kAccCols / CG * kF8Block; }
-template <int CG> __host__ __device__ constexpr size_t wide_smem() {
-    return 1024 + (size_t)wide_stages<CG>() * wide_stage_bytes<CG>() + kWideTakers * 32 * kStageRow + kScaleDepth * 128 * 8 + 2 * 128 * 4 + (kExpertMax + 1) * 4;
-}
-static_assert(wide_smem<1>() <= 232448 && wide_smem<2>() <= 232448, "shared memory");
+constexpr int kStages = 6, kStage = 2 * kCodesBytes;   // a CTA's 128 rows of x, and half of the matrix's
+constexpr size_t kWideSmem = 1024 + (size_t)kStages * kStage + kWideTakers * 32 * kStageRow + kScaleDepth * 128 * 8 + 2 * 128 * 4 + kExpertMax * 4;
+static_assert(kWideSmem <= 232448 - 1024, "shared memory");
 
-struct WideTile { int expert, row0, end, col; };   // rows row0 .. end - 1 (of which a tile has 128 CG at most), tile of columns
-
-// Tiles of the experts before each (experts 0: all rows are one expert's), then tile `t`.
-template <int CG>
-__device__ __forceinline__ WideTile wide_tile(const WideParams& p, const int* first_tile, int t) {
-    constexpr int ROWS = 128 * CG;
-    WideTile w{0, 0, p.rows, 0};
-    if (p.experts) {
-        int lo = 0, hi = p.experts - 1;   // the last expert whose tiles start at or before t
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (first_tile[mid] <= t) lo = mid; else hi = mid - 1;
-        }
-        w.expert = lo;
-        w.row0 = min(max(p.offsets[lo], 0), p.rows);
-        w.end = min(max(p.offsets[lo + 1], w.row0), p.rows);
-        t -= first_tile[lo];
-    }
-    // the shorter side first: what it sweeps stays in L2
-    const int row_tiles = (w.end - w.row0 + ROWS - 1) / ROWS;
-    int r;
-    if (row_tiles <= p.col_tiles) { r = t % row_tiles; w.col = t / row_tiles; }
-    else { w.col = t % p.col_tiles; r = t / p.col_tiles; }
-    w.row0 += r * ROWS;
-    return w;
-}
-
-template <int CG, bool GATED>
+template <bool GATED>
 __global__ void __launch_bounds__(kWideThreads, 1) f8_wide_kernel(const WideParams p, const __grid_constant__ CUtensorMap xmap,
                                                                   const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap upmap) {
-    constexpr int STAGES = wide_stages<CG>(), STAGE = wide_stage_bytes<CG>(), ROWS = 128 * CG, COLS = GATED ? 128 : 256;
+    constexpr int COLS = GATED ? 128 : 256;
     extern __shared__ __align__(1024) unsigned char wide_raw[];
     unsigned char* const ring = wide_raw + ((1024 - (smem_u32(wide_raw) & 1023)) & 1023);   // swizzle atoms
-    unsigned char* const staging = ring + STAGES * STAGE;
+    unsigned char* const staging = ring + kStages * kStage;
     float2* const scales = reinterpret_cast<float2*>(staging + kWideTakers * 32 * kStageRow);   // [kScaleDepth][128]
     unsigned* const tops = reinterpret_cast<unsigned*>(scales + kScaleDepth * 128);             // [2][128]
     int* const first_tile = reinterpret_cast<int*>(tops + 256);                                // [experts + 1]
-    __shared__ __align__(8) unsigned long long full[STAGES], empty[STAGES], sums_full[2], sums_empty[2];
+    __shared__ __align__(8) unsigned long long full[kStages], empty[kStages], sums_full[2], sums_empty[2];
     __shared__ unsigned tmem_base;
     __shared__ int warp_tiles[kWideWarps];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int rank = CG == 2 ? (int)(blockIdx.x & 1) : 0;
+    const int rank = (int)(blockIdx.x & 1);
     if (tid == 0) {
-        for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&sums_full[i], 1 + 2); mbar_init(&sums_empty[i], CG * kWideTakers); }
+        for (int s = 0; s < kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&sums_full[i], 1 + 2); mbar_init(&sums_empty[i], 2 * kWideTakers); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
-        if (CG == 1) {
-            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(2 * kAccCols) : "memory");
-            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-        } else {
-            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(2 * kAccCols) : "memory");
-            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-        }
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(2 * kAccCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     pdl_wait();
-    int tiles = (p.rows + ROWS - 1) / ROWS * p.col_tiles;
-    if (p.experts) {
-        constexpr int PER = (kExpertMax + kWideThreads - 1) / kWideThreads;
-        int c[PER], sum = 0;
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const int e = tid * PER + j;
-            c[j] = 0;
-            if (e < p.experts) {
-                const int from = min(max(p.offsets[e], 0), p.rows), to = min(max(p.offsets[e + 1], from), p.rows);
-                c[j] = (to - from + ROWS - 1) / ROWS * p.col_tiles;
-            }
-            sum += c[j];
-        }
-        int scan = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, scan, o);
-            if (lane >= o) scan += v;
-        }
-        if (lane == 31) warp_tiles[warp] = scan;
-        __syncthreads();
-        tiles = 0;
-        for (int w = 0; w < kWideWarps; ++w) { scan += w < warp ? warp_tiles[w] : 0; tiles += warp_tiles[w]; }
-        scan -= sum;
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const int e = tid * PER + j;
-            if (e < p.experts) first_tile[e] = scan;
-            scan += c[j];
-        }
-    }
+    const int tiles = count_tiles<kWideThreads>(p.tiles, first_tile, warp_tiles);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (CG == 2) cg::this_cluster().sync();   // both CTAs' barriers are ready
+    cg::this_cluster().sync();   // both CTAs' barriers are ready
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const unsigned tmem = tmem_base;
-    const int first = (int)blockIdx.x / CG, step = (int)gridDim.x / CG;
+    const int first = (int)blockIdx.x / 2, step = (int)gridDim.x / 2;
     if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 0) {
         // The warp runs its loop as a whole, one lane issues. Of a pair both CTAs' copies count on the barrier of the one that issues the MMAs.
         const bool el = elect_one();
-        const unsigned full0 = CG == 1 ? held_address(&full[0]) : cluster_place(smem_u32(&full[0]), 0), empty0 = held_address(&empty[0]), at = held_address(ring);
-        auto load = [&](unsigned dst, const CUtensorMap* map, int col, int row, int s) {
-            if (CG == 1) tma_load_2d(dst, map, col, row, full0 + 8u * s);
-            else tma_load_2d_pair(dst, map, col, row, full0 + 8u * s);
-        };
+        const unsigned full0 = cluster_place(smem_u32(&full[0]), 0), empty0 = held_address(&empty[0]), at = held_address(ring);
+        auto load = [&](unsigned dst, const CUtensorMap* map, int col, int row, int s) { tma_load_2d_pair(dst, map, col, row, full0 + 8u * s); };
         int s = 0, issued = 0;
         unsigned par = 1;
         bool ok = true;
         for (int t = first; t < tiles && ok; t += step) {
-            const WideTile tile = wide_tile<CG>(p, first_tile, t);
+            const Tile tile = tile_at(p.tiles, first_tile, t);
             const int x_row = tile.row0 + rank * 128, w_row = tile.expert * p.n + tile.col * COLS + rank * (COLS / 2);
             for (int b = 0; b < p.blocks; ++b) {
                 if (!mbar_wait_warp(empty0 + 8u * s, par)) { ok = false; break; }
                 if (el) {
-                    const unsigned dst = at + s * STAGE;
-                    if (rank == 0) mbar_expect(full0 + 8u * s, (unsigned)(CG * STAGE));
+                    const unsigned dst = at + s * kStage;
+                    if (rank == 0) mbar_expect(full0 + 8u * s, 2u * kStage);
                     load(dst, &xmap, b * kF8Block, x_row, s);
-                    if (GATED) {
-#pragma unroll
-                        for (int i = 0; i < 2 / CG; ++i) {
-                            load(dst + kCodesBytes * (1 + i), &wmap, b * kF8Block, w_row + 64 * i, s);
-                            load(dst + kCodesBytes * (1 + i) + kCodesBytes / 2, &upmap, b * kF8Block, w_row + 64 * i, s);
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 2 / CG; ++i) load(dst + kCodesBytes * (1 + i), &wmap, b * kF8Block, w_row + 128 * i, s);
-                    }
+                    load(dst + kCodesBytes, &wmap, b * kF8Block, w_row, s);
+                    if (GATED) load(dst + kCodesBytes + kCodesBytes / 2, &upmap, b * kF8Block, w_row, s);
                 }
                 __syncwarp();
                 ++issued;
-                if (++s == STAGES) { s = 0; par ^= 1u; }
+                if (++s == kStages) { s = 0; par ^= 1u; }
             }
         }
         if (!ok) {   // copies already requested still write shared memory (in a pair's second CTA, whose barrier this is not, the limit of the wait is the time they get)
             if (el) atomicExch_system(p.status, 11);
-            for (int i = max(issued - STAGES, 0); i < issued; ++i) mbar_wait_warp(&full[i % STAGES], (unsigned)((i / STAGES) & 1));
+            for (int i = max(issued - kStages, 0); i < issued; ++i) mbar_wait_warp(&full[i % kStages], (unsigned)((i / kStages) & 1));
         }
     } else if (warp == 1) {
         if (rank == 0) {
-            constexpr unsigned desc = idesc(128 * CG, kAccCols);
+            constexpr unsigned desc = idesc(256, kAccCols);
             const bool el = elect_one();
             const unsigned full0 = held_address(&full[0]), sums0 = held_address(&sums_empty[0]), at = umma_desc_lo(held_address(ring));
             int s = 0;
@@ -198,14 +120,14 @@ __global__ void __launch_bounds__(kWideThreads, 1) f8_wide_kernel(const WidePara
                     if (!ok) { if (el) atomicExch_system(p.status, 12); break; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     if (el) {
-                        const unsigned a = at + s * (STAGE / 16), w = a + kCodesBytes / 16, sums = tmem + buffer * kAccCols;
+                        const unsigned a = at + s * (kStage / 16), w = a + kCodesBytes / 16, sums = tmem + buffer * kAccCols;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) umma<CG>(sums, a + 2 * j, w + 2 * j, desc, j > 0);
-                        commit<CG>(&empty[s]);
-                        commit<CG>(&sums_full[buffer]);
+                        for (int j = 0; j < 4; ++j) umma<2>(sums, a + 2 * j, w + 2 * j, desc, j > 0);
+                        commit<2>(&empty[s]);
+                        commit<2>(&sums_full[buffer]);
                     }
                     __syncwarp();
-                    if (++s == STAGES) { s = 0; par ^= 1u; }
+                    if (++s == kStages) { s = 0; par ^= 1u; }
                     buffer ^= 1u;
                     sums_par ^= buffer ^ 1u;
                 }
@@ -218,10 +140,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) f8_wide_kernel(const WidePara
         const unsigned full0 = held_address(&sums_full[0]);
         float2* const mine = scales + r0;
         struct Ahead { float x[2], w[2]; } ahead[kScaleDepth];
-        WideTile tile{};
+        Tile tile{};
         int t = first, b = 0;      // the block that is asked for next
         bool any = t < tiles;
-        if (any) tile = wide_tile<CG>(p, first_tile, t);
+        if (any) tile = tile_at(p.tiles, first_tile, t);
         auto ask = [&](Ahead& a) {
             if (!any) return;
             const int row = tile.row0 + rank * 128 + r0, block = GATED ? tile.col : 2 * tile.col;
@@ -234,7 +156,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) f8_wide_kernel(const WidePara
             if (++b == p.blocks) {
                 b = 0; t += step;
                 any = t < tiles;
-                if (any) tile = wide_tile<CG>(p, first_tile, t);
+                if (any) tile = tile_at(p.tiles, first_tile, t);
             }
         };
         const int total = first < tiles ? (tiles - 1 - first) / step + 1 : 0;
@@ -262,7 +184,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) f8_wide_kernel(const WidePara
         // A warp has the 32 lanes of its quarter (warp & 3) and one half of the columns.
         const int taker = warp - 4, quarter = warp & 3, half = taker >> 2;
         const unsigned at = tmem + ((unsigned)(quarter * 32) << 16) + 128u * half;
-        const unsigned full0 = held_address(&sums_full[0]), given0 = CG == 1 ? held_address(&sums_empty[0]) : cluster_place(smem_u32(&sums_empty[0]), 0);
+        const unsigned full0 = held_address(&sums_full[0]), given0 = cluster_place(smem_u32(&sums_empty[0]), 0);
         const unsigned factors = held_address(scales) + 8u * (quarter * 32 + lane) + (GATED ? 0u : 4u * half);
         unsigned char* const out = staging + taker * 32 * kStageRow;
         unsigned buffer = 0, par = 0, slot = 0;
@@ -288,7 +210,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) f8_wide_kernel(const WidePara
                     if (c == 7) {   // all of them are in registers: the buffer is free
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                         __syncwarp();
-                        if (lane == 0) { if (CG == 1) arrive(given0 + 8u * buffer); else arrive_cluster(given0 + 8u * buffer); }
+                        if (lane == 0) arrive_cluster(given0 + 8u * buffer);
                     }
 #pragma unroll
                     for (int i = 0; i < 8; ++i) add_scaled(acc[8 * c + i], v[2 * i], v[2 * i + 1], c < 4 ? low : high);
@@ -298,7 +220,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) f8_wide_kernel(const WidePara
                 slot = (slot + 1024u) & (1024u * kScaleDepth - 1u);
             }
             if (!ok) break;
-            const WideTile done = wide_tile<CG>(p, first_tile, t);
+            const Tile done = tile_at(p.tiles, first_tile, t);
             // ---- results: value i of the thread is column col0 + i of its row ----
             constexpr int VALUES = GATED ? 64 : 128;
             float value[VALUES];
@@ -382,28 +304,27 @@ __global__ void __launch_bounds__(kWideThreads, 1) f8_wide_kernel(const WidePara
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (CG == 2) cg::this_cluster().sync();   // no MMA of the pair reads tensor memory or arrives at a barrier of a CTA that has left
+    cg::this_cluster().sync();   // no MMA of the pair reads tensor memory or arrives at a barrier of a CTA that has left
     if (warp == 1) {
-        if (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * kAccCols) : "memory");
-        else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * kAccCols) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * kAccCols) : "memory");
     }
 }
 
 // ---- launches ----------------------------------------------------------------------------------------------------------------
-template <int CG, bool GATED>
+template <bool GATED>
 int wide_attr() {
-    SWLM_CUDA(cudaFuncSetAttribute(f8_wide_kernel<CG, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)wide_smem<CG>()));
+    SWLM_CUDA(cudaFuncSetAttribute(f8_wide_kernel<GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kWideSmem));
     return SWLM_OK;
 }
 
-template <int CG, bool GATED>
+template <bool GATED>
 int wide_launch(const swlm_f8_product& a, int* status, cudaStream_t s) {
     constexpr int COLS = GATED ? 128 : 256;
     WideParams p{};
     p.x_scale = a.x.scale; p.x_scale_stride = a.x.scale_stride; p.w_scale = a.w.scale; p.up_scale = a.up.scale;
     p.y = static_cast<unsigned char*>(a.y); p.y_stride = a.y_stride; p.y_scale = a.y_scale; p.y_scale_stride = a.y_scale_stride;
-    p.offsets = a.offsets; p.status = status; p.rows = a.rows; p.n = a.n; p.blocks = f8_blocks(a.k); p.experts = a.experts;
-    p.col_blocks = f8_blocks(a.n); p.col_tiles = (a.n + COLS - 1) / COLS; p.dtype = a.dtype; p.act = a.act; p.alpha = a.alpha; p.limit = a.limit;
+    p.tiles = {a.offsets, a.rows, a.experts, 256, (a.n + COLS - 1) / COLS}; p.status = status; p.n = a.n; p.blocks = f8_blocks(a.k);
+    p.col_blocks = f8_blocks(a.n); p.dtype = a.dtype; p.act = a.act; p.alpha = a.alpha; p.limit = a.limit;
     const int64_t matrix_rows = (int64_t)std::max(a.experts, 1) * a.n;
     CUtensorMap xmap, wmap, upmap;
     int rc = code_map(a.x.codes, a.x.stride, a.rows, a.k, 128, &xmap);
@@ -412,24 +333,58 @@ int wide_launch(const swlm_f8_product& a, int* status, cudaStream_t s) {
     if (!rc && GATED) rc = code_map(a.up.codes, a.up.stride, matrix_rows, a.k, 64, &upmap);
     if (rc) return rc;
     // (at most this many tiles: an expert's last one may have a single row)
-    const int64_t tiles = std::min<int64_t>(((int64_t)a.rows / (128 * CG) + std::max(a.experts, 1)) * p.col_tiles, kSms / CG);
-    const cudaError_t e = launch_clusters(f8_wide_kernel<CG, GATED>, CG, dim3((unsigned)(CG * tiles)), dim3(kWideThreads), wide_smem<CG>(), s, p, xmap, wmap, upmap);
+    const int64_t tiles = std::min<int64_t>(((int64_t)a.rows / 256 + std::max(a.experts, 1)) * p.tiles.col_tiles, kSms / 2);
+    const cudaError_t e = launch_clusters(f8_wide_kernel<GATED>, 2, dim3((unsigned)(2 * tiles)), dim3(kWideThreads), kWideSmem, s, p, xmap, wmap, upmap);
     return e == cudaSuccess ? SWLM_OK : cuda_fail(e, "product launch");
+}
+
+// What a product takes, about (us): a block 0.38 while the pairs are few, 0.47 with all of them reading from L2, a tile's start and end 6; weights that are
+// read once come from memory at 3.2 TB/s.
+double wide_cost(int rows, int n, int k, int experts, bool gated) {
+    const int cols = gated ? 128 : 256, reached = experts ? std::min(experts, rows) : 1;
+    const double row_tiles = experts ? rows / 256.0 + 0.5 * reached : (rows + 255) / 256, tiles = row_tiles * ((n + cols - 1) / cols), pairs = kSms / 2;
+    const double waves = experts ? std::max(1.0, tiles / pairs) : (double)(int64_t)((tiles + pairs - 1) / pairs);
+    return std::max(waves * (f8_blocks(k) * (tiles > pairs / 2 ? 0.47 : 0.38) + 2), (double)reached * n * k * (gated ? 2 : 1) / 3.2e6) + 4;
 }
 
 }  // namespace
 
 int f8_product_init() {
     int rc;
-    if ((rc = f8_few_init()) || (rc = wide_attr<1, false>()) || (rc = wide_attr<1, true>()) || (rc = wide_attr<2, false>()) || (rc = wide_attr<2, true>())) return rc;
+    if ((rc = f8_few_init()) || (rc = wide_attr<false>()) || (rc = wide_attr<true>())) return rc;
     return SWLM_OK;
 }
 
 int launch_f8_product(const swlm_f8_product& a, int* status, cudaStream_t s) {
     if (a.rows == 0) return SWLM_OK;
-    const int each = (a.rows + std::max(a.experts, 1) - 1) / std::max(a.experts, 1);
-    if (each <= 128) return launch_f8_few(a, status, s);
-    return a.act != SWLM_F8_PLAIN ? wide_launch<2, true>(a, status, s) : wide_launch<2, false>(a, status, s);
+    const bool gated = a.act != SWLM_F8_PLAIN;
+    const F8FewForm few = f8_few_form(a.rows, a.n, a.k, a.experts, gated);
+    const double wide = wide_cost(a.rows, a.n, a.k, a.experts, gated), best = std::min(few.cost, wide);
+    // A last wave of few tiles leaves most pairs without work: the columns that fill whole waves may go first, and the rest as a product of its own, dealt out
+    // along K (777 rows x 5000 x 4100: 80 tiles on 74 pairs 38 us, 72 and 392 columns more 31).
+    const int cols = gated ? 128 : 256, row_tiles = (a.rows + 255) / 256, pairs = kSms / 2, waves = (int)((int64_t)row_tiles * ((a.n + cols - 1) / cols) / pairs);
+    const int full = (int)std::min<int64_t>((int64_t)waves * pairs / row_tiles * cols, a.n);
+    if (!a.experts && full > 0 && full < a.n) {
+        const F8FewForm last = f8_few_form(a.rows, a.n - full, a.k, 0, gated);
+        if (wide_cost(a.rows, full, a.k, 0, gated) + last.cost < best) {
+            swlm_f8_product head = a, tail = a;
+            head.n = full;
+            tail.n = a.n - full;
+            const int64_t codes = (int64_t)full, scales = (int64_t)(full / kF8Block) * f8_blocks(a.k);
+            tail.w.codes = static_cast<const unsigned char*>(a.w.codes) + codes * a.w.stride;
+            tail.w.scale += scales;
+            if (gated) {
+                tail.up.codes = static_cast<const unsigned char*>(a.up.codes) + codes * a.up.stride;
+                tail.up.scale += scales;
+            }
+            tail.y = static_cast<unsigned char*>(a.y) + codes * f8_size(a.dtype);
+            if (a.dtype == SWLM_F8_E4M3) tail.y_scale += full / kF8Block * a.y_scale_stride;
+            const int rc = gated ? wide_launch<true>(head, status, s) : wide_launch<false>(head, status, s);
+            return rc ? rc : launch_f8_few(tail, last, status, s);
+        }
+    }
+    if (few.cost <= wide) return launch_f8_few(a, few, status, s);
+    return gated ? wide_launch<true>(a, status, s) : wide_launch<false>(a, status, s);
 }
 
 }  // namespace swlm
