@@ -14,7 +14,7 @@ namespace {
 // A stable counting sort by one cluster: every warp has a run of neighbouring pairs and counts its experts; sums over warps and, through distributed
 // shared memory, over the cluster's CTAs give every warp its first row of every expert; then it numbers its pairs, 32 at a time, by those before
 // them of the same expert. No number depends on the order in which warps get there.
-constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortUnroll = 4, kSortCtas = 16;
+constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortUnroll = 8, kSortCtas = 16;
 
 __global__ void __launch_bounds__(kSortThreads) expert_sort_kernel(const swlm_expert_sort a) {
     extern __shared__ int counts[];        // [kSortWarps][experts]: pairs of each warp, then each warp's next row
@@ -27,13 +27,20 @@ __global__ void __launch_bounds__(kSortThreads) expert_sort_kernel(const swlm_ex
     int* const mine = counts + warp * E;
     for (int i = tid; i < kSortWarps * E; i += kSortThreads) counts[i] = 0;
     __syncthreads();
-    for (int i = first + lane; i < last; i += 32 * kSortUnroll) {
-        int e[kSortUnroll];
+    int e[kSortUnroll];   // choices of the pairs in question, -1 for none; where a warp has no more than these they are read once
+    auto read = [&](int i0) {
 #pragma unroll
-        for (int u = 0; u < kSortUnroll; ++u) e[u] = i + 32 * u < last ? a.choice[i + 32 * u] : -1;
+        for (int u = 0; u < kSortUnroll; ++u) {
+            const int i = i0 + 32 * u + lane;
+            e[u] = i < last ? a.choice[i] : -1;
+            if (e[u] >= E) e[u] = -1;
+        }
+    };
+    for (int i0 = first; i0 < last; i0 += 32 * kSortUnroll) {
+        read(i0);
 #pragma unroll
         for (int u = 0; u < kSortUnroll; ++u)
-            if (e[u] >= 0 && e[u] < E) atomicAdd(mine + e[u], 1);
+            if (e[u] >= 0) atomicAdd(mine + e[u], 1);
     }
     __syncthreads();
     int sum = 0;   // of expert `tid`
@@ -83,13 +90,7 @@ __global__ void __launch_bounds__(kSortThreads) expert_sort_kernel(const swlm_ex
     __syncthreads();
     for (int i = rows + rank * kSortThreads + tid; i < pairs; i += ctas * kSortThreads) a.source[i] = -1;
     for (int i0 = first; i0 < last; i0 += 32 * kSortUnroll) {
-        int e[kSortUnroll];
-#pragma unroll
-        for (int u = 0; u < kSortUnroll; ++u) {
-            const int i = i0 + 32 * u + lane;
-            e[u] = i < last ? a.choice[i] : -1;
-            if (e[u] >= E) e[u] = -1;
-        }
+        if (each > 32 * kSortUnroll) read(i0);
 #pragma unroll
         for (int u = 0; u < kSortUnroll; ++u) {
             const int i = i0 + 32 * u + lane;

@@ -91,6 +91,7 @@ __device__ __forceinline__ float gated(float g, float u, int act, float alpha, f
 }
 
 // Work as tiles of `rows` rows x a tile of columns, those of one expert after those of the other (experts 0: one has all rows). CTAs take them in turn.
+constexpr int kSweep = 8;
 struct TileShape { const int* offsets; int rows, experts, tile_rows, col_tiles; };
 struct Tile { int expert, row0, end, col; };   // rows row0 .. end - 1 (of which a tile has tile_rows at most), tile of columns
 
@@ -148,11 +149,15 @@ __device__ __forceinline__ Tile tile_at(const TileShape& p, const int* first_til
         w.expert = lo; w.row0 = r.x; w.end = r.y;
         t -= first_tile[lo];
     }
-    // the shorter side first: what it sweeps stays in L2
-    const int row_tiles = (w.end - w.row0 + p.tile_rows - 1) / p.tile_rows;
-    int r;
-    if (row_tiles <= p.col_tiles) { r = t % row_tiles; w.col = t / row_tiles; }
-    else { w.col = t % p.col_tiles; r = t / p.col_tiles; }
+    // Up to kSweep tiles of the shorter side, then those of the next place on the longer one: what CTAs at work together read is about as much of x as of the
+    // matrix, and stays in L2 (8192 rows x 4096 x 14336 with all 16 tiles of columns in a sweep read 526 MB from memory instead of the 175 there are).
+    const int row_tiles = (w.end - w.row0 + p.tile_rows - 1) / p.tile_rows, shorter = min(row_tiles, p.col_tiles), longer = max(row_tiles, p.col_tiles);
+    const int sweep = t / (kSweep * longer), width = min(kSweep, shorter - sweep * kSweep);
+    t -= sweep * kSweep * longer;
+    const int a = sweep * kSweep + t % width, b = t / width;
+    const bool rows_first = row_tiles <= p.col_tiles;
+    w.col = rows_first ? b : a;
+    const int r = rows_first ? a : b;
     w.row0 += r * p.tile_rows;
     return w;
 }

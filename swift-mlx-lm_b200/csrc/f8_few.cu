@@ -63,11 +63,31 @@ f8_few_kernel(const FewParams p, const __grid_constant__ CUtensorMap xmap, const
     const int range = (int)(blockIdx.x % p.ranges), first = (int)(blockIdx.x / p.ranges), step = (int)(gridDim.x / p.ranges);
     const int block0 = (int)((long long)p.blocks * range / p.ranges), blocks = (int)((long long)p.blocks * (range + 1) / p.ranges) - block0;
     pdl_wait();
-    if (tid == 0) {
-        for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        for (int i = 0; i < BUFFERS; ++i) { mbar_init(&sums_full[i], 1 + 1); mbar_init(&sums_empty[i], F::TAKERS); }
-        failed_word = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    auto load = [&](const Tile& tile, int b, int s) {   // by one thread
+        const unsigned dst = smem_u32(ring) + s * STAGE, bar = smem_u32(&full[s]);
+        const int col = (block0 + b) * kF8Block, w_row = tile.expert * p.n + tile.col * 128;
+        mbar_expect(bar, (unsigned)STAGE);
+        tma_load_2d(dst, &wmap, col, w_row, bar);
+        if (GATED) tma_load_2d(dst + kCodesBytes, &upmap, col, w_row, bar);
+        tma_load_2d(dst + MATS * kCodesBytes, &xmap, col, tile.row0, bar);
+    };
+    int early = 0;   // blocks of the first tile that are asked for before anything else is set up, where no table is needed to say which they are
+    if (warp == 0) {
+        if (lane == 0) {
+            for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+            for (int i = 0; i < BUFFERS; ++i) { mbar_init(&sums_full[i], 1 + 1); mbar_init(&sums_empty[i], F::TAKERS); }
+            failed_word = 0;
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        __syncwarp();
+        if (!p.tiles.experts && first < (p.tiles.rows + NT - 1) / NT * p.tiles.col_tiles) {
+            early = min(STAGES, blocks);
+            if (elect_one()) {
+                const Tile tile = tile_at(p.tiles, first_tile, first);
+                for (int b = 0; b < early; ++b) load(tile, b, b);
+            }
+            __syncwarp();
+        }
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(F::TMEM) : "memory");
@@ -87,23 +107,15 @@ f8_few_kernel(const FewParams p, const __grid_constant__ CUtensorMap xmap, const
 
     if (warp == 0) {
         const bool el = elect_one();
-        const unsigned full0 = held_address(&full[0]), empty0 = held_address(&empty[0]), at = held_address(ring);
-        int s = 0, issued = 0;
-        unsigned par = 1;
+        const unsigned full0 = held_address(&full[0]), empty0 = held_address(&empty[0]);
+        int s = early % STAGES, issued = early;
+        unsigned par = early == STAGES ? 0u : 1u;
         bool ok = true;
         for (int t = first; t < tiles; t += step) {
             const Tile tile = tile_at(p.tiles, first_tile, t);
-            const int w_row = tile.expert * p.n + tile.col * 128;
-            for (int b = 0; b < blocks && ok; ++b) {
+            for (int b = t == first ? early : 0; b < blocks && ok; ++b) {
                 if (!(ok = mbar_wait_warp(empty0 + 8u * s, par))) break;
-                if (el) {
-                    const unsigned dst = at + s * STAGE, bar = full0 + 8u * s;
-                    const int col = (block0 + b) * kF8Block;
-                    mbar_expect(bar, (unsigned)STAGE);
-                    tma_load_2d(dst, &wmap, col, w_row, bar);
-                    if (GATED) tma_load_2d(dst + kCodesBytes, &upmap, col, w_row, bar);
-                    tma_load_2d(dst + MATS * kCodesBytes, &xmap, col, tile.row0, bar);
-                }
+                if (el) load(tile, b, s);
                 __syncwarp();
                 ++issued;
                 if (++s == STAGES) { s = 0; par ^= 1u; }
