@@ -426,7 +426,8 @@ int swlm_op_kv8_lengths_dev(swlm_ctx* ctx, int batch, const int32_t* in, const i
  *
  * A held value is code * scale: rows have a scale per row and 128 columns, matrices one per 128 rows and 128 columns. All calls are enqueued on
  * `cuda_stream` (NULL = the context's own stream) without synchronising and without allocating, read choices and offsets on the device, and can be
- * captured into a graph. Pointers are device memory of the context's device. Calls at once may share what they only read; none has scratch. */
+ * captured into a graph. Pointers are device memory of the context's device, and are not looked at where there are no rows (tokens). Calls at once may
+ * share what they only read; none has scratch. */
 enum { SWLM_F8_BF16 = 0, SWLM_F8_FP16 = 1, SWLM_F8_FP32 = 2, SWLM_F8_E4M3 = 3 };   /* type of rows */
 enum { SWLM_F8_PLAIN = 0, SWLM_F8_SILU = 1, SWLM_F8_GELU = 2, SWLM_F8_CLAMPED = 3 };   /* swlm_f8_product.act */
 
@@ -443,7 +444,8 @@ typedef struct swlm_f8_weight {
     int64_t stride;         /* a multiple of 16 */
 } swlm_f8_weight;
 
-/* Row r of the result are the codes of row source[r] of x (NULL: row r; where source[r] is not within 0..x_rows-1 the row stays as it is). The
+/* Row r of the result are the codes of row source[r] of x (NULL: row r; where source[r] is not within 0..x_rows-1 the row stays as it is; out is not memory
+ * that the call reads). The
  * scale of 128 columns is the smallest power of two that is at least their largest |value| / 448, and not below 2^-126: a code is the e4m3 number nearest to
  * value / scale, ties to even, and nothing else is rounded. Columns among which is an infinity or a NaN get NaN as scale and codes. */
 typedef struct swlm_f8_quantize {
@@ -481,6 +483,9 @@ typedef struct swlm_f8_product {
     float alpha, limit;
 } swlm_f8_product;
 int swlm_op_f8_product_dev(swlm_ctx* ctx, const swlm_f8_product* how, void* cuda_stream);
+/* The form that a product takes, for tests that mean a certain one: form = {columns that pairs of SMs take in tiles of 256 rows, rows of a tile of the others (0:
+ * there are none), CTAs that share K for those}. */
+int swlm_op_f8_product_form(int rows, int n, int k, int experts, int gated, int* form);
 /* SWLM_ERR_TIMEOUT where a wait of the context's products has expired since the last call, which it forgets then. It does not wait: call it behind a
  * synchronisation of the streams in question. The replays of a captured product report nothing themselves, so whoever replays one asks here. */
 int swlm_op_f8_status(swlm_ctx* ctx);

@@ -1,5 +1,6 @@
 // Rows sorted by expert, and back at their tokens, weighted and added up.
 #include <algorithm>
+#include <atomic>
 
 #include <cooperative_groups.h>
 
@@ -224,22 +225,32 @@ template <int Y> void (*sum_kernel(int dtype))(swlm_expert_sum) {
 
 }  // namespace
 
+static std::atomic<int> g_sort_ctas{kSortCtas};   // most CTAs of a cluster that all devices in use take
+
 int expert_rows_init() {
     SWLM_CUDA(cudaFuncSetAttribute(expert_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortWarps * kExpertMax * 4));
     SWLM_CUDA(cudaFuncSetAttribute(expert_sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    // clusters of sixteen are not promised: a device that takes none does with eight
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kSortCtas; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(kSortCtas); cfg.blockDim = dim3(kSortThreads); cfg.dynamicSmemBytes = kSortWarps * kExpertMax * 4; cfg.attrs = attr; cfg.numAttrs = 1;
+    int fit = 0;
+    if (cudaOccupancyMaxActiveClusters(&fit, expert_sort_kernel, &cfg) != cudaSuccess) { cudaGetLastError(); fit = 0; }
+    if (fit < 1) g_sort_ctas.store(8, std::memory_order_relaxed);
     return SWLM_OK;
 }
 
 int launch_expert_sort(const swlm_expert_sort& a, cudaStream_t s) {
     const long long pairs = (long long)a.tokens * a.top;
     int ctas = 1;
-    while (ctas < kSortCtas && pairs > (long long)ctas * 2 * kSortThreads) ctas *= 2;
+    while (ctas < g_sort_ctas.load(std::memory_order_relaxed) && pairs > (long long)ctas * 2 * kSortThreads) ctas *= 2;
     const cudaError_t e = launch_clusters(expert_sort_kernel, ctas, dim3(ctas), dim3(kSortThreads), (size_t)kSortWarps * a.experts * 4, s, a);
     return e == cudaSuccess ? SWLM_OK : cuda_fail(e, "expert sort launch");
 }
 
 int launch_expert_sum(const swlm_expert_sum& a, cudaStream_t s) {
-    if (a.tokens == 0) return SWLM_OK;
     const long long threads = (long long)a.tokens * ((a.width + 7) / 8), ctas = (threads + kSumThreads - 1) / kSumThreads;
     if (ctas > 0x7FFFFFFFll) { set_error("f8: too many tokens for a width of %d", a.width); return SWLM_ERR_INVALID; }
     void (*kernel)(swlm_expert_sum) = a.y_dtype == SWLM_F8_FP32 ? sum_kernel<SWLM_F8_FP32>(a.dtype) : a.y_dtype == SWLM_F8_FP16 ? sum_kernel<SWLM_F8_FP16>(a.dtype) : sum_kernel<SWLM_F8_BF16>(a.dtype);

@@ -1,6 +1,7 @@
 // Rows in 8-bit floating point (quantization), and what the calls over such rows check. A code is value / scale rounded once: scales are powers of two, so the
 // quotient is exact, and results do not depend on the launch.
 #include <algorithm>
+#include <climits>
 #include <cmath>
 #include <type_traits>
 
@@ -87,7 +88,6 @@ __global__ void __launch_bounds__(kQuantThreads) f8_quantize_kernel(const swlm_f
 }  // namespace
 
 int launch_f8_quantize(const swlm_f8_quantize& a, cudaStream_t s) {
-    if (a.rows == 0) return SWLM_OK;
     const dim3 grid((a.rows + kQuantWarps - 1) / kQuantWarps, (f8_blocks(a.width) + kQuantBlocks - 1) / kQuantBlocks);
     void (*kernel)(swlm_f8_quantize) = a.dtype == SWLM_F8_FP32 ? f8_quantize_kernel<SWLM_F8_FP32> : a.dtype == SWLM_F8_FP16 ? f8_quantize_kernel<SWLM_F8_FP16> : f8_quantize_kernel<SWLM_F8_BF16>;
     const cudaError_t e = launch_k(kernel, grid, dim3(kQuantThreads), 0, s, a);
@@ -142,6 +142,7 @@ int swlm_op_f8_quantize_dev(swlm_ctx* ctx, const swlm_f8_quantize* how, void* cu
     if (a.rows < 0 || a.rows > kF8MaxRows || a.x_rows < 0 || a.x_rows > kF8MaxRows || a.width < 1 || a.width > kF8MaxWidth) return refuse("rows or width out of range");
     if (!a.source && a.x_rows < a.rows) return refuse("x has too few rows");
     if (!aligned(a.source, 4)) return refuse("source must be 4-byte aligned");
+    if (a.rows == 0 || a.x_rows == 0) return SWLM_OK;   // (no row of the result changes)
     if (!rows_ok(a.x, a.x_stride, a.width, f8_size(a.dtype))) return refuse("rows of x must be 16-byte aligned, their stride at least the width");
     const int rc = codes_ok(a.out, a.rows, a.width);
     if (rc) return rc;
@@ -157,15 +158,25 @@ int swlm_op_f8_product_dev(swlm_ctx* ctx, const swlm_f8_product* how, void* cuda
     if (a.rows < 0 || a.rows > kF8MaxRows || a.n < 1 || a.n > kF8MaxWidth || a.k < 1 || a.k > kF8MaxWidth) return refuse("rows, n or k out of range");
     if (a.experts < 0 || a.experts > kExpertMax) return refuse("experts out of range");
     if ((int64_t)std::max(a.experts, 1) * a.n > kF8MaxRows) return refuse("too many rows of all experts' matrices");
+    if (a.act == SWLM_F8_CLAMPED && (!std::isfinite(a.alpha) || !(a.limit >= 0.f))) return refuse("alpha must be finite, the limit not negative");
+    // (tiles are 32-bit numbers, also where offsets do not ascend and every expert has all rows)
+    if ((int64_t)std::max(a.experts, 1) * (a.rows / 16 + 1) * f8_blocks(a.n) > INT32_MAX) return refuse("too many rows, experts and columns together");
+    if (a.rows == 0) return SWLM_OK;
     if (a.experts && (!a.offsets || !aligned(a.offsets, 4))) return refuse("experts need offsets, 4-byte aligned");
     int rc = codes_ok(a.x, a.rows, a.k);
     if (rc || (rc = matrix_ok(a.w, a.k)) || (a.act != SWLM_F8_PLAIN && (rc = matrix_ok(a.up, a.k)))) return rc;
-    if (a.act == SWLM_F8_CLAMPED && (!std::isfinite(a.alpha) || !(a.limit >= 0.f))) return refuse("alpha must be finite, the limit not negative");
     if (!rows_ok(a.y, a.y_stride, a.n, f8_size(a.dtype))) return refuse("rows of y must be 16-byte aligned, their stride at least n");
     if (a.dtype == SWLM_F8_E4M3 && (!a.y_scale || !aligned(a.y_scale, 4) || a.y_scale_stride < a.rows || a.y_scale_stride > kMaxStride)) return refuse("codes need scales, 4-byte aligned, their stride at least the rows");
     SWLM_CUDA(cudaSetDevice(ctx->device));
     if ((rc = expired(__atomic_load_n(ctx->f8_status, __ATOMIC_RELAXED)))) return rc;
     return launch_f8_product(a, ctx->f8_status, stream_of(ctx, cuda_stream));
+}
+
+int swlm_op_f8_product_form(int rows, int n, int k, int experts, int gated, int* form) {
+    if (rows < 1 || rows > kF8MaxRows || n < 1 || n > kF8MaxWidth || k < 1 || k > kF8MaxWidth || experts < 0 || experts > kExpertMax || !form) return refuse("bad argument");
+    const F8ProductForm f = f8_product_form(rows, n, k, experts, gated != 0);
+    form[0] = f.wide; form[1] = f.wide == n ? 0 : f.few.nt; form[2] = f.wide == n ? 0 : f.few.ranges;
+    return SWLM_OK;
 }
 
 int swlm_op_f8_status(swlm_ctx* ctx) {
@@ -183,7 +194,7 @@ int swlm_op_expert_sort_dev(swlm_ctx* ctx, const swlm_expert_sort* how, void* cu
     if (!ctx || !how) return refuse("null argument");
     const swlm_expert_sort& a = *how;
     if (a.tokens < 0 || a.top < 1 || a.experts < 1 || a.experts > kExpertMax || (int64_t)a.tokens * a.top > kF8MaxRows) return refuse("tokens, top or experts out of range");
-    if (!a.choice || !a.offsets || !a.source || !a.place) return refuse("null argument");
+    if (!a.offsets || (a.tokens && (!a.choice || !a.source || !a.place))) return refuse("null argument");
     if (!aligned(a.choice, 4) || !aligned(a.offsets, 4) || !aligned(a.source, 4) || !aligned(a.place, 4)) return refuse("choices, offsets, source and place must be 4-byte aligned");
     SWLM_CUDA(cudaSetDevice(ctx->device));
     return launch_expert_sort(a, stream_of(ctx, cuda_stream));
@@ -195,8 +206,9 @@ int swlm_op_expert_sum_dev(swlm_ctx* ctx, const swlm_expert_sum* how, void* cuda
     if (!plain_type(a.dtype) || !plain_type(a.y_dtype)) return refuse("unknown dtype");
     if (a.tokens < 0 || a.top < 1 || (int64_t)a.tokens * a.top > kF8MaxRows || a.width < 1 || a.width > kF8MaxWidth || a.y_rows < 0 || a.y_rows > kF8MaxRows)
         return refuse("tokens, top, width or rows out of range");
+    if (a.tokens == 0) return SWLM_OK;
     if (!a.place || !a.weight || !aligned(a.place, 4) || !aligned(a.weight, 4)) return refuse("places and weights must be there, 4-byte aligned");
-    if (!rows_ok(a.y, a.y_stride, a.width, f8_size(a.y_dtype)) || !rows_ok(a.out, a.out_stride, a.width, f8_size(a.dtype)) ||
+    if ((a.y_rows && !rows_ok(a.y, a.y_stride, a.width, f8_size(a.y_dtype))) || !rows_ok(a.out, a.out_stride, a.width, f8_size(a.dtype)) ||
         (a.add && !rows_ok(a.add, a.add_stride, a.width, f8_size(a.dtype)))) return refuse("rows of y, add and out must be 16-byte aligned, their strides at least the width");
     SWLM_CUDA(cudaSetDevice(ctx->device));
     return launch_expert_sum(a, stream_of(ctx, cuda_stream));

@@ -12,6 +12,11 @@ constexpr int kF8MaxRows = 1 << 30;      // row numbers stay 32-bit ones, also a
 constexpr int kF8MaxWidth = 1 << 24;
 constexpr int kExpertMax = 1024;
 
+// A product of few rows: rows of x per tile, CTAs of a cluster that share K, and what it takes, about (us).
+struct F8FewForm { int nt, ranges; double cost; };
+// How a product runs: so many columns by pairs of SMs (many rows), the others, if any, in the form of few.
+struct F8ProductForm { int wide = 0; F8FewForm few{}; };
+F8ProductForm f8_product_form(int rows, int n, int k, int experts, bool gated);
 int f8_product_init();
 int expert_rows_init();
 int launch_f8_quantize(const swlm_f8_quantize& a, cudaStream_t s);

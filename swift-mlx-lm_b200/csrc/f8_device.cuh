@@ -178,8 +178,6 @@ inline int code_map(const void* p, int64_t stride, int64_t rows, int k, int box_
 
 }  // namespace f8
 
-// A product of few rows: rows of x per tile, CTAs of a cluster that share K, and what it takes, about (us).
-struct F8FewForm { int nt, ranges; double cost; };
 F8FewForm f8_few_form(int rows, int n, int k, int experts, bool gated);
 int f8_few_init();
 int launch_f8_few(const swlm_f8_product& a, const F8FewForm& form, int* status, cudaStream_t s);

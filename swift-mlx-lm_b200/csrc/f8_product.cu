@@ -355,36 +355,41 @@ int f8_product_init() {
     return SWLM_OK;
 }
 
-int launch_f8_product(const swlm_f8_product& a, int* status, cudaStream_t s) {
-    if (a.rows == 0) return SWLM_OK;
-    const bool gated = a.act != SWLM_F8_PLAIN;
-    const F8FewForm few = f8_few_form(a.rows, a.n, a.k, a.experts, gated);
-    const double wide = wide_cost(a.rows, a.n, a.k, a.experts, gated), best = std::min(few.cost, wide);
+F8ProductForm f8_product_form(int rows, int n, int k, int experts, bool gated) {
+    F8ProductForm f;
+    f.few = f8_few_form(rows, n, k, experts, gated);
+    const double wide = wide_cost(rows, n, k, experts, gated);
+    f.wide = f.few.cost > wide ? n : 0;
     // A last wave of few tiles leaves most pairs without work: the columns that fill whole waves may go first, and the rest as a product of its own, dealt out
-    // along K (777 rows x 5000 x 4100: 80 tiles on 74 pairs 38 us, 72 and 392 columns more 31).
-    const int cols = gated ? 128 : 256, row_tiles = (a.rows + 255) / 256, pairs = kSms / 2, waves = (int)((int64_t)row_tiles * ((a.n + cols - 1) / cols) / pairs);
-    const int full = (int)std::min<int64_t>((int64_t)waves * pairs / row_tiles * cols, a.n);
-    if (!a.experts && full > 0 && full < a.n) {
-        const F8FewForm last = f8_few_form(a.rows, a.n - full, a.k, 0, gated);
-        if (wide_cost(a.rows, full, a.k, 0, gated) + last.cost < best) {
-            swlm_f8_product head = a, tail = a;
-            head.n = full;
-            tail.n = a.n - full;
-            const int64_t codes = (int64_t)full, scales = (int64_t)(full / kF8Block) * f8_blocks(a.k);
-            tail.w.codes = static_cast<const unsigned char*>(a.w.codes) + codes * a.w.stride;
-            tail.w.scale += scales;
-            if (gated) {
-                tail.up.codes = static_cast<const unsigned char*>(a.up.codes) + codes * a.up.stride;
-                tail.up.scale += scales;
-            }
-            tail.y = static_cast<unsigned char*>(a.y) + codes * f8_size(a.dtype);
-            if (a.dtype == SWLM_F8_E4M3) tail.y_scale += full / kF8Block * a.y_scale_stride;
-            const int rc = gated ? wide_launch<true>(head, status, s) : wide_launch<false>(head, status, s);
-            return rc ? rc : launch_f8_few(tail, last, status, s);
-        }
+    // along K (777 rows x 5000 x 4100: 80 tiles on 74 pairs 37.8 us, 72 tiles and 392 columns more 36.0).
+    const int cols = gated ? 128 : 256, row_tiles = (rows + 255) / 256, pairs = kSms / 2, waves = (int)((int64_t)row_tiles * ((n + cols - 1) / cols) / pairs);
+    const int full = (int)std::min<int64_t>((int64_t)waves * pairs / row_tiles * cols, n);
+    if (!experts && full > 0 && full < n) {
+        const F8FewForm last = f8_few_form(rows, n - full, k, 0, gated);
+        if (wide_cost(rows, full, k, 0, gated) + last.cost < std::min(f.few.cost, wide)) f = {full, last};
     }
-    if (few.cost <= wide) return launch_f8_few(a, few, status, s);
-    return gated ? wide_launch<true>(a, status, s) : wide_launch<false>(a, status, s);
+    return f;
+}
+
+int launch_f8_product(const swlm_f8_product& a, int* status, cudaStream_t s) {
+    const bool gated = a.act != SWLM_F8_PLAIN;
+    const F8ProductForm form = f8_product_form(a.rows, a.n, a.k, a.experts, gated);
+    if (form.wide == 0) return launch_f8_few(a, form.few, status, s);
+    swlm_f8_product head = a, tail = a;
+    head.n = form.wide;
+    const int rc = gated ? wide_launch<true>(head, status, s) : wide_launch<false>(head, status, s);
+    if (rc || form.wide == a.n) return rc;
+    const int64_t scales = (int64_t)(form.wide / kF8Block) * f8_blocks(a.k);
+    tail.n = a.n - form.wide;
+    tail.w.codes = static_cast<const unsigned char*>(a.w.codes) + form.wide * a.w.stride;
+    tail.w.scale += scales;
+    if (gated) {
+        tail.up.codes = static_cast<const unsigned char*>(a.up.codes) + form.wide * a.up.stride;
+        tail.up.scale += scales;
+    }
+    tail.y = static_cast<unsigned char*>(a.y) + (int64_t)form.wide * f8_size(a.dtype);
+    if (a.dtype == SWLM_F8_E4M3) tail.y_scale += form.wide / kF8Block * a.y_scale_stride;
+    return launch_f8_few(tail, form.few, status, s);
 }
 
 }  // namespace swlm

@@ -286,6 +286,7 @@ SIGNATURES = {
     "swlm_op_kv8_lengths_dev": (_I, [_P, _I, _P, _P, _I, _I, _P, _P, _P]),
     "swlm_op_f8_quantize_dev": (_I, [_P, C.POINTER(F8Quantize), _P]),
     "swlm_op_f8_product_dev": (_I, [_P, C.POINTER(F8Product), _P]),
+    "swlm_op_f8_product_form": (_I, [_I, _I, _I, _I, _I, _P]),
     "swlm_op_f8_status": (_I, [_P]),
     "swlm_write_f8_status": (_I, [_P, _I]),
     "swlm_op_expert_sort_dev": (_I, [_P, C.POINTER(ExpertSort), _P]),

@@ -63,7 +63,8 @@ def test_matrices_that_are_refused(pkg, lib, bad):
                                  dict(rows=-1), dict(n=0), dict(k=0), dict(k=-8), dict(n=(1 << 24) + 16, y_stride=1 << 25), dict(experts=-1), dict(experts=1025, offsets=64),
                                  dict(experts=2), dict(experts=2, offsets=66), dict(dtype=3, y_scale=0), dict(dtype=3, y_scale=4097), dict(dtype=3, y_scale_stride=7),
                                  dict(act=3, alpha=float("nan")), dict(act=3, alpha=float("inf")), dict(act=3, limit=-1.0), dict(act=3, limit=float("nan")),
-                                 dict(experts=1024, offsets=64, n=1 << 21, y_stride=1 << 21)], ids=str)
+                                 dict(experts=1024, offsets=64, n=1 << 21, y_stride=1 << 21), dict(experts=1024, offsets=64, rows=1 << 29, n=4096, y_stride=4096, x=dict(scale_stride=1 << 29))],
+                         ids=str)
 def test_products_that_are_refused(pkg, lib, bad):
     assert lib.swlm_op_f8_product_dev(CTX, _product(pkg, **bad), None) == INVALID
 
@@ -91,3 +92,29 @@ def test_null_arguments(pkg, lib):
     assert lib.swlm_op_expert_sum_dev(None, _sum(pkg), None) == INVALID
     assert lib.swlm_op_expert_sum_dev(CTX, None, None) == INVALID
     assert lib.swlm_op_f8_status(None) == INVALID and lib.swlm_write_f8_status(None, 1) == INVALID
+
+
+def test_what_has_no_rows_is_not_looked_at(pkg, lib):
+    nothing = dict(codes=0, scale=0)
+    assert lib.swlm_op_f8_quantize_dev(CTX, _quantize(pkg, out=nothing, x=0, rows=0), None) == 0
+    assert lib.swlm_op_f8_quantize_dev(CTX, _quantize(pkg, out=nothing, x=0, x_rows=0, source=64), None) == 0
+    assert lib.swlm_op_f8_product_dev(CTX, _product(pkg, x=nothing, w=nothing, y=0, rows=0, experts=3), None) == 0
+    assert lib.swlm_op_expert_sum_dev(CTX, _sum(pkg, y=0, place=0, weight=0, out=0, tokens=0), None) == 0
+
+
+def test_forms(lib):
+    """The forms cover all columns; sizes out of range are refused."""
+    form = (C.c_int * 3)()
+    for rows in (1, 16, 17, 100, 777, 8192):
+        for n in (1, 128, 4096, 5000):
+            for k in (1, 129, 4100):
+                for experts in (0, 7):
+                    for gated in (0, 1):
+                        assert lib.swlm_op_f8_product_form(rows, n, k, experts, gated, form) == 0
+                        wide, tile, ctas = form
+                        assert 0 <= wide <= n and (wide == n) == (tile == 0) and (tile == 0) == (ctas == 0)
+                        assert tile in ((0, 16, 64) if gated else (0, 16, 32, 64, 128)) and ctas in (0, 1, 2, 4, 8) and wide % 128 * (n - wide) == 0
+                        assert experts == 0 or wide in (0, n)
+    for bad in ((0, 1, 1, 0), (1, 0, 1, 0), (1, 1, 0, 0), (1, 1, 1, -1), (1, 1, 1, 1025), ((1 << 30) + 1, 1, 1, 0)):
+        assert lib.swlm_op_f8_product_form(*bad[:3], bad[3], 0, form) == INVALID
+    assert lib.swlm_op_f8_product_form(1, 1, 1, 0, 0, None) == INVALID
