@@ -4,6 +4,8 @@
 // they are scaled and added; here the scales of the rows of x lie along a thread's registers. Where there are tiles for all SMs, CTAs take them in turn and
 // copies run ahead into the next tile. Where there are few, the blocks of K are dealt to the CTAs of a cluster: their parts then lie in shared memory, 128
 // columns of the result to a row of x, and a warp adds the cluster's parts of a row up in the order of the blocks.
+// What bounds it: memory, and what a launch takes to start and to end. One row x 4096 x 14336 takes 14.4 us of which its 59 MB are 9 (two, four, eight CTAs
+// along K: 21, 14.8, 15.1); 41 rows x 8192 x 2048, gated, 12.1 of 5.2; gate and up of 64 experts, 2048 x 1024, for 256 rows 52 (268 MB: 41).
 #include <algorithm>
 
 #include <cooperative_groups.h>
@@ -101,6 +103,9 @@ f8_few_kernel(const FewParams p, const __grid_constant__ CUtensorMap xmap, const
     const cg::cluster_group cluster = cg::this_cluster();
     auto fail = [&](int code) { if (lane == 0) { atomicExch_system(p.status, code); *failed = 1; } __syncwarp(); };
 
+    // A launch behind this one may set itself up (behind the allocation: it cannot get at tensor memory in between): 0.6 us of a chain of products. Not with
+    // experts, where its CTAs would take places that this one's still want (routed 32 x 2048: 84 us, with it 87).
+    if (!p.tiles.experts) pdl_launch_dependents();
     // Alone every warp runs through all tiles by itself; the CTAs of a cluster meet behind each. A wait that expires ends a warp's work; the cluster's barriers are kept.
     const bool alone = p.ranges == 1;
     auto meet = [&] { if (!alone) cluster.sync(); };
@@ -247,9 +252,8 @@ f8_few_kernel(const FewParams p, const __grid_constant__ CUtensorMap xmap, const
             const Tile tile = tile_at(p.tiles, first_tile, t);
             const int rows = min(NT, tile.end - tile.row0);
             if (alone) {
-                if (!ok) continue;
                 // ---- results of one CTA: a lane has a column, its registers are rows of x ----
-                const int col = tile.col * 128 + quarter * 32 + lane, row0 = tile.row0 + half * EACH, count = rows - half * EACH;
+                const int col = tile.col * 128 + quarter * 32 + lane, row0 = tile.row0 + half * EACH, count = ok ? rows - half * EACH : 0;   // (a warp whose wait has expired stores nothing, but keeps the takers' barriers)
                 const bool there = col < p.n;
                 float value[EACH];
 #pragma unroll

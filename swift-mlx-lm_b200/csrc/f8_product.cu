@@ -15,12 +15,16 @@ using namespace f8;
 namespace {
 
 // ---- many rows ---------------------------------------------------------------------------------------------------------------
-// Persistent pairs of CTAs that share a tile of 256 rows x 256 columns of accumulators: lanes of tensor memory are rows of
-// x, a thread has one row and 128 of the columns. A warp for the copies, one for the MMAs, eight that take a block's sums out of one of two buffers of
-// tensor memory while the next block's are multiplied into the other. GATED: the accumulators of 64 columns of w lie before those of the same 64
-// of `up`, so that a thread has both, and a tile gives 128 columns of the result.
-// Registers are dealt out anew after the start: 128 threads x 56 for the first four warps, two of which have nothing to do, 256 x 224 for the takers' 128 sums
-// and the 64 that are on their way, together the 384 x 168 of the launch.
+// Persistent pairs of CTAs that share a tile of 256 rows x 256 columns of accumulators: lanes of tensor memory are rows of x, a thread has one row and 128 of
+// the columns. A warp for the copies, one for the MMAs, two for the scales, eight that take a block's sums out of one of two buffers of tensor memory while the
+// next block's are multiplied into the other. GATED: the accumulators of 64 columns of w lie before those of the same 64 of `up`, so that a thread has both,
+// and a tile gives 128 columns of the result.
+// What bounds it: a pair's block is 64 KB from L2, which gives all SMs together some 10 TB/s: 0.47 us, 365 us for 8192 rows x 4096 x 14336 without any product
+// or sum, and 400 with them (2.4 PFLOP/s). Kept up for seconds it is bound by power: 990 W, the SM clock falls from 1965 to 1240 MHz, 470 to 510 us. One CTA
+// per tile of 128 rows moved half as much again and was never faster by more than a last wave's tiles.
+// The takers: 16 columns at a time, so that nothing spills (439 clocks a block by themselves; with 32 columns on their way while 32 are added ptxas spills, and
+// a block took 1090). Registers are dealt out anew after the start: 128 threads x 56 for the first four warps and 256 x 224 for the takers and their 128 sums,
+// together the 384 x 168 of the launch.
 constexpr int kWideWarps = 12, kWideThreads = kWideWarps * 32, kWideTakers = 8;
 constexpr int kAccCols = 256;
 constexpr int kScaleDepth = 4;      // blocks whose scales are on their way, and that have room for theirs in shared memory
@@ -51,7 +55,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) f8_wide_kernel(const WidePara
     unsigned char* const staging = ring + kStages * kStage;
     float2* const scales = reinterpret_cast<float2*>(staging + kWideTakers * 32 * kStageRow);   // [kScaleDepth][128]
     unsigned* const tops = reinterpret_cast<unsigned*>(scales + kScaleDepth * 128);             // [2][128]
-    int* const first_tile = reinterpret_cast<int*>(tops + 256);                                // [experts + 1]
+    int* const first_tile = reinterpret_cast<int*>(tops + 256);                                // [experts]
     __shared__ __align__(8) unsigned long long full[kStages], empty[kStages], sums_full[2], sums_empty[2];
     __shared__ unsigned tmem_base;
     __shared__ int warp_tiles[kWideWarps];
@@ -75,110 +79,110 @@ __global__ void __launch_bounds__(kWideThreads, 1) f8_wide_kernel(const WidePara
     const unsigned tmem = tmem_base;
     const int first = (int)blockIdx.x / 2, step = (int)gridDim.x / 2;
     if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 0) {
-        // The warp runs its loop as a whole, one lane issues. Of a pair both CTAs' copies count on the barrier of the one that issues the MMAs.
-        const bool el = elect_one();
-        const unsigned full0 = cluster_place(smem_u32(&full[0]), 0), empty0 = held_address(&empty[0]), at = held_address(ring);
-        auto load = [&](unsigned dst, const CUtensorMap* map, int col, int row, int s) { tma_load_2d_pair(dst, map, col, row, full0 + 8u * s); };
-        int s = 0, issued = 0;
-        unsigned par = 1;
-        bool ok = true;
-        for (int t = first; t < tiles && ok; t += step) {
-            const Tile tile = tile_at(p.tiles, first_tile, t);
-            const int x_row = tile.row0 + rank * 128, w_row = tile.expert * p.n + tile.col * COLS + rank * (COLS / 2);
-            for (int b = 0; b < p.blocks; ++b) {
-                if (!mbar_wait_warp(empty0 + 8u * s, par)) { ok = false; break; }
-                if (el) {
-                    const unsigned dst = at + s * kStage;
-                    if (rank == 0) mbar_expect(full0 + 8u * s, 2u * kStage);
-                    load(dst, &xmap, b * kF8Block, x_row, s);
-                    load(dst + kCodesBytes, &wmap, b * kF8Block, w_row, s);
-                    if (GATED) load(dst + kCodesBytes + kCodesBytes / 2, &upmap, b * kF8Block, w_row, s);
-                }
-                __syncwarp();
-                ++issued;
-                if (++s == kStages) { s = 0; par ^= 1u; }
-            }
-        }
-        if (!ok) {   // copies already requested still write shared memory (in a pair's second CTA, whose barrier this is not, the limit of the wait is the time they get)
-            if (el) atomicExch_system(p.status, 11);
-            for (int i = max(issued - kStages, 0); i < issued; ++i) mbar_wait_warp(&full[i % kStages], (unsigned)((i / kStages) & 1));
-        }
-    } else if (warp == 1) {
-        if (rank == 0) {
-            constexpr unsigned desc = idesc(256, kAccCols);
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 0) {
+            // The warp runs its loop as a whole, one lane issues. Of a pair both CTAs' copies count on the barrier of the one that issues the MMAs.
             const bool el = elect_one();
-            const unsigned full0 = held_address(&full[0]), sums0 = held_address(&sums_empty[0]), at = umma_desc_lo(held_address(ring));
-            int s = 0;
-            unsigned par = 0, buffer = 0, sums_par = 1;
+            const unsigned full0 = cluster_place(smem_u32(&full[0]), 0), empty0 = held_address(&empty[0]), at = held_address(ring);
+            auto load = [&](unsigned dst, const CUtensorMap* map, int col, int row, int s) { tma_load_2d_pair(dst, map, col, row, full0 + 8u * s); };
+            int s = 0, issued = 0;
+            unsigned par = 1;
             bool ok = true;
-            for (int t = first; t < tiles && ok; t += step)
+            for (int t = first; t < tiles && ok; t += step) {
+                const Tile tile = tile_at(p.tiles, first_tile, t);
+                const int x_row = tile.row0 + rank * 128, w_row = tile.expert * p.n + tile.col * COLS + rank * (COLS / 2);
                 for (int b = 0; b < p.blocks; ++b) {
-                    // (what the barriers guard is read by the tensor cores: no ordinary load has to see another CTA's stores)
-                    ok = mbar_wait_warp(full0 + 8u * s, par) && mbar_wait_warp(sums0 + 8u * buffer, sums_par);
-                    if (!ok) { if (el) atomicExch_system(p.status, 12); break; }
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (!mbar_wait_warp(empty0 + 8u * s, par)) { ok = false; break; }
                     if (el) {
-                        const unsigned a = at + s * (kStage / 16), w = a + kCodesBytes / 16, sums = tmem + buffer * kAccCols;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) umma<2>(sums, a + 2 * j, w + 2 * j, desc, j > 0);
-                        commit<2>(&empty[s]);
-                        commit<2>(&sums_full[buffer]);
+                        const unsigned dst = at + s * kStage;
+                        if (rank == 0) mbar_expect(full0 + 8u * s, 2u * kStage);
+                        load(dst, &xmap, b * kF8Block, x_row, s);
+                        load(dst + kCodesBytes, &wmap, b * kF8Block, w_row, s);
+                        if (GATED) load(dst + kCodesBytes + kCodesBytes / 2, &upmap, b * kF8Block, w_row, s);
                     }
                     __syncwarp();
+                    ++issued;
                     if (++s == kStages) { s = 0; par ^= 1u; }
-                    buffer ^= 1u;
-                    sums_par ^= buffer ^ 1u;
                 }
-        }
-    } else {
-        // Two warps for the scales, 64 rows each: what the accumulators of a row are worth, as two factors (of the two halves of the columns, or of w's
-        // and up's), is in shared memory before the sums are said to be there. A slot is free again by then: the takers have left block
-        // it - 4 before block it - 2 was multiplied.
-        const int r0 = (warp - 2) * 64 + 2 * lane;
-        const unsigned full0 = held_address(&sums_full[0]);
-        float2* const mine = scales + r0;
-        struct Ahead { float x[2], w[2]; } ahead[kScaleDepth];
-        Tile tile{};
-        int t = first, b = 0;      // the block that is asked for next
-        bool any = t < tiles;
-        if (any) tile = tile_at(p.tiles, first_tile, t);
-        auto ask = [&](Ahead& a) {
-            if (!any) return;
-            const int row = tile.row0 + rank * 128 + r0, block = GATED ? tile.col : 2 * tile.col;
-            const float* x = p.x_scale + b * p.x_scale_stride + row;
-            const long long at = ((long long)tile.expert * p.col_blocks + block) * p.blocks + b;
-            a.x[0] = row < tile.end ? *x : 0.f;
-            a.x[1] = row + 1 < tile.end ? x[1] : 0.f;
-            a.w[0] = p.w_scale[at];
-            a.w[1] = GATED ? p.up_scale[at] : block + 1 < p.col_blocks ? p.w_scale[at + p.blocks] : 0.f;
-            if (++b == p.blocks) {
-                b = 0; t += step;
-                any = t < tiles;
-                if (any) tile = tile_at(p.tiles, first_tile, t);
             }
-        };
-        const int total = first < tiles ? (tiles - 1 - first) / step + 1 : 0;
-        const int all = total * p.blocks;
+            if (!ok) {   // copies already requested still write shared memory (in a pair's second CTA, whose barrier this is not, the limit of the wait is the time they get)
+                if (el) atomicExch_system(p.status, 11);
+                for (int i = max(issued - kStages, 0); i < issued; ++i) mbar_wait_warp(&full[i % kStages], (unsigned)((i / kStages) & 1));
+            }
+        } else if (warp == 1) {
+            if (rank == 0) {
+                constexpr unsigned desc = idesc(256, kAccCols);
+                const bool el = elect_one();
+                const unsigned full0 = held_address(&full[0]), sums0 = held_address(&sums_empty[0]), at = umma_desc_lo(held_address(ring));
+                int s = 0;
+                unsigned par = 0, buffer = 0, sums_par = 1;
+                bool ok = true;
+                for (int t = first; t < tiles && ok; t += step)
+                    for (int b = 0; b < p.blocks; ++b) {
+                        // (what the barriers guard is read by the tensor cores: no ordinary load has to see another CTA's stores)
+                        ok = mbar_wait_warp(full0 + 8u * s, par) && mbar_wait_warp(sums0 + 8u * buffer, sums_par);
+                        if (!ok) { if (el) atomicExch_system(p.status, 12); break; }
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        if (el) {
+                            const unsigned a = at + s * (kStage / 16), w = a + kCodesBytes / 16, sums = tmem + buffer * kAccCols;
 #pragma unroll
-        for (int u = 0; u < kScaleDepth; ++u) ask(ahead[u]);
-        bool ok = true;
-        for (int it0 = 0; it0 < all && ok; it0 += kScaleDepth) {
+                            for (int j = 0; j < 4; ++j) umma<2>(sums, a + 2 * j, w + 2 * j, desc, j > 0);
+                            commit<2>(&empty[s]);
+                            commit<2>(&sums_full[buffer]);
+                        }
+                        __syncwarp();
+                        if (++s == kStages) { s = 0; par ^= 1u; }
+                        buffer ^= 1u;
+                        sums_par ^= buffer ^ 1u;
+                    }
+            }
+        } else {
+            // Two warps for the scales, 64 rows each: what the accumulators of a row are worth, as two factors (of the two halves of the columns, or of w's
+            // and up's), is in shared memory before the sums are said to be there. A slot is free again by then: the takers have left block
+            // it - 4 before block it - 2 was multiplied.
+            const int r0 = (warp - 2) * 64 + 2 * lane;
+            const unsigned full0 = held_address(&sums_full[0]);
+            float2* const mine = scales + r0;
+            struct Ahead { float x[2], w[2]; } ahead[kScaleDepth];
+            Tile tile{};
+            int t = first, b = 0;      // the block that is asked for next
+            bool any = t < tiles;
+            if (any) tile = tile_at(p.tiles, first_tile, t);
+            auto ask = [&](Ahead& a) {
+                if (!any) return;
+                const int row = tile.row0 + rank * 128 + r0, block = GATED ? tile.col : 2 * tile.col;
+                const float* x = p.x_scale + b * p.x_scale_stride + row;
+                const long long at = ((long long)tile.expert * p.col_blocks + block) * p.blocks + b;
+                a.x[0] = row < tile.end ? *x : 0.f;
+                a.x[1] = row + 1 < tile.end ? x[1] : 0.f;
+                a.w[0] = p.w_scale[at];
+                a.w[1] = GATED ? p.up_scale[at] : block + 1 < p.col_blocks ? p.w_scale[at + p.blocks] : 0.f;
+                if (++b == p.blocks) {
+                    b = 0; t += step;
+                    any = t < tiles;
+                    if (any) tile = tile_at(p.tiles, first_tile, t);
+                }
+            };
+            const int total = first < tiles ? (tiles - 1 - first) / step + 1 : 0;
+            const int all = total * p.blocks;
 #pragma unroll
-            for (int u = 0; u < kScaleDepth; ++u) {
-                const int it = it0 + u;
-                if (it >= all || !ok) break;
-                if (it >= 2) ok = mbar_wait_warp(full0 + 8u * (u & 1), (unsigned)(((it >> 1) - 1) & 1));
-                if (!ok) { if (lane == 0) atomicExch_system(p.status, 14); break; }
-                const Ahead now = ahead[u];
-                *reinterpret_cast<float4*>(mine + u * 128) = make_float4(now.x[0] * now.w[0], now.x[0] * now.w[1], now.x[1] * now.w[0], now.x[1] * now.w[1]);
-                __syncwarp();
-                if (lane == 0) arrive(full0 + 8u * (u & 1));
-                ask(ahead[u]);
+            for (int u = 0; u < kScaleDepth; ++u) ask(ahead[u]);
+            bool ok = true;
+            for (int it0 = 0; it0 < all && ok; it0 += kScaleDepth) {
+#pragma unroll
+                for (int u = 0; u < kScaleDepth; ++u) {
+                    const int it = it0 + u;
+                    if (it >= all || !ok) break;
+                    if (it >= 2) ok = mbar_wait_warp(full0 + 8u * (u & 1), (unsigned)(((it >> 1) - 1) & 1));
+                    if (!ok) { if (lane == 0) atomicExch_system(p.status, 14); break; }
+                    const Ahead now = ahead[u];
+                    *reinterpret_cast<float4*>(mine + u * 128) = make_float4(now.x[0] * now.w[0], now.x[0] * now.w[1], now.x[1] * now.w[0], now.x[1] * now.w[1]);
+                    __syncwarp();
+                    if (lane == 0) arrive(full0 + 8u * (u & 1));
+                    ask(ahead[u]);
+                }
             }
         }
-    }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         // A warp has the 32 lanes of its quarter (warp & 3) and one half of the columns.
@@ -189,13 +193,13 @@ __global__ void __launch_bounds__(kWideThreads, 1) f8_wide_kernel(const WidePara
         unsigned char* const out = staging + taker * 32 * kStageRow;
         unsigned buffer = 0, par = 0, slot = 0;
         bool ok = true;
-        for (int t = first; t < tiles && ok; t += step) {
+        for (int t = first; t < tiles; t += step) {
             unsigned long long acc[64];
 #pragma unroll
             for (int i = 0; i < 64; ++i) acc[i] = 0;
-            for (int b = 0; b < p.blocks; ++b) {
+            for (int b = 0; b < p.blocks && ok; ++b) {
                 ok = mbar_wait_warp(full0 + 8u * buffer, par);
-                if (!ok) { if (lane == 0) atomicExch_system(p.status, 13); break; }
+                if (!ok) { if (lane == 0) atomicExch_system(p.status, 13); break; }   // (it stores nothing more, but keeps the takers' barriers)
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const unsigned from = at + buffer * kAccCols;
                 float s_low, s_high;
@@ -219,7 +223,6 @@ __global__ void __launch_bounds__(kWideThreads, 1) f8_wide_kernel(const WidePara
                 par ^= buffer ^ 1u;
                 slot = (slot + 1024u) & (1024u * kScaleDepth - 1u);
             }
-            if (!ok) break;
             const Tile done = tile_at(p.tiles, first_tile, t);
             // ---- results: value i of the thread is column col0 + i of its row ----
             constexpr int VALUES = GATED ? 64 : 128;
@@ -246,10 +249,11 @@ __global__ void __launch_bounds__(kWideThreads, 1) f8_wide_kernel(const WidePara
                     asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
                 }
                 const F8Scale s(top);
-                if (row0 + lane < done.end && col0 < p.n && !(GATED && half)) p.y_scale[(long long)(col0 / kF8Block) * p.y_scale_stride + row0 + lane] = s.scale;
+                if (ok && row0 + lane < done.end && col0 < p.n && !(GATED && half)) p.y_scale[(long long)(col0 / kF8Block) * p.y_scale_stride + row0 + lane] = s.scale;
 #pragma unroll
                 for (int i = 0; i < VALUES; ++i) value[i] *= s.inverse;
             }
+            if (!ok) continue;
             auto send = [&](int col) {   // 64 bytes of each row, from column `col` on, are in the staging rows
                 __syncwarp();
                 const int per = 16 / size, c = col + (lane & 3) * per, rest = p.n - c;
