@@ -47,17 +47,6 @@ __device__ __forceinline__ unsigned f8_codes4(float a, float b, float c, float d
         : "=r"(word) : "f"(a), "f"(b), "f"(c), "f"(d));
     return word;
 }
-// The gated activations (swlm_op_f8_product_dev); a NaN stays one. tanh-GELU as g / (1 + e^-2u).
-__device__ __forceinline__ float f8_gated(float g, float u, int act, float alpha, float limit) {
-    float z = g;
-    if (act == SWLM_F8_GELU) z = 1.5957691216f * (g + 0.044715f * g * g * g);
-    if (act == SWLM_F8_CLAMPED) {
-        g = g > limit ? limit : g;
-        u = (u > limit ? limit : u < -limit ? -limit : u) + 1.0f;
-        z = alpha * g;
-    }
-    return g / (1.0f + expf(-z)) * u;
-}
 #endif
 
 }  // namespace swlm

@@ -79,15 +79,20 @@ __device__ __forceinline__ unsigned pack2(float a, float b, bool f16) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const unsigned*>(&h);
 }
-// f8_gated without a branch between values: their exponentials overlap
+// The gated activations (swlm_op_f8_product_dev); a NaN stays one; tanh-GELU as g / (1 + e^-2u). An exponential and a reciprocal of the special function unit, two
+// in the last place each, and |z| 2^-24 for its argument; no branch between values, so that they overlap.
 __device__ __forceinline__ float gated(float g, float u, int act, float alpha, float limit) {
-    const bool clamped = act == SWLM_F8_CLAMPED;
-    if (clamped) {
+    float z = g;
+    if (act == SWLM_F8_GELU) z = 1.5957691216f * (g + 0.044715f * g * g * g);
+    if (act == SWLM_F8_CLAMPED) {
         g = g > limit ? limit : g;
         u = (u > limit ? limit : u < -limit ? -limit : u) + 1.0f;
+        z = alpha * g;
     }
-    const float z = act == SWLM_F8_GELU ? 1.5957691216f * (g + 0.044715f * g * g * g) : clamped ? alpha * g : g;
-    return 0.25f * g * four_over(1.0f + expf(-z)) * u;
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-1.4426950408889634f * z));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return g * r * u;
 }
 
 // Work as tiles of `rows` rows x a tile of columns, those of one expert after those of the other (experts 0: one has all rows). CTAs take them in turn.

@@ -3,6 +3,7 @@
 // The products of a block's codes are exact and summed in fp32 in tensor memory; two scales belong to every block, so its sums leave tensor memory before the
 // next block's are added: registers hold acc += (sx sw) sums, in fp32. A block is 128 bytes of a row, one swizzle row and four MMAs of K = 32.
 #include <algorithm>
+#include <type_traits>
 
 #include <cooperative_groups.h>
 
@@ -237,7 +238,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) f8_wide_kernel(const WidePara
                     value[i + 1] = gated(g.y, u.y, p.act, p.alpha, p.limit);
                 }
             }
-            const int row0 = done.row0 + rank * 128 + quarter * 32, col0 = done.col * COLS + half * VALUES, size = f8_size(p.dtype);
+            const int row0 = done.row0 + rank * 128 + quarter * 32, col0 = done.col * COLS + half * VALUES;
             if (p.dtype == SWLM_F8_E4M3) {
                 unsigned top = 0;
 #pragma unroll
@@ -254,31 +255,46 @@ __global__ void __launch_bounds__(kWideThreads, 1) f8_wide_kernel(const WidePara
                 for (int i = 0; i < VALUES; ++i) value[i] *= s.inverse;
             }
             if (!ok) continue;
-            auto send = [&](int col) {   // 64 bytes of each row, from column `col` on, are in the staging rows
+            // 64 bytes of each row at a time, by way of the staging rows: a lane then stores sixteen of every eighth row
+            const int live = done.end - row0 - (lane >> 2);
+            const uint4* const got = reinterpret_cast<const uint4*>(out + (lane >> 2) * kStageRow + (lane & 3) * 16);
+            uint4* const put = reinterpret_cast<uint4*>(out + lane * kStageRow);
+            auto send = [&](auto size, int c) {   // columns c .. of the warp's are in the staging rows
+                constexpr int SIZE = decltype(size)::value, PER = 16 / SIZE;
+                unsigned char* dst = p.y + ((long long)(row0 + (lane >> 2)) * p.y_stride + col0 + c) * SIZE + (lane & 3) * 16;
+                const long long step8 = 8 * p.y_stride * SIZE;
+                const int rest = p.n - col0 - c - (lane & 3) * PER;
                 __syncwarp();
-                const int per = 16 / size, c = col + (lane & 3) * per, rest = p.n - c;
+                uint4 v[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int r = (lane >> 2) + 8 * i;
-                    const unsigned char* src = out + r * kStageRow + (lane & 3) * 16;
-                    if (row0 + r < done.end && rest > 0) {
-                        unsigned char* dst = p.y + ((long long)(row0 + r) * p.y_stride + c) * size;
-                        if (rest >= per) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
-                        else if (size == 1) { for (int e = 0; e < rest; ++e) dst[e] = src[e]; }
-                        else if (size == 2) { for (int e = 0; e < rest; ++e) reinterpret_cast<unsigned short*>(dst)[e] = reinterpret_cast<const unsigned short*>(src)[e]; }
-                        else { for (int e = 0; e < rest; ++e) reinterpret_cast<unsigned*>(dst)[e] = reinterpret_cast<const unsigned*>(src)[e]; }
+                for (int i = 0; i < 4; ++i) v[i] = got[i * (8 * kStageRow / 16)];
+                __syncwarp();
+                if (rest >= PER) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (8 * i < live) *reinterpret_cast<uint4*>(dst + i * step8) = v[i];
+                } else if (rest > 0) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (8 * i >= live) continue;
+                        const unsigned w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+                        for (int e = 0; e < PER - 1; ++e) {
+                            if (e >= rest) continue;
+                            if (SIZE == 4) reinterpret_cast<unsigned*>(dst + i * step8)[e] = w[e & 3];
+                            else if (SIZE == 2) reinterpret_cast<unsigned short*>(dst + i * step8)[e] = (unsigned short)(w[(e >> 1) & 3] >> (16 * (e & 1)));
+                            else (dst + i * step8)[e] = (unsigned char)(w[e >> 2] >> (8 * (e & 3)));
+                        }
                     }
                 }
-                __syncwarp();
             };
-            uint4* const put = reinterpret_cast<uint4*>(out + lane * kStageRow);
             if (p.dtype == SWLM_F8_FP32) {
 #pragma unroll
                 for (int c = 0; c < VALUES; c += 16) {
                     if (col0 + c >= p.n) break;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) put[i] = make_uint4(__float_as_uint(value[c + 4 * i]), __float_as_uint(value[c + 4 * i + 1]), __float_as_uint(value[c + 4 * i + 2]), __float_as_uint(value[c + 4 * i + 3]));
-                    send(col0 + c);
+                    send(std::integral_constant<int, 4>(), c);
                 }
             } else if (p.dtype == SWLM_F8_E4M3) {
 #pragma unroll
@@ -289,7 +305,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) f8_wide_kernel(const WidePara
                         const float* f = value + c + 16 * i;
                         put[i] = make_uint4(f8_codes4(f[0], f[1], f[2], f[3]), f8_codes4(f[4], f[5], f[6], f[7]), f8_codes4(f[8], f[9], f[10], f[11]), f8_codes4(f[12], f[13], f[14], f[15]));
                     }
-                    send(col0 + c);
+                    send(std::integral_constant<int, 1>(), c);
                 }
             } else {
                 const bool f16 = p.dtype == SWLM_F8_FP16;
@@ -301,7 +317,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) f8_wide_kernel(const WidePara
                         const float* f = value + c + 8 * i;
                         put[i] = make_uint4(pack2(f[0], f[1], f16), pack2(f[2], f[3], f16), pack2(f[4], f[5], f16), pack2(f[6], f[7], f16));
                     }
-                    send(col0 + c);
+                    send(std::integral_constant<int, 2>(), c);
                 }
             }
         }
