@@ -15,18 +15,20 @@ namespace {
 // A stable counting sort by one cluster: every warp has a run of neighbouring pairs and counts its experts; sums over warps and, through distributed
 // shared memory, over the cluster's CTAs give every warp its first row of every expert; then it numbers its pairs, 32 at a time, by those before
 // them of the same expert. No number depends on the order in which warps get there.
-constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortUnroll = 8, kSortCtas = 16;
+// What bounds it is latency: a few pairs take as many warps as they need (16 tokens x 8: 32 warps 5.9 us replayed, four 3.0), many a cluster of sixteen CTAs
+// (131072 pairs: eight 21 us, sixteen 13.4; rows' tokens put in order in shared memory before they are stored gained nothing).
+constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortUnroll = 8, kSortCtas = 16;   // at most
 
 __global__ void __launch_bounds__(kSortThreads) expert_sort_kernel(const swlm_expert_sort a) {
-    extern __shared__ int counts[];        // [kSortWarps][experts]: pairs of each warp, then each warp's next row
+    extern __shared__ int counts[];        // [warps][experts]: pairs of each warp, then each warp's next row
     __shared__ int total[kExpertMax], before[kSortWarps];
     pdl_wait();
     const cg::cluster_group cluster = cg::this_cluster();
-    const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, E = a.experts;
-    const int pairs = a.tokens * a.top, runs = ctas * kSortWarps, each = (pairs + 32 * runs - 1) / (32 * runs) * 32;   // (at most 2^30 + 2^14)
-    const int first = (int)min((long long)(rank * kSortWarps + warp) * each, (long long)pairs), last = min(first + each, pairs);
+    const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, E = a.experts, threads = blockDim.x, warps = threads >> 5;
+    const int pairs = a.tokens * a.top, runs = ctas * warps, each = (pairs + 32 * runs - 1) / (32 * runs) * 32;   // (at most 2^30 + 2^14)
+    const int first = (int)min((long long)(rank * warps + warp) * each, (long long)pairs), last = min(first + each, pairs);
     int* const mine = counts + warp * E;
-    for (int i = tid; i < kSortWarps * E; i += kSortThreads) counts[i] = 0;
+    for (int i = tid; i < warps * E; i += threads) counts[i] = 0;
     __syncthreads();
     int e[kSortUnroll];   // choices of the pairs in question, -1 for none; where a warp has no more than these they are read once
     auto read = [&](int i0) {
@@ -48,11 +50,15 @@ __global__ void __launch_bounds__(kSortThreads) expert_sort_kernel(const swlm_ex
     if (tid < E) {
 #pragma unroll
         for (int w0 = 0; w0 < kSortWarps; w0 += 16) {   // pairs of the warps before each
+            if (w0 >= warps) break;
             int c[16];
 #pragma unroll
-            for (int w = 0; w < 16; ++w) c[w] = counts[(w0 + w) * E + tid];
+            for (int w = 0; w < 16; ++w) c[w] = w0 + w < warps ? counts[(w0 + w) * E + tid] : 0;
 #pragma unroll
-            for (int w = 0; w < 16; ++w) { counts[(w0 + w) * E + tid] = sum; sum += c[w]; }
+            for (int w = 0; w < 16; ++w) {
+                if (w0 + w < warps) counts[(w0 + w) * E + tid] = sum;
+                sum += c[w];
+            }
         }
         total[tid] = sum;
     }
@@ -66,34 +72,34 @@ __global__ void __launch_bounds__(kSortThreads) expert_sort_kernel(const swlm_ex
             all += v;
         }
     }
-    int scan = all;   // rows of the experts up to this one
+    auto running = [&](int v) {   // sum over the lanes up to this one
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, scan, o);
-        if (lane >= o) scan += v;
-    }
+        for (int o = 1; o < 32; o <<= 1) {
+            const int w = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += w;
+        }
+        return v;
+    };
+    const int scan = running(all);   // rows of the experts up to this one, the warp's first on
     if (lane == 31) before[warp] = scan;
     __syncthreads();
-    int base = 0, rows = 0;
-    for (int w = 0; w < kSortWarps; ++w) {
-        base += w < warp ? before[w] : 0;
-        rows += before[w];
-    }
-    base += scan - all;
+    const int upto = running(lane < warps ? before[lane] : 0), rows = __shfl_sync(0xffffffffu, upto, 31);
+    const int base = (warp ? __shfl_sync(0xffffffffu, upto, (warp + 31) & 31) : 0) + scan - all;
     if (tid < E) {
         if (rank == 0) {
             a.offsets[tid] = base;
             if (tid == E - 1) a.offsets[E] = rows;
         }
 #pragma unroll 16
-        for (int w = 0; w < kSortWarps; ++w) atomicAdd(counts + w * E + tid, base + others);   // (no thread waits for what it reads)
+        for (int w = 0; w < warps; ++w) atomicAdd(counts + w * E + tid, base + others);   // (no thread waits for what it reads)
     }
     __syncthreads();
-    for (int i = rows + rank * kSortThreads + tid; i < pairs; i += ctas * kSortThreads) a.source[i] = -1;
+    for (int i = rows + rank * threads + tid; i < pairs; i += ctas * threads) a.source[i] = -1;
     for (int i0 = first; i0 < last; i0 += 32 * kSortUnroll) {
         if (each > 32 * kSortUnroll) read(i0);
 #pragma unroll
         for (int u = 0; u < kSortUnroll; ++u) {
+            if (i0 + 32 * u >= last) break;   // (the same for the warp)
             const int i = i0 + 32 * u + lane;
             const unsigned same = __match_any_sync(0xffffffffu, e[u]);
             const int next = e[u] >= 0 ? mine[e[u]] : 0;
@@ -246,7 +252,9 @@ int launch_expert_sort(const swlm_expert_sort& a, cudaStream_t s) {
     const long long pairs = (long long)a.tokens * a.top;
     int ctas = 1;
     while (ctas < g_sort_ctas.load(std::memory_order_relaxed) && pairs > (long long)ctas * 2 * kSortThreads) ctas *= 2;
-    const cudaError_t e = launch_clusters(expert_sort_kernel, ctas, dim3(ctas), dim3(kSortThreads), (size_t)kSortWarps * a.experts * 4, s, a);
+    // a thread per expert, and as many warps as have pairs
+    const int threads = (int)std::min<long long>(kSortThreads, std::max<long long>((a.experts + 31) / 32 * 32, (pairs + 31) / 32 * 32));
+    const cudaError_t e = launch_clusters(expert_sort_kernel, ctas, dim3(ctas), dim3(threads), (size_t)threads / 32 * a.experts * 4, s, a);
     return e == cudaSuccess ? SWLM_OK : cuda_fail(e, "expert sort launch");
 }
 
