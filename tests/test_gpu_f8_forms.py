@@ -180,3 +180,56 @@ def test_nothing_to_do(calls, pkg):
     lib.check(lib.swlm_op_expert_sum_dev(h, call, calls.stream))
     torch.cuda.synchronize()
     assert (offsets == 0).all() and torch.equal(out, add)
+
+
+def far(compact, stride):
+    """The same rows, each `stride` entries behind the one before it."""
+    out = torch.zeros((compact.shape[0] * stride,), dtype=torch.uint8 if compact.element_size() == 1 else compact.dtype, device="cuda")
+    view = torch.as_strided(out.view(compact.dtype), compact.shape, (stride, 1))
+    (view.view(torch.uint8) if compact.element_size() == 1 else view).copy_(compact.view(torch.uint8) if compact.element_size() == 1 else compact)
+    return view
+
+
+def test_rows_that_lie_far_apart(calls):
+    """Offsets in bytes that pass 32 bits, in rows, experts' matrices and results: the bits are those of the same rows close together."""
+    rows, n, k, experts, stride, w_stride = 3, 130, 200, 3, 5 << 28, 12 << 20
+    g = generator(5)
+    x = torch.randn((rows, k), generator=g, device="cuda").bfloat16()
+    near, apart = code_room(rows, k), code_room(rows, k)
+    calls.quantize(x, near)
+    wide = far(x, stride)
+    calls.quantize(wide, apart)
+    torch.cuda.synchronize()
+    assert torch.equal(near[0].view(torch.uint8), apart[0].view(torch.uint8)) and torch.equal(near[1], apart[1])
+    del wide
+    w = matrix(g, n, k, experts)
+    w_far = torch.as_strided(torch.zeros((experts * n * w_stride,), dtype=torch.uint8, device="cuda").view(E4M3), (experts, n, k), (n * w_stride, w_stride, 1))
+    w_far.view(torch.uint8).copy_(w[0].view(torch.uint8))
+    offsets = torch.tensor([0, 1, 1, rows], dtype=torch.int32, device="cuda")
+    y, y_far = room(rows, n, torch.bfloat16), far(room(rows, n, torch.bfloat16), stride)
+    calls.product(near, w, y, offsets=offsets)
+    calls.product((far(near[0], 2 * stride), near[1]), (w_far, w[1]), y_far, offsets=offsets)
+    torch.cuda.synchronize()
+    assert torch.equal(y, y_far)
+    out = room(rows, n, torch.bfloat16)
+    calls.sum(y_far, torch.arange(rows, dtype=torch.int32, device="cuda").view(rows, 1), torch.ones((rows, 1), device="cuda"), out)
+    torch.cuda.synchronize()
+    assert torch.equal(out, y)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, E4M3], ids=str)
+def test_many_rows_that_lie_far_apart(calls, dtype):
+    """The same where pairs of SMs take a product."""
+    rows, n, k, stride = 1100, 2600, 300, 5 << 20
+    assert form_of(calls.lib, rows, n, k, 0, False)[0] == "wide"
+    g = generator(6)
+    x, w = rows_of(g, rows, k), matrix(g, n, k)
+    y = code_room(rows, n) if dtype == E4M3 else room(rows, n, dtype)
+    held = y[0] if dtype == E4M3 else y
+    y_far = far(held, stride)
+    scale = torch.zeros_like(y[1]) if dtype == E4M3 else None
+    calls.product(x, w, y)
+    calls.product((far(x[0], stride), x[1]), w, (y_far, scale) if dtype == E4M3 else y_far)
+    torch.cuda.synchronize()
+    same = torch.equal(held.view(torch.uint8), y_far.view(torch.uint8)) if dtype == E4M3 else torch.equal(held, y_far)
+    assert same and (dtype != E4M3 or torch.equal(scale, y[1]))
