@@ -399,8 +399,8 @@ int f8_few_init() {
     return SWLM_OK;
 }
 
-// A block takes a tile 0.22 to 0.36 (twice the matrices: 0.36 to 0.4), a launch's tile starts and ends in 6, further tiles of a CTA in 1, the exchange of a cluster
-// takes 1; weights come from memory at 6.2 TB/s. Gated tiles of 128 rows took three times as long as two of 64, those of 32 as long as those of 64.
+// A block takes a tile 0.22 to 0.36 (twice the matrices: 0.36 to 0.4), a launch's first tile starts and ends in 4.5 to 7.5, further ones in 1, the exchange of a cluster
+// takes 0.5; weights come from memory at 6.2 TB/s. Gated tiles of 128 rows took three times as long as two of 64, those of 32 as long as those of 64.
 F8FewForm f8_few_form(int rows, int n, int k, int experts, bool gated) {
     F8FewForm best{0, 0, 1e30};
     const int blocks = f8_blocks(k), reached = experts ? std::min(experts, rows) : 1;
@@ -409,15 +409,16 @@ F8FewForm f8_few_form(int rows, int n, int k, int experts, bool gated) {
         if (gated && nt == 32) continue;
         const int per_sm = nt <= 32 ? 2 : 1;
         const double alone = gated ? (nt <= 16 ? 0.36 : 0.39) : nt == 16 ? 0.22 : nt == 32 ? 0.24 : nt == 64 ? 0.27 : 0.36;
+        const double ends = nt <= 32 ? 3.5 : nt == 128 ? 6.5 : gated ? 5.0 : 4.0;
         // rows of an expert end inside a tile
         const double row_tiles = experts ? rows / (double)nt + 0.5 * reached : (rows + nt - 1) / nt, tiles = std::max(row_tiles, (double)reached) * f8_blocks(n);
         for (int ranges = 1; ranges <= 8 && ranges <= blocks; ranges *= 2) {
-            // clusters of eight leave some SMs without one
-            const double slots = (ranges == 8 ? 128 : ranges == 4 ? 144 : kSms) * per_sm, waves = (double)(int64_t)((tiles * ranges + slots - 1) / slots);
+            // larger clusters leave some SMs without one: of eight CTAs fourteen run at once and sixteen take two turns, of four 36 do
+            const double slots = ranges == 8 ? (per_sm == 2 ? 128 : 112) : (ranges == 4 ? 132 : kSms) * per_sm, waves = (double)(int64_t)((tiles * ranges + slots - 1) / slots);
             if (ranges > 1 && waves > 1) break;
             const double both = per_sm == 2 && tiles * ranges > slots / 2 ? 1.5 : 1.0;   // two CTAs on an SM share it
             const double ctas = std::min(tiles * ranges, slots), step = std::max(alone * both, ctas * ((gated ? 2 : 1) * kCodesBytes + nt * kF8Block) / 10e6);   // L2 gives 10 TB/s
-            const double cost = std::max(waves * ((blocks + ranges - 1) / ranges * step + 1), memory) + 5 + (ranges > 1 ? 1 : 0);
+            const double cost = std::max(waves * ((blocks + ranges - 1) / ranges * step + 1), memory) + ends + (ranges > 1 ? 0.5 : 0.0);
             if (cost < best.cost) best = {nt, ranges, cost};
         }
     }

@@ -358,13 +358,16 @@ int wide_launch(const swlm_f8_product& a, int* status, cudaStream_t s) {
     return e == cudaSuccess ? SWLM_OK : cuda_fail(e, "product launch");
 }
 
-// What a product takes, about (us): a block 0.38 while the pairs are few, 0.47 with all of them reading from L2, a tile's start and end 6; weights that are
-// read once come from memory at 3.2 TB/s.
+// What a product takes, about (us): a block 0.38 while the pairs are few, 0.47 with all of them reading from L2, a launch and its first tile's start and end 7.5; weights
+// that are read once come from memory at 3.2 TB/s.
 double wide_cost(int rows, int n, int k, int experts, bool gated) {
     const int cols = gated ? 128 : 256, reached = experts ? std::min(experts, rows) : 1;
-    const double row_tiles = experts ? rows / 256.0 + 0.5 * reached : (rows + 255) / 256, tiles = row_tiles * ((n + cols - 1) / cols), pairs = kSms / 2;
-    const double waves = experts ? std::max(1.0, tiles / pairs) : (double)(int64_t)((tiles + pairs - 1) / pairs);
-    return std::max(waves * (f8_blocks(k) * (tiles > pairs / 2 ? 0.47 : 0.38) + 2), (double)reached * n * k * (gated ? 2 : 1) / 3.2e6) + 4;
+    const double row_tiles = experts ? std::max(rows / 256.0 + 0.5 * reached, (double)reached) : (rows + 255) / 256, tiles = row_tiles * ((n + cols - 1) / cols), pairs = kSms / 2;
+    auto wave = [&](double busy) { return f8_blocks(k) * (busy > pairs / 2 ? 0.47 : 0.38) + 2; };
+    const double full = (double)(int64_t)(tiles / pairs), rest = tiles - full * pairs;
+    // (how full an expert's tiles are is not known: their waves are not counted one by one)
+    const double run = experts ? std::max(1.0, tiles / pairs) * wave(tiles) : full * wave(pairs) + (rest > 0 ? wave(rest) : 0.0);
+    return std::max(run, (double)reached * n * k * (gated ? 2 : 1) / 3.2e6) + 5.5;
 }
 
 }  // namespace
@@ -386,7 +389,7 @@ F8ProductForm f8_product_form(int rows, int n, int k, int experts, bool gated) {
     const int full = (int)std::min<int64_t>((int64_t)waves * pairs / row_tiles * cols, n);
     if (!experts && full > 0 && full < n) {
         const F8FewForm last = f8_few_form(rows, n - full, k, 0, gated);
-        if (wide_cost(rows, full, k, 0, gated) + last.cost < std::min(f.few.cost, wide)) f = {full, last};
+        if (wide_cost(rows, full, k, 0, gated) + last.cost < 0.95 * std::min(f.few.cost, wide)) f = {full, last};   // (within what the model is off by, one launch)
     }
     return f;
 }

@@ -40,14 +40,14 @@ def form_of(lib, rows, n, k, experts, gated):
 
 # what each size is there for: the form of the other columns than those that pairs of SMs take
 FORMS = [
-    (False, 2100, 1, 17, "few", 32, 1), (False, 1, 2100, 1030, "few", 16, 4), (False, 1, 9300, 2049, "few", 16, 2), (False, 3, 1, 1030, "few", 16, 8),
-    (False, 17, 2100, 1030, "few", 32, 4), (False, 17, 9300, 2049, "few", 32, 2), (False, 300, 1, 1030, "few", 32, 8), (False, 2100, 129, 17, "few", 64, 1),
-    (False, 2100, 1, 1030, "few", 64, 4), (False, 33, 5000, 2049, "few", 64, 2), (False, 513, 1, 1030, "few", 64, 8), (False, 200, 5000, 17, "few", 128, 1),
-    (False, 70, 6000, 2049, "few", 128, 2), (False, 1500, 129, 1030, "few", 128, 4), (False, 1030, 1, 1030, "few", 128, 8), (False, 130, 9300, 17, "wide", 0, 0),
-    (False, 1100, 2600, 300, "wide", 0, 0), (False, 2900, 2800, 700, "wide", 0, 0), (False, 777, 5000, 2049, "both", 128, 4), (False, 2100, 2100, 2049, "both", 64, 4),
-    (True, 1, 5000, 700, "few", 16, 2), (True, 1, 1, 700, "few", 16, 4), (True, 5, 130, 1030, "few", 16, 8), (True, 17, 9300, 17, "few", 64, 1),
-    (True, 17, 5000, 1030, "few", 64, 2), (True, 513, 1, 700, "few", 64, 4), (True, 256, 1, 1030, "few", 64, 8), (True, 2100, 1, 17, "wide", 0, 0),
-    (True, 1000, 1500, 260, "wide", 0, 0), (True, 2900, 1500, 700, "wide", 0, 0), (True, 300, 5000, 2049, "both", 64, 8), (True, 400, 5000, 2049, "both", 64, 4),
+    (False, 1, 5000, 700, "few", 16, 2), (False, 1, 1, 700, "few", 16, 4), (False, 3, 130, 1030, "few", 16, 8), (False, 513, 264, 100, "few", 16, 1),
+    (False, 2100, 1, 17, "few", 32, 1), (False, 1100, 1, 700, "few", 32, 2), (False, 513, 1, 700, "few", 32, 4), (False, 130, 1, 1030, "few", 32, 8),
+    (False, 777, 5000, 17, "few", 64, 1), (False, 2900, 1, 2049, "few", 64, 2), (False, 1100, 1, 2600, "few", 64, 4), (False, 513, 1, 2600, "few", 64, 8),
+    (False, 2100, 4100, 17, "few", 128, 1), (False, 70, 9300, 4100, "few", 128, 2), (False, 1100, 2100, 17, "wide", 0, 0), (False, 1100, 2600, 300, "wide", 0, 0),
+    (False, 2900, 2800, 700, "wide", 0, 0), (False, 777, 5000, 2600, "both", 64, 2), (False, 2100, 2100, 2049, "both", 64, 4),
+    (True, 2, 2957, 290, "few", 16, 1), (True, 600, 1, 700, "few", 16, 2), (True, 1, 1, 700, "few", 16, 4), (True, 5, 130, 1030, "few", 16, 8), (True, 2900, 129, 17, "few", 64, 1),
+    (True, 2900, 1, 700, "few", 64, 2), (True, 1500, 1, 1030, "few", 64, 4), (True, 600, 1, 2049, "few", 64, 8), (True, 2900, 392, 17, "wide", 0, 0),
+    (True, 1000, 1500, 260, "wide", 0, 0), (True, 2900, 1500, 700, "wide", 0, 0), (True, 300, 5000, 4100, "both", 64, 4),
 ]
 
 
@@ -82,8 +82,8 @@ def spread(rows, experts, seed):
     return torch.cat([torch.zeros(1, dtype=torch.int32), ends]).cuda()
 
 
-EXPERTS = [(False, 3000, 700, 150, 5, "wide"), (True, 3000, 700, 150, 5, "wide"), (False, 6000, 300, 260, 40, "wide"), (True, 200, 1100, 300, 64, "few"), (False, 200, 1100, 300, 64, "few"),
-           (False, 1000, 640, 520, 33, "wide"), (False, 500, 640, 520, 33, "few"), (True, 400, 640, 520, 33, "few"), (False, 5, 260, 1100, 9, "few"), (True, 1, 130, 2100, 300, "few"), (False, 2000, 130, 130, 1024, "few")]
+EXPERTS = [(False, 3000, 700, 150, 5, "few"), (True, 3000, 700, 150, 5, "wide"), (False, 6000, 300, 260, 40, "wide"), (True, 200, 1100, 300, 64, "few"), (False, 200, 1100, 300, 64, "few"),
+           (False, 1000, 640, 520, 33, "few"), (False, 500, 640, 520, 33, "few"), (True, 400, 640, 520, 33, "few"), (False, 5, 260, 1100, 9, "few"), (True, 1, 130, 2100, 300, "few"), (False, 2000, 130, 130, 1024, "few")]
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, E4M3], ids=str)
@@ -110,7 +110,7 @@ def test_forms_of_experts(calls, gated, rows, n, k, experts, kind, dtype):
                 check(y[at], *want)
 
 
-SOME = [(False, 1100, 2600, 300), (True, 1000, 1500, 260), (False, 777, 5000, 2049), (False, 33, 5000, 2049), (True, 17, 5000, 1030), (False, 1, 2100, 1030)]
+SOME = [(False, 1100, 2600, 300), (True, 1000, 1500, 260), (False, 777, 5000, 2600), (False, 513, 1, 2600), (False, 2100, 4100, 17), (True, 600, 1, 2049), (False, 1, 5000, 700)]
 
 
 def prepared(calls, seed=0):
