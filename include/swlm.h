@@ -463,7 +463,7 @@ int swlm_op_f8_quantize_dev(swlm_ctx* ctx, const swlm_f8_quantize* how, void* cu
  * fp32. act other than SWLM_F8_PLAIN: y = act(w x) * (up x), `up` a second matrix of w's shape: SiLU, GELU (tanh) or, as the clamped experts of
  * SWLM_STEP_ROUTED_MLP have it, g = min(w x, limit), u = clamp(up x, -limit, limit), g * sigmoid(alpha * g) * (u + 1).
  * dtype SWLM_F8_E4M3: the result is quantized as swlm_op_f8_quantize_dev does, into codes y and scales y_scale.
- * experts > 0: rows offsets[e] .. offsets[e + 1] - 1 meet matrix e; offsets [experts + 1] ascend, what exceeds `rows` is cut off, and rows of y that no expert
+ * experts > 0 (at most 1024): rows offsets[e] .. offsets[e + 1] - 1 meet matrix e; offsets [experts + 1] ascend, what exceeds `rows` is cut off, and rows of y that no expert
  * has stay as they are. experts 0: all rows meet the one matrix.
  * A product of two scales is one fp32 number (2^-126 .. 2^127), as is every partial sum.
  * Waits on the device are bounded. Once one has expired, results since then are not valid, and the context's swlm_op_f8_product_dev returns
