@@ -233,3 +233,32 @@ def test_many_rows_that_lie_far_apart(calls, dtype):
     torch.cuda.synchronize()
     same = torch.equal(held.view(torch.uint8), y_far.view(torch.uint8)) if dtype == E4M3 else torch.equal(held, y_far)
     assert same and (dtype != E4M3 or torch.equal(scale, y[1]))
+
+
+@pytest.mark.parametrize("gated,rows,n,k,kind", [(False, 1100, 2600, 300, "wide"), (True, 1000, 1500, 260, "wide"), (False, 777, 5000, 2600, "both"), (False, 513, 1, 2600, "few"),
+                                                 (True, 5, 130, 1030, "few"), (True, 2900, 129, 17, "few")])
+def test_what_is_not_a_number_stays_in_its_place(calls, gated, rows, n, k, kind):
+    """A NaN among a row's codes, and one in a row's scale, make that row's codes and scales NaN and leave the others' bits as they are; so do NaN rows of
+    other experts that share a tile with them."""
+    assert form_of(calls.lib, rows, n, k, 0, gated)[0] == kind
+    g = generator(rows + 9)
+    x, pair = rows_of(g, rows, k), [matrix(g, n, k, 2), matrix(g, n, k, 2) if gated else None]
+    w, up = ((m[0][:1], m[1][:1]) if m is not None else None for m in pair)
+    act = "silu" if gated else "plain"
+    want, got = code_room(rows, n), code_room(rows, n)
+    calls.product(x, w, want, up, act)
+    bad = sorted({rows // 3, rows - 1})
+    x[0].view(torch.uint8)[bad[0], k - 1] = 0xFF
+    x[1][blocks(k) - 1, bad[-1]] = float("nan")
+    calls.product(x, w, got, up, act)
+    torch.cuda.synchronize()
+    fine = torch.ones(rows, dtype=torch.bool, device="cuda")
+    fine[bad] = False
+    assert torch.equal(got[0].view(torch.uint8)[fine], want[0].view(torch.uint8)[fine]) and torch.equal(got[1][:, fine], want[1][:, fine])
+    assert got[0][~fine].float().isnan().all() and got[1][:, ~fine].isnan().all()
+    if rows > 2:   # one expert has the rows before the first bad one, another those from it on
+        cut = torch.tensor([0, bad[0], rows], dtype=torch.int32, device="cuda")
+        y = room(rows, n, torch.float32)
+        calls.product(x, pair[0], y, pair[1], act, cut)
+        torch.cuda.synchronize()
+        assert y[:bad[0]].isfinite().all() and y[bad].isnan().all()
