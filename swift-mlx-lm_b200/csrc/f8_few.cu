@@ -416,7 +416,7 @@ F8FewForm f8_few_form(int rows, int n, int k, int experts, bool gated) {
             // larger clusters leave some SMs without one: of eight CTAs fourteen run at once and sixteen take two turns, of four 36 do
             const double slots = ranges == 8 ? (per_sm == 2 ? 128 : 112) : (ranges == 4 ? 132 : kSms) * per_sm, waves = (double)(int64_t)((tiles * ranges + slots - 1) / slots);
             if (ranges > 1 && waves > 1) break;
-            const double both = per_sm == 2 && tiles * ranges > slots / 2 ? 1.5 : 1.0;   // two CTAs on an SM share it
+            const double both = per_sm == 2 && tiles * ranges > kSms ? 1.5 : 1.0;   // two CTAs on an SM share it
             const double ctas = std::min(tiles * ranges, slots), step = std::max(alone * both, ctas * ((gated ? 2 : 1) * kCodesBytes + nt * kF8Block) / 10e6);   // L2 gives 10 TB/s
             const double cost = std::max(waves * ((blocks + ranges - 1) / ranges * step + 1), memory) + ends + (ranges > 1 ? 0.5 : 0.0);
             if (cost < best.cost) best = {nt, ranges, cost};

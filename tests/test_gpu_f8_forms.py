@@ -41,8 +41,8 @@ def form_of(lib, rows, n, k, experts, gated):
 # what each size is there for: the form of the other columns than those that pairs of SMs take
 FORMS = [
     (False, 1, 5000, 700, "few", 16, 2), (False, 1, 1, 700, "few", 16, 4), (False, 3, 130, 1030, "few", 16, 8), (False, 513, 264, 100, "few", 16, 1),
-    (False, 2100, 1, 17, "few", 32, 1), (False, 1100, 1, 700, "few", 32, 2), (False, 513, 1, 700, "few", 32, 4), (False, 130, 1, 1030, "few", 32, 8),
-    (False, 777, 5000, 17, "few", 64, 1), (False, 2900, 1, 2049, "few", 64, 2), (False, 1100, 1, 2600, "few", 64, 4), (False, 513, 1, 2600, "few", 64, 8),
+    (False, 2100, 1, 17, "few", 32, 1), (False, 1500, 1, 700, "few", 32, 2), (False, 513, 1, 700, "few", 32, 4), (False, 300, 1, 1030, "few", 32, 8),
+    (False, 777, 5000, 17, "few", 64, 1), (False, 2900, 1, 2049, "few", 64, 2), (False, 1500, 1, 2049, "few", 64, 4), (False, 513, 1, 2600, "few", 64, 8),
     (False, 2100, 4100, 17, "few", 128, 1), (False, 70, 9300, 4100, "few", 128, 2), (False, 1100, 2100, 17, "wide", 0, 0), (False, 1100, 2600, 300, "wide", 0, 0),
     (False, 2900, 2800, 700, "wide", 0, 0), (False, 777, 5000, 2600, "both", 64, 2), (False, 2100, 2100, 2049, "both", 64, 4),
     (True, 2, 2957, 290, "few", 16, 1), (True, 600, 1, 700, "few", 16, 2), (True, 1, 1, 700, "few", 16, 4), (True, 5, 130, 1030, "few", 16, 8), (True, 2900, 129, 17, "few", 64, 1),
