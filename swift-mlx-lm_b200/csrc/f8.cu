@@ -120,6 +120,14 @@ int matrix_ok(const swlm_f8_weight& w, int k) {
     if (!w.scale || !aligned(w.scale, 4)) return refuse("a matrix's scales must be 4-byte aligned");
     return SWLM_OK;
 }
+// What a product may have of rows, columns and experts. An expert has its own rows and a last tile of its own.
+const char* size_refused(int rows, int n, int k, int experts) {
+    if (rows < 0 || rows > kF8MaxRows || n < 1 || n > kF8MaxWidth || k < 1 || k > kF8MaxWidth) return "rows, n or k out of range";
+    if (experts < 0 || experts > kExpertMax) return "experts out of range";
+    if ((int64_t)std::max(experts, 1) * n > kF8MaxRows) return "too many rows of all experts' matrices";
+    if (((int64_t)rows / 16 + std::max(experts, 1)) * f8_blocks(n) > kF8MaxTiles) return "too many rows, experts and columns together";
+    return nullptr;
+}
 bool plain_type(int dtype) { return dtype == SWLM_F8_BF16 || dtype == SWLM_F8_FP16 || dtype == SWLM_F8_FP32; }
 
 // (`code`: what the kernels left in the context's word)
@@ -155,12 +163,8 @@ int swlm_op_f8_product_dev(swlm_ctx* ctx, const swlm_f8_product* how, void* cuda
     const swlm_f8_product& a = *how;
     if (!plain_type(a.dtype) && a.dtype != SWLM_F8_E4M3) return refuse("unknown dtype");
     if (a.act < SWLM_F8_PLAIN || a.act > SWLM_F8_CLAMPED) return refuse("unknown activation");
-    if (a.rows < 0 || a.rows > kF8MaxRows || a.n < 1 || a.n > kF8MaxWidth || a.k < 1 || a.k > kF8MaxWidth) return refuse("rows, n or k out of range");
-    if (a.experts < 0 || a.experts > kExpertMax) return refuse("experts out of range");
-    if ((int64_t)std::max(a.experts, 1) * a.n > kF8MaxRows) return refuse("too many rows of all experts' matrices");
+    if (const char* why = size_refused(a.rows, a.n, a.k, a.experts)) return refuse(why);
     if (a.act == SWLM_F8_CLAMPED && (!std::isfinite(a.alpha) || !(a.limit >= 0.f))) return refuse("alpha must be finite, the limit not negative");
-    // (tiles are 32-bit numbers, also where offsets do not ascend and every expert has all rows)
-    if ((int64_t)std::max(a.experts, 1) * (a.rows / 16 + 1) * f8_blocks(a.n) > INT32_MAX) return refuse("too many rows, experts and columns together");
     if (a.rows == 0) return SWLM_OK;
     if (a.experts && (!a.offsets || !aligned(a.offsets, 4))) return refuse("experts need offsets, 4-byte aligned");
     int rc = codes_ok(a.x, a.rows, a.k);
@@ -173,7 +177,8 @@ int swlm_op_f8_product_dev(swlm_ctx* ctx, const swlm_f8_product* how, void* cuda
 }
 
 int swlm_op_f8_product_form(int rows, int n, int k, int experts, int gated, int* form) {
-    if (rows < 1 || rows > kF8MaxRows || n < 1 || n > kF8MaxWidth || k < 1 || k > kF8MaxWidth || experts < 0 || experts > kExpertMax || !form) return refuse("bad argument");
+    if (const char* why = size_refused(rows, n, k, experts)) return refuse(why);
+    if (rows < 1 || !form) return refuse("bad argument");
     const F8ProductForm f = f8_product_form(rows, n, k, experts, gated != 0);
     form[0] = f.wide; form[1] = f.wide == n ? 0 : f.few.nt; form[2] = f.wide == n ? 0 : f.few.ranges;
     return SWLM_OK;

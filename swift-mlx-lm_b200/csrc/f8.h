@@ -11,6 +11,7 @@ constexpr int kF8Block = 128;            // columns of a row's scale, rows and c
 constexpr int kF8MaxRows = 1 << 30;      // row numbers stay 32-bit ones, also a tile behind the last
 constexpr int kF8MaxWidth = 1 << 24;
 constexpr int kExpertMax = 1024;
+constexpr int kF8MaxTiles = 1 << 30;     // tiles of a product, of 16 rows x 128 columns or more: two terabytes of results have no more
 
 // A product of few rows: rows of x per tile, CTAs of a cluster that share K, and what it takes, about (us).
 struct F8FewForm { int nt, ranges; double cost; };

@@ -106,12 +106,14 @@ __device__ __forceinline__ int2 expert_rows(const TileShape& p, int e) {
     return make_int2(from, min(max(p.offsets[e + 1], from), p.rows));
 }
 // Fills first_tile [experts] with the tiles of the experts before each, by all threads of a CTA, and returns the number of tiles; `warps`: a number per warp. A
-// barrier has to follow.
+// barrier has to follow. Sums stop at what offsets that ascend come to at most, which is within kF8MaxTiles: of others, where experts share rows, later tiles are left out.
 template <int THREADS>
 __device__ __forceinline__ int count_tiles(const TileShape& p, int* first_tile, int* warps) {
     if (!p.experts) return (p.rows + p.tile_rows - 1) / p.tile_rows * p.col_tiles;
     constexpr int PER = (kExpertMax + THREADS - 1) / THREADS;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const unsigned most = (unsigned)(p.rows / p.tile_rows + p.experts) * p.col_tiles;
+    auto add = [&](int a, int b) { return (int)min((unsigned)a + (unsigned)b, most); };
     int c[PER], sum = 0;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
@@ -121,24 +123,24 @@ __device__ __forceinline__ int count_tiles(const TileShape& p, int* first_tile, 
             const int2 r = expert_rows(p, e);
             c[j] = (r.y - r.x + p.tile_rows - 1) / p.tile_rows * p.col_tiles;
         }
-        sum += c[j];
+        sum = add(sum, c[j]);
     }
     int scan = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, scan, o);
-        if (lane >= o) scan += v;
+        if (lane >= o) scan = add(scan, v);
     }
     if (lane == 31) warps[warp] = scan;
     __syncthreads();
-    int tiles = 0;
-    for (int w = 0; w < THREADS / 32; ++w) { scan += w < warp ? warps[w] : 0; tiles += warps[w]; }
-    scan -= sum;
+    int tiles = 0, before = __shfl_up_sync(0xffffffffu, scan, 1);
+    if (lane == 0) before = 0;
+    for (int w = 0; w < THREADS / 32; ++w) { before = add(before, w < warp ? warps[w] : 0); tiles = add(tiles, warps[w]); }
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
         const int e = tid * PER + j;
-        if (e < p.experts) first_tile[e] = scan;
-        scan += c[j];
+        if (e < p.experts) first_tile[e] = before;
+        before = add(before, c[j]);
     }
     return tiles;
 }
