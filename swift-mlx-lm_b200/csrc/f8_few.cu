@@ -20,6 +20,13 @@ namespace {
 
 constexpr int kPartPitch = 132;   // floats of a row's part (four more than its columns)
 
+// Clusters of 1, 2, 4 and 8 CTAs, where an SM takes one CTA and where it takes two. A cluster stays within a GPC, so that larger ones leave some SMs without a CTA.
+// kAtOnce: how many run at once, by the starts and ends of the CTAs of a launch of many (fourteen of eight on a GPU whose GPCs have other SMs): a launch has no more,
+// since others would start when those end. kChosenFor: tiles up to which the choice of a form deals K to clusters of that size. Fewer where an SM takes two: with 71
+// and 33 for 66 and 16 one size in forty takes another form, and 80 such sizes drawn at random took 1.02 times as long (0.81 to 1.26).
+constexpr int kAtOnce[2][4] = {{148, 74, 33, 15}, {296, 148, 71, 33}}, kChosenFor[2][4] = {{148, 74, 33, 14}, {296, 148, 66, 16}};
+constexpr int cluster_size(int ranges) { return ranges == 1 ? 0 : ranges == 2 ? 1 : ranges == 4 ? 2 : 3; }
+
 struct FewParams {
     const float *x_scale, *w_scale, *up_scale;
     long long x_scale_stride, y_stride, y_scale_stride;
@@ -385,7 +392,7 @@ int few_launch(const swlm_f8_product& a, int ranges, int* status, cudaStream_t s
     if (!rc && GATED) rc = code_map(a.up.codes, a.up.stride, matrix_rows, a.k, 128, &upmap);
     if (rc) return rc;
     // (at most this many tiles: an expert's last one may have a single row)
-    const int64_t tiles = std::min<int64_t>(((int64_t)a.rows / NT + std::max(a.experts, 1)) * p.col_blocks, kSms * F::PER_SM / ranges);
+    const int64_t tiles = std::min<int64_t>(((int64_t)a.rows / NT + std::max(a.experts, 1)) * p.col_blocks, kAtOnce[F::PER_SM - 1][cluster_size(ranges)]);
     const cudaError_t e = launch_clusters(f8_few_kernel<NT, GATED>, ranges, dim3((unsigned)(tiles * ranges)), dim3(F::THREADS), F::SMEM, s, p, xmap, wmap, upmap);
     return e == cudaSuccess ? SWLM_OK : cuda_fail(e, "product launch");
 }
@@ -413,8 +420,7 @@ F8FewForm f8_few_form(int rows, int n, int k, int experts, bool gated) {
         // rows of an expert end inside a tile
         const double row_tiles = experts ? rows / (double)nt + 0.5 * reached : (rows + nt - 1) / nt, tiles = std::max(row_tiles, (double)reached) * f8_blocks(n);
         for (int ranges = 1; ranges <= 8 && ranges <= blocks; ranges *= 2) {
-            // larger clusters leave some SMs without one: of eight CTAs fourteen run at once and sixteen take two turns, of four 36 do
-            const double slots = ranges == 8 ? (per_sm == 2 ? 128 : 112) : (ranges == 4 ? 132 : kSms) * per_sm, waves = (double)(int64_t)((tiles * ranges + slots - 1) / slots);
+            const double slots = ranges * kChosenFor[per_sm - 1][cluster_size(ranges)], waves = (double)(int64_t)((tiles * ranges + slots - 1) / slots);
             if (ranges > 1 && waves > 1) break;
             const double both = per_sm == 2 && tiles * ranges > kSms ? 1.5 : 1.0;   // two CTAs on an SM share it
             const double ctas = std::min(tiles * ranges, slots), step = std::max(alone * both, ctas * ((gated ? 2 : 1) * kCodesBytes + nt * kF8Block) / 10e6);   // L2 gives 10 TB/s
