@@ -461,7 +461,8 @@ int swlm_op_f8_quantize_dev(swlm_ctx* ctx, const swlm_f8_quantize* how, void* cu
 
 /* y[r][c] = sum over blocks b of 128 columns: x.scale[b][r] * w.scale[c / 128][b] * (codes of row r . codes of w's row c within the block), the sums in
  * fp32. act other than SWLM_F8_PLAIN: y = act(w x) * (up x), `up` a second matrix of w's shape: SiLU, GELU (tanh) or, as the clamped experts of
- * SWLM_STEP_ROUTED_MLP have it, g = min(w x, limit), u = clamp(up x, -limit, limit), g * sigmoid(alpha * g) * (u + 1).
+ * SWLM_STEP_ROUTED_MLP have it, g = min(w x, limit), u = clamp(up x, -limit, limit), g * sigmoid(alpha * g) * (u + 1). Beside what the sums are off, such a
+ * result is off by (16 + 8 |z|) 2^-24 of itself at most, z the exponential's argument: g, 1.596 (g + 0.0447 g^3) or alpha * g; where z is below -87 it may be zero.
  * dtype SWLM_F8_E4M3: the result is quantized as swlm_op_f8_quantize_dev does, into codes y and scales y_scale.
  * experts > 0 (at most 1024): rows offsets[e] .. offsets[e + 1] - 1 meet matrix e; offsets [experts + 1] ascend, what exceeds `rows` is cut off, and rows of y that no expert
  * has stay as they are (of offsets that do not ascend only this is promised). experts 0: all rows meet the one matrix.

@@ -79,8 +79,8 @@ __device__ __forceinline__ unsigned pack2(float a, float b, bool f16) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const unsigned*>(&h);
 }
-// The gated activations (swlm_op_f8_product_dev); a NaN stays one; tanh-GELU as g / (1 + e^-2u). An exponential and a reciprocal of the special function unit, two
-// in the last place each, and |z| 2^-24 for its argument; no branch between values, so that they overlap.
+// The gated activations (swlm_op_f8_product_dev); a NaN stays one; tanh-GELU as g / (1 + e^-2u). An exponential and a reciprocal of the special function unit, within
+// three and two 2^-24 of their values, and |z| 2^-24 for each rounding of the exponential's argument (GELU's has the most, seven); no branch between values, so that they overlap.
 __device__ __forceinline__ float gated(float g, float u, int act, float alpha, float limit) {
     float z = g;
     if (act == SWLM_F8_GELU) z = 1.5957691216f * (g + 0.044715f * g * g * g);
@@ -157,7 +157,7 @@ __device__ __forceinline__ Tile tile_at(const TileShape& p, const int* first_til
         t -= first_tile[lo];
     }
     // Up to kSweep tiles of the shorter side, then those of the next place on the longer one: what CTAs at work together read is about as much of x as of the
-    // matrix, and stays in L2 (8192 rows x 4096 x 14336 with all 16 tiles of columns in a sweep read 526 MB from memory instead of the 175 there are).
+    // matrix, and stays in L2 for longer (8192 rows x 4096 x 14336, 176 MB: 445 MB are read from memory, with all 16 tiles of columns in a sweep 526).
     const int row_tiles = (w.end - w.row0 + p.tile_rows - 1) / p.tile_rows, shorter = min(row_tiles, p.col_tiles), longer = max(row_tiles, p.col_tiles);
     const int sweep = t / (kSweep * longer), width = min(kSweep, shorter - sweep * kSweep);
     t -= sweep * kSweep * longer;

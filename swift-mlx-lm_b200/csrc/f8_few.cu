@@ -4,8 +4,8 @@
 // they are scaled and added; here the scales of the rows of x lie along a thread's registers. Where there are tiles for all SMs, CTAs take them in turn and
 // copies run ahead into the next tile. Where there are few, the blocks of K are dealt to the CTAs of a cluster: their parts then lie in shared memory, 128
 // columns of the result to a row of x, and a warp adds the cluster's parts of a row up in the order of the blocks.
-// What bounds it: memory, and what a launch takes to start and to end. One row x 4096 x 14336 takes 14.4 us of which its 59 MB are 9 (two, four, eight CTAs
-// along K: 21, 14.8, 15.1); 41 rows x 8192 x 2048, gated, 12.1 of 5.2; gate and up of 64 experts, 2048 x 1024, for 256 rows 52 (268 MB: 41).
+// What bounds it: memory, and what a launch takes to start and to end. One row x 4096 x 14336 takes 14.1 us of which its 59 MB are 9 (one, two, four, eight
+// CTAs along K: 35.3, 20.6, 14.1, 14.0); 41 rows x 8192 x 2048, gated, 12 to 13 of 5.2; gate and up of 64 experts, 2048 x 1024, for 256 rows 52 (268 MB: 41).
 #include <algorithm>
 
 #include <cooperative_groups.h>
@@ -111,7 +111,7 @@ f8_few_kernel(const FewParams p, const __grid_constant__ CUtensorMap xmap, const
     auto fail = [&](int code) { if (lane == 0) { atomicExch_system(p.status, code); *failed = 1; } __syncwarp(); };
 
     // A launch behind this one may set itself up (behind the allocation: it cannot get at tensor memory in between): 0.6 us of a chain of products. Not with
-    // experts, where its CTAs would take places that this one's still want (routed 32 x 2048: 84 us, with it 87).
+    // experts, where its CTAs would take places that this one's still want (routed 32 x 2048: 82.6 us, with it 85.8).
     if (!p.tiles.experts) pdl_launch_dependents();
     // Alone every warp runs through all tiles by itself; the CTAs of a cluster meet behind each. A wait that expires ends a warp's work; the cluster's barriers are kept.
     const bool alone = p.ranges == 1;

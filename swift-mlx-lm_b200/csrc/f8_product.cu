@@ -384,7 +384,7 @@ F8ProductForm f8_product_form(int rows, int n, int k, int experts, bool gated) {
     const double wide = wide_cost(rows, n, k, experts, gated);
     f.wide = f.few.cost > wide ? n : 0;
     // A last wave of few tiles leaves most pairs without work: the columns that fill whole waves may go first, and the rest as a product of its own, dealt out
-    // along K (777 rows x 5000 x 4100: 80 tiles on 74 pairs 37.8 us, 72 tiles and 392 columns more 36.0).
+    // along K (777 rows x 5000 x 4100: 80 tiles on 74 pairs 35.7 us, 72 tiles and 392 columns more 34.0).
     const int cols = gated ? 128 : 256, row_tiles = (rows + 255) / 256, pairs = kSms / 2, waves = (int)((int64_t)row_tiles * ((n + cols - 1) / cols) / pairs);
     const int full = (int)std::min<int64_t>((int64_t)waves * pairs / row_tiles * cols, n);
     if (!experts && full > 0 && full < n) {
