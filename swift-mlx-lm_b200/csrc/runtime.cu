@@ -167,9 +167,9 @@ int add_q4_raw(swlm_ctx* ctx, const char* name, int n, int k, const uint32_t* w,
     if ((rc = dev_alloc(&r.biases, (size_t)r.n * lg, &ctx->bytes))) return rc;
     for (int part = 0; part < sl.parts; ++part) {
         const size_t src_row = (size_t)part * sl.part_stride + sl.row0, dst_row = (size_t)part * sl.rows;
-        SWLM_CUDA(cudaMemcpy2D(r.w + dst_row * lw, (size_t)lw * 4, w + src_row * wpr + sl.col0 / 8, (size_t)wpr * 4, (size_t)lw * 4, sl.rows, cudaMemcpyHostToDevice));
-        SWLM_CUDA(cudaMemcpy2D(r.scales + dst_row * lg, (size_t)lg * 2, s + src_row * gpr + sl.col0 / 64, (size_t)gpr * 2, (size_t)lg * 2, sl.rows, cudaMemcpyHostToDevice));
-        SWLM_CUDA(cudaMemcpy2D(r.biases + dst_row * lg, (size_t)lg * 2, b + src_row * gpr + sl.col0 / 64, (size_t)gpr * 2, (size_t)lg * 2, sl.rows, cudaMemcpyHostToDevice));
+        SWLM_CUDA(copy_in_2d(r.w + dst_row * lw, (size_t)lw * 4, w + src_row * wpr + sl.col0 / 8, (size_t)wpr * 4, (size_t)lw * 4, sl.rows));
+        SWLM_CUDA(copy_in_2d(r.scales + dst_row * lg, (size_t)lg * 2, s + src_row * gpr + sl.col0 / 64, (size_t)gpr * 2, (size_t)lg * 2, sl.rows));
+        SWLM_CUDA(copy_in_2d(r.biases + dst_row * lg, (size_t)lg * 2, b + src_row * gpr + sl.col0 / 64, (size_t)gpr * 2, (size_t)lg * 2, sl.rows));
     }
     ctx->raw[name] = r;
     return SWLM_OK;
@@ -203,7 +203,7 @@ int rope_table_for(swlm_plan* plan, int rope_dim, float base, int* index) {
     RopeTable t{rope_dim, base, nullptr};
     int rc = dev_alloc(&t.inv_freq, f.size());
     if (rc) return rc;
-    SWLM_CUDA(cudaMemcpy(t.inv_freq, f.data(), f.size() * 4, cudaMemcpyHostToDevice));
+    SWLM_CUDA(copy_in(t.inv_freq, f.data(), f.size() * 4));
     plan->rope_tables.push_back(t);
     *index = (int)plan->rope_tables.size() - 1;
     return SWLM_OK;
@@ -1492,7 +1492,7 @@ int swlm_weights_add_dense_bf16(swlm_ctx* ctx, const char* name, int64_t rows, i
         // the same shape: new values in the old place, so that plans compiled against the tensor stay valid; another shape
         // replaces it, and those plans must be rebuilt
         if (old->second.rows == sl.rows && old->second.cols == cols && old->second.shard_kind == shard_kind) {
-            SWLM_CUDA(cudaMemcpy(old->second.data, data + (size_t)sl.row0 * cols, (size_t)sl.rows * cols * 2, cudaMemcpyHostToDevice));
+            SWLM_CUDA(copy_in(old->second.data, data + (size_t)sl.row0 * cols, (size_t)sl.rows * cols * 2));
             return SWLM_OK;
         }
         cudaFree(old->second.data);
@@ -1502,7 +1502,7 @@ int swlm_weights_add_dense_bf16(swlm_ctx* ctx, const char* name, int64_t rows, i
     DenseTensor t;
     t.rows = sl.rows; t.cols = cols; t.shard_kind = shard_kind;
     if ((rc = dev_alloc(&t.data, (size_t)t.rows * cols, &ctx->bytes))) return rc;
-    SWLM_CUDA(cudaMemcpy(t.data, data + (size_t)sl.row0 * cols, (size_t)t.rows * cols * 2, cudaMemcpyHostToDevice));
+    SWLM_CUDA(copy_in(t.data, data + (size_t)sl.row0 * cols, (size_t)t.rows * cols * 2));
     ctx->dense[name] = t;
     return SWLM_OK;
 }
@@ -1515,7 +1515,7 @@ int swlm_weights_add_dense_f32(swlm_ctx* ctx, const char* name, int64_t count, c
     if (old != ctx->densef.end()) {
         SWLM_CUDA(cudaDeviceSynchronize());
         if (old->second.count == count) {   // in place, as above
-            SWLM_CUDA(cudaMemcpy(old->second.data, data, (size_t)count * 4, cudaMemcpyHostToDevice));
+            SWLM_CUDA(copy_in(old->second.data, data, (size_t)count * 4));
             return SWLM_OK;
         }
         cudaFree(old->second.data);
@@ -1525,7 +1525,7 @@ int swlm_weights_add_dense_f32(swlm_ctx* ctx, const char* name, int64_t count, c
     DenseF32 t;
     t.count = count;
     if ((rc = dev_alloc(&t.data, (size_t)count, &ctx->bytes))) return rc;
-    SWLM_CUDA(cudaMemcpy(t.data, data, (size_t)count * 4, cudaMemcpyHostToDevice));
+    SWLM_CUDA(copy_in(t.data, data, (size_t)count * 4));
     ctx->densef[name] = t;
     return SWLM_OK;
 }
@@ -1548,7 +1548,7 @@ int swlm_weights_add_matrix_bf16(swlm_ctx* ctx, const char* name, int n, int k, 
         if (m.ld != k) SWLM_CUDA(cudaMemset(m.data, 0, (size_t)n * m.ld * 2));
     }
     SWLM_CUDA(cudaDeviceSynchronize());
-    SWLM_CUDA(cudaMemcpy2D(m.data, (size_t)m.ld * 2, data, (size_t)k * 2, (size_t)k * 2, n, cudaMemcpyHostToDevice));
+    SWLM_CUDA(copy_in_2d(m.data, (size_t)m.ld * 2, data, (size_t)k * 2, (size_t)k * 2, n));
     return SWLM_OK;
 }
 
@@ -1657,12 +1657,12 @@ int swlm_state_create(swlm_plan* plan, swlm_state** out) {
         s->rotor_layer_elems = (size_t)d.kv_heads * groups * 4;
         kv_rotor_init_host(d.kv_layers, d.kv_heads, groups, &s->rotors_host);
         if ((rc = dev_alloc(&s->rotors, s->rotors_host.size()))) return fail(rc);
-        cudaError_t ce = cudaMemcpy(s->rotors, s->rotors_host.data(), s->rotors_host.size() * 2, cudaMemcpyHostToDevice);
+        cudaError_t ce = copy_in(s->rotors, s->rotors_host.data(), s->rotors_host.size() * 2);
         if (ce != cudaSuccess) return fail(cuda_fail(ce, "cudaMemcpy(rotors)"));
         if (d.kv_qjl_dim > 0) {
             kv_qjl_matrix_init_host(d.head_dim, d.kv_qjl_dim, &s->qjl_matrix_host);
             if ((rc = dev_alloc(&s->qjl_matrix, s->qjl_matrix_host.size()))) return fail(rc);
-            ce = cudaMemcpy(s->qjl_matrix, s->qjl_matrix_host.data(), s->qjl_matrix_host.size() * 2, cudaMemcpyHostToDevice);
+            ce = copy_in(s->qjl_matrix, s->qjl_matrix_host.data(), s->qjl_matrix_host.size() * 2);
             if (ce != cudaSuccess) return fail(cuda_fail(ce, "cudaMemcpy(projection matrix)"));
             s->qjl_layer_elems = (size_t)d.max_batch * d.kv_heads * d.max_seq * d.kv_qjl_dim;
             if ((rc = dev_alloc(&s->qjl_res, (size_t)d.kv_layers * s->qjl_layer_elems))) return fail(rc);
@@ -1925,7 +1925,7 @@ int swlm_prefill(swlm_state* s, const int32_t* tokens, int n, int32_t* first_tok
         for (int b = 0; b < m; ++b) seqs[b] = b;
         rc = stream_run(s, m, seqs.data(), counts.data(), tokens, ones.data(), last.data(), nullptr, first_token, s->prefill_chunk > 0 ? s->prefill_chunk : 2048);
         if (rc) { for (int b = 0; b < m; ++b) first_token[b] = -1; return rc; }
-        SWLM_CUDA(cudaMemcpy(s->token_in, first_token, sizeof(int32_t) * m, cudaMemcpyHostToDevice));
+        SWLM_CUDA(copy_in(s->token_in, first_token, sizeof(int32_t) * m));
         return SWLM_OK;
     }
     // several sequences with prompts long enough for chunks: one sequence after the other through the row-wise path
@@ -1991,7 +1991,7 @@ int swlm_prefill_seq(swlm_state* s, int seq, const int32_t* tokens, int n, int32
         int rc = ensure_device(s->plan->ctx);
         if (!rc) rc = stream_run(s, 1, &q, &c, tokens, &one, &last, nullptr, first_token, s->prefill_chunk > 0 ? s->prefill_chunk : 2048);
         if (rc) { *first_token = -1; return rc; }
-        SWLM_CUDA(cudaMemcpy(s->token_in + seq, first_token, sizeof(int32_t), cudaMemcpyHostToDevice));
+        SWLM_CUDA(copy_in(s->token_in + seq, first_token, sizeof(int32_t)));
         return SWLM_OK;
     }
     if (!rows_capable(s->plan)) { set_error("this plan cannot ingest a prompt into one sequence (tensor parallel, head_dim > 128 or an in-place product)"); return SWLM_ERR_UNSUPPORTED; }
@@ -2097,11 +2097,11 @@ int swlm_write_buffer(swlm_state* s, int buf, const uint16_t* src, int count_per
     if (s && s->plan->stream()) { set_error("this plan keeps fp32 buffers: use the _f32 form"); return SWLM_ERR_UNSUPPORTED; }
     if (!s || !src || !buf_ok(buf) || count_per_row > s->width[buf]) { set_error("bad buffer write"); return SWLM_ERR_INVALID; }
     SWLM_CUDA(cudaStreamSynchronize(s->stream));
-    SWLM_CUDA(cudaMemcpy2D(s->buf[buf], (size_t)s->width[buf] * 2, src, (size_t)count_per_row * 2, (size_t)count_per_row * 2,
-                           s->plan->desc.max_batch, cudaMemcpyHostToDevice));
+    SWLM_CUDA(copy_in_2d(s->buf[buf], (size_t)s->width[buf] * 2, src, (size_t)count_per_row * 2, (size_t)count_per_row * 2,
+                           s->plan->desc.max_batch));
     if (buf == SWLM_BUF_RESIDUAL)
-        SWLM_CUDA(cudaMemcpy2D(s->res2, (size_t)s->width[buf] * 2, src, (size_t)count_per_row * 2, (size_t)count_per_row * 2,
-                               s->plan->desc.max_batch, cudaMemcpyHostToDevice));
+        SWLM_CUDA(copy_in_2d(s->res2, (size_t)s->width[buf] * 2, src, (size_t)count_per_row * 2, (size_t)count_per_row * 2,
+                               s->plan->desc.max_batch));
     return SWLM_OK;
 }
 
@@ -2203,13 +2203,13 @@ int swlm_write_kv(swlm_state* s, int which, int layer, int b, int head, int coun
                 }
             }
         }
-        SWLM_CUDA(cudaMemcpy(p, rows.data(), rows.size(), cudaMemcpyHostToDevice));
+        SWLM_CUDA(copy_in(p, rows.data(), rows.size()));
         if (qjl > 0)
-            SWLM_CUDA(cudaMemcpy(s->qjl_res + (size_t)layer * s->qjl_layer_elems + ((size_t)b * d.kv_heads + head) * d.max_seq * qjl,
-                                 res.data(), res.size() * 2, cudaMemcpyHostToDevice));
+            SWLM_CUDA(copy_in(s->qjl_res + (size_t)layer * s->qjl_layer_elems + ((size_t)b * d.kv_heads + head) * d.max_seq * qjl,
+                                 res.data(), res.size() * 2));
         return SWLM_OK;
     }
-    SWLM_CUDA(cudaMemcpy(p, src, (size_t)count * s->plan->desc.head_dim * 2, cudaMemcpyHostToDevice));
+    SWLM_CUDA(copy_in(p, src, (size_t)count * s->plan->desc.head_dim * 2));
     return SWLM_OK;
 }
 
@@ -2229,7 +2229,7 @@ int swlm_state_set_rotors(swlm_state* s, const uint16_t* src, size_t count) {
     if (rc) return rc;
     SWLM_CUDA(cudaStreamSynchronize(s->stream));
     s->rotors_host.assign(src, src + count);
-    SWLM_CUDA(cudaMemcpy(s->rotors, src, count * 2, cudaMemcpyHostToDevice));
+    SWLM_CUDA(copy_in(s->rotors, src, count * 2));
     return SWLM_OK;
 }
 
@@ -2294,9 +2294,9 @@ int swlm_run_step(swlm_state* s, const swlm_step* step, const int32_t* token_in,
     for (RopeTable& t : tmp.rope_tables) cudaFree(t.inv_freq);
     if (rc) return rc;
     if (e != cudaSuccess) return cuda_fail(e, "run_step sync");
-    SWLM_CUDA(cudaMemcpy(s->position, saved_pos.data(), sizeof(int32_t) * m, cudaMemcpyHostToDevice));
+    SWLM_CUDA(copy_in(s->position, saved_pos.data(), sizeof(int32_t) * m));
     const int32_t saved_steps = (int32_t)s->steps_host;
-    SWLM_CUDA(cudaMemcpy(s->step_counter, &saved_steps, 4, cudaMemcpyHostToDevice));
+    SWLM_CUDA(copy_in(s->step_counter, &saved_steps, 4));
     if (token_out) SWLM_CUDA(cudaMemcpy(token_out, s->token_out, sizeof(int32_t) * m, cudaMemcpyDeviceToHost));
     return SWLM_OK;
 }
@@ -2342,8 +2342,8 @@ int swlm_write_buffer_f32(swlm_state* s, int buf, int rows, int count_per_row, c
     if (!f32) { h.resize((size_t)rows * count_per_row); for (size_t i = 0; i < h.size(); ++i) h[i] = float_to_bf16_bits(src[i]); }
     const size_t e = f32 ? 4 : 2;
     const void* from = f32 ? static_cast<const void*>(src) : h.data();
-    SWLM_CUDA(cudaMemcpy2D(b.buf[buf], (size_t)s->width[buf] * e, from, (size_t)count_per_row * e, (size_t)count_per_row * e, rows, cudaMemcpyHostToDevice));
-    if (buf == SWLM_BUF_RESIDUAL) SWLM_CUDA(cudaMemcpy2D(b.res2, (size_t)s->width[buf] * e, from, (size_t)count_per_row * e, (size_t)count_per_row * e, rows, cudaMemcpyHostToDevice));
+    SWLM_CUDA(copy_in_2d(b.buf[buf], (size_t)s->width[buf] * e, from, (size_t)count_per_row * e, (size_t)count_per_row * e, rows));
+    if (buf == SWLM_BUF_RESIDUAL) SWLM_CUDA(copy_in_2d(b.res2, (size_t)s->width[buf] * e, from, (size_t)count_per_row * e, (size_t)count_per_row * e, rows));
     return SWLM_OK;
 }
 int swlm_read_logits_f32(swlm_state* s, float* dst, size_t count) {

@@ -119,7 +119,7 @@ int stream_rope_table(swlm_plan* plan, const swlm_step& st, int* index) {
     }
     int rc = dev_alloc(&t.inv_freq, f.size());
     if (rc) return rc;
-    SWLM_CUDA(cudaMemcpy(t.inv_freq, f.data(), f.size() * 4, cudaMemcpyHostToDevice));
+    SWLM_CUDA(copy_in(t.inv_freq, f.data(), f.size() * 4));
     plan->rope_tables.push_back(t);
     *index = (int)plan->rope_tables.size() - 1;
     return SWLM_OK;
@@ -1082,7 +1082,7 @@ int stream_state_create(swlm_state* s) {
     if ((rc = dev_alloc(&s->seq_identity, d.max_batch))) return rc;
     std::vector<int32_t> ident(d.max_batch);
     for (int i = 0; i < d.max_batch; ++i) ident[i] = i;
-    SWLM_CUDA(cudaMemcpy(s->seq_identity, ident.data(), ident.size() * 4, cudaMemcpyHostToDevice));
+    SWLM_CUDA(copy_in(s->seq_identity, ident.data(), ident.size() * 4));
     if (!s->pf_status) {
         if ((rc = dev_alloc(&s->pf_status, 1))) return rc;
         SWLM_CUDA(cudaMemset(s->pf_status, 0, sizeof(int)));
