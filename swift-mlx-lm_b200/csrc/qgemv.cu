@@ -1128,7 +1128,7 @@ int qgemv_init() {
     const char* tr = getenv("SWLM_TRACE");
     if (tr && tr[0] == '1' && !g_trace_buf) {
         SWLM_CUDA(cudaMalloc((void**)&g_trace_buf, (size_t)kTraceSlots * kTraceCtas * 4 * 8));
-        SWLM_CUDA(cudaMemset(g_trace_buf, 0, (size_t)kTraceSlots * kTraceCtas * 4 * 8));
+        SWLM_CUDA(clear(g_trace_buf, (size_t)kTraceSlots * kTraceCtas * 4 * 8));
     }
     if ((rc = opt_in_smem(qgemv_kernel<1, 0, false>))) return rc;
     if ((rc = opt_in_smem(qgemv_kernel<1, 1, false>))) return rc;

@@ -957,7 +957,7 @@ int grow_scratch(swlm_state* s, size_t attn_floats, size_t partial_floats, size_
         SWLM_CUDA(cudaStreamSynchronize(s->stream));
         cudaFree(s->qgemv_counters); s->qgemv_counters = nullptr; s->qgemv_counters_cap = 0;
         if ((rc = dev_alloc(&s->qgemv_counters, counters))) return rc;
-        SWLM_CUDA(cudaMemset(s->qgemv_counters, 0, counters * sizeof(unsigned)));
+        SWLM_CUDA(clear(s->qgemv_counters, counters * sizeof(unsigned)));
         s->qgemv_counters_cap = counters;
     }
     return SWLM_OK;
@@ -1096,7 +1096,7 @@ int ensure_pf_status(swlm_state* s) {
     if (s->pf_status) return SWLM_OK;
     int rc;
     if ((rc = dev_alloc(&s->pf_status, 1))) return rc;
-    SWLM_CUDA(cudaMemset(s->pf_status, 0, sizeof(int)));
+    SWLM_CUDA(clear(s->pf_status, sizeof(int)));
     return SWLM_OK;
 }
 
@@ -1106,7 +1106,7 @@ int check_pf_status(swlm_state* s) {
     int st = 0;
     SWLM_CUDA(cudaMemcpy(&st, s->pf_status, sizeof(int), cudaMemcpyDeviceToHost));
     if (!st) return SWLM_OK;
-    SWLM_CUDA(cudaMemset(s->pf_status, 0, sizeof(int)));
+    SWLM_CUDA(clear(s->pf_status, sizeof(int)));
     set_error("a bounded wait in the tensor-core product expired");
     return SWLM_ERR_TIMEOUT;
 }
@@ -1128,7 +1128,7 @@ int prefill_workspace(swlm_state* s, int rows) {
     if ((rc = dev_alloc(&s->pf_xh, qgemm_tc_scratch_bytes(rows, widest_activation(s))))) return rc;
     const size_t n_ctr = (size_t)rows * std::max(1, s->plan->desc.kv_heads);
     if ((rc = dev_alloc(&s->pf_attn_counters, n_ctr))) return rc;
-    SWLM_CUDA(cudaMemset(s->pf_attn_counters, 0, n_ctr * sizeof(unsigned)));
+    SWLM_CUDA(clear(s->pf_attn_counters, n_ctr * sizeof(unsigned)));
     size_t attn_floats = 0;
     for (const swlm_step& st : s->plan->steps)
         if (st.kind == SWLM_STEP_ATTN_DECODE) attn_floats = std::max(attn_floats, attn_scratch_floats(rows, st.heads, st.head_dim, 1));
@@ -1545,7 +1545,7 @@ int swlm_weights_add_matrix_bf16(swlm_ctx* ctx, const char* name, int n, int k, 
     if (!m.data) {
         m.n = n; m.k = k; m.ld = (k + 7) / 8 * 8;
         if ((rc = dev_alloc(&m.data, (size_t)n * m.ld, &ctx->bytes))) { ctx->matrices.erase(name); return rc; }
-        if (m.ld != k) SWLM_CUDA(cudaMemset(m.data, 0, (size_t)n * m.ld * 2));
+        if (m.ld != k) SWLM_CUDA(clear(m.data, (size_t)n * m.ld * 2));
     }
     SWLM_CUDA(cudaDeviceSynchronize());
     SWLM_CUDA(copy_in_2d(m.data, (size_t)m.ld * 2, data, (size_t)k * 2, (size_t)k * 2, n));
@@ -1666,7 +1666,7 @@ int swlm_state_create(swlm_plan* plan, swlm_state** out) {
             if (ce != cudaSuccess) return fail(cuda_fail(ce, "cudaMemcpy(projection matrix)"));
             s->qjl_layer_elems = (size_t)d.max_batch * d.kv_heads * d.max_seq * d.kv_qjl_dim;
             if ((rc = dev_alloc(&s->qjl_res, (size_t)d.kv_layers * s->qjl_layer_elems))) return fail(rc);
-            ce = cudaMemset(s->qjl_res, 0, (size_t)d.kv_layers * s->qjl_layer_elems * 2);
+            ce = clear(s->qjl_res, (size_t)d.kv_layers * s->qjl_layer_elems * 2);
             if (ce != cudaSuccess) return fail(cuda_fail(ce, "cudaMemset(residual rows)"));
         }
     }
@@ -1689,7 +1689,7 @@ int swlm_state_create(swlm_plan* plan, swlm_state** out) {
     if ((rc = grow_scratch(s, plan->attn_scratch, plan->qgemv_partial, plan->qgemv_counters))) return fail(rc);
     if ((rc = dev_alloc(&s->attn_counters, (size_t)d.max_batch * std::max(1, d.kv_heads)))) return fail(rc);
     {
-        cudaError_t ce = cudaMemset(s->attn_counters, 0, (size_t)d.max_batch * std::max(1, d.kv_heads) * sizeof(unsigned));
+        cudaError_t ce = clear(s->attn_counters, (size_t)d.max_batch * std::max(1, d.kv_heads) * sizeof(unsigned));
         if (ce != cudaSuccess) return fail(cuda_fail(ce, "cudaMemset"));
     }
     if (d.max_batch > kQGemvMaxRows && !plan->stream()) {
@@ -2390,10 +2390,10 @@ int swlm_tp_export(swlm_state* s, void* handle_out) {
         s->tp.lay = TpLayout{ctx->tp_size, s->plan->desc.max_batch, s->plan->desc.hidden, prefill_batchable(s->plan) ? kTpChunkRows : 0};
         unsigned char* buf = nullptr;
         if ((rc = dev_alloc(&buf, s->tp.lay.total()))) return rc;
-        SWLM_CUDA(cudaMemset(buf, 0, s->tp.lay.total()));
+        SWLM_CUDA(clear(buf, s->tp.lay.total()));
         s->tp.peer[ctx->tp_rank] = buf;
         if ((rc = dev_alloc(&s->tp_words, 8))) return rc;
-        SWLM_CUDA(cudaMemset(s->tp_words, 0, 32));
+        SWLM_CUDA(clear(s->tp_words, 32));
         s->tp.epoch = s->tp_words; s->tp.done = reinterpret_cast<unsigned*>(s->tp_words + 1); s->tp.status = s->tp_words + 2;
         s->tp.host_status = s->tc_status;
         SWLM_CUDA(cudaDeviceSynchronize());
@@ -2512,7 +2512,7 @@ static int op_scratch_sized(swlm_ctx* ctx, size_t pf, size_t cc) {
         ctx->op_counters = nullptr; ctx->op_counter_count = 0;
         int rc = dev_alloc(&ctx->op_counters, cc);
         if (rc) return rc;
-        SWLM_CUDA(cudaMemset(ctx->op_counters, 0, cc * sizeof(unsigned)));
+        SWLM_CUDA(clear(ctx->op_counters, cc * sizeof(unsigned)));
         ctx->op_counter_count = cc;
     }
     return SWLM_OK;
@@ -2579,7 +2579,7 @@ int swlm_op_qgemm(swlm_ctx* ctx, const char* weight, int m, const uint16_t* x_bf
         SWLM_CUDA(cudaMemcpy(&st, ctx->tc_status, sizeof(int), cudaMemcpyDeviceToHost));
         if (st) {
             set_error("qgemm: a bounded wait in a tensor-core kernel expired (code %d)", st);
-            cudaMemset(ctx->tc_status, 0, sizeof(int));
+            clear(ctx->tc_status, sizeof(int));
             return SWLM_ERR_TIMEOUT;
         }
     }
@@ -2646,7 +2646,7 @@ int swlm_op_flash_decode_dev(swlm_ctx* ctx, int b, int heads, int kv_heads, int 
         cudaFree(ctx->op_attn_counters);
         ctx->op_attn_counters = nullptr; ctx->op_attn_counter_count = 0;
         if ((rc = dev_alloc(&ctx->op_attn_counters, need))) return rc;
-        SWLM_CUDA(cudaMemset(ctx->op_attn_counters, 0, need * sizeof(unsigned)));
+        SWLM_CUDA(clear(ctx->op_attn_counters, need * sizeof(unsigned)));
         ctx->op_attn_counter_count = need;
     }
     return launch_flash_decode_plain(b, heads, kv_heads, hd, ctx_len, ctx_stride, scale, static_cast<const __nv_bfloat16*>(q_dev),

@@ -49,9 +49,9 @@ int concat_matrices(swlm_ctx* ctx, const std::vector<std::string>& names, const 
         Matrix& m = ctx->matrices.at(nm);
         if (m.ld != cat.ld) { set_error("matrix '%s' is already part of a product over side-by-side matrices", nm.c_str()); return SWLM_ERR_UNSUPPORTED; }
         SWLM_CUDA(cudaMemcpy(cat.data + row * cat.ld, m.data, (size_t)m.n * m.ld * 2, cudaMemcpyDeviceToDevice));
+        // the copy is there before a plan's first launch; plans built earlier may hold the old address: their kernels are ordered before the free by the device
+        SWLM_CUDA(cudaDeviceSynchronize());
         if (!m.view) {
-            // plans built earlier may hold the old address: their kernels are ordered before the free by the device
-            SWLM_CUDA(cudaDeviceSynchronize());
             cudaFree(m.data);
             ctx->bytes -= (int64_t)m.n * m.ld * 2;
         }
@@ -76,7 +76,7 @@ int join_matrices(swlm_ctx* ctx, const char* left, const char* right, const Matr
     if (part[0]->view || part[1]->view || !strcmp(left, right)) { set_error("matrices '%s' and '%s' are already part of a concatenated matrix", left, right); return SWLM_ERR_UNSUPPORTED; }
     const int rc = dev_alloc(&both.data, (size_t)both.n * both.ld, &ctx->bytes);
     if (rc) return rc;
-    SWLM_CUDA(cudaMemset(both.data, 0, (size_t)both.n * both.ld * 2));
+    SWLM_CUDA(clear(both.data, (size_t)both.n * both.ld * 2));
     for (int i = 0; i < 2; ++i) {
         Matrix& m = *part[i];
         SWLM_CUDA(cudaMemcpy2D(both.data + at[i], (size_t)both.ld * 2, m.data, (size_t)m.ld * 2, (size_t)m.k * 2, m.n, cudaMemcpyDeviceToDevice));
@@ -1043,7 +1043,7 @@ int stream_state_create(swlm_state* s) {
         s->pool.push_back(p);
         s->pool_bytes.push_back(bytes);
         // a page is read whole: rows nobody has written must hold finite numbers
-        if (bytes) SWLM_CUDA(cudaMemset(p, 0, bytes));
+        if (bytes) SWLM_CUDA(clear(p, bytes));
     }
     for (const GroupedLayer& l : plan->grouped) {
         const size_t bytes = (size_t)s->pool_pages * l.row.groups * l.row.block * elem;
@@ -1051,7 +1051,7 @@ int stream_state_create(swlm_state* s) {
         if ((rc = dev_alloc(&p, bytes))) return rc;
         s->pool.push_back(p);
         s->pool_bytes.push_back(bytes);
-        if (bytes) SWLM_CUDA(cudaMemset(p, 0, bytes));
+        if (bytes) SWLM_CUDA(clear(p, bytes));
     }
     for (const DeltaLayer& l : plan->delta) {
         float* st = nullptr;
@@ -1062,18 +1062,18 @@ int stream_state_create(swlm_state* s) {
         if ((rc = dev_alloc(&ring, bytes))) return rc;
         s->delta_ring.push_back(ring);
         // (a sequence at position 0 starts from zeros whatever its slot holds; this is for positions that are set)
-        if (bytes) SWLM_CUDA(cudaMemset(ring, 0, bytes));
-        if (st) SWLM_CUDA(cudaMemset(st, 0, (size_t)d.max_batch * l.state_elems() * 4));
+        if (bytes) SWLM_CUDA(clear(ring, bytes));
+        if (st) SWLM_CUDA(clear(st, (size_t)d.max_batch * l.state_elems() * 4));
     }
     for (const StreamConv& c : plan->convs) {   // (as above: a sequence at position 0 starts from zeros)
         const size_t count = (size_t)d.max_batch * std::max(0, c.taps - 1) * d.hidden;
         float* p = nullptr;
         if ((rc = dev_alloc(&p, count))) return rc;
         s->conv_state.push_back(p);
-        if (count) SWLM_CUDA(cudaMemset(p, 0, count * 4));
+        if (count) SWLM_CUDA(clear(p, count * 4));
     }
     if ((rc = dev_alloc(&s->routed_counts, kMaxExperts))) return rc;
-    SWLM_CUDA(cudaMemset(s->routed_counts, 0, kMaxExperts * 4));
+    SWLM_CUDA(clear(s->routed_counts, kMaxExperts * 4));
     s->seq_pages.assign(d.max_batch, {});
     s->page_table_host.assign((size_t)d.max_batch * s->pages_per_seq, 0);
     if ((rc = dev_alloc(&s->page_table, s->page_table_host.size()))) return rc;
@@ -1085,7 +1085,7 @@ int stream_state_create(swlm_state* s) {
     SWLM_CUDA(copy_in(s->seq_identity, ident.data(), ident.size() * 4));
     if (!s->pf_status) {
         if ((rc = dev_alloc(&s->pf_status, 1))) return rc;
-        SWLM_CUDA(cudaMemset(s->pf_status, 0, sizeof(int)));
+        SWLM_CUDA(clear(s->pf_status, sizeof(int)));
     }
     if ((rc = bufs_rows(s, &s->dec, d.max_batch, d.max_batch))) return rc;
     if ((rc = grow(&s->dec.meta, &s->dec.meta_cap, (size_t)3 * d.max_batch, s->stream))) return rc;
@@ -1143,7 +1143,7 @@ int stream_check_status(swlm_state* s) {
     int st = 0;
     SWLM_CUDA(cudaMemcpy(&st, s->pf_status, sizeof(int), cudaMemcpyDeviceToHost));
     if (!st) return SWLM_OK;
-    SWLM_CUDA(cudaMemset(s->pf_status, 0, sizeof(int)));
+    SWLM_CUDA(clear(s->pf_status, sizeof(int)));
     set_error("a bounded wait in a kernel expired (code %d)", st);
     return SWLM_ERR_TIMEOUT;
 }

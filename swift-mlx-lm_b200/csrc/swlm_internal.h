@@ -26,13 +26,14 @@ int cuda_fail(cudaError_t e, const char* what);  // records the message, returns
     } while (0)
 
 // ---- copies --------------------------------------------------------------------
-// Host to device; the values are there when the call returns. (A plain copy from pageable memory returns when it has been staged, and its way to the device is ordered
+// Host to device, and zeros; they are there when the call returns. (A plain copy from pageable memory returns when it has been staged, a memset at once, and both are ordered
 // with the legacy stream only: the library's streams do not wait for that one, and a kernel launched next could still read what was there before.)
 inline cudaError_t landed(cudaError_t e) { return e == cudaSuccess ? cudaStreamSynchronize(cudaStreamLegacy) : e; }
 inline cudaError_t copy_in(void* dst, const void* src, size_t bytes) { return landed(cudaMemcpy(dst, src, bytes, cudaMemcpyHostToDevice)); }
 inline cudaError_t copy_in_2d(void* dst, size_t dst_pitch, const void* src, size_t src_pitch, size_t row_bytes, size_t rows) {
     return landed(cudaMemcpy2D(dst, dst_pitch, src, src_pitch, row_bytes, rows, cudaMemcpyHostToDevice));
 }
+inline cudaError_t clear(void* p, size_t bytes) { return landed(cudaMemset(p, 0, bytes)); }
 
 // ---- launches ------------------------------------------------------------------
 // Every kernel of the decode step is launched with programmatic stream serialization (programmatic

@@ -95,3 +95,36 @@ def test_weights_in_place(pkg, store, busy):
 
     turns(busy, lambda i: store.add_dense("up.embed", table[i]), look)
     m.close()
+
+
+def test_counters_that_a_first_call_makes_are_zero_before_its_kernel(pkg):
+    """They come from memory that others have filled, and are cleared while another stream keeps the SMs busy."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    heads, kv_heads, dim, length = 32, 8, 128, 4096
+    q, k, v = (torch.randn((h, n, dim), generator=g, device="cuda").bfloat16() for h, n in ((heads, 1), (kv_heads, length), (kv_heads, length)))
+    a = torch.randn((4096, 4096), device="cuda", dtype=torch.bfloat16)
+    other, mine = torch.cuda.Stream(), torch.cuda.Stream()
+    want = None
+    for busy_first in (False, True, True, True):
+        s = pkg.WeightStore(0)
+        filled = torch.full((1 << 30,), 0xFF, dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        del filled
+        torch.cuda.empty_cache()
+        out = torch.zeros((heads, dim), dtype=torch.bfloat16, device="cuda")
+        scratch = torch.zeros(s.lib.swlm_op_flash_decode_scratch_bytes(1, heads, kv_heads, dim, length), dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        if busy_first:
+            with torch.cuda.stream(other):
+                for _ in range(50):
+                    a @ a
+        s.lib.check(s.lib.swlm_op_flash_decode_dev(s.handle, 1, heads, kv_heads, dim, length, length, dim ** -0.5, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                                                   scratch.data_ptr(), mine.cuda_stream))
+        torch.cuda.synchronize()
+        if want is None:
+            want = out.clone()
+            ref = torch.softmax((q.float().view(kv_heads, heads // kv_heads, dim) @ k.float().transpose(1, 2)) * dim ** -0.5, dim=-1) @ v.float()
+            # (the result rounds to bf16, by 2^-8 of itself at most; as much again for weights of which 16 bits meet the values)
+            assert (out.float() - ref.view(heads, dim)).abs().max() <= 2.0 ** -7 * ref.abs().max()
+        assert torch.equal(out, want)
+        s.close()
