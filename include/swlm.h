@@ -466,7 +466,7 @@ int swlm_op_f8_quantize_dev(swlm_ctx* ctx, const swlm_f8_quantize* how, void* cu
  * dtype SWLM_F8_E4M3: the result is quantized as swlm_op_f8_quantize_dev does, into codes y and scales y_scale.
  * experts > 0 (at most 1024): rows offsets[e] .. offsets[e + 1] - 1 meet matrix e; offsets [experts + 1] ascend, what exceeds `rows` is cut off, and rows of y that no expert
  * has stay as they are (of offsets that do not ascend only this is promised). experts 0: all rows meet the one matrix.
- * rows are at most 2^30, n and k 2^24, the rows of all experts' matrices 2^30, and (rows / 16 + max(experts, 1)) * ceil(n / 128), rounded down, 2^30.
+ * rows are at most 2^30, n and k 2^24, the rows of all experts' matrices 2^30, and (floor(rows / 16) + max(experts, 1)) * ceil(n / 128) 2^30.
  * A product of two scales is one fp32 number (2^-126 .. 2^127), as is every partial sum.
  * Waits on the device are bounded. Once one has expired, results since then are not valid, and the context's swlm_op_f8_product_dev returns
  * SWLM_ERR_TIMEOUT without doing anything until swlm_op_f8_status has reported it. */

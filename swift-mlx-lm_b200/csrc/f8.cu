@@ -1,7 +1,6 @@
 // Rows in 8-bit floating point (quantization), and what the calls over such rows check. A code is value / scale rounded once: scales are powers of two, so the
 // quotient is exact, and results do not depend on the launch.
 #include <algorithm>
-#include <climits>
 #include <cmath>
 #include <type_traits>
 
